@@ -1,0 +1,51 @@
+// ttc_ops_common.hpp -- types, conversions and reductions shared by the sequence operators' kernels.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <initializer_list>
+#include <type_traits>
+
+#include "ttc_lqr.h"
+#include "ttc_ops.h"
+
+namespace ttc {
+
+// 16 bytes of T: what a lane loads or stores at once
+template <class T>
+struct alignas(16) Pack {
+  static constexpr int N = 16 / sizeof(T);
+  T v[N];
+};
+
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(__bf16 x) { return (float)x; }
+template <class T>
+__device__ __forceinline__ T from_f(float x) { return (T)x; }  // bf16: to nearest, ties to even
+
+// sum over aligned groups of `width` lanes (a power of two up to 64), in every lane
+__device__ __forceinline__ float lane_sum(float v, int width) {
+  for (int m = width >> 1; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+  return v;
+}
+
+__device__ __forceinline__ float sigmoid(float z) { return 1.0f / (1.0f + __expf(-z)); }
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline int launched() { return hipGetLastError() == hipSuccess ? TTC_LQR_OK : TTC_LQR_ELAUNCH; }
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// whether sizes of at least 0 have a product of at most 2^58, so that byte counts and offsets of several such arrays
+// stay within 64 bits
+inline bool countable(std::initializer_list<int64_t> sizes) {
+  __int128 p = 1;
+  for (int64_t v : sizes) {
+    p *= v > 1 ? v : 1;  // an empty array's other sizes are bounded too
+    if (p > ((__int128)1 << 58)) return false;
+  }
+  return true;
+}
+
+constexpr int64_t MAX_GRID = 0x7fffffff;
+
+}  // namespace ttc

@@ -1,0 +1,701 @@
+// ttc_ops_norm.hip -- group norm with an activation or a gate over channels-last data, forward and backward.
+//
+//   y0 = (x - mean) rstd w + b over the l positions and the c / G channels of a group;
+//   y = act(y0), or y0 act(gate)
+//   backward, with dy0 = dy act'(y0) or dy act(gate):  dxhat = dy0 w,
+//   dx = rstd (dxhat - mean(dxhat) - xhat mean(dxhat xhat)),  dw = sum dy0 xhat,  db = sum dy0,
+//   dgate = dy y0 act'(gate).
+//
+// Bound: memory.  Two forms:
+//  * one position (l = 1: a norm over each head of a token): a group is contiguous, up to 64 lanes hold it in
+//    registers, so x is read once and the variance is that of the centred values;
+//  * any l: slabs of positions, each reduced over whole rows of c channels (coalesced); sums per channel are taken
+//    about the slab's first position (a large common mean costs no digits) and joined as (mean, sum of squares)
+//    pairs; a second pass reads x again and writes y.
+#include "ttc_ops_common.hpp"
+
+namespace ttc {
+
+struct Affine {  // weight and bias of type float or bf16, or none
+  const void *w, *b;
+  bool bf16;
+  __device__ __forceinline__ float weight(int64_t c) const {
+    if (w == nullptr) return 1.0f;
+    return bf16 ? to_f(static_cast<const __bf16*>(w)[c]) : static_cast<const float*>(w)[c];
+  }
+  __device__ __forceinline__ float bias(int64_t c) const {
+    if (b == nullptr) return 0.0f;
+    return bf16 ? to_f(static_cast<const __bf16*>(b)[c]) : static_cast<const float*>(b)[c];
+  }
+};
+
+// act(z) and its slope
+template <bool SILU>
+__device__ __forceinline__ float act(float z) {
+  return SILU ? z * sigmoid(z) : z;
+}
+template <bool SILU>
+__device__ __forceinline__ void act_slope(float z, float& on, float& slope) {
+  if (SILU) {
+    const float s = sigmoid(z);
+    on = z * s;
+    slope = s * (1.0f + z * (1.0f - s));
+  } else {
+    on = z;
+    slope = 1.0f;
+  }
+}
+
+template <bool SILU, bool GATE>
+__device__ __forceinline__ float out_of(float y0, float gate) {
+  return GATE ? y0 * act<SILU>(gate) : act<SILU>(y0);
+}
+// gradient of y0 and of the gate
+template <bool SILU, bool GATE>
+__device__ __forceinline__ float back_of(float dy, float y0, float gate, float& dgate) {
+  float on, slope;
+  act_slope<SILU>(GATE ? gate : y0, on, slope);
+  dgate = GATE ? dy * y0 * slope : 0.0f;
+  return GATE ? dy * on : dy * slope;
+}
+
+template <class T, int V>
+struct alignas(V * sizeof(T)) Vec {
+  T v[V];
+};
+
+// ---- one position: rows of `cg` contiguous channels ---------------------------------------------------------
+
+// `lanes` (a power of two) lanes a row, NV vectors of V elements each
+template <class T, int V, int NV, bool SILU, bool GATE>
+__global__ __launch_bounds__(256) void norm_row_kernel(const T* __restrict__ x, const T* __restrict__ gate, Affine aff,
+                                                       int64_t rows, int G, int cg, int lanes, float eps,
+                                                       T* __restrict__ y, float* __restrict__ mean_out,
+                                                       float* __restrict__ rstd_out) {
+  const int lane = threadIdx.x % lanes;
+  const int64_t row = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+  const bool live = row < rows;
+  const int64_t base = row * cg;
+  const int ch0 = (int)(row % G) * cg;
+  Vec<T, V> xv[NV], gv[NV];
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * lanes + lane) * V;
+    if (live && c < cg) {
+      xv[i] = *reinterpret_cast<const Vec<T, V>*>(x + base + c);
+      if (GATE) gv[i] = *reinterpret_cast<const Vec<T, V>*>(gate + base + c);
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum += to_f(xv[i].v[j]);
+    }
+  }
+  const float mean = lane_sum(sum, lanes) / cg;
+  float sq = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (live && (i * lanes + lane) * V < cg) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = to_f(xv[i].v[j]) - mean;
+        sq = fmaf(d, d, sq);
+      }
+    }
+  const float rstd = 1.0f / sqrtf(lane_sum(sq, lanes) / cg + eps);
+  if (!live) return;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * lanes + lane) * V;
+    if (c >= cg) break;
+    Vec<T, V> out;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float y0 = fmaf((to_f(xv[i].v[j]) - mean) * rstd, aff.weight(ch0 + c + j), aff.bias(ch0 + c + j));
+      out.v[j] = from_f<T>(out_of<SILU, GATE>(y0, GATE ? to_f(gv[i].v[j]) : 0.0f));
+    }
+    *reinterpret_cast<Vec<T, V>*>(y + base + c) = out;
+  }
+  if (lane == 0 && mean_out) {
+    mean_out[row] = mean;
+    rstd_out[row] = rstd;
+  }
+}
+
+// Backward: a thread keeps its channels (group, lane) and walks down a slab of the n rows, so the sums over n of
+// the weight's and bias's gradients stay in registers.  A workgroup covers 256 / lanes groups of a row of G, or
+// several rows at once where G is smaller (`gper` groups, `rper` rows).  partial: [parts, 2, c] fp32.
+template <class T, int V, int NV, bool SILU, bool GATE>
+__global__ __launch_bounds__(256) void norm_row_backward_kernel(
+    const T* __restrict__ x, const T* __restrict__ gate, const T* __restrict__ dy, Affine aff, int64_t n, int G, int cg,
+    int lanes, int gper, int rper, int gblocks, int slab, const float* __restrict__ mean_in,
+    const float* __restrict__ rstd_in, T* __restrict__ dx, T* __restrict__ dgate, float* __restrict__ partial) {
+  const int lane = threadIdx.x % lanes, unit = threadIdx.x / lanes;
+  const int gb = blockIdx.x % gblocks;
+  const int64_t sl = blockIdx.x / gblocks;
+  const int r = unit / gper, g = gb * gper + unit % gper;
+  if (r >= rper || g >= G) return;  // no barrier follows; a row's lanes leave together
+  const int64_t n0 = sl * slab, n1 = n0 + slab < n ? n0 + slab : n;
+  float w[NV][V], b[NV][V], dw[NV][V], db[NV][V];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int c = (i * lanes + lane) * V + j;
+      w[i][j] = c < cg ? aff.weight(g * cg + c) : 0.0f;
+      b[i][j] = c < cg ? aff.bias(g * cg + c) : 0.0f;
+      dw[i][j] = db[i][j] = 0.0f;
+    }
+  const float inv = 1.0f / cg;
+  for (int64_t m = n0 + r; m < n1; m += rper) {
+    const int64_t row = m * G + g, base = row * cg;
+    const float mean = mean_in[row], rstd = rstd_in[row];
+    float xh[NV][V], dh[NV][V], s1 = 0.0f, s2 = 0.0f;
+    Vec<T, V> xv[NV], dv[NV], gv[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * lanes + lane) * V;
+      if (c < cg) {
+        xv[i] = *reinterpret_cast<const Vec<T, V>*>(x + base + c);
+        dv[i] = *reinterpret_cast<const Vec<T, V>*>(dy + base + c);
+        if (GATE) gv[i] = *reinterpret_cast<const Vec<T, V>*>(gate + base + c);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * lanes + lane) * V;
+      if (c < cg) {
+        Vec<T, V> dg;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          xh[i][j] = (to_f(xv[i].v[j]) - mean) * rstd;
+          float dgj;
+          const float d0 = back_of<SILU, GATE>(to_f(dv[i].v[j]), fmaf(xh[i][j], w[i][j], b[i][j]),
+                                               GATE ? to_f(gv[i].v[j]) : 0.0f, dgj);
+          dg.v[j] = from_f<T>(dgj);
+          dw[i][j] = fmaf(d0, xh[i][j], dw[i][j]);
+          db[i][j] += d0;
+          dh[i][j] = d0 * w[i][j];
+          s1 += dh[i][j];
+          s2 = fmaf(dh[i][j], xh[i][j], s2);
+        }
+        if (GATE && dgate) *reinterpret_cast<Vec<T, V>*>(dgate + base + c) = dg;
+      }
+    }
+    s1 = lane_sum(s1, lanes) * inv;
+    s2 = lane_sum(s2, lanes) * inv;
+    if (dx) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * lanes + lane) * V;
+        if (c < cg) {
+          Vec<T, V> out;
+#pragma unroll
+          for (int j = 0; j < V; ++j) out.v[j] = from_f<T>(rstd * (dh[i][j] - s1 - xh[i][j] * s2));
+          *reinterpret_cast<Vec<T, V>*>(dx + base + c) = out;
+        }
+      }
+    }
+  }
+  if (partial) {
+    float* p = partial + (sl * rper + r) * 2 * (int64_t)G * cg + g * cg;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int c = (i * lanes + lane) * V + j;
+        if (c < cg) {
+          p[c] = dw[i][j];
+          p[(int64_t)G * cg + c] = db[i][j];
+        }
+      }
+  }
+}
+
+// Sums of [parts, 2, c] over the parts, in 64 bits: 16 channels a workgroup, 16 threads each
+template <class W>
+__global__ __launch_bounds__(256) void norm_affine_sum_kernel(const float* __restrict__ partial, int64_t parts, int64_t c,
+                                                              W* __restrict__ dw, W* __restrict__ db) {
+  __shared__ double sw[16][17], sb[16][17];
+  const int cx = threadIdx.x % 16, py = threadIdx.x / 16;
+  const int64_t ch = (int64_t)blockIdx.x * 16 + cx;
+  double w = 0.0, b = 0.0;
+  if (ch < c)
+    for (int64_t p = py; p < parts; p += 16) {
+      w += partial[p * 2 * c + ch];
+      b += partial[(p * 2 + 1) * c + ch];
+    }
+  sw[py][cx] = w;
+  sb[py][cx] = b;
+  __syncthreads();
+  if (py == 0 && ch < c) {
+    for (int i = 1; i < 16; ++i) {
+      w += sw[i][cx];
+      b += sb[i][cx];
+    }
+    if (dw) dw[ch] = from_f<W>((float)w);
+    if (db) db[ch] = from_f<W>((float)b);
+  }
+}
+
+// ---- any number of positions ---------------------------------------------------------------------------------
+
+// Slab kernels: a workgroup reads `slab` positions of one n, all channels in blocks of 256 / rper vectors; thread
+// (r, column) walks down positions r, r + rper, ...
+struct Slab {
+  int64_t L, slab, slabs;
+  int C, G, cg, cols, rper, cblocks;  // cols: vectors of a row
+};
+
+// (mean, M2) of `count` values per (n, slab, channel) -> partial [n, slabs, 2, c]
+template <class T, int V>
+__global__ __launch_bounds__(256) void norm_slab_stats_kernel(const T* __restrict__ x, Slab S,
+                                                              float* __restrict__ partial) {
+  __shared__ float s1[256 * V], s2[256 * V];
+  const int cper = 256 / S.rper;
+  const int r = threadIdx.x / cper, cc = threadIdx.x % cper;
+  int64_t blk = blockIdx.x;
+  const int cb = (int)(blk % S.cblocks);
+  blk /= S.cblocks;
+  const int64_t sl = blk % S.slabs, n = blk / S.slabs;
+  const int col = cb * cper + cc;
+  const bool live = r < S.rper && col < S.cols;
+  const int64_t l0 = sl * S.slab, l1 = l0 + S.slab < S.L ? l0 + S.slab : S.L;
+  float a[V], q[V], k[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) a[j] = q[j] = k[j] = 0.0f;
+  if (live) {
+    const T* p = x + n * S.L * S.C + (int64_t)col * V;
+    const Vec<T, V> first = *reinterpret_cast<const Vec<T, V>*>(p + l0 * S.C);
+#pragma unroll
+    for (int j = 0; j < V; ++j) k[j] = to_f(first.v[j]);
+#pragma unroll 4
+    for (int64_t l = l0 + r; l < l1; l += S.rper) {
+      const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(p + l * S.C);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = to_f(v.v[j]) - k[j];
+        a[j] += d;
+        q[j] = fmaf(d, d, q[j]);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    s1[j * 256 + threadIdx.x] = a[j];
+    s2[j * 256 + threadIdx.x] = q[j];
+  }
+  __syncthreads();
+  if (r == 0 && col < S.cols) {
+    const float cnt = (float)(l1 - l0);
+    float* out = partial + ((n * S.slabs + sl) * 2) * S.C + (int64_t)col * V;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      for (int i = 1; i < S.rper; ++i) {
+        a[j] += s1[j * 256 + i * cper + cc];
+        q[j] += s2[j * 256 + i * cper + cc];
+      }
+      out[j] = k[j] + a[j] / cnt;
+      out[S.C + j] = fmaxf(q[j] - a[j] * (a[j] / cnt), 0.0f);
+    }
+  }
+}
+
+// joins them: one workgroup per (n, group)
+__global__ __launch_bounds__(256) void norm_slab_join_kernel(const float* __restrict__ partial, Slab S, float eps,
+                                                             float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+  __shared__ double sh[256];
+  const int64_t ng = blockIdx.x, n = ng / S.G;
+  const int g = (int)(ng % S.G);
+  const int64_t all = S.slabs * S.cg;
+  const float* p = partial + n * S.slabs * 2 * S.C + g * S.cg;
+  auto sum = [&](double v) {
+    sh[threadIdx.x] = v;
+    __syncthreads();
+    for (int m = 128; m >= 1; m >>= 1) {
+      if ((int)threadIdx.x < m) sh[threadIdx.x] += sh[threadIdx.x + m];
+      __syncthreads();
+    }
+    const double r = sh[0];
+    __syncthreads();
+    return r;
+  };
+  auto count = [&](int64_t sl) { return (double)(sl + 1 < S.slabs ? S.slab : S.L - sl * S.slab); };
+  double acc = 0.0;
+  for (int64_t i = threadIdx.x; i < all; i += 256) {
+    const int64_t sl = i / S.cg, c = i % S.cg;
+    acc += count(sl) * p[sl * 2 * S.C + c];
+  }
+  const double total = (double)S.L * S.cg, mean = sum(acc) / total;
+  acc = 0.0;
+  for (int64_t i = threadIdx.x; i < all; i += 256) {
+    const int64_t sl = i / S.cg, c = i % S.cg;
+    const double d = p[sl * 2 * S.C + c] - mean;
+    acc += p[(sl * 2 + 1) * S.C + c] + count(sl) * d * d;
+  }
+  const double var = sum(acc) / total;
+  if (threadIdx.x == 0) {
+    mean_out[ng] = (float)mean;
+    rstd_out[ng] = (float)(1.0 / sqrt(var + eps));
+  }
+}
+
+template <class T, int V, bool SILU, bool GATE>
+__global__ __launch_bounds__(256) void norm_slab_apply_kernel(const T* __restrict__ x, const T* __restrict__ gate,
+                                                              Affine aff, Slab S, const float* __restrict__ mean,
+                                                              const float* __restrict__ rstd, T* __restrict__ y) {
+  const int cper = 256 / S.rper;
+  const int r = threadIdx.x / cper, cc = threadIdx.x % cper;
+  int64_t blk = blockIdx.x;
+  const int cb = (int)(blk % S.cblocks);
+  blk /= S.cblocks;
+  const int64_t sl = blk % S.slabs, n = blk / S.slabs;
+  const int col = cb * cper + cc;
+  if (r >= S.rper || col >= S.cols) return;
+  const int64_t l0 = sl * S.slab, l1 = l0 + S.slab < S.L ? l0 + S.slab : S.L;
+  float m[V], k[V], w[V], b[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int c = col * V + j, g = c / S.cg;
+    m[j] = mean[n * S.G + g];
+    k[j] = rstd[n * S.G + g];
+    w[j] = aff.weight(c);
+    b[j] = aff.bias(c);
+  }
+  const int64_t base = n * S.L * S.C + (int64_t)col * V;
+#pragma unroll 4
+  for (int64_t l = l0 + r; l < l1; l += S.rper) {
+    const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(x + base + l * S.C);
+    Vec<T, V> gt, out;
+    if (GATE) gt = *reinterpret_cast<const Vec<T, V>*>(gate + base + l * S.C);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      out.v[j] = from_f<T>(
+          out_of<SILU, GATE>(fmaf((to_f(v.v[j]) - m[j]) * k[j], w[j], b[j]), GATE ? to_f(gt.v[j]) : 0.0f));
+    *reinterpret_cast<Vec<T, V>*>(y + base + l * S.C) = out;
+  }
+}
+
+// sums over a slab of dy0 xhat and dy0 per channel -> partial [n, slabs, 2, c]; writes dgate on the way
+template <class T, int V, bool SILU, bool GATE>
+__global__ __launch_bounds__(256) void norm_slab_back_stats_kernel(const T* __restrict__ x, const T* __restrict__ gate,
+                                                                   const T* __restrict__ dy, Affine aff, Slab S,
+                                                                   const float* __restrict__ mean,
+                                                                   const float* __restrict__ rstd, T* __restrict__ dgate,
+                                                                   float* __restrict__ partial) {
+  __shared__ float s1[256 * V], s2[256 * V];
+  const int cper = 256 / S.rper;
+  const int r = threadIdx.x / cper, cc = threadIdx.x % cper;
+  int64_t blk = blockIdx.x;
+  const int cb = (int)(blk % S.cblocks);
+  blk /= S.cblocks;
+  const int64_t sl = blk % S.slabs, n = blk / S.slabs;
+  const int col = cb * cper + cc;
+  const bool live = r < S.rper && col < S.cols;
+  const int64_t l0 = sl * S.slab, l1 = l0 + S.slab < S.L ? l0 + S.slab : S.L;
+  float a[V], q[V], m[V], k[V], w[V], b[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) a[j] = q[j] = 0.0f;
+  if (live) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int c = col * V + j, g = c / S.cg;
+      m[j] = mean[n * S.G + g];
+      k[j] = rstd[n * S.G + g];
+      w[j] = aff.weight(c);
+      b[j] = aff.bias(c);
+    }
+    const int64_t base = n * S.L * S.C + (int64_t)col * V;
+#pragma unroll 4
+    for (int64_t l = l0 + r; l < l1; l += S.rper) {
+      const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(x + base + l * S.C);
+      const Vec<T, V> d = *reinterpret_cast<const Vec<T, V>*>(dy + base + l * S.C);
+      Vec<T, V> gt, dg;
+      if (GATE) gt = *reinterpret_cast<const Vec<T, V>*>(gate + base + l * S.C);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float xh = (to_f(v.v[j]) - m[j]) * k[j];
+        float dgj;
+        const float d0 =
+            back_of<SILU, GATE>(to_f(d.v[j]), fmaf(xh, w[j], b[j]), GATE ? to_f(gt.v[j]) : 0.0f, dgj);
+        dg.v[j] = from_f<T>(dgj);
+        a[j] = fmaf(d0, xh, a[j]);
+        q[j] += d0;
+      }
+      if (GATE && dgate) *reinterpret_cast<Vec<T, V>*>(dgate + base + l * S.C) = dg;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    s1[j * 256 + threadIdx.x] = a[j];
+    s2[j * 256 + threadIdx.x] = q[j];
+  }
+  __syncthreads();
+  if (r == 0 && col < S.cols) {
+    float* out = partial + ((n * S.slabs + sl) * 2) * S.C + (int64_t)col * V;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      for (int i = 1; i < S.rper; ++i) {
+        a[j] += s1[j * 256 + i * cper + cc];
+        q[j] += s2[j * 256 + i * cper + cc];
+      }
+      out[j] = a[j];
+      out[S.C + j] = q[j];
+    }
+  }
+}
+
+// means over each group of dxhat xhat and dxhat -> sums [n, g, 2]
+__global__ __launch_bounds__(256) void norm_slab_back_join_kernel(const float* __restrict__ partial, Affine aff, Slab S,
+                                                                  float* __restrict__ sums) {
+  __shared__ double s1[256], s2[256];
+  const int64_t ng = blockIdx.x, n = ng / S.G;
+  const int g = (int)(ng % S.G);
+  const int64_t all = S.slabs * S.cg;
+  const float* p = partial + n * S.slabs * 2 * S.C + g * S.cg;
+  double a = 0.0, q = 0.0;
+  for (int64_t i = threadIdx.x; i < all; i += 256) {
+    const int64_t sl = i / S.cg, c = i % S.cg;
+    const double w = aff.weight(g * S.cg + c);
+    a += w * p[sl * 2 * S.C + c];
+    q += w * p[(sl * 2 + 1) * S.C + c];
+  }
+  s1[threadIdx.x] = a;
+  s2[threadIdx.x] = q;
+  __syncthreads();
+  for (int m = 128; m >= 1; m >>= 1) {
+    if ((int)threadIdx.x < m) {
+      s1[threadIdx.x] += s1[threadIdx.x + m];
+      s2[threadIdx.x] += s2[threadIdx.x + m];
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    const double total = (double)S.L * S.cg;
+    sums[2 * ng] = (float)(s1[0] / total);
+    sums[2 * ng + 1] = (float)(s2[0] / total);
+  }
+}
+
+template <class T, int V, bool SILU, bool GATE>
+__global__ __launch_bounds__(256) void norm_slab_back_apply_kernel(const T* __restrict__ x, const T* __restrict__ gate,
+                                                                   const T* __restrict__ dy, Affine aff, Slab S,
+                                                                   const float* __restrict__ mean,
+                                                                   const float* __restrict__ rstd,
+                                                                   const float* __restrict__ sums, T* __restrict__ dx) {
+  const int cper = 256 / S.rper;
+  const int r = threadIdx.x / cper, cc = threadIdx.x % cper;
+  int64_t blk = blockIdx.x;
+  const int cb = (int)(blk % S.cblocks);
+  blk /= S.cblocks;
+  const int64_t sl = blk % S.slabs, n = blk / S.slabs;
+  const int col = cb * cper + cc;
+  if (r >= S.rper || col >= S.cols) return;
+  const int64_t l0 = sl * S.slab, l1 = l0 + S.slab < S.L ? l0 + S.slab : S.L;
+  float m[V], k[V], w[V], b[V], c1[V], c2[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int c = col * V + j;
+    const int64_t g = n * S.G + c / S.cg;
+    m[j] = mean[g];
+    k[j] = rstd[g];
+    c2[j] = sums[2 * g];
+    c1[j] = sums[2 * g + 1];
+    w[j] = aff.weight(c);
+    b[j] = aff.bias(c);
+  }
+  const int64_t base = n * S.L * S.C + (int64_t)col * V;
+#pragma unroll 4
+  for (int64_t l = l0 + r; l < l1; l += S.rper) {
+    const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(x + base + l * S.C);
+    const Vec<T, V> d = *reinterpret_cast<const Vec<T, V>*>(dy + base + l * S.C);
+    Vec<T, V> gt, out;
+    if (GATE) gt = *reinterpret_cast<const Vec<T, V>*>(gate + base + l * S.C);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float xh = (to_f(v.v[j]) - m[j]) * k[j];
+      float dgj;
+      const float d0 = back_of<SILU, GATE>(to_f(d.v[j]), fmaf(xh, w[j], b[j]), GATE ? to_f(gt.v[j]) : 0.0f, dgj);
+      out.v[j] = from_f<T>(k[j] * (d0 * w[j] - c1[j] - xh * c2[j]));
+    }
+    *reinterpret_cast<Vec<T, V>*>(dx + base + l * S.C) = out;
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------
+
+struct NormPlan {
+  bool rows;              // the one-position form
+  int V, lanes, NV;       // rows: lanes and vectors a group
+  int gper, rper, gblocks, slab;
+  int64_t slabs;
+  Slab S;
+  size_t floats;          // workspace
+};
+
+inline bool norm_wide(const ttc_group_norm_args& A) {
+  const int V = A.dtype == TTC_DTYPE_F32 ? 4 : 8;
+  return A.c % V == 0 && aligned16(A.x) && aligned16(A.gate) && aligned16(A.y) && aligned16(A.dy) &&
+         aligned16(A.dx) && aligned16(A.dgate);
+}
+
+// Everything but the vector width follows from sizes alone, so that the workspace's size does too: it is computed for
+// both widths and the larger taken.
+inline NormPlan norm_plan(const ttc_group_norm_args& A, bool wide) {
+  NormPlan P{};
+  const int full = A.dtype == TTC_DTYPE_F32 ? 4 : 8;
+  const int64_t cg = A.c / A.groups;
+  const int Vr = wide && cg % full == 0 ? full : 1;
+  const int64_t vecs = ceil_div(cg, Vr);
+  P.rows = A.l == 1 && vecs <= 64 * 4;
+  if (P.rows) {
+    P.V = Vr;
+    P.lanes = 1;
+    while (P.lanes < 64 && P.lanes < vecs) P.lanes *= 2;
+    const int need = (int)ceil_div(vecs, P.lanes);
+    P.NV = need <= 1 ? 1 : need <= 2 ? 2 : 4;
+    if (A.backward) {
+      const int units = 256 / P.lanes;
+      P.gper = A.groups < units ? (int)A.groups : units;
+      P.rper = units / P.gper;
+      P.gblocks = (int)ceil_div(A.groups, P.gper);
+      // 2,048 workgroups fill the GPU eight waves a SIMD deep; more rows each keep the partial sums small
+      const int64_t want = 2048 / P.gblocks > 0 ? 2048 / P.gblocks : 1;
+      int64_t slab = ceil_div(A.n, want);
+      slab = slab < P.rper ? P.rper : slab;
+      P.slab = (int)slab;
+      P.slabs = ceil_div(A.n, slab);
+      if (A.dweight || A.dbias) P.floats = (size_t)(P.slabs * P.rper * 2 * A.c);
+    }
+    return P;
+  }
+  Slab& S = P.S;
+  P.V = wide ? full : 1;
+  S.L = A.l;
+  S.C = (int)A.c;
+  S.G = (int)A.groups;
+  S.cg = (int)cg;
+  S.cols = (int)(A.c / P.V);
+  const int cper = S.cols < 256 ? S.cols : 256;
+  S.rper = 256 / cper;
+  S.cblocks = (int)ceil_div(S.cols, 256 / S.rper);
+  const int64_t want = ceil_div(2048, A.n * S.cblocks);
+  int64_t slab = ceil_div(A.l, want);
+  slab = slab < 4 * S.rper ? 4 * S.rper : slab;
+  S.slab = slab < A.l ? slab : A.l;
+  S.slabs = ceil_div(A.l, S.slab);
+  P.floats = (size_t)(A.n * S.slabs * 2 * A.c) + (size_t)(A.n * A.groups * 2);
+  return P;
+}
+
+template <class T, int V, bool SILU, bool GATE>
+int norm_run(const ttc_group_norm_args& A, const NormPlan& P, hipStream_t s) {
+  const T *x = static_cast<const T*>(A.x), *gate = static_cast<const T*>(A.gate), *dy = static_cast<const T*>(A.dy);
+  const Affine aff{A.weight, A.bias, A.weight_dtype == TTC_DTYPE_BF16};
+  const float eps = (float)A.eps;
+  float* ws = static_cast<float*>(A.workspace);
+  const int G = (int)A.groups, cg = (int)(A.c / A.groups);
+  int64_t parts = 0;
+  if (P.rows) {
+    auto go = [&](auto nv) {
+      constexpr int NV = decltype(nv)::value;
+      if (!A.backward) {
+        const int64_t rows = A.n * G, blocks = ceil_div(rows, 256 / P.lanes);
+        if (blocks > MAX_GRID) return TTC_LQR_EINVAL;
+        hipLaunchKernelGGL((norm_row_kernel<T, V, NV, SILU, GATE>), dim3((unsigned)blocks), dim3(256), 0, s, x, gate, aff,
+                           rows, G, cg, P.lanes, eps, static_cast<T*>(A.y), A.mean, A.rstd);
+        return launched();
+      }
+      const int64_t blocks = P.slabs * P.gblocks;
+      if (blocks > MAX_GRID) return TTC_LQR_EINVAL;
+      float* part = A.dweight || A.dbias ? ws : nullptr;
+      hipLaunchKernelGGL((norm_row_backward_kernel<T, V, NV, SILU, GATE>), dim3((unsigned)blocks), dim3(256), 0, s, x,
+                         gate, dy, aff, A.n, G, cg, P.lanes, P.gper, P.rper, P.gblocks, P.slab, A.mean, A.rstd,
+                         static_cast<T*>(A.dx), static_cast<T*>(A.dgate), part);
+      return launched();
+    };
+    const int rc = P.NV == 1   ? go(std::integral_constant<int, 1>{})
+                   : P.NV == 2 ? go(std::integral_constant<int, 2>{})
+                               : go(std::integral_constant<int, 4>{});
+    if (rc != TTC_LQR_OK) return rc;
+    parts = P.slabs * P.rper;
+  } else {
+    const Slab& S = P.S;
+    const int64_t blocks = A.n * S.slabs * S.cblocks;
+    if (blocks > MAX_GRID || A.n * G > MAX_GRID) return TTC_LQR_EINVAL;
+    const dim3 grid((unsigned)blocks), block(256), join((unsigned)(A.n * G));
+    float* extra = ws + A.n * S.slabs * 2 * A.c;
+    if (!A.backward) {
+      float* mean = A.mean ? A.mean : extra;
+      float* rstd = A.mean ? A.rstd : extra + A.n * G;
+      hipLaunchKernelGGL((norm_slab_stats_kernel<T, V>), grid, block, 0, s, x, S, ws);
+      hipLaunchKernelGGL(norm_slab_join_kernel, join, block, 0, s, ws, S, eps, mean, rstd);
+      hipLaunchKernelGGL((norm_slab_apply_kernel<T, V, SILU, GATE>), grid, block, 0, s, x, gate, aff, S, mean, rstd,
+                         static_cast<T*>(A.y));
+      return launched();
+    }
+    hipLaunchKernelGGL((norm_slab_back_stats_kernel<T, V, SILU, GATE>), grid, block, 0, s, x, gate, dy, aff, S, A.mean,
+                       A.rstd, static_cast<T*>(A.dgate), ws);
+    if (A.dx) {
+      hipLaunchKernelGGL(norm_slab_back_join_kernel, join, block, 0, s, ws, aff, S, extra);
+      hipLaunchKernelGGL((norm_slab_back_apply_kernel<T, V, SILU, GATE>), grid, block, 0, s, x, gate, dy, aff, S, A.mean,
+                         A.rstd, extra, static_cast<T*>(A.dx));
+    }
+    parts = A.n * S.slabs;
+  }
+  if (A.dweight || A.dbias) {
+    const dim3 grid((unsigned)ceil_div(A.c, 16));
+    if (A.weight_dtype == TTC_DTYPE_BF16)
+      hipLaunchKernelGGL(norm_affine_sum_kernel<__bf16>, grid, dim3(256), 0, s, ws, parts, A.c,
+                         static_cast<__bf16*>(A.dweight), static_cast<__bf16*>(A.dbias));
+    else
+      hipLaunchKernelGGL(norm_affine_sum_kernel<float>, grid, dim3(256), 0, s, ws, parts, A.c,
+                         static_cast<float*>(A.dweight), static_cast<float*>(A.dbias));
+  }
+  return launched();
+}
+
+template <class T, int V>
+int norm_dispatch(const ttc_group_norm_args& A, const NormPlan& P, hipStream_t s) {
+  if (A.activation == 1) return A.gate ? norm_run<T, V, true, true>(A, P, s) : norm_run<T, V, true, false>(A, P, s);
+  return A.gate ? norm_run<T, V, false, true>(A, P, s) : norm_run<T, V, false, false>(A, P, s);
+}
+
+// 0, or the status that the block's sizes and types deserve
+inline int norm_check(const ttc_group_norm_args& A) {
+  const int64_t lim = 1 << 24;
+  if (A.n < 0 || A.l < 0 || A.c < 0 || A.c > lim || A.groups <= 0 || A.c % A.groups || A.activation < 0 ||
+      A.activation > 1 || !(A.eps >= 0.0) || !countable({A.n, A.l, A.c}))
+    return TTC_LQR_EINVAL;
+  auto known = [](int64_t t) { return t == TTC_DTYPE_F32 || t == TTC_DTYPE_BF16; };
+  if (!known(A.dtype) || !known(A.weight_dtype)) return TTC_LQR_EUNSUPPORTED;
+  return TTC_LQR_OK;
+}
+
+inline size_t norm_floats(const ttc_group_norm_args& A) {
+  const size_t a = norm_plan(A, false).floats, b = norm_plan(A, true).floats;
+  return a > b ? a : b;
+}
+
+}  // namespace ttc
+
+extern "C" size_t ttc_group_norm_workspace_bytes(const ttc_group_norm_args* args) {
+  using namespace ttc;
+  if (!args || norm_check(*args) != TTC_LQR_OK || args->n == 0 || args->l == 0 || args->c == 0) return 0;
+  return norm_floats(*args) * sizeof(float);
+}
+
+extern "C" int ttc_group_norm(const ttc_group_norm_args* args, void* stream) {
+  using namespace ttc;
+  if (!args) return TTC_LQR_EINVAL;
+  const ttc_group_norm_args& A = *args;
+  if (const int rc = norm_check(A)) return rc;
+  if (A.n == 0 || A.l == 0 || A.c == 0) return TTC_LQR_OK;
+  if (!A.x || !A.weight != !A.bias || !A.mean != !A.rstd) return TTC_LQR_EINVAL;
+  if (A.backward ? !A.dy || !A.mean || (A.dgate && !A.gate) : !A.y) return TTC_LQR_EINVAL;
+  const size_t need = norm_floats(A) * sizeof(float);
+  if (need > 0 && (!A.workspace || A.workspace_bytes < 0 || (size_t)A.workspace_bytes < need)) return TTC_LQR_EINVAL;
+  const NormPlan P = norm_plan(A, norm_wide(A));
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (A.dtype == TTC_DTYPE_F32)
+    return P.V == 4 ? norm_dispatch<float, 4>(A, P, s) : norm_dispatch<float, 1>(A, P, s);
+  return P.V == 8 ? norm_dispatch<__bf16, 8>(A, P, s) : norm_dispatch<__bf16, 1>(A, P, s);
+}

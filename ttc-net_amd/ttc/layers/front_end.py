@@ -14,6 +14,7 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
+from .._dispatch import traced as _traced
 from ..solvers._lib import lib, check
 
 __all__ = ["front_end", "front_end_torch", "l2norm"]
@@ -96,18 +97,6 @@ class _FrontEndFunc(torch.autograd.Function):
             d_bias = torch.cat([zero(grads[5], 1), zero(grads[6], ud), zero(grads[7], hd)])
             d_bias = d_bias.masked_fill(bias >= 0, 0.0)  # relu's gradient: 0 where it is off, NaN passes
         return d_proj, d_bias, None
-
-
-def _traced(*xs) -> bool:
-    """Whether operators are observed one by one (functorch transforms, batched gradients, forward-mode
-    tangents, tracing and compilation, dispatch modes such as ``make_fx``'s, tensor subclasses such as fake
-    tensors): none of these sees the kernel."""
-    if torch.compiler.is_compiling():  # first: a full-graph compilation can trace none of the rest
-        return True
-    return (any(type(x) not in (torch.Tensor, torch.nn.Parameter) or not torch._C._has_storage(x)
-                for x in xs if x is not None)
-            or torch._C._are_functorch_transforms_active() or torch._C._len_torch_dispatch_stack() > 0
-            or torch.autograd.forward_ad._current_level >= 0 or torch.jit.is_tracing())
 
 
 def front_end(proj: torch.Tensor, bias: torch.Tensor | None, dims):

@@ -1,4 +1,5 @@
-"""ctypes binding of ``libttc_lqr.so`` (the C ABI declared in ``include/ttc_lqr.h``).
+"""ctypes binding of ``libttc_lqr.so`` (the C ABI declared in ``include/ttc_lqr.h``, ``ttc_frontend.h`` and
+``ttc_ops.h``).
 
 The library is built in-tree by ``ttc-net_amd/csrc/build.py`` into
 ``ttc-net_amd/lib/libttc_lqr.so``.  There is no fallback: if the library is
@@ -110,6 +111,11 @@ def _load():
     L.ttc_lqr_backward_host.restype = ctypes.c_int
     L.ttc_lqr_backward_host.argtypes = ([f32p] * 10 + [i64, i32, i32, i32, i32] + [f32p] * 9
                                         + [ctypes.c_float, f32p, i32])
+    for name in ("ttc_rotary", "ttc_group_norm"):  # (argument block, stream)
+        getattr(L, name).restype = ctypes.c_int
+        getattr(L, name).argtypes = [ctypes.c_char_p, ctypes.c_void_p]
+    L.ttc_group_norm_workspace_bytes.restype = sz
+    L.ttc_group_norm_workspace_bytes.argtypes = [ctypes.c_char_p]
     for suffix in ("", "_bf16"):
         getattr(L, "ttc_lqr_forward_factored" + suffix).restype = ctypes.c_int
         getattr(L, "ttc_lqr_forward_factored" + suffix).argtypes = L.ttc_lqr_forward_factored.argtypes
