@@ -63,6 +63,59 @@ typedef struct {
 size_t ttc_group_norm_workspace_bytes(const ttc_group_norm_args* args);
 int ttc_group_norm(const ttc_group_norm_args* args, void* stream);
 
+/* ---- Linear attention with a decay for each head ----
+ * For each sequence and head, with a state S [dk, dv] held in fp32 and g = log_gamma of the token and head,
+ *   S_t = e^{g_t} S_{t-1} + k_t v_t',   o_t = scale S_t' q_t.
+ * A log_gamma below TTC_RESET_LOG_GAMMA (e^g is 0 in fp32; -inf included) drops the state: what came before has no
+ * effect on what follows, whatever it held.  Tokens after t have no effect on o_t, whatever they hold.
+ * q, k [batch, tokens, q_heads / k_heads, dk], v [batch, tokens, v_heads, dv]: unit stride along the last dimension;
+ * each head count divides `heads`, and head h reads head h / (heads / q_heads) of q.  log_gamma: any strides over
+ * batch, tokens and heads (0 for batch and tokens: one decay for each head), of type gamma_dtype (fp32, or dtype).
+ * dk, dv: 1 to TTC_LINEAR_ATTENTION_MAX_DIM.  initial_state (NULL: zero), final_state (NULL: not wanted)
+ * [batch, heads, dk, dv] fp32 contiguous; o [batch, tokens, heads, dv] contiguous.
+ * The backward takes d_o (unit stride along dv) and d_final_state (NULL: zero) and writes dq, dk_out, dv_out (contiguous,
+ * of q's, k's and v's shapes), d_log_gamma (contiguous [batch, tokens, heads], or [heads] with gamma_per_head) and
+ * d_initial_state; NULL: not wanted.
+ * workspace: ttc_linear_attention_workspace_bytes() of the same block (the backward's where `backward` is set). */
+#define TTC_LINEAR_ATTENTION_MAX_DIM 128
+#define TTC_RESET_LOG_GAMMA -104.0f
+typedef struct {
+  int64_t dtype, gamma_dtype, gamma_per_head, backward;
+  int64_t batch, tokens, heads, q_heads, k_heads, v_heads, dk, dv;
+  double scale;
+  const void *q, *k, *v, *log_gamma;
+  int64_t q_stride[3], k_stride[3], v_stride[3], gamma_stride[3]; /* batch, token, head */
+  const float* initial_state;
+  void* o;
+  float* final_state;
+  const void* d_o;
+  int64_t d_o_stride[3];
+  const float* d_final_state;
+  void *dq, *dk_out, *dv_out, *d_log_gamma;
+  float* d_initial_state;
+  void* workspace;
+  int64_t workspace_bytes;
+} ttc_linear_attention_args;
+
+size_t ttc_linear_attention_workspace_bytes(const ttc_linear_attention_args* args);
+int ttc_linear_attention(const ttc_linear_attention_args* args, void* stream);
+
+/* One token of each sequence, its state updated in place: q, k, v, log_gamma as above without the token dimension,
+ * o [batch, heads, dv] contiguous.  state [slots, heads, dk, dv] fp32 contiguous; row b's state is slot slot_index[b]
+ * (int32; NULL: slot b, and slots = batch).  A row whose index lies outside [0, slots) is skipped: its output is 0 and
+ * no state changes.  Rows must not share a slot. */
+typedef struct {
+  int64_t dtype, gamma_dtype, batch, heads, q_heads, k_heads, v_heads, dk, dv, slots;
+  double scale;
+  const void *q, *k, *v, *log_gamma;
+  int64_t q_stride[2], k_stride[2], v_stride[2], gamma_stride[2]; /* batch, head */
+  float* state;
+  const int32_t* slot_index;
+  void* o;
+} ttc_linear_attention_step_args;
+
+int ttc_linear_attention_step(const ttc_linear_attention_step_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

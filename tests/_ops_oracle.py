@@ -58,3 +58,36 @@ def quotient(f, xs, ds, cs, h):
         out = out if isinstance(out, tuple) else (out,)
         return sum(float((o.detach().double().cpu() * c.double().cpu()).sum()) for o, c in zip(out, cs) if c is not None)
     return (at(1.0) - at(-1.0)) / (2 * h)
+
+
+def linear64(q, k, v, g, scale, state=None, d_o=None, d_state=None):
+    """Token by token: o, the final state, and for gradients d_o (and d_state) those of q, k, v, g and the state, from the
+    formulas (R: the gradient of the state).  ``g`` [batch, tokens, heads]; shared heads' gradients are summed.  A decay
+    of 0 drops the state whatever it holds."""
+    H = g.shape[-1]
+    wide = lambda x: x.detach().double().cpu().repeat_interleave(H // x.shape[2], dim=2)  # noqa: E731
+    Q, K, V, G = wide(q), wide(k), wide(v), g.detach().double().cpu()
+    (B, T), dk, dv = Q.shape[:2], Q.shape[-1], V.shape[-1]
+    S = torch.zeros(B, H, dk, dv, dtype=torch.float64) if state is None else state.detach().double().cpu()
+    before, after, o = [], [], torch.zeros(B, T, H, dv, dtype=torch.float64)
+    decay, gone = G.exp(), (G < -104)[..., None, None]
+    kept = lambda t, X: torch.where(gone[:, t], torch.zeros_like(X), X * decay[:, t, :, None, None])  # noqa: E731
+    for t in range(T):
+        before.append(S)
+        S = kept(t, S) + K[:, t, :, :, None] * V[:, t, :, None, :]
+        after.append(S)
+        o[:, t] = scale * (S * Q[:, t, :, :, None]).sum(-2)
+    if d_o is None:
+        return {"o": o, "state": S}
+    D = d_o.detach().double().cpu()
+    R = torch.zeros_like(S) if d_state is None else d_state.detach().double().cpu()
+    dq, dk_, dv_, dg = torch.zeros_like(Q), torch.zeros_like(K), torch.zeros_like(V), torch.zeros_like(G)
+    for t in reversed(range(T)):
+        dq[:, t] = scale * (after[t] * D[:, t, :, None, :]).sum(-1)
+        R = R + scale * Q[:, t, :, :, None] * D[:, t, :, None, :]
+        dk_[:, t] = (R * V[:, t, :, None, :]).sum(-1)
+        dv_[:, t] = (R * K[:, t, :, :, None]).sum(-2)
+        dg[:, t] = (R * kept(t, before[t])).sum((-1, -2))
+        R = kept(t, R)
+    shared = lambda x, d: d.unflatten(2, (x.shape[2], -1)).sum(3)  # noqa: E731
+    return {"o": o, "state": S, "q": shared(q, dq), "k": shared(k, dk_), "v": shared(v, dv_), "g": dg, "d_state": R}

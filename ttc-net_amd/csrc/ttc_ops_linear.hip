@@ -1,0 +1,428 @@
+// ttc_ops_linear.hip -- linear attention with a decay for each head: the token-by-token sweep (single tokens of a serving
+// batch, short inputs), the joining kernels of the backward, and the C entries (the roles: ttc_ops_linear.hpp).
+#include "ttc_ops_linear.hpp"
+
+namespace ttc {
+
+// Token by token with the state in registers: a workgroup holds 32 columns of one head's state, a thread 4 of them for
+// RPT rows.  For one token it reads and writes the state once (8 bytes an element against 5 flops): bound by memory.
+template <class T, int RPT>
+__global__ __launch_bounds__(256) void token_sweep_kernel(Sweep A, int tiles, bool wide) {
+  __shared__ float part[2][4][32];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int tile = (int)(blockIdx.x % tiles);
+  const int64_t bh = blockIdx.x / tiles, b = bh / A.H;
+  const int h = (int)(bh % A.H);
+  const int e0 = tile * 32 + (lane & 7) * 4, r0 = wave * 8 + (lane >> 3);
+  const int64_t slot = A.slots ? A.slots[b] : b;
+  T* out = static_cast<T*>(A.out) + (b * A.T * A.H + h) * (int64_t)A.vd;
+  float* outf = static_cast<float*>(A.out) + (b * A.T * A.H + h) * (int64_t)A.vd;
+  if (slot < 0 || slot >= A.nslots) {  // a row without a state
+    for (int64_t t = 0; t < A.T; ++t)
+      for (int j = threadIdx.x; j < 32 && tile * 32 + j < A.vd; j += 256) {
+        const int64_t at = t * A.H * (int64_t)A.vd + tile * 32 + j;
+        if (A.out_f32) outf[at] = 0.0f; else out[at] = from_f<T>(0.0f);
+      }
+    return;
+  }
+  const int64_t base = (slot * A.H + h) * (int64_t)A.kd * A.vd;
+  float S[RPT][4];
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const int r = r0 + 32 * i;
+    if (A.state_in == nullptr || r >= A.kd) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) S[i][j] = 0.0f;
+    } else if (wide) {
+      const float4 f = e0 < A.vd ? *reinterpret_cast<const float4*>(A.state_in + base + r * A.sr + e0)
+                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+      S[i][0] = f.x, S[i][1] = f.y, S[i][2] = f.z, S[i][3] = f.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) S[i][j] = e0 + j < A.vd ? A.state_in[base + r * A.sr + (e0 + j) * A.sc] : 0.0f;
+    }
+  }
+  const T *q = A.q.at<T>(b, h), *k = A.k.at<T>(b, h), *v = A.v.at<T>(b, h);
+  const T* x = A.x.p ? A.x.at<T>(b, h) : nullptr;
+  const int64_t g = b * A.gb + h * A.gh;
+  for (int64_t n = 0; n < A.T; ++n) {
+    const int64_t t = A.reverse ? A.T - 1 - n : n;
+    const float lg = !A.reverse ? gamma_at(A, g + t * A.gt) : n == 0 ? 0.0f : gamma_at(A, g + (t + 1) * A.gt);
+    const float decay = expf(lg);
+    float vv[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) vv[j] = e0 + j < A.vd ? to_f(v[t * A.v.st + e0 + j]) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+      const int r = r0 + 32 * i;
+      if (r < A.kd) {
+        const float kk = to_f(k[t * A.k.st + r]) * A.key_scale, qq = to_f(q[t * A.q.st + r]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          S[i][j] = lg < RESET ? kk * vv[j] : fmaf(S[i][j], decay, kk * vv[j]);
+          acc[j] = fmaf(qq, S[i][j], acc[j]);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int m = 8; m <= 32; m <<= 1) acc[j] += __shfl_xor(acc[j], m, 64);
+      if (lane < 8) part[n & 1][wave][lane * 4 + j] = acc[j];
+    }
+    __syncthreads();  // the next token writes the other buffer, and meets this barrier before it comes back to this one
+    if (threadIdx.x < 32) {
+      const int j = threadIdx.x, e = tile * 32 + j;
+      float o = (part[n & 1][0][j] + part[n & 1][1][j] + part[n & 1][2][j] + part[n & 1][3][j]) * A.out_scale;
+      const int64_t at = t * A.H * (int64_t)A.vd + e;
+      if (e < A.vd && A.out) {
+        if (A.out_f32) outf[at] = o; else out[at] = from_f<T>(o);
+      }
+      if (x) {
+        const float d = lane_sum(e < A.vd ? o * to_f(x[t * A.x.st + e]) : 0.0f, 32);
+        if (j == 0) A.dots[(tile * A.B * A.H + bh) * A.T + t] = d;
+      }
+    }
+  }
+  if (A.state_out == nullptr) return;
+  const float lg = A.reverse && A.T > 0 ? gamma_at(A, g) : 0.0f;
+  const float last = expf(lg);
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const int r = r0 + 32 * i;
+    if (r >= A.kd) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) S[i][j] = !A.reverse ? S[i][j] : lg < RESET ? 0.0f : S[i][j] * last;
+    if (wide) {
+      if (e0 < A.vd)
+        *reinterpret_cast<float4*>(A.state_out + base + r * A.sr + e0) = make_float4(S[i][0], S[i][1], S[i][2], S[i][3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (e0 + j < A.vd) A.state_out[base + r * A.sr + (e0 + j) * A.sc] = S[i][j];
+    }
+  }
+}
+
+int launch_token_sweep(const Sweep& A, bool bf16, hipStream_t s) {
+  const int tiles = token_tiles(A.vd);
+  const int64_t blocks = A.B * A.H * tiles;
+  if (blocks == 0) return TTC_LQR_OK;
+  if (blocks > MAX_GRID) return TTC_LQR_EINVAL;
+  const bool wide = A.sc == 1 && A.vd % 4 == 0 && aligned16(A.state_in) && aligned16(A.state_out);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, s, A, tiles, wide);
+    return launched();
+  };
+  if (bf16)
+    return A.kd <= 32 ? go(token_sweep_kernel<__bf16, 1>) : A.kd <= 64 ? go(token_sweep_kernel<__bf16, 2>)
+                                                                       : go(token_sweep_kernel<__bf16, 4>);
+  return A.kd <= 32 ? go(token_sweep_kernel<float, 1>) : A.kd <= 64 ? go(token_sweep_kernel<float, 2>)
+                                                                    : go(token_sweep_kernel<float, 4>);
+}
+
+// Gradients of shared heads: out [rows, heads / share, d] = sums over `share` heads of in [rows, heads, d]
+template <class T>
+__global__ __launch_bounds__(256) void share_sum_kernel(const float* __restrict__ in, T* __restrict__ out, int64_t n,
+                                                        int share, int d) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const int64_t head = i / d;
+  const float* p = in + head * share * d + i % d;
+  float a = 0.0f;
+  for (int j = 0; j < share; ++j) a += p[(int64_t)j * d];
+  out[i] = from_f<T>(a);
+}
+
+// dg_t = sum_{u >= t} (r_u - c_u) + <S_T, dS_T>, one wave per sequence and head, from the end, 8 tokens a lane at a time, in
+// 64 bits (the sum's terms cancel).  A reset's own gradient is 0, and nothing after it reaches tokens before it.
+constexpr int GATE_TOKENS = 8;
+__global__ __launch_bounds__(64) void gate_kernel(Sweep A, const float* __restrict__ r, const float* __restrict__ c,
+                                                  int rtiles, int ctiles, const float* __restrict__ last,
+                                                  const float* __restrict__ dlast, int64_t elems, void* d_gamma,
+                                                  double* __restrict__ per_head) {
+  const int lane = threadIdx.x;
+  const int64_t bh = blockIdx.x, b = bh / A.H, BHT = A.B * A.H * A.T;
+  const int h = (int)(bh % A.H);
+  double carry = 0.0, total = 0.0;
+  if (dlast) {
+    for (int64_t i = lane; i < elems; i += 64) carry += (double)last[bh * elems + i] * dlast[bh * elems + i];
+    for (int m = 32; m >= 1; m >>= 1) carry += __shfl_xor(carry, m, 64);
+  }
+  for (int64_t end = A.T; end > 0; end -= 64 * GATE_TOKENS) {
+    const int64_t hi = end - lane * GATE_TOKENS;  // this lane: tokens hi - 1 down to hi - 8
+    double sum[GATE_TOKENS], run = 0.0;
+    bool cut[GATE_TOKENS], cuts = false;
+#pragma unroll
+    for (int i = 0; i < GATE_TOKENS; ++i) {
+      const int64_t t = hi - 1 - i;
+      cut[i] = false;
+      if (t >= 0) {
+        double d = 0.0;
+        for (int j = 0; j < rtiles; ++j) d += r[j * BHT + bh * A.T + t];
+        for (int j = 0; j < ctiles; ++j) d -= c[j * BHT + bh * A.T + t];
+        run += d;
+        cut[i] = gamma_at(A, b * A.gb + h * A.gh + t * A.gt) < RESET;
+      }
+      if (cut[i]) run = 0.0, cuts = true;
+      sum[i] = run;
+    }
+    // what the lanes before this one pass on: their runs since the last reset among them
+    double in = run;
+    bool stop = cuts;
+    for (int m = 1; m < 64; m <<= 1) {
+      const double up = __shfl_up(in, m, 64);
+      const bool sup = __shfl_up((int)stop, m, 64);
+      if (lane >= m) {
+        if (!stop) in += up;
+        stop = stop || sup;
+      }
+    }
+    double before = __shfl_up(in, 1, 64);
+    const bool sbefore = __shfl_up((int)stop, 1, 64);
+    if (lane == 0) before = carry;
+    else if (!sbefore) before += carry;
+    const double whole = __shfl(in, 63, 64);
+    carry = __shfl((int)stop, 63, 64) ? whole : whole + carry;
+    bool open = true;
+#pragma unroll
+    for (int i = 0; i < GATE_TOKENS; ++i) {
+      const int64_t t = hi - 1 - i;
+      open = open && !cut[i];
+      const double d = cut[i] ? 0.0 : open ? sum[i] + before : sum[i];
+      if (t < 0) continue;
+      total += d;
+      if (per_head == nullptr) {
+        const int64_t at = (b * A.T + t) * A.H + h;
+        if (A.gamma_bf16) static_cast<__bf16*>(d_gamma)[at] = from_f<__bf16>((float)d);
+        else static_cast<float*>(d_gamma)[at] = (float)d;
+      }
+    }
+  }
+  if (per_head) {
+    for (int m = 32; m >= 1; m >>= 1) total += __shfl_xor(total, m, 64);
+    if (lane == 0) per_head[bh] = total;
+  }
+}
+
+__global__ __launch_bounds__(64) void gate_head_kernel(const double* __restrict__ per_head, int64_t B, int H, bool bf16,
+                                                       void* d_gamma) {
+  const int h = blockIdx.x * 64 + threadIdx.x;
+  if (h >= H) return;
+  double a = 0.0;
+  for (int64_t b = 0; b < B; ++b) a += per_head[b * H + h];
+  if (bf16) static_cast<__bf16*>(d_gamma)[h] = from_f<__bf16>((float)a);
+  else static_cast<float*>(d_gamma)[h] = (float)a;
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------
+
+struct Layout {  // the backward's workspace, in bytes from its start; 0 bytes: not needed
+  int64_t dq, dk, dv, r, c, last, per_head, total;
+  bool gate;
+};
+
+inline bool shared_out(int64_t heads, int64_t own) { return heads != own; }
+
+inline Layout layout_of(const ttc_linear_attention_args& A) {
+  Layout W{};
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t p = at;
+    at += (bytes + 255) / 256 * 256;
+    return p;
+  };
+  if (!A.backward) return W;
+  const int64_t rows = A.batch * A.tokens * A.heads;
+  W.gate = A.d_log_gamma != nullptr;
+  W.dq = take(shared_out(A.heads, A.q_heads) && (A.dq || W.gate) ? rows * A.dk * 4 : !A.dq && W.gate ? rows * A.dk * 4 : 0);
+  W.dk = take(shared_out(A.heads, A.k_heads) && (A.dk_out || W.gate) ? rows * A.dk * 4
+              : !A.dk_out && W.gate                                    ? rows * A.dk * 4
+                                                                       : 0);
+  W.dv = take(shared_out(A.heads, A.v_heads) && A.dv_out ? rows * A.dv * 4 : 0);
+  if (W.gate) {
+    const int64_t tiles = token_tiles((int)A.dk);
+    W.r = take(rows * tiles * 4);
+    W.c = take(rows * tiles * 4);
+    W.last = take(A.d_final_state ? A.batch * A.heads * A.dk * A.dv * 4 : 0);
+    W.per_head = take(A.gamma_per_head ? A.batch * A.heads * 8 : 0);
+  }
+  W.total = at;
+  return W;
+}
+
+inline int linear_check(int64_t dtype, int64_t gamma_dtype, std::initializer_list<int64_t> sizes, int64_t heads,
+                        int64_t qh, int64_t kh, int64_t vh, int64_t dk, int64_t dv) {
+  for (int64_t v : sizes)
+    if (v < 0) return TTC_LQR_EINVAL;
+  if (heads < 1 || heads > (1 << 24) || qh < 1 || kh < 1 || vh < 1 || heads % qh || heads % kh || heads % vh || dk < 1 ||
+      dk > MAX_DIM || dv < 1 || dv > MAX_DIM || !countable(sizes))
+    return TTC_LQR_EINVAL;
+  if (dtype != TTC_DTYPE_F32 && dtype != TTC_DTYPE_BF16) return TTC_LQR_EUNSUPPORTED;
+  if (gamma_dtype != TTC_DTYPE_F32 && gamma_dtype != dtype) return TTC_LQR_EUNSUPPORTED;
+  return TTC_LQR_OK;
+}
+
+inline int args_check(const ttc_linear_attention_args& A) {
+  return linear_check(A.dtype, A.gamma_dtype, {A.batch, A.tokens, A.heads, MAX_DIM, MAX_DIM}, A.heads, A.q_heads, A.k_heads,
+                      A.v_heads, A.dk, A.dv);
+}
+
+inline Side side_of(const void* p, const int64_t* st, int64_t heads, int64_t own) {
+  return Side{p, st[0], st[1], st[2], (int)(heads / own)};
+}
+
+template <class T>
+int share_sum(const float* in, void* out, int64_t rows, int64_t own, int64_t heads, int64_t d, hipStream_t s) {
+  const int64_t n = rows * own * d, blocks = ceil_div(n, 256);
+  if (blocks > MAX_GRID) return TTC_LQR_EINVAL;
+  hipLaunchKernelGGL(share_sum_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, in, static_cast<T*>(out), n,
+                     (int)(heads / own), (int)d);
+  return launched();
+}
+
+inline Sweep sweep_of(const ttc_linear_attention_args& A) {
+  Sweep S{};
+  S.gamma = A.log_gamma;
+  S.gb = A.gamma_stride[0], S.gt = A.gamma_stride[1], S.gh = A.gamma_stride[2];
+  S.gamma_bf16 = A.gamma_dtype == TTC_DTYPE_BF16;
+  S.H = (int)A.heads;
+  S.B = A.batch;
+  S.T = A.tokens;
+  S.nslots = A.batch;
+  S.key_scale = S.out_scale = 1.0f;
+  return S;
+}
+
+inline int run_sweep(const Sweep& S, bool bf16, hipStream_t s) { return launch_token_sweep(S, bf16, s); }
+
+}  // namespace ttc
+
+extern "C" size_t ttc_linear_attention_workspace_bytes(const ttc_linear_attention_args* args) {
+  using namespace ttc;
+  if (!args || args_check(*args) != TTC_LQR_OK) return 0;
+  return (size_t)layout_of(*args).total;
+}
+
+extern "C" int ttc_linear_attention(const ttc_linear_attention_args* args, void* stream) {
+  using namespace ttc;
+  if (!args) return TTC_LQR_EINVAL;
+  const ttc_linear_attention_args& A = *args;
+  if (const int rc = args_check(A)) return rc;
+  const bool some = A.batch > 0 && A.tokens > 0, bf16 = A.dtype == TTC_DTYPE_BF16;
+  if (some && (!A.q || !A.k || !A.v || !A.log_gamma)) return TTC_LQR_EINVAL;
+  const Layout W = layout_of(A);
+  if (W.total > 0 && (!A.workspace || A.workspace_bytes < W.total)) return TTC_LQR_EINVAL;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const Side q = side_of(A.q, A.q_stride, A.heads, A.q_heads), k = side_of(A.k, A.k_stride, A.heads, A.k_heads),
+             v = side_of(A.v, A.v_stride, A.heads, A.v_heads), none{};
+  Sweep S = sweep_of(A);
+  if (!A.backward) {
+    if (some && !A.o) return TTC_LQR_EINVAL;
+    S.q = q, S.k = k, S.v = v;
+    S.kd = (int)A.dk, S.vd = (int)A.dv;
+    S.out_scale = (float)A.scale;
+    S.state_in = A.initial_state;
+    S.state_out = A.final_state;
+    S.sr = S.vd, S.sc = 1;
+    S.out = A.o;
+    return run_sweep(S, bf16, s);
+  }
+  if (some && !A.d_o) return TTC_LQR_EINVAL;
+  const Side d_o = side_of(A.d_o, A.d_o_stride, A.heads, A.heads);
+  char* ws = static_cast<char*>(A.workspace);
+  auto space = [&](int64_t at) { return reinterpret_cast<float*>(ws + at); };
+  const int dk = (int)A.dk, dv = (int)A.dv;
+  const bool gate = W.gate && some;
+  int rc = TTC_LQR_OK;
+  if (some && (A.dq || gate)) {  // S transposed: [dv, dk]
+    S.q = d_o, S.k = v, S.v = k;
+    S.x = gate ? q : none;
+    S.kd = dv, S.vd = dk;
+    S.out_scale = (float)A.scale;
+    S.state_in = A.initial_state;
+    S.state_out = gate && A.d_final_state ? space(W.last) : nullptr;
+    S.sr = 1, S.sc = dv;
+    S.dots = space(W.r);
+    S.out_f32 = shared_out(A.heads, A.q_heads) || !A.dq;
+    S.out = S.out_f32 ? space(W.dq) : A.dq;
+    if ((rc = run_sweep(S, bf16, s))) return rc;
+  }
+  S = sweep_of(A);
+  S.reverse = true;
+  S.key_scale = (float)A.scale;
+  S.state_in = A.d_final_state;
+  if (some && (A.dk_out || gate)) {  // R transposed: [dv, dk]
+    S.q = v, S.k = d_o, S.v = q;
+    S.x = gate ? k : none;
+    S.kd = dv, S.vd = dk;
+    S.sr = 1, S.sc = dv;
+    S.dots = space(W.c);
+    S.out_f32 = shared_out(A.heads, A.k_heads) || !A.dk_out;
+    S.out = S.out_f32 ? space(W.dk) : A.dk_out;
+    if ((rc = run_sweep(S, bf16, s))) return rc;
+  }
+  if ((some && A.dv_out) || A.d_initial_state) {
+    S.q = k, S.k = q, S.v = d_o;
+    S.x = none;
+    S.kd = dk, S.vd = dv;
+    S.sr = dv, S.sc = 1;
+    S.state_out = A.d_initial_state;
+    S.out_f32 = shared_out(A.heads, A.v_heads) && A.dv_out;
+    S.out = S.out_f32 ? space(W.dv) : A.dv_out;
+    if ((rc = run_sweep(S, bf16, s))) return rc;
+  }
+  if (some) {
+    const int64_t rows = A.batch * A.tokens;
+    auto join = [&](const float* in, void* out, int64_t own, int64_t d) {
+      return bf16 ? share_sum<__bf16>(in, out, rows, own, A.heads, d, s) : share_sum<float>(in, out, rows, own, A.heads, d, s);
+    };
+    if (A.dq && shared_out(A.heads, A.q_heads) && (rc = join(space(W.dq), A.dq, A.q_heads, A.dk))) return rc;
+    if (A.dk_out && shared_out(A.heads, A.k_heads) && (rc = join(space(W.dk), A.dk_out, A.k_heads, A.dk))) return rc;
+    if (A.dv_out && shared_out(A.heads, A.v_heads) && (rc = join(space(W.dv), A.dv_out, A.v_heads, A.dv))) return rc;
+  }
+  if (W.gate) {  // of one decay for each head: zero where there are no tokens
+    const int64_t bh = A.batch * A.heads;
+    if (bh > MAX_GRID) return TTC_LQR_EINVAL;
+    S = sweep_of(A);
+    const int tiles = token_tiles(dk);
+    double* per_head = A.gamma_per_head ? reinterpret_cast<double*>(space(W.per_head)) : nullptr;
+    if (bh > 0)
+      hipLaunchKernelGGL(gate_kernel, dim3((unsigned)bh), dim3(64), 0, s, S, space(W.r), space(W.c), tiles, tiles,
+                       space(W.last), some ? A.d_final_state : nullptr, (int64_t)dk * dv, A.d_log_gamma, per_head);
+    if (per_head)
+      hipLaunchKernelGGL(gate_head_kernel, dim3((unsigned)ceil_div(A.heads, 64)), dim3(64), 0, s, per_head, A.batch,
+                         (int)A.heads, S.gamma_bf16, A.d_log_gamma);
+  }
+  return launched();
+}
+
+extern "C" int ttc_linear_attention_step(const ttc_linear_attention_step_args* args, void* stream) {
+  using namespace ttc;
+  if (!args) return TTC_LQR_EINVAL;
+  const ttc_linear_attention_step_args& A = *args;
+  if (const int rc = linear_check(A.dtype, A.gamma_dtype, {A.batch, A.heads, MAX_DIM, MAX_DIM}, A.heads, A.q_heads,
+                                  A.k_heads, A.v_heads, A.dk, A.dv))
+    return rc;
+  if (A.slots < 0 || !countable({A.slots, A.heads, MAX_DIM, MAX_DIM}) || (!A.slot_index && A.slots != A.batch))
+    return TTC_LQR_EINVAL;
+  if (A.batch == 0) return TTC_LQR_OK;
+  if (!A.q || !A.k || !A.v || !A.log_gamma || !A.o || (A.slots > 0 && !A.state)) return TTC_LQR_EINVAL;
+  auto side = [&](const void* p, const int64_t* st, int64_t own) { return Side{p, st[0], 0, st[1], (int)(A.heads / own)}; };
+  Sweep S{};
+  S.q = side(A.q, A.q_stride, A.q_heads);
+  S.k = side(A.k, A.k_stride, A.k_heads);
+  S.v = side(A.v, A.v_stride, A.v_heads);
+  S.gamma = A.log_gamma;
+  S.gb = A.gamma_stride[0], S.gh = A.gamma_stride[1];
+  S.gamma_bf16 = A.gamma_dtype == TTC_DTYPE_BF16;
+  S.kd = (int)A.dk, S.vd = (int)A.dv, S.H = (int)A.heads;
+  S.B = A.batch, S.T = 1;
+  S.key_scale = 1.0f, S.out_scale = (float)A.scale;
+  S.state_in = S.state_out = A.state;
+  S.sr = S.vd, S.sc = 1;
+  S.slots = A.slot_index;
+  S.nslots = A.slots;
+  S.out = A.o;
+  return launch_token_sweep(S, A.dtype == TTC_DTYPE_BF16, reinterpret_cast<hipStream_t>(stream));
+}

@@ -1,0 +1,55 @@
+// ttc_ops_linear.hpp -- linear attention with a decay for each head: the one sweep that all its passes are.
+//
+//   S_t = e^{g_t} S_{t-1} + k_t v_t',   o_t = scale S_t' q_t
+// and with R_t the gradient of S_t,
+//   dq_t = scale S_t do_t,   R_t = scale q_t do_t' + e^{g_{t+1}} R_{t+1},   dk_t = R_t v_t,   dv_t = R_t' k_t,
+// so that, written sweep(query, key, value) -> out,
+//   o = sweep(q, k, v),  dq = sweep(do, v, k),  dv = reverse sweep(k, q, do),  dk = reverse sweep(v, do, q):
+// one kernel, in four roles (the state transposed where the roles of dk and dv swap).  In reverse order the decay that
+// is applied before token t is that of token t + 1 (none before the last token), and that of token 0 after the end.
+// The decays' gradient needs no state either: with the dots r_t = q_t.dq_t and c_t = k_t.dk_t,
+//   dg_t = sum_{u >= t} (r_u - c_u) + <S_T, dS_T>.
+#pragma once
+#include "ttc_ops_common.hpp"
+
+namespace ttc {
+
+constexpr float RESET = TTC_RESET_LOG_GAMMA;
+constexpr int MAX_DIM = TTC_LINEAR_ATTENTION_MAX_DIM;
+
+struct Side {  // one of the sweep's inputs: [batch, token, head, dim], heads shared by `div` heads of the sweep
+  const void* p;
+  int64_t sb, st, sh;
+  int div;
+  template <class T>
+  __device__ __forceinline__ const T* at(int64_t b, int h) const {
+    return static_cast<const T*>(p) + b * sb + (h / div) * sh;
+  }
+};
+
+struct Sweep {
+  Side q, k, v;            // query and key of kd elements, value of vd
+  Side x;                  // x.p: the dots out_t . x_t are wanted (vd elements)
+  const void* gamma;
+  int64_t gb, gt, gh;
+  bool gamma_bf16, reverse, out_f32;
+  int kd, vd, H;
+  int64_t B, T;
+  float key_scale, out_scale;  // of the state's products; of the output
+  const float* state_in;       // [slot, head, ...]: element (i, j) at i * sr + j * sc
+  float* state_out;
+  int sr, sc;
+  const int32_t* slots;        // NULL: slot b
+  int64_t nslots;
+  void* out;                   // [B, T, H, vd] contiguous, of the inputs' type or fp32
+  float* dots;                 // [B, H, T], with one more such array for each further tile of columns
+};
+
+__device__ __forceinline__ float gamma_at(const Sweep& A, int64_t i) {
+  return A.gamma_bf16 ? to_f(static_cast<const __bf16*>(A.gamma)[i]) : static_cast<const float*>(A.gamma)[i];
+}
+
+int launch_token_sweep(const Sweep& A, bool bf16, hipStream_t s);
+inline int token_tiles(int vd) { return (vd + 31) / 32; }
+
+}  // namespace ttc

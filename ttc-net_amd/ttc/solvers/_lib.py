@@ -111,11 +111,12 @@ def _load():
     L.ttc_lqr_backward_host.restype = ctypes.c_int
     L.ttc_lqr_backward_host.argtypes = ([f32p] * 10 + [i64, i32, i32, i32, i32] + [f32p] * 9
                                         + [ctypes.c_float, f32p, i32])
-    for name in ("ttc_rotary", "ttc_group_norm"):  # (argument block, stream)
+    for name in ("ttc_rotary", "ttc_group_norm", "ttc_linear_attention", "ttc_linear_attention_step"):  # (block, stream)
         getattr(L, name).restype = ctypes.c_int
         getattr(L, name).argtypes = [ctypes.c_char_p, ctypes.c_void_p]
-    L.ttc_group_norm_workspace_bytes.restype = sz
-    L.ttc_group_norm_workspace_bytes.argtypes = [ctypes.c_char_p]
+    for name in ("ttc_group_norm_workspace_bytes", "ttc_linear_attention_workspace_bytes"):
+        getattr(L, name).restype = sz
+        getattr(L, name).argtypes = [ctypes.c_char_p]
     for suffix in ("", "_bf16"):
         getattr(L, "ttc_lqr_forward_factored" + suffix).restype = ctypes.c_int
         getattr(L, "ttc_lqr_forward_factored" + suffix).argtypes = L.ttc_lqr_forward_factored.argtypes
