@@ -104,6 +104,8 @@ __global__ __launch_bounds__(256) void token_sweep_kernel(Sweep A, int tiles, bo
   }
 }
 
+inline int token_tiles(int vd) { return (vd + 31) / 32; }
+
 int launch_token_sweep(const Sweep& A, bool bf16, hipStream_t s) {
   const int tiles = token_tiles(A.vd);
   const int64_t blocks = A.B * A.H * tiles;
@@ -119,6 +121,22 @@ int launch_token_sweep(const Sweep& A, bool bf16, hipStream_t s) {
                                                                        : go(token_sweep_kernel<__bf16, 4>);
   return A.kd <= 32 ? go(token_sweep_kernel<float, 1>) : A.kd <= 64 ? go(token_sweep_kernel<float, 2>)
                                                                     : go(token_sweep_kernel<float, 4>);
+}
+
+// Segments' own contributions to the states in front of them: state_in, then decay * state + contribution
+__global__ __launch_bounds__(256) void segment_join_kernel(Sweep A, Segments G, int64_t blocks_a_head) {
+  const int64_t bh = blockIdx.x / blocks_a_head, elems = (int64_t)A.kd * A.vd;
+  const int64_t i = blockIdx.x % blocks_a_head * 256 + threadIdx.x;
+  if (i >= elems) return;
+  float run = A.state_in ? A.state_in[bh * elems + i / A.vd * A.sr + i % A.vd * A.sc] : 0.0f;
+  float* p = G.state + bh * G.count * elems + i;
+  const float* w = G.decay + bh * G.count;
+  for (int j = 0; j + 1 < G.count; ++j) {
+    const float own = p[j * elems];
+    p[j * elems] = run;
+    run = w[j] == 0.0f ? own : fmaf(w[j], run, own);
+  }
+  p[(G.count - 1) * elems] = run;
 }
 
 // Gradients of shared heads: out [rows, heads / share, d] = sums over `share` heads of in [rows, heads, d]
@@ -217,8 +235,25 @@ __global__ __launch_bounds__(64) void gate_head_kernel(const double* __restrict_
 
 // ---- host ----------------------------------------------------------------------------------------------------
 
-struct Layout {  // the backward's workspace, in bytes from its start; 0 bytes: not needed
-  int64_t dq, dk, dv, r, c, last, per_head, total;
+// Up to this many tokens are swept one by one; more in chunks
+constexpr int64_t TOKEN_SWEEP = 4;
+
+// Segments of a chunked sweep: enough workgroups to fill the GPU's 256 CUs twice; a segment's keys and values are read once
+// more for the state behind it, so heads that fill the GPU by themselves are not split
+inline Segments segments_of(const ttc_linear_attention_args& A) {
+  Segments G{};
+  const int64_t chunks = ceil_div(A.tokens, chunk_tokens(A.dtype == TTC_DTYPE_BF16)), heads = A.batch * A.heads;
+  int64_t count = heads > 0 ? 512 / heads : 1;
+  if (count > chunks / 2) count = chunks / 2;
+  if (count < 1) count = 1;
+  G.chunks = ceil_div(chunks, count);
+  G.count = (int)(chunks > 0 ? ceil_div(chunks, G.chunks) : 1);
+  return G;
+}
+
+struct Layout {  // the workspace, in bytes from its start; 0 bytes: not needed
+  int64_t seg_state, seg_decay, dq, dk, dv, r, c, last, per_head, total;
+  int dot_tiles;
   bool gate;
 };
 
@@ -232,6 +267,13 @@ inline Layout layout_of(const ttc_linear_attention_args& A) {
     at += (bytes + 255) / 256 * 256;
     return p;
   };
+  if (A.tokens > TOKEN_SWEEP) {
+    const int64_t n = segments_of(A).count, all = A.batch * A.heads * n;
+    W.seg_state = take(n > 1 ? all * A.dk * A.dv * 4 : 0);
+    W.seg_decay = take(n > 1 ? all * 4 : 0);
+  }
+  W.dot_tiles = A.tokens > TOKEN_SWEEP ? 1 : token_tiles((int)A.dk);
+  W.total = at;
   if (!A.backward) return W;
   const int64_t rows = A.batch * A.tokens * A.heads;
   W.gate = A.d_log_gamma != nullptr;
@@ -241,9 +283,8 @@ inline Layout layout_of(const ttc_linear_attention_args& A) {
                                                                        : 0);
   W.dv = take(shared_out(A.heads, A.v_heads) && A.dv_out ? rows * A.dv * 4 : 0);
   if (W.gate) {
-    const int64_t tiles = token_tiles((int)A.dk);
-    W.r = take(rows * tiles * 4);
-    W.c = take(rows * tiles * 4);
+    W.r = take(rows * W.dot_tiles * 4);
+    W.c = take(rows * W.dot_tiles * 4);
     W.last = take(A.d_final_state ? A.batch * A.heads * A.dk * A.dv * 4 : 0);
     W.per_head = take(A.gamma_per_head ? A.batch * A.heads * 8 : 0);
   }
@@ -294,7 +335,37 @@ inline Sweep sweep_of(const ttc_linear_attention_args& A) {
   return S;
 }
 
-inline int run_sweep(const Sweep& S, bool bf16, hipStream_t s) { return launch_token_sweep(S, bf16, s); }
+// exact: the sweep's dots are wanted
+int run_sweep(const ttc_linear_attention_args& A, const Layout& W, const Sweep& S, bool exact, hipStream_t s) {
+  const bool bf16 = A.dtype == TTC_DTYPE_BF16;
+  if (A.tokens <= TOKEN_SWEEP) return launch_token_sweep(S, bf16, s);
+  if (A.batch == 0) return TTC_LQR_OK;
+  Segments G = segments_of(A);
+  char* ws = static_cast<char*>(A.workspace);
+  G.state = reinterpret_cast<float*>(ws + W.seg_state);
+  G.decay = reinterpret_cast<float*>(ws + W.seg_decay);
+  const int vec = bf16 ? 8 : 4;
+  auto wide = [&](const Side& x, int dim) {
+    return dim % vec == 0 && aligned16(x.p) && x.sb % vec == 0 && x.st % vec == 0 && x.sh % vec == 0;
+  };
+  const Wides V{wide(S.q, S.kd), wide(S.k, S.kd), wide(S.v, S.vd), S.vd % 4 == 0 && aligned16(S.out)};
+  auto launch = [&](int mode) {
+    if (bf16)
+      return S.kd <= 32   ? launch_chunk_kd32<__bf16>(S, G, V, mode, s)
+             : S.kd <= 64 ? launch_chunk_kd64<__bf16>(S, G, V, mode, s)
+                          : launch_chunk_kd128<__bf16>(S, G, V, mode, s);
+    return S.kd <= 32   ? launch_chunk_kd32<float>(S, G, V, mode, s)
+           : S.kd <= 64 ? launch_chunk_kd64<float>(S, G, V, mode, s)
+                        : launch_chunk_kd128<float>(S, G, V, mode, s);
+  };
+  if (G.count > 1) {
+    if (const int rc = launch(STATE_ONLY)) return rc;
+    const int64_t per = ceil_div((int64_t)S.kd * S.vd, 256), blocks = A.batch * A.heads * per;
+    if (blocks > MAX_GRID) return TTC_LQR_EINVAL;
+    hipLaunchKernelGGL(segment_join_kernel, dim3((unsigned)blocks), dim3(256), 0, s, S, G, per);
+  }
+  return launch(exact ? EXACT : FAST);
+}
 
 }  // namespace ttc
 
@@ -326,7 +397,7 @@ extern "C" int ttc_linear_attention(const ttc_linear_attention_args* args, void*
     S.state_out = A.final_state;
     S.sr = S.vd, S.sc = 1;
     S.out = A.o;
-    return run_sweep(S, bf16, s);
+    return run_sweep(A, W, S, false, s);
   }
   if (some && !A.d_o) return TTC_LQR_EINVAL;
   const Side d_o = side_of(A.d_o, A.d_o_stride, A.heads, A.heads);
@@ -346,7 +417,7 @@ extern "C" int ttc_linear_attention(const ttc_linear_attention_args* args, void*
     S.dots = space(W.r);
     S.out_f32 = shared_out(A.heads, A.q_heads) || !A.dq;
     S.out = S.out_f32 ? space(W.dq) : A.dq;
-    if ((rc = run_sweep(S, bf16, s))) return rc;
+    if ((rc = run_sweep(A, W, S, gate, s))) return rc;
   }
   S = sweep_of(A);
   S.reverse = true;
@@ -360,17 +431,18 @@ extern "C" int ttc_linear_attention(const ttc_linear_attention_args* args, void*
     S.dots = space(W.c);
     S.out_f32 = shared_out(A.heads, A.k_heads) || !A.dk_out;
     S.out = S.out_f32 ? space(W.dk) : A.dk_out;
-    if ((rc = run_sweep(S, bf16, s))) return rc;
+    if ((rc = run_sweep(A, W, S, gate, s))) return rc;
   }
   if ((some && A.dv_out) || A.d_initial_state) {
     S.q = k, S.k = q, S.v = d_o;
     S.x = none;
+    S.dots = nullptr;
     S.kd = dk, S.vd = dv;
     S.sr = dv, S.sc = 1;
     S.state_out = A.d_initial_state;
     S.out_f32 = shared_out(A.heads, A.v_heads) && A.dv_out;
     S.out = S.out_f32 ? space(W.dv) : A.dv_out;
-    if ((rc = run_sweep(S, bf16, s))) return rc;
+    if ((rc = run_sweep(A, W, S, false, s))) return rc;
   }
   if (some) {
     const int64_t rows = A.batch * A.tokens;
@@ -385,10 +457,9 @@ extern "C" int ttc_linear_attention(const ttc_linear_attention_args* args, void*
     const int64_t bh = A.batch * A.heads;
     if (bh > MAX_GRID) return TTC_LQR_EINVAL;
     S = sweep_of(A);
-    const int tiles = token_tiles(dk);
     double* per_head = A.gamma_per_head ? reinterpret_cast<double*>(space(W.per_head)) : nullptr;
     if (bh > 0)
-      hipLaunchKernelGGL(gate_kernel, dim3((unsigned)bh), dim3(64), 0, s, S, space(W.r), space(W.c), tiles, tiles,
+      hipLaunchKernelGGL(gate_kernel, dim3((unsigned)bh), dim3(64), 0, s, S, space(W.r), space(W.c), W.dot_tiles, W.dot_tiles,
                        space(W.last), some ? A.d_final_state : nullptr, (int64_t)dk * dv, A.d_log_gamma, per_head);
     if (per_head)
       hipLaunchKernelGGL(gate_head_kernel, dim3((unsigned)ceil_div(A.heads, 64)), dim3(64), 0, s, per_head, A.batch,

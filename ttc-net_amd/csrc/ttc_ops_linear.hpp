@@ -49,7 +49,29 @@ __device__ __forceinline__ float gamma_at(const Sweep& A, int64_t i) {
   return A.gamma_bf16 ? to_f(static_cast<const __bf16*>(A.gamma)[i]) : static_cast<const float*>(A.gamma)[i];
 }
 
-int launch_token_sweep(const Sweep& A, bool bf16, hipStream_t s);
-inline int token_tiles(int vd) { return (vd + 31) / 32; }
+// ---- segments: where heads are few, their tokens are split -----------------------------------------------------
+
+struct Segments {
+  int count;          // segments a head
+  int64_t chunks;     // chunks a segment
+  float* state;       // [batch, head, segment, kd, vd]: a segment's own contribution, then the state in front of it
+  float* decay;       // [batch, head, segment]: its whole decay
+};
+
+// Where 16-byte loads, and stores of 4 elements at once, are possible
+struct Wides {
+  bool q, k, v, out;
+};
+
+enum { STATE_ONLY = 0, FAST = 1, EXACT = 2 };  // what a chunked sweep gives: ttc_ops_linear_chunk.hpp
+
+template <class T>
+int launch_chunk_kd32(const Sweep& A, const Segments& G, const Wides& W, int mode, hipStream_t s);
+template <class T>
+int launch_chunk_kd64(const Sweep& A, const Segments& G, const Wides& W, int mode, hipStream_t s);
+template <class T>
+int launch_chunk_kd128(const Sweep& A, const Segments& G, const Wides& W, int mode, hipStream_t s);
+
+inline int chunk_tokens(bool bf16) { return bf16 ? 64 : 32; }
 
 }  // namespace ttc
