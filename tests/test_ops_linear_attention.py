@@ -217,6 +217,21 @@ def test_gradients_of_decays(device, dtype, kind, T):
         within(one, each.double().sum((0, 1)), 2 * T * 2 * EPS * each.abs().sum((0, 1)) + 1e-30)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kind,case", [
+    (torch.float32, "mixed", (1, 1100, 2, 2, 1, 2, 24, 40)), (torch.bfloat16, "mixed", (1, 2100, 2, 2, 2, 2, 40, 24)),
+    (torch.bfloat16, "reset", (1, 1025, 1, 1, 1, 1, 64, 64)), (torch.float32, "none", (2, 513, 1, 1, 1, 1, 16, 16))])
+def test_gradients_of_long_inputs(dtype, kind, case):
+    """Several stretches of the decays' gradient."""
+    x = inputs(*case, dtype, "cuda", True, kind)
+    B, T, H, dk, dv = case[0], case[1], case[2], case[6], case[7]
+    d_o, d_state = make((B, T, H, dv), dtype, "cuda", 9), make((B, H, dk, dv), torch.float32, "cuda", 10)
+    got = grads(x, d_o, d_state, 0.2)
+    check_grads(x, got, d_o, d_state, 0.2)
+    want = linear64(x["q"], x["k"], x["v"], x["g"], 0.2, x["state"], d_o, d_state)["g"]
+    assert float((got["g"].double().cpu() - want).norm() / want.norm()) < 1e-5  # the bounds above grow with the length
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("T", [7, 100])
 def test_gradients_against_differences(device, T):

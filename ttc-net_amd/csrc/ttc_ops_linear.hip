@@ -152,22 +152,27 @@ __global__ __launch_bounds__(256) void share_sum_kernel(const float* __restrict_
   out[i] = from_f<T>(a);
 }
 
-// dg_t = sum_{u >= t} (r_u - c_u) + <S_T, dS_T>, one wave per sequence and head, from the end, 8 tokens a lane at a time, in
-// 64 bits (the sum's terms cancel).  A reset's own gradient is 0, and nothing after it reaches tokens before it.
+// dg_t = sum_{u >= t} (r_u - c_u) + what the boundary behind passes on: one wave per sequence, head and stretch between
+// boundaries, from its end, 8 tokens a lane at a time, in 64 bits (the sum's terms cancel).  A reset's own gradient is 0,
+// and nothing after it reaches tokens before it.
 constexpr int GATE_TOKENS = 8;
 __global__ __launch_bounds__(64) void gate_kernel(Sweep A, const float* __restrict__ r, const float* __restrict__ c,
-                                                  int rtiles, int ctiles, const float* __restrict__ last,
+                                                  int tiles, int waves, const float* __restrict__ last,
                                                   const float* __restrict__ dlast, int64_t elems, void* d_gamma,
                                                   double* __restrict__ per_head) {
   const int lane = threadIdx.x;
-  const int64_t bh = blockIdx.x, b = bh / A.H, BHT = A.B * A.H * A.T;
+  const int64_t bh = blockIdx.x / A.marks, mark = blockIdx.x % A.marks, b = bh / A.H, BHT = A.B * A.H * A.T;
   const int h = (int)(bh % A.H);
+  const int64_t first = mark * A.mark_tokens, behind = first + A.mark_tokens < A.T ? first + A.mark_tokens : A.T;
   double carry = 0.0, total = 0.0;
-  if (dlast) {
+  if (A.joins) {
+    if (mark + 1 < A.marks || dlast)
+      for (int w = 0; w < waves; ++w) carry += A.joins[(bh * (A.marks + 1) + mark + 1) * MAX_WAVES + w];
+  } else if (dlast) {
     for (int64_t i = lane; i < elems; i += 64) carry += (double)last[bh * elems + i] * dlast[bh * elems + i];
     for (int m = 32; m >= 1; m >>= 1) carry += __shfl_xor(carry, m, 64);
   }
-  for (int64_t end = A.T; end > 0; end -= 64 * GATE_TOKENS) {
+  for (int64_t end = behind; end > first; end -= 64 * GATE_TOKENS) {
     const int64_t hi = end - lane * GATE_TOKENS;  // this lane: tokens hi - 1 down to hi - 8
     double sum[GATE_TOKENS], run = 0.0;
     bool cut[GATE_TOKENS], cuts = false;
@@ -175,10 +180,9 @@ __global__ __launch_bounds__(64) void gate_kernel(Sweep A, const float* __restri
     for (int i = 0; i < GATE_TOKENS; ++i) {
       const int64_t t = hi - 1 - i;
       cut[i] = false;
-      if (t >= 0) {
+      if (t >= first) {
         double d = 0.0;
-        for (int j = 0; j < rtiles; ++j) d += r[j * BHT + bh * A.T + t];
-        for (int j = 0; j < ctiles; ++j) d -= c[j * BHT + bh * A.T + t];
+        for (int j = 0; j < tiles; ++j) d += (double)r[j * BHT + bh * A.T + t] - c[j * BHT + bh * A.T + t];
         run += d;
         cut[i] = gamma_at(A, b * A.gb + h * A.gh + t * A.gt) < RESET;
       }
@@ -208,7 +212,7 @@ __global__ __launch_bounds__(64) void gate_kernel(Sweep A, const float* __restri
       const int64_t t = hi - 1 - i;
       open = open && !cut[i];
       const double d = cut[i] ? 0.0 : open ? sum[i] + before : sum[i];
-      if (t < 0) continue;
+      if (t < first) continue;
       total += d;
       if (per_head == nullptr) {
         const int64_t at = (b * A.T + t) * A.H + h;
@@ -219,16 +223,17 @@ __global__ __launch_bounds__(64) void gate_kernel(Sweep A, const float* __restri
   }
   if (per_head) {
     for (int m = 32; m >= 1; m >>= 1) total += __shfl_xor(total, m, 64);
-    if (lane == 0) per_head[bh] = total;
+    if (lane == 0) per_head[blockIdx.x] = total;
   }
 }
 
-__global__ __launch_bounds__(64) void gate_head_kernel(const double* __restrict__ per_head, int64_t B, int H, bool bf16,
-                                                       void* d_gamma) {
-  const int h = blockIdx.x * 64 + threadIdx.x;
-  if (h >= H) return;
+__global__ __launch_bounds__(64) void gate_head_kernel(const double* __restrict__ per_head, int64_t B, int H,
+                                                       int64_t marks, bool bf16, void* d_gamma) {
+  const int h = blockIdx.x;
   double a = 0.0;
-  for (int64_t b = 0; b < B; ++b) a += per_head[b * H + h];
+  for (int64_t i = threadIdx.x; i < B * marks; i += 64) a += per_head[(i / marks * H + h) * marks + i % marks];
+  for (int m = 32; m >= 1; m >>= 1) a += __shfl_xor(a, m, 64);
+  if (threadIdx.x != 0) return;
   if (bf16) static_cast<__bf16*>(d_gamma)[h] = from_f<__bf16>((float)a);
   else static_cast<float*>(d_gamma)[h] = (float)a;
 }
@@ -252,7 +257,8 @@ inline Segments segments_of(const ttc_linear_attention_args& A) {
 }
 
 struct Layout {  // the workspace, in bytes from its start; 0 bytes: not needed
-  int64_t seg_state, seg_decay, dq, dk, dv, r, c, last, per_head, total;
+  int64_t seg_state, seg_decay, dq, dk, dv, r, c, last, states, joins, per_head, total;
+  int64_t mark_tokens, marks;  // one stretch where the tokens are swept one by one
   int dot_tiles;
   bool gate;
 };
@@ -286,7 +292,14 @@ inline Layout layout_of(const ttc_linear_attention_args& A) {
     W.r = take(rows * W.dot_tiles * 4);
     W.c = take(rows * W.dot_tiles * 4);
     W.last = take(A.d_final_state ? A.batch * A.heads * A.dk * A.dv * 4 : 0);
-    W.per_head = take(A.gamma_per_head ? A.batch * A.heads * 8 : 0);
+    const int64_t stretch = 16 * chunk_tokens(A.dtype == TTC_DTYPE_BF16);
+    W.mark_tokens = A.tokens > TOKEN_SWEEP ? stretch : TOKEN_SWEEP;
+    W.marks = A.tokens > 0 ? ceil_div(A.tokens, W.mark_tokens) : 1;
+    if (A.tokens > TOKEN_SWEEP) {
+      W.states = take(W.marks > 1 ? A.batch * A.heads * W.marks * A.dk * A.dv * 4 : 0);
+      W.joins = take(A.batch * A.heads * (W.marks + 1) * MAX_WAVES * 4);
+    }
+    W.per_head = take(A.gamma_per_head ? A.batch * A.heads * W.marks * 8 : 0);
   }
   W.total = at;
   return W;
@@ -346,9 +359,11 @@ int run_sweep(const ttc_linear_attention_args& A, const Layout& W, const Sweep& 
   G.decay = reinterpret_cast<float*>(ws + W.seg_decay);
   const int vec = bf16 ? 8 : 4;
   auto wide = [&](const Side& x, int dim) {
-    return dim % vec == 0 && aligned16(x.p) && x.sb % vec == 0 && x.st % vec == 0 && x.sh % vec == 0;
+    return dim % vec == 0 && aligned16(x.p) && x.sb % vec == 0 && x.st % vec == 0 && x.sh % vec == 0 && x.st >= 0 &&
+           x.st < (1 << 22);  // a chunk's rows within 2^29 bytes of its lowest address
   };
-  const Wides V{wide(S.q, S.kd), wide(S.k, S.kd), wide(S.v, S.vd), S.vd % 4 == 0 && aligned16(S.out)};
+  const Wides V{wide(S.q, S.kd) && wide(S.k, S.kd) && wide(S.v, S.vd) && (!S.x.p || wide(S.x, S.vd)),
+                S.vd % 4 == 0 && aligned16(S.out)};
   auto launch = [&](int mode) {
     if (bf16)
       return S.kd <= 32   ? launch_chunk_kd32<__bf16>(S, G, V, mode, s)
@@ -415,6 +430,8 @@ extern "C" int ttc_linear_attention(const ttc_linear_attention_args* args, void*
     S.state_out = gate && A.d_final_state ? space(W.last) : nullptr;
     S.sr = 1, S.sc = dv;
     S.dots = space(W.r);
+    S.mark_tokens = W.mark_tokens, S.marks = W.marks;
+    S.states = gate && W.marks > 1 ? space(W.states) : nullptr;
     S.out_f32 = shared_out(A.heads, A.q_heads) || !A.dq;
     S.out = S.out_f32 ? space(W.dq) : A.dq;
     if ((rc = run_sweep(A, W, S, gate, s))) return rc;
@@ -429,6 +446,10 @@ extern "C" int ttc_linear_attention(const ttc_linear_attention_args* args, void*
     S.kd = dv, S.vd = dk;
     S.sr = 1, S.sc = dv;
     S.dots = space(W.c);
+    S.mark_tokens = W.mark_tokens, S.marks = W.marks;
+    S.states = gate && W.marks > 1 ? space(W.states) : nullptr;
+    S.joins = gate ? space(W.joins) : nullptr;
+    S.last = gate && A.d_final_state ? space(W.last) : nullptr;
     S.out_f32 = shared_out(A.heads, A.k_heads) || !A.dk_out;
     S.out = S.out_f32 ? space(W.dk) : A.dk_out;
     if ((rc = run_sweep(A, W, S, gate, s))) return rc;
@@ -436,7 +457,8 @@ extern "C" int ttc_linear_attention(const ttc_linear_attention_args* args, void*
   if ((some && A.dv_out) || A.d_initial_state) {
     S.q = k, S.k = q, S.v = d_o;
     S.x = none;
-    S.dots = nullptr;
+    S.dots = S.states = S.joins = nullptr;
+    S.last = nullptr;
     S.kd = dk, S.vd = dv;
     S.sr = dv, S.sc = 1;
     S.state_out = A.d_initial_state;
@@ -454,16 +476,19 @@ extern "C" int ttc_linear_attention(const ttc_linear_attention_args* args, void*
     if (A.dv_out && shared_out(A.heads, A.v_heads) && (rc = join(space(W.dv), A.dv_out, A.v_heads, A.dv))) return rc;
   }
   if (W.gate) {  // of one decay for each head: zero where there are no tokens
-    const int64_t bh = A.batch * A.heads;
-    if (bh > MAX_GRID) return TTC_LQR_EINVAL;
+    const int64_t stretches = A.batch * A.heads * W.marks;
+    if (stretches > MAX_GRID) return TTC_LQR_EINVAL;
     S = sweep_of(A);
+    S.mark_tokens = W.mark_tokens, S.marks = W.marks;
+    S.joins = A.tokens > TOKEN_SWEEP ? space(W.joins) : nullptr;
+    const int waves = dk <= 32 ? 2 : dk <= 64 ? 4 : 8;  // of the sweep of dk
     double* per_head = A.gamma_per_head ? reinterpret_cast<double*>(space(W.per_head)) : nullptr;
-    if (bh > 0)
-      hipLaunchKernelGGL(gate_kernel, dim3((unsigned)bh), dim3(64), 0, s, S, space(W.r), space(W.c), W.dot_tiles, W.dot_tiles,
-                       space(W.last), some ? A.d_final_state : nullptr, (int64_t)dk * dv, A.d_log_gamma, per_head);
+    if (stretches > 0)
+      hipLaunchKernelGGL(gate_kernel, dim3((unsigned)stretches), dim3(64), 0, s, S, space(W.r), space(W.c), W.dot_tiles,
+                         waves, space(W.last), some ? A.d_final_state : nullptr, (int64_t)dk * dv, A.d_log_gamma, per_head);
     if (per_head)
-      hipLaunchKernelGGL(gate_head_kernel, dim3((unsigned)ceil_div(A.heads, 64)), dim3(64), 0, s, per_head, A.batch,
-                         (int)A.heads, S.gamma_bf16, A.d_log_gamma);
+      hipLaunchKernelGGL(gate_head_kernel, dim3((unsigned)A.heads), dim3(64), 0, s, per_head, A.batch, (int)A.heads, W.marks,
+                         S.gamma_bf16, A.d_log_gamma);
   }
   return launched();
 }

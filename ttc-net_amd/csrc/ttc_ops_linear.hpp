@@ -8,7 +8,9 @@
 // one kernel, in four roles (the state transposed where the roles of dk and dv swap).  In reverse order the decay that
 // is applied before token t is that of token t + 1 (none before the last token), and that of token 0 after the end.
 // The decays' gradient needs no state either: with the dots r_t = q_t.dq_t and c_t = k_t.dk_t,
-//   dg_t = sum_{u >= t} (r_u - c_u) + <S_T, dS_T>.
+//   dg_t = sum_{u >= t} (r_u - c_u) + <S_T, dS_T>,
+// and, so that the rounding of a long sum of cancelling terms does not add up, dg_t = e^{g_t} <S_{t-1}, R_t> itself at a
+// boundary every 16 chunks, where the two sweeps' states meet.
 #pragma once
 #include "ttc_ops_common.hpp"
 
@@ -16,6 +18,7 @@ namespace ttc {
 
 constexpr float RESET = TTC_RESET_LOG_GAMMA;
 constexpr int MAX_DIM = TTC_LINEAR_ATTENTION_MAX_DIM;
+constexpr int MAX_WAVES = MAX_DIM / 16;  // of a chunked sweep's workgroup
 
 struct Side {  // one of the sweep's inputs: [batch, token, head, dim], heads shared by `div` heads of the sweep
   const void* p;
@@ -43,6 +46,13 @@ struct Sweep {
   int64_t nslots;
   void* out;                   // [B, T, H, vd] contiguous, of the inputs' type or fp32
   float* dots;                 // [B, H, T], with one more such array for each further tile of columns
+  // Boundaries every mark_tokens tokens of a chunked sweep (NULL: none), marks of them with the one before token 0.
+  // The sweep of dq leaves the state in front of each, [B, H, marks, kd, vd]; the sweep of dk joins its own state there to
+  // the decay's gradient, [B, H, marks + 1, MAX_WAVES] in parts, the last from `last`, the state behind all tokens (laid out
+  // as state_out; NULL: none).
+  float *states, *joins;
+  const float* last;
+  int64_t mark_tokens, marks;
 };
 
 __device__ __forceinline__ float gamma_at(const Sweep& A, int64_t i) {
@@ -58,9 +68,9 @@ struct Segments {
   float* decay;       // [batch, head, segment]: its whole decay
 };
 
-// Where 16-byte loads, and stores of 4 elements at once, are possible
+// Where 16-byte loads of all inputs, and stores of 4 elements at once, are possible
 struct Wides {
-  bool q, k, v, out;
+  bool in, out;
 };
 
 enum { STATE_ONLY = 0, FAST = 1, EXACT = 2 };  // what a chunked sweep gives: ttc_ops_linear_chunk.hpp

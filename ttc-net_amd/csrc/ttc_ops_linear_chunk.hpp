@@ -162,111 +162,137 @@ __device__ __forceinline__ float kept(float w, float x) { return w == 0.0f ? 0.0
 
 template <class T, int KD, int VD>
 struct ChunkShape {
-  static constexpr int WAVES = VD == 32 ? 2 : 4, NT = WAVES * 64, VW = VD / WAVES, ET = VW / 16;
+  static constexpr int WAVES = VD / 16, NT = WAVES * 64;  // at most MAX_WAVES; a wave's 16 columns: 32 registers of state for 128 rows
   static constexpr int C = Operand<T>::CHUNK, TT = C / 16, KB = C / 32, DB = KD / 32, DT = KD / 16;
   static constexpr int VEC = 16 / sizeof(T), QS = KD + Operand<T>::PAD, VS = VD + Operand<T>::PAD;
-  static constexpr int KV = C * KD / VEC / NT, VV = C * VD / VEC / NT;  // 16-byte loads a thread
+  static constexpr int KV = (C * KD / VEC + NT - 1) / NT, VV = (C * VD / VEC + NT - 1) / NT;  // 16-byte loads a thread
 };
 
-// 16 bytes of a row from element c on, zero beyond `dim`
+// 16 bytes of a row from element c on, zero beyond `dim`, for rows of any alignment
 template <class T>
-__device__ __forceinline__ u32x4 load16(const T* p, int c, int dim, bool wide) {
+__device__ __forceinline__ u32x4 load_any(const T* p, int c, int dim) {
   constexpr int VEC = 16 / sizeof(T);
-  u32x4 r = {0, 0, 0, 0};
-  if (wide) {
-    if (c < dim) r = *reinterpret_cast<const u32x4*>(p + c);
-  } else {
-    T e[VEC];
+  u32x4 r;
+  T e[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) e[j] = c + j < dim ? p[c + j] : from_f<T>(0.0f);
-    __builtin_memcpy(&r, e, 16);
-  }
+  for (int j = 0; j < VEC; ++j) e[j] = c + j < dim ? p[c + j] : from_f<T>(0.0f);
+  __builtin_memcpy(&r, e, 16);
   return r;
 }
 
-template <class T, int KD, int VD, int MODE>
+// A chunk's rows of one input, for loads that give 0 past the bound instead of branching: all loads of a chunk are in
+// flight at once.  Offsets from the chunk's lowest address are below 2^30 bytes (the host sees to it).
+constexpr int BEYOND = 0x7ffffff0;
+template <class T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const T* p) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, 1 << 30, 0x00027000);
+}
+
+// WIDE: rows of 16-byte multiples at 16-byte addresses
+template <class T, int KD, int VD, int MODE, bool WIDE>
 __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_kernel(Sweep A, Segments G, Wides W) {
   using Z = ChunkShape<T, KD, VD>;
   using Op = Operand<T>;
   using PT = std::conditional_t<MODE == EXACT, float, T>;  // the weighted scores in shared memory
+  constexpr bool DOTS = MODE == EXACT || (MODE == FAST && sizeof(T) == 4);
   constexpr int C = Z::C, NT = Z::NT, VEC = Z::VEC, QS = Z::QS, VS = Z::VS, PS = C + 16 / (int)sizeof(PT);
   __shared__ __attribute__((aligned(16))) T Qs[MODE == STATE_ONLY ? 1 : C * QS];
   __shared__ __attribute__((aligned(16))) T Ks[C * QS];
   __shared__ __attribute__((aligned(16))) T Vs[C * VS];
   __shared__ __attribute__((aligned(16))) PT Ps[MODE == STATE_ONLY ? 1 : C * PS];
   __shared__ __attribute__((aligned(16))) float Hi[2][C], Lo[2][C], In[2][C], Up[2][C];
-  __shared__ float Whole[2], Dot[MODE == EXACT || sizeof(T) == 4 ? Z::WAVES : 1][C];
+  __shared__ float Whole[2], Dot[DOTS ? Z::WAVES : 1][C];
   __shared__ int Odd[Z::WAVES];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, n = lane & 15;
   const int segs = MODE == STATE_ONLY ? G.count - 1 : G.count;  // the last one's own contribution is not needed
   const int seg = (int)(blockIdx.x % segs);
-  const int64_t bh = blockIdx.x / segs, b = bh / A.H;
+  const int64_t bh = blockIdx.x / segs, b = bh / A.H, elems = (int64_t)A.kd * A.vd;
   const int h = (int)(bh % A.H);
   const T *q = MODE == STATE_ONLY ? nullptr : A.q.at<T>(b, h), *k = A.k.at<T>(b, h), *v = A.v.at<T>(b, h);
+  const T* x = DOTS && A.x.p ? A.x.at<T>(b, h) : nullptr;
   const int64_t gbase = b * A.gb + h * A.gh;
-  const int64_t u0 = seg * G.chunks * C;  // tokens in the sweep's order
-  const int64_t u1 = u0 + G.chunks * C < A.T ? u0 + G.chunks * C : A.T;
-  const int e0 = wave * Z::VW;
+  // Places in the sweep's order: whole chunks, whose boundaries lie between the same tokens in both orders
+  const int64_t places = (A.T + C - 1) / C * C, u0 = seg * G.chunks * C;
+  const int64_t u1 = u0 + G.chunks * C < places ? u0 + G.chunks * C : places;
+  const int e0 = wave * 16;  // the wave's columns
+  auto token = [&](int64_t u) { return A.reverse ? places - 1 - u : u; };  // >= T: none
 
-  f32x4 S[Z::DT][Z::ET];
+  // S: lane's rows 16 d + 4 g + i, column e0 + n.  The lane's place is hidden from the compiler, which would otherwise keep
+  // 32 addresses in registers over the whole loop.
+  auto each = [&](auto f) {
+    int r = 4 * g, c = e0 + n;
+    asm volatile("" : "+v"(r), "+v"(c));
+#pragma unroll
+    for (int d = 0; d < Z::DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f(d, i, 16 * d + r + i, c);
+  };
+  f32x4 S[Z::DT];
   {
     const float* p = nullptr;
     int sr = A.sr, sc = A.sc;
     if (MODE != STATE_ONLY) {
       if (G.count > 1) {
-        p = G.state + (bh * G.count + seg) * (int64_t)A.kd * A.vd;
+        p = G.state + (bh * G.count + seg) * elems;
         sr = A.vd, sc = 1;
       } else if (A.state_in) {
-        p = A.state_in + bh * (int64_t)A.kd * A.vd;
+        p = A.state_in + bh * elems;
       }
     }
-#pragma unroll
-    for (int d = 0; d < Z::DT; ++d)
-#pragma unroll
-      for (int e = 0; e < Z::ET; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 16 * d + 4 * g + i, c = e0 + 16 * e + n;
-          S[d][e][i] = p && r < A.kd && c < A.vd ? p[(int64_t)r * sr + (int64_t)c * sc] : 0.0f;
-        }
+    each([&](int d, int i, int r, int c) {
+      S[d][i] = p && r < A.kd && c < A.vd ? p[r * sr + c * sc] : 0.0f;
+    });
   }
+  // <S, p>, the wave's part of it: the decays' gradient at a boundary
+  auto meet = [&](const float* p, int sr, int sc, float w, int64_t mark) {
+    float d = 0.0f;
+    each([&](int dt, int i, int r, int c) {
+      if (r < A.kd && c < A.vd) d = fmaf(S[dt][i], p[r * sr + c * sc], d);
+    });
+    d = lane_sum(d, 64);
+    if (lane == 0) A.joins[(bh * (A.marks + 1) + mark) * MAX_WAVES + wave] = kept(w, d);
+  };
+  if (DOTS && A.joins && A.reverse && seg == 0 && A.last) meet(A.last + bh * elems, A.sr, A.sc, 1.0f, A.marks);
 
   u32x4 qr[Z::KV], kr[Z::KV], vr[Z::VV];
-  auto token = [&](int64_t u) { return A.reverse ? A.T - 1 - u : u; };
-  auto fetch = [&](int64_t at) {
+  auto fetch_side = [&](const T* p, int64_t st, int dim, int64_t at, auto& r, auto width) {
+    constexpr int D = decltype(width)::value;
+    const auto rows = rows_of(p + (A.reverse ? token(at + C - 1) : at) * st);
 #pragma unroll
-    for (int j = 0; j < Z::KV; ++j) {
-      const int i = tid + j * NT, row = i / (KD / VEC), c = i % (KD / VEC) * VEC;
-      const u32x4 zero = {0, 0, 0, 0};
-      const bool in = at + row < u1;
-      const int64_t t = token(at + row);
-      kr[j] = in ? load16(k + t * A.k.st, c, A.kd, W.k) : zero;
-      if (MODE != STATE_ONLY) qr[j] = in ? load16(q + t * A.q.st, c, A.kd, W.q) : zero;
-    }
-#pragma unroll
-    for (int j = 0; j < Z::VV; ++j) {
-      const int i = tid + j * NT, row = i / (VD / VEC), c = i % (VD / VEC) * VEC;
-      const u32x4 zero = {0, 0, 0, 0};
-      vr[j] = at + row < u1 ? load16(v + token(at + row) * A.v.st, c, A.vd, W.v) : zero;
+    for (int j = 0; j < (int)(sizeof(r) / sizeof(r[0])); ++j) {
+      const int i = tid + j * NT, row = i / (D / VEC), c = i % (D / VEC) * VEC;
+      const bool in = row < C && token(at + row) < A.T;
+      if constexpr (WIDE) {
+        const int off = (A.reverse ? C - 1 - row : row) * (int)(st * (int)sizeof(T)) + c * (int)sizeof(T);
+        r[j] = __builtin_amdgcn_raw_buffer_load_b128(rows, in && c < dim ? off : BEYOND, 0, 0);
+      } else {
+        const u32x4 zero = {0, 0, 0, 0};
+        r[j] = in ? load_any(p + token(at + row) * st, c, dim) : zero;
+      }
     }
   };
-  // wave 0: the chunk's decays.  Tokens beyond the end have none.
+  auto fetch = [&](int64_t at) {
+    fetch_side(k, A.k.st, A.kd, at, kr, std::integral_constant<int, KD>{});
+    if constexpr (MODE != STATE_ONLY) fetch_side(q, A.q.st, A.kd, at, qr, std::integral_constant<int, KD>{});
+    fetch_side(v, A.v.st, A.vd, at, vr, std::integral_constant<int, VD>{});
+  };
+  // wave 0: the chunk's decays; before a token in reverse order, that of the one after it
   auto gate_of = [&](int64_t u) {
-    if (lane >= C || u >= u1 || (A.reverse && u == 0)) return 0.0f;
-    return gamma_at(A, gbase + (A.reverse ? A.T - u : u) * A.gt);
+    const int64_t t = token(u) + (A.reverse ? 1 : 0);
+    return lane < C && t < A.T ? gamma_at(A, gbase + t * A.gt) : 0.0f;
   };
   auto gates = [&](float lg, int buf) {
-    double x = (double)lg * 1.4426950408889634;
-    x = x < -4096.0 ? -4096.0 : x;
+    double y = (double)lg * 1.4426950408889634;
+    y = y < -4096.0 ? -4096.0 : y;
 #pragma unroll
     for (int m = 1; m < C; m <<= 1) {
-      const double y = __shfl_up(x, m, 64);
-      if (lane >= m) x += y;
+      const double z = __shfl_up(y, m, 64);
+      if (lane >= m) y += z;
     }
-    const double all = __shfl(x, C - 1, 64), rest = all - x;
+    const double rest = __shfl(y, C - 1, 64) - y;
     if (lane < C) {
-      const float hi = (float)x, lo = (float)(x - (double)hi), uh = (float)rest, ul = (float)(rest - (double)uh);
+      const float hi = (float)y, lo = (float)(y - (double)hi), uh = (float)rest, ul = (float)(rest - (double)uh);
       Hi[buf][lane] = hi;
       Lo[buf][lane] = lo;
       const float in = exp2_of(hi) * exp2_of(lo);
@@ -275,51 +301,76 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
       if (lane == C - 1) Whole[buf] = in;
     }
   };
+  auto put_dots = [&](int64_t at) {  // after the barrier behind the chunk
+    if constexpr (DOTS) {
+      if (x && tid < C && token(at + tid) < A.T) {
+        float d = 0.0f;
+#pragma unroll
+        for (int w = 0; w < Z::WAVES; ++w) d += Dot[w][tid];
+        A.dots[bh * A.T + token(at + tid)] = d;
+      }
+    }
+  };
 
   fetch(u0);
   if (wave == 0) gates(gate_of(u0 + lane), 0);
   float whole_decay = 1.0f;
   int buf = 0;
-  int64_t dot_at = -1;
-  auto put_dots = [&]() {  // of the chunk before, after a barrier
-    if constexpr (MODE == EXACT || sizeof(T) == 4) {
-      if (A.x.p != nullptr && dot_at >= 0 && tid < C && dot_at + tid < u1) {
-        float d = 0.0f;
-#pragma unroll
-        for (int w = 0; w < Z::WAVES; ++w) d += Dot[w][tid];
-        A.dots[bh * A.T + token(dot_at + tid)] = d;
-      }
-    }
-  };
-
   for (int64_t at = u0; at < u1; at += C, buf ^= 1) {
     // the chunk's tokens to shared memory, and whether all keys and values are finite
     uint32_t most = 0;
+    auto stage = [&](T* to, int stride, auto& r, auto width, bool look) {
+      constexpr int D = decltype(width)::value;
 #pragma unroll
-    for (int j = 0; j < Z::KV; ++j) {
-      const int i = tid + j * NT, row = i / (KD / VEC), c = i % (KD / VEC) * VEC;
-      Op::largest(kr[j], most);
-      *reinterpret_cast<u32x4*>(&Ks[row * QS + c]) = kr[j];
-      if (MODE != STATE_ONLY) *reinterpret_cast<u32x4*>(&Qs[row * QS + c]) = qr[j];
-    }
-#pragma unroll
-    for (int j = 0; j < Z::VV; ++j) {
-      const int i = tid + j * NT, row = i / (VD / VEC), c = i % (VD / VEC) * VEC;
-      Op::largest(vr[j], most);
-      *reinterpret_cast<u32x4*>(&Vs[row * VS + c]) = vr[j];
-    }
+      for (int j = 0; j < (int)(sizeof(r) / sizeof(r[0])); ++j) {
+        const int i = tid + j * NT, row = i / (D / VEC), c = i % (D / VEC) * VEC;
+        if (look) Op::largest(r[j], most);
+        if (C * D / VEC % NT == 0 || row < C) *reinterpret_cast<u32x4*>(&to[row * stride + c]) = r[j];
+      }
+    };
+    stage(Ks, QS, kr, std::integral_constant<int, KD>{}, true);
+    if constexpr (MODE != STATE_ONLY) stage(Qs, QS, qr, std::integral_constant<int, KD>{}, false);
+    stage(Vs, VS, vr, std::integral_constant<int, VD>{}, true);
     const bool odd_here = __ballot(!Op::finite(most)) != 0;
     if (lane == 0) Odd[wave] = odd_here;
     __syncthreads();
-    put_dots();
+    if (at > u0) put_dots(at - C);
     bool odd = false;
 #pragma unroll
     for (int w = 0; w < Z::WAVES; ++w) odd = odd || Odd[w];
     if (at + C < u1) fetch(at + C);
-    const float next_gate = wave == 0 ? gate_of(at + C + lane) : 0.0f;
+    const float next_gate = wave == 0 && at + C < u1 ? gate_of(at + C + lane) : 0.0f;
     const float whole = Whole[buf];
+    struct alignas(4 * sizeof(T)) Four { T v[4]; };
+    Four xs[DOTS ? Z::TT : 1];
+    if constexpr (DOTS) {
+      if (x) {
+#pragma unroll
+        for (int t = 0; t < Z::TT; ++t) {
+          const int64_t tok = token(at + 16 * t + n);
+          const int c = e0 + 4 * g;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) xs[t].v[i] = from_f<T>(0.0f);
+          if (tok < A.T) {
+            if (WIDE) {
+              if (c < A.vd) xs[t] = *reinterpret_cast<const Four*>(x + tok * A.x.st + c);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (c + i < A.vd) xs[t].v[i] = x[tok * A.x.st + c + i];
+            }
+          }
+        }
+      }
+      if (A.states && !A.reverse && at > 0 && at % A.mark_tokens == 0) {  // the state in front of a boundary
+        float* p = A.states + (bh * A.marks + at / A.mark_tokens) * elems;
+        each([&](int d, int i, int r, int c) {
+          if (r < A.kd && c < A.vd) p[r * A.vd + c] = S[d][i];
+        });
+      }
+    }
 
-    f32x4 O[Z::TT][Z::ET];
+    f32x4 O[Z::TT];
     if constexpr (MODE != STATE_ONLY) {
       // scores, tile by tile over the waves: (ti, si <= ti), and zeros where a later product's 32 tokens reach past ti
       int turn = 0;
@@ -343,51 +394,39 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
               p[i] = si < ti || 4 * g + i <= n ? kept(w, p[i]) : 0.0f;
             }
           }
-          struct alignas(4 * sizeof(PT)) Four { PT v[4]; };
-          Four f;
+          struct alignas(4 * sizeof(PT)) Scores { PT v[4]; };
+          Scores f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) f.v[i] = from_f<PT>(p[i]);
-          *reinterpret_cast<Four*>(&Ps[(16 * ti + n) * PS + 16 * si + 4 * g]) = f;
+          *reinterpret_cast<Scores*>(&Ps[(16 * ti + n) * PS + 16 * si + 4 * g]) = f;
         }
       // the state's part
 #pragma unroll
-      for (int t = 0; t < Z::TT; ++t)
-#pragma unroll
-        for (int e = 0; e < Z::ET; ++e) O[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < Z::TT; ++t) O[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int d = 0; d < Z::DB; ++d) {
-        using Given = std::conditional_t<MODE == EXACT, typename Op::Wide, typename Op::Frag>;
-        Given s[Z::ET];
+        float y[8];
 #pragma unroll
-        for (int e = 0; e < Z::ET; ++e) {
-          float x[8];
+        for (int i = 0; i < 4; ++i) y[i] = S[2 * d][i], y[4 + i] = S[2 * d + 1][i];
+        auto by = [&](const auto& s) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = S[2 * d][e][i], x[4 + i] = S[2 * d + 1][e][i];
-          if constexpr (MODE == EXACT) s[e] = Op::wide(x); else s[e] = Op::narrow(x);
-        }
-#pragma unroll
-        for (int t = 0; t < Z::TT; ++t) {
-          const typename Op::Frag f = Op::row_split(&Qs[(16 * t + n) * QS + 32 * d + 4 * g]);
-#pragma unroll
-          for (int e = 0; e < Z::ET; ++e) O[t][e] = Op::mma(s[e], f, O[t][e]);
-        }
+          for (int t = 0; t < Z::TT; ++t)
+            O[t] = Op::mma(s, Op::row_split(&Qs[(16 * t + n) * QS + 32 * d + 4 * g]), O[t]);
+        };
+        if constexpr (MODE == EXACT) by(Op::wide(y)); else by(Op::narrow(y));
       }
 #pragma unroll
       for (int t = 0; t < Z::TT; ++t) {
         const float w = In[buf][16 * t + n];
 #pragma unroll
-        for (int e = 0; e < Z::ET; ++e)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) O[t][e][i] = kept(w, O[t][e][i]);
+        for (int i = 0; i < 4; ++i) O[t][i] = kept(w, O[t][i]);
       }
       __syncthreads();
     }
 
-    typename Op::Frag vf[Z::KB][Z::ET];
+    typename Op::Frag vf[Z::KB];
 #pragma unroll
-    for (int s = 0; s < Z::KB; ++s)
-#pragma unroll
-      for (int e = 0; e < Z::ET; ++e) vf[s][e] = Op::column(&Vs[32 * s * VS], VS, e0 + 16 * e, lane);
+    for (int s = 0; s < Z::KB; ++s) vf[s] = Op::column(&Vs[32 * s * VS], VS, e0, lane);
 
     if constexpr (MODE != STATE_ONLY) {
       if (!odd) {
@@ -395,16 +434,13 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
         for (int t = 0; t < Z::TT; ++t)
 #pragma unroll
           for (int s = 0; s <= t / 2; ++s) {
+            const PT* p = &Ps[(16 * t + n) * PS + 32 * s + 8 * g];
             if constexpr (MODE == EXACT) {
-              float x[8];
-              Operand<float>::values(Operand<float>::row(&Ps[(16 * t + n) * PS + 32 * s + 8 * g]), x);
-              const auto p = Op::wide(x);
-#pragma unroll
-              for (int e = 0; e < Z::ET; ++e) O[t][e] = Op::mma(vf[s][e], p, O[t][e]);
+              float y[8];
+              Operand<float>::values(Operand<float>::row(p), y);
+              O[t] = Op::mma(vf[s], Op::wide(y), O[t]);
             } else {
-              const typename Op::Frag p = Op::row(&Ps[(16 * t + n) * PS + 32 * s + 8 * g]);
-#pragma unroll
-              for (int e = 0; e < Z::ET; ++e) O[t][e] = Op::mma(vf[s][e], p, O[t][e]);
+              O[t] = Op::mma(vf[s], Op::row(p), O[t]);
             }
           }
       } else {
@@ -416,162 +452,124 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
             if (s > tt || w == 0.0f) continue;
             const float p = to_f(Ps[tt * PS + s]);
 #pragma unroll
-            for (int e = 0; e < Z::ET; ++e)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) O[t][e][i] = fmaf(p, to_f(Vs[s * VS + e0 + 16 * e + 4 * g + i]), O[t][e][i]);
+            for (int i = 0; i < 4; ++i) O[t][i] = fmaf(p, to_f(Vs[s * VS + e0 + 4 * g + i]), O[t][i]);
           }
         }
       }
       // out: a lane holds 4 neighbouring columns of one token
-      const bool dots = (MODE == EXACT || sizeof(T) == 4) && A.x.p != nullptr;
+      const int c = e0 + 4 * g;
 #pragma unroll
       for (int t = 0; t < Z::TT; ++t) {
-        const int64_t u = at + 16 * t + n;
-        const int64_t tok = token(u);
-        float dot = 0.0f;
+        const int64_t tok = token(at + 16 * t + n), o = ((b * A.T + tok) * A.H + h) * A.vd + c;
+        f32x4 r = O[t];
 #pragma unroll
-        for (int e = 0; e < Z::ET; ++e) {
-          const int c = e0 + 16 * e + 4 * g;
-          const int64_t o = ((b * A.T + tok) * A.H + h) * A.vd + c;
-          f32x4 r = O[t][e];
+        for (int i = 0; i < 4; ++i) r[i] *= A.out_scale;
+        if (tok < A.T && A.out != nullptr) {
+          auto put = [&](auto* y) {
+            using Y = std::remove_pointer_t<decltype(y)>;
+            struct alignas(4 * sizeof(Y)) Columns { Y v[4]; };
+            Columns f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) r[i] *= A.out_scale;
-          if (u < u1) {
-            if (A.out == nullptr) {
-            } else if (A.out_f32) {
-              float* y = static_cast<float*>(A.out) + o;
-              if (W.out) {
-                if (c < A.vd) *reinterpret_cast<f32x4*>(y) = r;
-              } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  if (c + i < A.vd) y[i] = r[i];
-              }
+            for (int i = 0; i < 4; ++i) f.v[i] = from_f<Y>(r[i]);
+            if (W.out) {
+              if (c < A.vd) *reinterpret_cast<Columns*>(y + o) = f;
             } else {
-              T* y = static_cast<T*>(A.out) + o;
-              struct alignas(4 * sizeof(T)) Four { T v[4]; };
-              Four f;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) f.v[i] = from_f<T>(r[i]);
-              if (W.out) {
-                if (c < A.vd) *reinterpret_cast<Four*>(y) = f;
-              } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  if (c + i < A.vd) y[i] = f.v[i];
-              }
-            }
-            if (dots) {
-              const T* x = A.x.at<T>(b, h) + tok * A.x.st + c;
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                if (c + i < A.vd) dot = fmaf(r[i], to_f(x[i]), dot);
+                if (c + i < A.vd) y[o + i] = f.v[i];
             }
-          }
+          };
+          if (A.out_f32) put(static_cast<float*>(A.out)); else put(static_cast<T*>(A.out));
         }
-        if constexpr (MODE == EXACT || sizeof(T) == 4) {
-          if (dots) {
+        if constexpr (DOTS) {
+          if (x) {
+            float dot = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dot = fmaf(r[i], to_f(xs[t].v[i]), dot);
             dot += __shfl_xor(dot, 16, 64);
             dot += __shfl_xor(dot, 32, 64);
             if (g == 0) Dot[wave][16 * t + n] = dot;
           }
         }
       }
-      dot_at = at;
     }
 
     // the state behind the chunk
 #pragma unroll
     for (int d = 0; d < Z::DT; ++d)
 #pragma unroll
-      for (int e = 0; e < Z::ET; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) S[d][e][i] = kept(whole, S[d][e][i]);
+      for (int i = 0; i < 4; ++i) S[d][i] = kept(whole, S[d][i]);
     whole_decay *= whole;
     if (!odd) {
 #pragma unroll
       for (int s = 0; s < Z::KB; ++s) {
         const f32x4 wa = *reinterpret_cast<const f32x4*>(&Up[buf][32 * s + 8 * g]),
                     wb = *reinterpret_cast<const f32x4*>(&Up[buf][32 * s + 8 * g + 4]);
-        typename Op::Wide wv[Z::ET];
+        float y[8];
+        Op::values(vf[s], y);
 #pragma unroll
-        for (int e = 0; e < Z::ET; ++e) {
-          float x[8];
-          Op::values(vf[s][e], x);
+        for (int j = 0; j < 8; ++j) y[j] *= j < 4 ? wa[j] : wb[j - 4];
+        const typename Op::Wide wv = Op::wide(y);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] *= j < 4 ? wa[j] : wb[j - 4];
-          wv[e] = Op::wide(x);
-        }
-#pragma unroll
-        for (int d = 0; d < Z::DT; ++d) {
-          const typename Op::Frag f = Op::column(&Ks[32 * s * QS], QS, 16 * d, lane);
-#pragma unroll
-          for (int e = 0; e < Z::ET; ++e) S[d][e] = Op::mma(f, wv[e], S[d][e]);
-        }
+        for (int d = 0; d < Z::DT; ++d) S[d] = Op::mma(Op::column(&Ks[32 * s * QS], QS, 16 * d, lane), wv, S[d]);
       }
     } else {
       for (int s = 0; s < C; ++s) {
         const float w = Up[buf][s];
         if (w == 0.0f) continue;
-#pragma unroll
-        for (int e = 0; e < Z::ET; ++e) {
-          const float x = w * to_f(Vs[s * VS + e0 + 16 * e + n]);
-#pragma unroll
-          for (int d = 0; d < Z::DT; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) S[d][e][i] = fmaf(to_f(Ks[s * QS + 16 * d + 4 * g + i]), x, S[d][e][i]);
-        }
+        const float y = w * to_f(Vs[s * VS + e0 + n]);
+        each([&](int d, int i, int r, int) { S[d][i] = fmaf(to_f(Ks[s * QS + r]), y, S[d][i]); });
+      }
+    }
+    if (DOTS && A.joins && A.reverse) {  // a boundary in front of token t: its decay's gradient
+      const int64_t t = token(at + C - 1);
+      if (t > 0 && t % A.mark_tokens == 0) {
+        const float lg = gamma_at(A, gbase + t * A.gt);
+        meet(A.states + (bh * A.marks + t / A.mark_tokens) * elems, A.vd, 1, lg < RESET ? 0.0f : expf(lg), t / A.mark_tokens);
       }
     }
     if (wave == 0 && at + C < u1) gates(next_gate, buf ^ 1);
     __syncthreads();
   }
-  put_dots();
+  put_dots(u1 - C);
 
   float* p = nullptr;
   int sr = A.sr, sc = A.sc;
   if (MODE == STATE_ONLY) {
-    p = G.state + (bh * G.count + seg) * (int64_t)A.kd * A.vd;
+    p = G.state + (bh * G.count + seg) * elems;
     sr = A.vd, sc = 1;
     if (tid == 0) G.decay[bh * G.count + seg] = whole_decay;
   } else if (A.state_out && seg == G.count - 1) {
-    p = A.state_out + bh * (int64_t)A.kd * A.vd;
-    if (A.reverse && A.T > 0) {
+    p = A.state_out + bh * elems;
+    if (A.reverse) {
       const float lg = gamma_at(A, gbase), last = lg < RESET ? 0.0f : expf(lg);
-#pragma unroll
-      for (int d = 0; d < Z::DT; ++d)
-#pragma unroll
-        for (int e = 0; e < Z::ET; ++e)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) S[d][e][i] = kept(last, S[d][e][i]);
+      each([&](int d, int i, int, int) { S[d][i] = kept(last, S[d][i]); });
     }
   }
-  if (p) {
-#pragma unroll
-    for (int d = 0; d < Z::DT; ++d)
-#pragma unroll
-      for (int e = 0; e < Z::ET; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 16 * d + 4 * g + i, c = e0 + 16 * e + n;
-          if (r < A.kd && c < A.vd) p[(int64_t)r * sr + (int64_t)c * sc] = S[d][e][i];
-        }
-  }
+  if (p)
+    each([&](int d, int i, int r, int c) {
+      if (r < A.kd && c < A.vd) p[r * sr + c * sc] = S[d][i];
+    });
+}
+
+template <class T, int KD, int VD, int MODE>
+int launch_mode(const Sweep& A, const Segments& G, const Wides& W, hipStream_t s) {
+  using Z = ChunkShape<T, KD, VD>;
+  const int64_t blocks = A.B * A.H * (MODE == STATE_ONLY ? G.count - 1 : G.count);
+  if (blocks > MAX_GRID) return TTC_LQR_EINVAL;
+  const dim3 grid((unsigned)blocks), block(Z::NT);
+  if (W.in)
+    hipLaunchKernelGGL((chunk_sweep_kernel<T, KD, VD, MODE, true>), grid, block, 0, s, A, G, W);
+  else
+    hipLaunchKernelGGL((chunk_sweep_kernel<T, KD, VD, MODE, false>), grid, block, 0, s, A, G, W);
+  return launched();
 }
 
 template <class T, int KD, int VD>
 int launch_chunk(const Sweep& A, const Segments& G, const Wides& W, int mode, hipStream_t s) {
-  using Z = ChunkShape<T, KD, VD>;
-  const int64_t blocks = A.B * A.H * (mode == STATE_ONLY ? G.count - 1 : G.count);
-  if (blocks > MAX_GRID) return TTC_LQR_EINVAL;
-  const dim3 grid((unsigned)blocks), block(Z::NT);
-  if (mode == STATE_ONLY)
-    hipLaunchKernelGGL((chunk_sweep_kernel<T, KD, VD, STATE_ONLY>), grid, block, 0, s, A, G, W);
-  else if (mode == FAST || sizeof(T) == 4)  // fp32 products are exact enough as they are
-    hipLaunchKernelGGL((chunk_sweep_kernel<T, KD, VD, FAST>), grid, block, 0, s, A, G, W);
-  else
-    hipLaunchKernelGGL((chunk_sweep_kernel<T, KD, VD, sizeof(T) == 4 ? FAST : EXACT>), grid, block, 0, s, A, G, W);
-  return launched();
+  if (mode == STATE_ONLY) return launch_mode<T, KD, VD, STATE_ONLY>(A, G, W, s);
+  if (mode == FAST || sizeof(T) == 4) return launch_mode<T, KD, VD, FAST>(A, G, W, s);  // fp32 products are exact enough
+  return launch_mode<T, KD, VD, sizeof(T) == 4 ? FAST : EXACT>(A, G, W, s);
 }
 
 }  // namespace ttc
