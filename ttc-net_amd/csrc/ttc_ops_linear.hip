@@ -359,11 +359,11 @@ int run_sweep(const ttc_linear_attention_args& A, const Layout& W, const Sweep& 
   G.decay = reinterpret_cast<float*>(ws + W.seg_decay);
   const int vec = bf16 ? 8 : 4;
   auto wide = [&](const Side& x, int dim) {
-    return dim % vec == 0 && aligned16(x.p) && x.sb % vec == 0 && x.st % vec == 0 && x.sh % vec == 0 && x.st >= 0 &&
-           x.st < (1 << 22);  // a chunk's rows within 2^29 bytes of its lowest address
+    return dim % vec == 0 && aligned16(x.p) && x.sb % vec == 0 && x.st % vec == 0 && x.sh % vec == 0 &&
+           x.st >= dim && x.st < (1 << 22);  // rows that do not overlap, a chunk's within 2^30 bytes
   };
   const Wides V{wide(S.q, S.kd) && wide(S.k, S.kd) && wide(S.v, S.vd) && (!S.x.p || wide(S.x, S.vd)),
-                S.vd % 4 == 0 && aligned16(S.out)};
+                S.vd % 4 == 0 && aligned16(S.out) && (int64_t)S.H * S.vd < (1 << 22)};
   auto launch = [&](int mode) {
     if (bf16)
       return S.kd <= 32   ? launch_chunk_kd32<__bf16>(S, G, V, mode, s)

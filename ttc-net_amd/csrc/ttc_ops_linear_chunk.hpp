@@ -180,12 +180,11 @@ __device__ __forceinline__ u32x4 load_any(const T* p, int c, int dim) {
   return r;
 }
 
-// A chunk's rows of one input, for loads that give 0 past the bound instead of branching: all loads of a chunk are in
-// flight at once.  Offsets from the chunk's lowest address are below 2^30 bytes (the host sees to it).
+// `bytes` from p on, for loads that give 0 and stores that do nothing past the bound instead of branching: all loads of a
+// chunk are in flight at once.  A chunk's offsets are below 2^30 bytes (the host sees to it).
 constexpr int BEYOND = 0x7ffffff0;
-template <class T>
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const T* p) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, 1 << 30, 0x00027000);
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t bounded(const void* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00027000);
 }
 
 // WIDE: rows of 16-byte multiples at 16-byte addresses
@@ -204,7 +203,7 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
   __shared__ float Whole[2], Dot[DOTS ? Z::WAVES : 1][C];
   __shared__ int Odd[Z::WAVES];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, n = lane & 15;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, n = lane & 15;
   const int segs = MODE == STATE_ONLY ? G.count - 1 : G.count;  // the last one's own contribution is not needed
   const int seg = (int)(blockIdx.x % segs);
   const int64_t bh = blockIdx.x / segs, b = bh / A.H, elems = (int64_t)A.kd * A.vd;
@@ -216,7 +215,11 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
   const int64_t places = (A.T + C - 1) / C * C, u0 = seg * G.chunks * C;
   const int64_t u1 = u0 + G.chunks * C < places ? u0 + G.chunks * C : places;
   const int e0 = wave * 16;  // the wave's columns
-  auto token = [&](int64_t u) { return A.reverse ? places - 1 - u : u; };  // >= T: none
+  // A chunk holds tokens low .. low + left - 1 (left <= C: the last ones may be missing); the sweep's row r is its token
+  // place(r)
+  auto low_of = [&](int64_t at) { return A.reverse ? places - C - at : at; };
+  auto left_of = [&](int64_t at) { return (int)(A.T - low_of(at) < C ? A.T - low_of(at) : C); };
+  auto place = [&](int r) { return A.reverse ? C - 1 - r : r; };
 
   // S: lane's rows 16 d + 4 g + i, column e0 + n.  The lane's place is hidden from the compiler, which would otherwise keep
   // 32 addresses in registers over the whole loop.
@@ -256,34 +259,52 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
   if (DOTS && A.joins && A.reverse && seg == 0 && A.last) meet(A.last + bh * elems, A.sr, A.sc, 1.0f, A.marks);
 
   u32x4 qr[Z::KV], kr[Z::KV], vr[Z::VV];
-  auto fetch_side = [&](const T* p, int64_t st, int dim, int64_t at, auto& r, auto width) {
+  int ko[Z::KV], qo[Z::KV], vo[Z::VV];  // offsets of this thread's 16 bytes from the chunk's lowest address
+  auto offsets = [&](int64_t st, int dim, auto& o, auto width) {
     constexpr int D = decltype(width)::value;
-    const auto rows = rows_of(p + (A.reverse ? token(at + C - 1) : at) * st);
+#pragma unroll
+    for (int j = 0; j < (int)(sizeof(o) / sizeof(o[0])); ++j) {
+      const int i = tid + j * NT, row = i / (D / VEC), c = i % (D / VEC) * VEC;
+      o[j] = row < C && c < dim ? (place(row) * (int)st + c) * (int)sizeof(T) : BEYOND;
+    }
+  };
+  if constexpr (WIDE) {
+    offsets(A.k.st, A.kd, ko, std::integral_constant<int, KD>{});
+    if constexpr (MODE != STATE_ONLY) offsets(A.q.st, A.kd, qo, std::integral_constant<int, KD>{});
+    offsets(A.v.st, A.vd, vo, std::integral_constant<int, VD>{});
+  }
+  auto fetch_side = [&](const T* p, int64_t st, int dim, int64_t at, auto& r, const auto& o, auto width) {
+    constexpr int D = decltype(width)::value;
+    const T* from = p + low_of(at) * st;
+    const int left = left_of(at);
+    const auto rows = bounded(from, left * (int)st * (int)sizeof(T));  // rows do not overlap: st >= dim
 #pragma unroll
     for (int j = 0; j < (int)(sizeof(r) / sizeof(r[0])); ++j) {
-      const int i = tid + j * NT, row = i / (D / VEC), c = i % (D / VEC) * VEC;
-      const bool in = row < C && token(at + row) < A.T;
       if constexpr (WIDE) {
-        const int off = (A.reverse ? C - 1 - row : row) * (int)(st * (int)sizeof(T)) + c * (int)sizeof(T);
-        r[j] = __builtin_amdgcn_raw_buffer_load_b128(rows, in && c < dim ? off : BEYOND, 0, 0);
+        r[j] = __builtin_amdgcn_raw_buffer_load_b128(rows, o[j], 0, 0);
       } else {
+        const int i = tid + j * NT, row = i / (D / VEC), c = i % (D / VEC) * VEC;
         const u32x4 zero = {0, 0, 0, 0};
-        r[j] = in ? load_any(p + token(at + row) * st, c, dim) : zero;
+        r[j] = row < C && place(row) < left ? load_any(from + place(row) * st, c, dim) : zero;
       }
     }
   };
   auto fetch = [&](int64_t at) {
-    fetch_side(k, A.k.st, A.kd, at, kr, std::integral_constant<int, KD>{});
-    if constexpr (MODE != STATE_ONLY) fetch_side(q, A.q.st, A.kd, at, qr, std::integral_constant<int, KD>{});
-    fetch_side(v, A.v.st, A.vd, at, vr, std::integral_constant<int, VD>{});
+    fetch_side(k, A.k.st, A.kd, at, kr, ko, std::integral_constant<int, KD>{});
+    if constexpr (MODE != STATE_ONLY) fetch_side(q, A.q.st, A.kd, at, qr, qo, std::integral_constant<int, KD>{});
+    fetch_side(v, A.v.st, A.vd, at, vr, vo, std::integral_constant<int, VD>{});
   };
-  // wave 0: the chunk's decays; before a token in reverse order, that of the one after it
-  auto gate_of = [&](int64_t u) {
-    const int64_t t = token(u) + (A.reverse ? 1 : 0);
-    return lane < C && t < A.T ? gamma_at(A, gbase + t * A.gt) : 0.0f;
+  // One wave: a chunk's decays, one a lane (before a token in reverse order, that of the one after it), as they are stored
+  constexpr int GATES = Z::WAVES - 1;
+  auto gate_bits = [&](int64_t at) {
+    const int r = place(lane) + (A.reverse ? 1 : 0);
+    const int64_t t = low_of(at) + r;
+    if (lane >= C || at >= u1 || t >= A.T) return 0u;
+    const int64_t i = gbase + t * A.gt;
+    return A.gamma_bf16 ? (uint32_t) static_cast<const uint16_t*>(A.gamma)[i] : static_cast<const uint32_t*>(A.gamma)[i];
   };
-  auto gates = [&](float lg, int buf) {
-    double y = (double)lg * 1.4426950408889634;
+  auto gates = [&](uint32_t bits, int buf) {
+    double y = (double)__uint_as_float(A.gamma_bf16 ? bits << 16 : bits) * 1.4426950408889634;
     y = y < -4096.0 ? -4096.0 : y;
 #pragma unroll
     for (int m = 1; m < C; m <<= 1) {
@@ -303,17 +324,21 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
   };
   auto put_dots = [&](int64_t at) {  // after the barrier behind the chunk
     if constexpr (DOTS) {
-      if (x && tid < C && token(at + tid) < A.T) {
+      if (x && tid < C && place(tid) < left_of(at)) {
         float d = 0.0f;
 #pragma unroll
         for (int w = 0; w < Z::WAVES; ++w) d += Dot[w][tid];
-        A.dots[bh * A.T + token(at + tid)] = d;
+        A.dots[bh * A.T + low_of(at) + place(tid)] = d;
       }
     }
   };
 
   fetch(u0);
-  if (wave == 0) gates(gate_of(u0 + lane), 0);
+  uint32_t gate = 0;
+  if (wave == GATES) {
+    gates(gate_bits(u0), 0);
+    gate = gate_bits(u0 + C);
+  }
   float whole_decay = 1.0f;
   int buf = 0;
   for (int64_t at = u0; at < u1; at += C, buf ^= 1) {
@@ -339,25 +364,30 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
 #pragma unroll
     for (int w = 0; w < Z::WAVES; ++w) odd = odd || Odd[w];
     if (at + C < u1) fetch(at + C);
-    const float next_gate = wave == 0 && at + C < u1 ? gate_of(at + C + lane) : 0.0f;
     const float whole = Whole[buf];
+    const int64_t low = low_of(at);
+    const int left = left_of(at);
+    if (wave == GATES && at + C < u1) {
+      gates(gate, buf ^ 1);
+      gate = gate_bits(at + 2 * C);
+    }
     struct alignas(4 * sizeof(T)) Four { T v[4]; };
     Four xs[DOTS ? Z::TT : 1];
     if constexpr (DOTS) {
       if (x) {
 #pragma unroll
         for (int t = 0; t < Z::TT; ++t) {
-          const int64_t tok = token(at + 16 * t + n);
-          const int c = e0 + 4 * g;
+          const int r = place(16 * t + n), c = e0 + 4 * g;
+          const T* p = x + (low + r) * A.x.st;
 #pragma unroll
           for (int i = 0; i < 4; ++i) xs[t].v[i] = from_f<T>(0.0f);
-          if (tok < A.T) {
+          if (r < left) {
             if (WIDE) {
-              if (c < A.vd) xs[t] = *reinterpret_cast<const Four*>(x + tok * A.x.st + c);
+              if (c < A.vd) xs[t] = *reinterpret_cast<const Four*>(p + c);
             } else {
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                if (c + i < A.vd) xs[t].v[i] = x[tok * A.x.st + c + i];
+                if (c + i < A.vd) xs[t].v[i] = p[c + i];
             }
           }
         }
@@ -458,28 +488,34 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
       }
       // out: a lane holds 4 neighbouring columns of one token
       const int c = e0 + 4 * g;
+      const int64_t first = ((b * A.T + low) * A.H + h) * A.vd;
+      auto put = [&](auto* y, int r, const f32x4& o) {
+        using Y = std::remove_pointer_t<decltype(y)>;
+        const int row = A.H * A.vd;
+        Y f[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = from_f<Y>(o[i]);
+        if (W.out) {
+          const auto rows = bounded(y + first, ((left - 1) * row + A.vd) * (int)sizeof(Y));
+          const int off = c < A.vd ? (r * row + c) * (int)sizeof(Y) : BEYOND;
+          if constexpr (sizeof(Y) == 4)
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f), rows, off, 0, 0);
+          else
+            __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f), rows, off, 0, 0);
+        } else if (r < left) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (c + i < A.vd) y[first + (int64_t)r * row + c + i] = f[i];
+        }
+      };
 #pragma unroll
       for (int t = 0; t < Z::TT; ++t) {
-        const int64_t tok = token(at + 16 * t + n), o = ((b * A.T + tok) * A.H + h) * A.vd + c;
         f32x4 r = O[t];
 #pragma unroll
         for (int i = 0; i < 4; ++i) r[i] *= A.out_scale;
-        if (tok < A.T && A.out != nullptr) {
-          auto put = [&](auto* y) {
-            using Y = std::remove_pointer_t<decltype(y)>;
-            struct alignas(4 * sizeof(Y)) Columns { Y v[4]; };
-            Columns f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) f.v[i] = from_f<Y>(r[i]);
-            if (W.out) {
-              if (c < A.vd) *reinterpret_cast<Columns*>(y + o) = f;
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (c + i < A.vd) y[o + i] = f.v[i];
-            }
-          };
-          if (A.out_f32) put(static_cast<float*>(A.out)); else put(static_cast<T*>(A.out));
+        if (A.out != nullptr) {
+          if (A.out_f32) put(static_cast<float*>(A.out), place(16 * t + n), r);
+          else put(static_cast<T*>(A.out), place(16 * t + n), r);
         }
         if constexpr (DOTS) {
           if (x) {
@@ -522,13 +558,12 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
       }
     }
     if (DOTS && A.joins && A.reverse) {  // a boundary in front of token t: its decay's gradient
-      const int64_t t = token(at + C - 1);
+      const int64_t t = low;
       if (t > 0 && t % A.mark_tokens == 0) {
         const float lg = gamma_at(A, gbase + t * A.gt);
         meet(A.states + (bh * A.marks + t / A.mark_tokens) * elems, A.vd, 1, lg < RESET ? 0.0f : expf(lg), t / A.mark_tokens);
       }
     }
-    if (wave == 0 && at + C < u1) gates(next_gate, buf ^ 1);
     __syncthreads();
   }
   put_dots(u1 - C);
