@@ -131,12 +131,20 @@ __global__ __launch_bounds__(256) void segment_join_kernel(Sweep A, Segments G, 
   float run = A.state_in ? A.state_in[bh * elems + i / A.vd * A.sr + i % A.vd * A.sc] : 0.0f;
   float* p = G.state + bh * G.count * elems + i;
   const float* w = G.decay + bh * G.count;
-  for (int j = 0; j + 1 < G.count; ++j) {
-    const float own = p[j * elems];
-    p[j * elems] = run;
-    run = w[j] == 0.0f ? own : fmaf(w[j], run, own);
+  constexpr int AHEAD = 8;  // contributions in flight
+  for (int j = 0; j < G.count; j += AHEAD) {
+    float own[AHEAD], decay[AHEAD];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      own[a] = j + a + 1 < G.count ? p[(j + a) * elems] : 0.0f;
+      decay[a] = j + a + 1 < G.count ? w[j + a] : 0.0f;
+    }
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      if (j + a < G.count) p[(j + a) * elems] = run;
+      run = decay[a] == 0.0f ? own[a] : fmaf(decay[a], run, own[a]);
+    }
   }
-  p[(G.count - 1) * elems] = run;
 }
 
 // Gradients of shared heads: out [rows, heads / share, d] = sums over `share` heads of in [rows, heads, d]
@@ -481,7 +489,7 @@ extern "C" int ttc_linear_attention(const ttc_linear_attention_args* args, void*
     S = sweep_of(A);
     S.mark_tokens = W.mark_tokens, S.marks = W.marks;
     S.joins = A.tokens > TOKEN_SWEEP ? space(W.joins) : nullptr;
-    const int waves = dk <= 32 ? 2 : dk <= 64 ? 4 : 8;  // of the sweep of dk
+    const int waves = sweep_waves(dk);  // of the sweep of dk
     double* per_head = A.gamma_per_head ? reinterpret_cast<double*>(space(W.per_head)) : nullptr;
     if (stretches > 0)
       hipLaunchKernelGGL(gate_kernel, dim3((unsigned)stretches), dim3(64), 0, s, S, space(W.r), space(W.c), W.dot_tiles,

@@ -29,7 +29,8 @@ using i16x4 = __attribute__((ext_vector_type(4))) short;
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 using u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
 
-// ---- operands: 8 values a lane, row or column lane % 16, contraction index 8 (lane / 16) + j ------------------
+// ---- operands: 8 values a lane, row or column lane % 16; which of the 32 contracted indices a lane holds is free as long
+// as both sides agree: 8 g + j (row), or 4 g + j and 16 + 4 g + j (row_split, column, accumulators), g = lane / 16
 
 template <class T>
 struct Operand;
@@ -40,7 +41,8 @@ struct Operand<__bf16> {
   struct Wide {  // a value as the exact sum of three bf16 numbers
     Frag h, m, l;
   };
-  static constexpr int CHUNK = 64, PAD = 8;  // chunk_tokens()
+  // rows read along them: 4 banks apart (mod 32); rows read across them, 8 rows at once, 8 banks apart
+  static constexpr int ROW_PAD = 8, COL_PAD = 16;
   static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
@@ -56,14 +58,14 @@ struct Operand<__bf16> {
     const bf16x4 a = *reinterpret_cast<const bf16x4*>(p), b = *reinterpret_cast<const bf16x4*>(p + 16);
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
-  // column col0 + lane % 16, rows 8 (lane / 16) .. + 7 of the 32 from p's row on.  A transposing read gives each lane of 16
-  // one column of 4 rows, whose 16 columns lie in 4 lanes' 8 bytes a row.
+  // column col0 + lane % 16, rows 4 g .. + 3 and 16 + 4 g .. + 3 of the 32 from p's row on (g = lane / 16).  A transposing
+  // read gives each lane of 16 one column of 4 rows, whose 16 columns lie in 4 lanes' 8 bytes a row.
   static __device__ __forceinline__ Frag column(const __bf16* p, int stride, int col0, int lane) {
     const int g = lane >> 4, i = lane & 15;
-    const __bf16* a = p + (8 * g + (i >> 2)) * stride + col0 + (i & 3) * 4;
+    const __bf16* a = p + (4 * g + (i >> 2)) * stride + col0 + (i & 3) * 4;
     typedef __attribute__((address_space(3))) i16x4 lds;
     const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)(a));
-    const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)(a + 4 * stride));
+    const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)(a + 16 * stride));
     return __builtin_bit_cast(Frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
   }
   static __device__ __forceinline__ Frag narrow(const float (&x)[8]) {
@@ -116,7 +118,7 @@ struct Operand<float> {
     float v[8];
   };
   using Wide = Frag;
-  static constexpr int CHUNK = 32, PAD = 4;  // chunk_tokens()
+  static constexpr int ROW_PAD = 4, COL_PAD = 4;
   static __device__ __forceinline__ f32x4 mma(const Frag& a, const Frag& b, f32x4 c) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j], b.v[j], c, 0, 0, 0);
@@ -129,10 +131,10 @@ struct Operand<float> {
   static __device__ __forceinline__ Frag row(const float* p) { return two(p, p + 4); }
   static __device__ __forceinline__ Frag row_split(const float* p) { return two(p, p + 16); }
   static __device__ __forceinline__ Frag column(const float* p, int stride, int col0, int lane) {
-    const float* a = p + 8 * (lane >> 4) * stride + col0 + (lane & 15);
+    const float* a = p + 4 * (lane >> 4) * stride + col0 + (lane & 15);
     Frag r;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) r.v[j] = a[j * stride];
+    for (int j = 0; j < 8; ++j) r.v[j] = a[(j < 4 ? j : 12 + j) * stride];
     return r;
   }
   static __device__ __forceinline__ Frag narrow(const float (&x)[8]) { return wide(x); }
@@ -162,9 +164,10 @@ __device__ __forceinline__ float kept(float w, float x) { return w == 0.0f ? 0.0
 
 template <class T, int KD, int VD>
 struct ChunkShape {
-  static constexpr int WAVES = VD / 16, NT = WAVES * 64;  // at most MAX_WAVES; a wave's 16 columns: 32 registers of state for 128 rows
-  static constexpr int C = Operand<T>::CHUNK, TT = C / 16, KB = C / 32, DB = KD / 32, DT = KD / 16;
-  static constexpr int VEC = 16 / sizeof(T), QS = KD + Operand<T>::PAD, VS = VD + Operand<T>::PAD;
+  static constexpr int WAVES = sweep_waves(VD), NT = WAVES * 64, ET = VD / 16 / WAVES;  // a wave's columns: 16 ET
+  static constexpr int C = chunk_tokens(sizeof(T) == 2), TT = C / 16, KB = C / 32, DB = KD / 32, DT = KD / 16;
+  static constexpr int VEC = 16 / sizeof(T), QS = KD + Operand<T>::ROW_PAD, KS = KD + Operand<T>::COL_PAD,
+                       VS = VD + Operand<T>::COL_PAD;
   static constexpr int KV = (C * KD / VEC + NT - 1) / NT, VV = (C * VD / VEC + NT - 1) / NT;  // 16-byte loads a thread
 };
 
@@ -194,16 +197,18 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
   using Op = Operand<T>;
   using PT = std::conditional_t<MODE == EXACT, float, T>;  // the weighted scores in shared memory
   constexpr bool DOTS = MODE == EXACT || (MODE == FAST && sizeof(T) == 4);
-  constexpr int C = Z::C, NT = Z::NT, VEC = Z::VEC, QS = Z::QS, VS = Z::VS, PS = C + 16 / (int)sizeof(PT);
+  constexpr int C = Z::C, NT = Z::NT, VEC = Z::VEC, QS = Z::QS, KS = Z::KS, VS = Z::VS, PS = C + 16 / (int)sizeof(PT);
   __shared__ __attribute__((aligned(16))) T Qs[MODE == STATE_ONLY ? 1 : C * QS];
-  __shared__ __attribute__((aligned(16))) T Ks[C * QS];
+  __shared__ __attribute__((aligned(16))) T Ks[C * KS];
   __shared__ __attribute__((aligned(16))) T Vs[C * VS];
   __shared__ __attribute__((aligned(16))) PT Ps[MODE == STATE_ONLY ? 1 : C * PS];
   __shared__ __attribute__((aligned(16))) float Hi[2][C], Lo[2][C], In[2][C], Up[2][C];
   __shared__ float Whole[2], Dot[DOTS ? Z::WAVES : 1][C];
   __shared__ int Odd[Z::WAVES];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, n = lane & 15;
+  int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int lane = tid & 63, g = lane >> 4, n = lane & 15;
   const int segs = MODE == STATE_ONLY ? G.count - 1 : G.count;  // the last one's own contribution is not needed
   const int seg = (int)(blockIdx.x % segs);
   const int64_t bh = blockIdx.x / segs, b = bh / A.H, elems = (int64_t)A.kd * A.vd;
@@ -214,24 +219,26 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
   // Places in the sweep's order: whole chunks, whose boundaries lie between the same tokens in both orders
   const int64_t places = (A.T + C - 1) / C * C, u0 = seg * G.chunks * C;
   const int64_t u1 = u0 + G.chunks * C < places ? u0 + G.chunks * C : places;
-  const int e0 = wave * 16;  // the wave's columns
+  const int e0 = wave * 16 * Z::ET;  // the wave's columns
   // A chunk holds tokens low .. low + left - 1 (left <= C: the last ones may be missing); the sweep's row r is its token
   // place(r)
   auto low_of = [&](int64_t at) { return A.reverse ? places - C - at : at; };
   auto left_of = [&](int64_t at) { return (int)(A.T - low_of(at) < C ? A.T - low_of(at) : C); };
   auto place = [&](int r) { return A.reverse ? C - 1 - r : r; };
 
-  // S: lane's rows 16 d + 4 g + i, column e0 + n.  The lane's place is hidden from the compiler, which would otherwise keep
+  // S: lane's rows 16 d + 4 g + i, columns e0 + 16 e + n.  The lane's place is hidden from the compiler, which would otherwise keep
   // 32 addresses in registers over the whole loop.
+  f32x4 S[Z::DT][Z::ET];
   auto each = [&](auto f) {
     int r = 4 * g, c = e0 + n;
     asm volatile("" : "+v"(r), "+v"(c));
 #pragma unroll
     for (int d = 0; d < Z::DT; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f(d, i, 16 * d + r + i, c);
+      for (int e = 0; e < Z::ET; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) S[d][e][i] = f((float)S[d][e][i], 16 * d + r + i, c + 16 * e);
   };
-  f32x4 S[Z::DT];
   {
     const float* p = nullptr;
     int sr = A.sr, sc = A.sc;
@@ -243,15 +250,14 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
         p = A.state_in + bh * elems;
       }
     }
-    each([&](int d, int i, int r, int c) {
-      S[d][i] = p && r < A.kd && c < A.vd ? p[r * sr + c * sc] : 0.0f;
-    });
+    each([&](float, int r, int c) { return p && r < A.kd && c < A.vd ? p[r * sr + c * sc] : 0.0f; });
   }
   // <S, p>, the wave's part of it: the decays' gradient at a boundary
   auto meet = [&](const float* p, int sr, int sc, float w, int64_t mark) {
     float d = 0.0f;
-    each([&](int dt, int i, int r, int c) {
-      if (r < A.kd && c < A.vd) d = fmaf(S[dt][i], p[r * sr + c * sc], d);
+    each([&](float s, int r, int c) {
+      if (r < A.kd && c < A.vd) d = fmaf(s, p[r * sr + c * sc], d);
+      return s;
     });
     d = lane_sum(d, 64);
     if (lane == 0) A.joins[(bh * (A.marks + 1) + mark) * MAX_WAVES + wave] = kept(w, d);
@@ -317,7 +323,7 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
       Hi[buf][lane] = hi;
       Lo[buf][lane] = lo;
       const float in = exp2_of(hi) * exp2_of(lo);
-      In[buf][lane] = in;
+      In[buf][lane] = in * A.out_scale;
       Up[buf][lane] = exp2_of(uh) * exp2_of(ul) * A.key_scale;
       if (lane == C - 1) Whole[buf] = in;
     }
@@ -342,6 +348,10 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
   float whole_decay = 1.0f;
   int buf = 0;
   for (int64_t at = u0; at < u1; at += C, buf ^= 1) {
+    // Addresses follow from the lane: hidden from the compiler, which would otherwise keep some 70 of them in registers
+    // over the whole loop and spill
+    asm volatile("" : "+v"(lane), "+v"(tid));
+    g = lane >> 4, n = lane & 15;
     // the chunk's tokens to shared memory, and whether all keys and values are finite
     uint32_t most = 0;
     auto stage = [&](T* to, int stride, auto& r, auto width, bool look) {
@@ -353,7 +363,7 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
         if (C * D / VEC % NT == 0 || row < C) *reinterpret_cast<u32x4*>(&to[row * stride + c]) = r[j];
       }
     };
-    stage(Ks, QS, kr, std::integral_constant<int, KD>{}, true);
+    stage(Ks, KS, kr, std::integral_constant<int, KD>{}, true);
     if constexpr (MODE != STATE_ONLY) stage(Qs, QS, qr, std::integral_constant<int, KD>{}, false);
     stage(Vs, VS, vr, std::integral_constant<int, VD>{}, true);
     const bool odd_here = __ballot(!Op::finite(most)) != 0;
@@ -364,7 +374,7 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
 #pragma unroll
     for (int w = 0; w < Z::WAVES; ++w) odd = odd || Odd[w];
     if (at + C < u1) fetch(at + C);
-    const float whole = Whole[buf];
+    const float whole = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(Whole[buf])));
     const int64_t low = low_of(at);
     const int left = left_of(at);
     if (wave == GATES && at + C < u1) {
@@ -372,35 +382,40 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
       gate = gate_bits(at + 2 * C);
     }
     struct alignas(4 * sizeof(T)) Four { T v[4]; };
-    Four xs[DOTS ? Z::TT : 1];
+    Four xs[DOTS ? Z::TT : 1][Z::ET];
     if constexpr (DOTS) {
       if (x) {
 #pragma unroll
         for (int t = 0; t < Z::TT; ++t) {
-          const int r = place(16 * t + n), c = e0 + 4 * g;
+          const int r = place(16 * t + n);
           const T* p = x + (low + r) * A.x.st;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) xs[t].v[i] = from_f<T>(0.0f);
-          if (r < left) {
-            if (WIDE) {
-              if (c < A.vd) xs[t] = *reinterpret_cast<const Four*>(p + c);
-            } else {
+          for (int e = 0; e < Z::ET; ++e) {
+            const int c = e0 + 16 * e + 4 * g;
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (c + i < A.vd) xs[t].v[i] = p[c + i];
+            for (int i = 0; i < 4; ++i) xs[t][e].v[i] = from_f<T>(0.0f);
+            if (r < left) {
+              if (WIDE) {
+                if (c < A.vd) xs[t][e] = *reinterpret_cast<const Four*>(p + c);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if (c + i < A.vd) xs[t][e].v[i] = p[c + i];
+              }
             }
           }
         }
       }
       if (A.states && !A.reverse && at > 0 && at % A.mark_tokens == 0) {  // the state in front of a boundary
         float* p = A.states + (bh * A.marks + at / A.mark_tokens) * elems;
-        each([&](int d, int i, int r, int c) {
-          if (r < A.kd && c < A.vd) p[r * A.vd + c] = S[d][i];
+        each([&](float s, int r, int c) {
+          if (r < A.kd && c < A.vd) p[r * A.vd + c] = s;
+          return s;
         });
       }
     }
 
-    f32x4 O[Z::TT];
+    f32x4 O[Z::TT][Z::ET];
     if constexpr (MODE != STATE_ONLY) {
       // scores, tile by tile over the waves: (ti, si <= ti), and zeros where a later product's 32 tokens reach past ti
       int turn = 0;
@@ -413,14 +428,14 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
           if (si <= ti) {
 #pragma unroll
             for (int d = 0; d < Z::DB; ++d)
-              p = Op::mma(Op::row(&Ks[(16 * si + n) * QS + 32 * d + 8 * g]), Op::row(&Qs[(16 * ti + n) * QS + 32 * d + 8 * g]),
+              p = Op::mma(Op::row(&Ks[(16 * si + n) * KS + 32 * d + 8 * g]), Op::row(&Qs[(16 * ti + n) * QS + 32 * d + 8 * g]),
                           p);
             const float th = Hi[buf][16 * ti + n], tl = Lo[buf][16 * ti + n];
             const f32x4 sh = *reinterpret_cast<const f32x4*>(&Hi[buf][16 * si + 4 * g]),
                         sl = *reinterpret_cast<const f32x4*>(&Lo[buf][16 * si + 4 * g]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float w = exp2_of((th - sh[i]) + (tl - sl[i])) * A.key_scale;
+              const float w = exp2_of((th - sh[i]) + (tl - sl[i])) * (A.key_scale * A.out_scale);
               p[i] = si < ti || 4 * g + i <= n ? kept(w, p[i]) : 0.0f;
             }
           }
@@ -432,31 +447,47 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
         }
       // the state's part
 #pragma unroll
-      for (int t = 0; t < Z::TT; ++t) O[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < Z::TT; ++t)
+#pragma unroll
+        for (int e = 0; e < Z::ET; ++e) O[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int d = 0; d < Z::DB; ++d) {
-        float y[8];
+        std::conditional_t<MODE == EXACT, typename Op::Wide, typename Op::Frag> s[Z::ET];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = S[2 * d][i], y[4 + i] = S[2 * d + 1][i];
-        auto by = [&](const auto& s) {
+        for (int e = 0; e < Z::ET; ++e) {
+          float y[8];
 #pragma unroll
-          for (int t = 0; t < Z::TT; ++t)
-            O[t] = Op::mma(s, Op::row_split(&Qs[(16 * t + n) * QS + 32 * d + 4 * g]), O[t]);
-        };
-        if constexpr (MODE == EXACT) by(Op::wide(y)); else by(Op::narrow(y));
+          for (int i = 0; i < 4; ++i) y[i] = S[2 * d][e][i], y[4 + i] = S[2 * d + 1][e][i];
+          if constexpr (MODE == EXACT) s[e] = Op::wide(y); else s[e] = Op::narrow(y);
+        }
+#pragma unroll
+        for (int t = 0; t < Z::TT; ++t) {
+          const typename Op::Frag f = Op::row_split(&Qs[(16 * t + n) * QS + 32 * d + 4 * g]);
+#pragma unroll
+          for (int e = 0; e < Z::ET; ++e) O[t][e] = Op::mma(s[e], f, O[t][e]);
+        }
       }
 #pragma unroll
       for (int t = 0; t < Z::TT; ++t) {
         const float w = In[buf][16 * t + n];
+        if (__ballot(w == 0.0f) == 0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) O[t][i] = kept(w, O[t][i]);
+          for (int e = 0; e < Z::ET; ++e) O[t][e] *= w;
+        } else {
+#pragma unroll
+          for (int e = 0; e < Z::ET; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) O[t][e][i] = kept(w, O[t][e][i]);
+        }
       }
       __syncthreads();
     }
 
-    typename Op::Frag vf[Z::KB];
+    typename Op::Frag vf[Z::KB][Z::ET];
 #pragma unroll
-    for (int s = 0; s < Z::KB; ++s) vf[s] = Op::column(&Vs[32 * s * VS], VS, e0, lane);
+    for (int s = 0; s < Z::KB; ++s)
+#pragma unroll
+      for (int e = 0; e < Z::ET; ++e) vf[s][e] = Op::column(&Vs[32 * s * VS], VS, e0 + 16 * e, lane);
 
     if constexpr (MODE != STATE_ONLY) {
       if (!odd) {
@@ -464,13 +495,17 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
         for (int t = 0; t < Z::TT; ++t)
 #pragma unroll
           for (int s = 0; s <= t / 2; ++s) {
-            const PT* p = &Ps[(16 * t + n) * PS + 32 * s + 8 * g];
+            const PT* p = &Ps[(16 * t + n) * PS + 32 * s + 4 * g];
+            auto by = [&](const auto& f) {
+#pragma unroll
+              for (int e = 0; e < Z::ET; ++e) O[t][e] = Op::mma(vf[s][e], f, O[t][e]);
+            };
             if constexpr (MODE == EXACT) {
               float y[8];
-              Operand<float>::values(Operand<float>::row(p), y);
-              O[t] = Op::mma(vf[s], Op::wide(y), O[t]);
+              Operand<float>::values(Operand<float>::row_split(p), y);
+              by(Op::wide(y));
             } else {
-              O[t] = Op::mma(vf[s], Op::row(p), O[t]);
+              by(Op::row_split(p));
             }
           }
       } else {
@@ -482,14 +517,15 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
             if (s > tt || w == 0.0f) continue;
             const float p = to_f(Ps[tt * PS + s]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) O[t][i] = fmaf(p, to_f(Vs[s * VS + e0 + 4 * g + i]), O[t][i]);
+            for (int e = 0; e < Z::ET; ++e)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) O[t][e][i] = fmaf(p, to_f(Vs[s * VS + e0 + 16 * e + 4 * g + i]), O[t][e][i]);
           }
         }
       }
       // out: a lane holds 4 neighbouring columns of one token
-      const int c = e0 + 4 * g;
       const int64_t first = ((b * A.T + low) * A.H + h) * A.vd;
-      auto put = [&](auto* y, int r, const f32x4& o) {
+      auto put = [&](auto* y, int r, int c, const f32x4& o) {
         using Y = std::remove_pointer_t<decltype(y)>;
         const int row = A.H * A.vd;
         Y f[4];
@@ -510,18 +546,24 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
       };
 #pragma unroll
       for (int t = 0; t < Z::TT; ++t) {
-        f32x4 r = O[t];
+        float dot = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] *= A.out_scale;
-        if (A.out != nullptr) {
-          if (A.out_f32) put(static_cast<float*>(A.out), place(16 * t + n), r);
-          else put(static_cast<T*>(A.out), place(16 * t + n), r);
+        for (int e = 0; e < Z::ET; ++e) {
+          const int c = e0 + 16 * e + 4 * g;
+          const f32x4 r = O[t][e];
+          if (A.out != nullptr) {
+            if (A.out_f32) put(static_cast<float*>(A.out), place(16 * t + n), c, r);
+            else put(static_cast<T*>(A.out), place(16 * t + n), c, r);
+          }
+          if constexpr (DOTS) {
+            if (x) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) dot = fmaf(r[i], to_f(xs[t][e].v[i]), dot);
+            }
+          }
         }
         if constexpr (DOTS) {
           if (x) {
-            float dot = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) dot = fmaf(r[i], to_f(xs[t].v[i]), dot);
             dot += __shfl_xor(dot, 16, 64);
             dot += __shfl_xor(dot, 32, 64);
             if (g == 0) Dot[wave][16 * t + n] = dot;
@@ -534,27 +576,34 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
 #pragma unroll
     for (int d = 0; d < Z::DT; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) S[d][i] = kept(whole, S[d][i]);
+      for (int e = 0; e < Z::ET; ++e) S[d][e] = whole == 0.0f ? f32x4{0.f, 0.f, 0.f, 0.f} : S[d][e] * whole;
     whole_decay *= whole;
     if (!odd) {
 #pragma unroll
       for (int s = 0; s < Z::KB; ++s) {
-        const f32x4 wa = *reinterpret_cast<const f32x4*>(&Up[buf][32 * s + 8 * g]),
-                    wb = *reinterpret_cast<const f32x4*>(&Up[buf][32 * s + 8 * g + 4]);
-        float y[8];
-        Op::values(vf[s], y);
+        const f32x4 wa = *reinterpret_cast<const f32x4*>(&Up[buf][32 * s + 4 * g]),
+                    wb = *reinterpret_cast<const f32x4*>(&Up[buf][32 * s + 16 + 4 * g]);
+        typename Op::Wide wv[Z::ET];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] *= j < 4 ? wa[j] : wb[j - 4];
-        const typename Op::Wide wv = Op::wide(y);
+        for (int e = 0; e < Z::ET; ++e) {
+          float y[8];
+          Op::values(vf[s][e], y);
 #pragma unroll
-        for (int d = 0; d < Z::DT; ++d) S[d] = Op::mma(Op::column(&Ks[32 * s * QS], QS, 16 * d, lane), wv, S[d]);
+          for (int j = 0; j < 8; ++j) y[j] *= j < 4 ? wa[j] : wb[j - 4];
+          wv[e] = Op::wide(y);
+        }
+#pragma unroll
+        for (int d = 0; d < Z::DT; ++d) {
+          const typename Op::Frag f = Op::column(&Ks[32 * s * KS], KS, 16 * d, lane);
+#pragma unroll
+          for (int e = 0; e < Z::ET; ++e) S[d][e] = Op::mma(f, wv[e], S[d][e]);
+        }
       }
     } else {
       for (int s = 0; s < C; ++s) {
         const float w = Up[buf][s];
         if (w == 0.0f) continue;
-        const float y = w * to_f(Vs[s * VS + e0 + n]);
-        each([&](int d, int i, int r, int) { S[d][i] = fmaf(to_f(Ks[s * QS + r]), y, S[d][i]); });
+        each([&](float o, int r, int c) { return fmaf(to_f(Ks[s * KS + r]), w * to_f(Vs[s * VS + c]), o); });
       }
     }
     if (DOTS && A.joins && A.reverse) {  // a boundary in front of token t: its decay's gradient
@@ -578,12 +627,13 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
     p = A.state_out + bh * elems;
     if (A.reverse) {
       const float lg = gamma_at(A, gbase), last = lg < RESET ? 0.0f : expf(lg);
-      each([&](int d, int i, int, int) { S[d][i] = kept(last, S[d][i]); });
+      each([&](float s, int, int) { return kept(last, s); });
     }
   }
   if (p)
-    each([&](int d, int i, int r, int c) {
-      if (r < A.kd && c < A.vd) p[r * sr + c * sc] = S[d][i];
+    each([&](float s, int r, int c) {
+      if (r < A.kd && c < A.vd) p[r * sr + c * sc] = s;
+      return s;
     });
 }
 
