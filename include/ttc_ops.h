@@ -76,6 +76,8 @@ int ttc_group_norm(const ttc_group_norm_args* args, void* stream);
  * The backward takes d_o (unit stride along dv) and d_final_state (NULL: zero) and writes dq, dk_out, dv_out (contiguous,
  * of q's, k's and v's shapes), d_log_gamma (contiguous [batch, tokens, heads], or [heads] with gamma_per_head) and
  * d_initial_state; NULL: not wanted.
+ * saved: NULL, or ttc_linear_attention_saved_bytes() that the forward fills (states between the parts that long inputs are
+ * swept in) and the backward of the same inputs reads instead of computing them again.
  * workspace: ttc_linear_attention_workspace_bytes() of the same block (the backward's where `backward` is set). */
 #define TTC_LINEAR_ATTENTION_MAX_DIM 128
 #define TTC_RESET_LOG_GAMMA -104.0f
@@ -93,11 +95,14 @@ typedef struct {
   const float* d_final_state;
   void *dq, *dk_out, *dv_out, *d_log_gamma;
   float* d_initial_state;
+  float* saved;
+  int64_t saved_bytes;
   void* workspace;
   int64_t workspace_bytes;
 } ttc_linear_attention_args;
 
 size_t ttc_linear_attention_workspace_bytes(const ttc_linear_attention_args* args);
+size_t ttc_linear_attention_saved_bytes(const ttc_linear_attention_args* args);
 int ttc_linear_attention(const ttc_linear_attention_args* args, void* stream);
 
 /* One token of each sequence, its state updated in place: q, k, v, log_gamma as above without the token dimension,

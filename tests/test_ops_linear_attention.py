@@ -381,7 +381,7 @@ def test_c_entries_refuse():
     from ttc.ops.linear_attention import _BLOCK, _STEP_BLOCK
     names = (["dtype", "gdtype", "per_head", "backward", "B", "T", "H", "Hq", "Hk", "Hv", "dk", "dv", "scale", "q", "k", "v",
               "g"] + [f"s{i}" for i in range(12)] + ["state", "o", "final", "d_o", "d0", "d1", "d2", "d_final", "dq", "dk_",
-                                                     "dv_", "dg", "d_state", "ws", "size"])
+                                                     "dv_", "dg", "d_state", "saved", "saved_size", "ws", "size"])
     base = dict.fromkeys(names, 0) | dict(B=1, T=2, H=4, Hq=4, Hk=2, Hv=4, dk=8, dv=8, scale=1.0, q=64, k=64, v=64, g=64, o=64)
     pack = lambda **kw: _BLOCK.pack(*(base | kw).values())  # noqa: E731
     back = dict(backward=1, d_o=64, dq=64, dk_=64, dv_=64, dg=64)
@@ -392,6 +392,10 @@ def test_c_entries_refuse():
                      (dict(v=0), 1), (dict(g=0), 1), (dict(o=0), 1), (dict(B=1 << 40, T=1 << 40), 1), (back, 1),
                      (back | dict(ws=64, size=need - 1), 1), (back | dict(d_o=0, ws=64, size=need), 1)]:
         assert lib.ttc_linear_attention(pack(**kw), None) == code, kw
+    long = back | dict(T=4096, ws=64, size=1 << 40)
+    kept = lib.ttc_linear_attention_saved_bytes(pack(**long))
+    assert kept > 0 and lib.ttc_linear_attention_saved_bytes(pack()) == 0
+    assert lib.ttc_linear_attention(pack(**long, saved=64, saved_size=kept - 1), None) == 1
     assert lib.ttc_linear_attention(None, None) == 1 and lib.ttc_linear_attention(pack(B=0), None) == 0
     names = ["dtype", "gdtype", "B", "H", "Hq", "Hk", "Hv", "dk", "dv", "slots", "scale", "q", "k", "v", "g"] + \
         [f"s{i}" for i in range(8)] + ["state", "index", "o"]

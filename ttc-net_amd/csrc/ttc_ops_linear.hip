@@ -184,16 +184,22 @@ __global__ __launch_bounds__(64) void gate_kernel(Sweep A, const float* __restri
     const int64_t hi = end - lane * GATE_TOKENS;  // this lane: tokens hi - 1 down to hi - 8
     double sum[GATE_TOKENS], run = 0.0;
     bool cut[GATE_TOKENS], cuts = false;
+    float rs[GATE_TOKENS], cs[GATE_TOKENS];
+#pragma unroll
+    for (int i = 0; i < GATE_TOKENS; ++i) {  // all loads at once, from the stretch's first token where there is none
+      const int64_t t = hi - 1 - i < first ? first : hi - 1 - i;
+      rs[i] = r[bh * A.T + t];
+      cs[i] = c[bh * A.T + t];
+      cut[i] = gamma_at(A, b * A.gb + h * A.gh + t * A.gt) < RESET;
+    }
 #pragma unroll
     for (int i = 0; i < GATE_TOKENS; ++i) {
       const int64_t t = hi - 1 - i;
-      cut[i] = false;
-      if (t >= first) {
-        double d = 0.0;
-        for (int j = 0; j < tiles; ++j) d += (double)r[j * BHT + bh * A.T + t] - c[j * BHT + bh * A.T + t];
-        run += d;
-        cut[i] = gamma_at(A, b * A.gb + h * A.gh + t * A.gt) < RESET;
-      }
+      double d = (double)rs[i] - cs[i];
+      if (tiles > 1 && t >= first)
+        for (int j = 1; j < tiles; ++j) d += (double)r[j * BHT + bh * A.T + t] - c[j * BHT + bh * A.T + t];
+      cut[i] = cut[i] && t >= first;
+      if (t >= first) run += d;
       if (cut[i]) run = 0.0, cuts = true;
       sum[i] = run;
     }
@@ -264,6 +270,12 @@ inline Segments segments_of(const ttc_linear_attention_args& A) {
   return G;
 }
 
+// The states in front of the segments: 0 where the tokens are not split
+inline int64_t saved_bytes(const ttc_linear_attention_args& A) {
+  const int64_t n = A.tokens > TOKEN_SWEEP ? segments_of(A).count : 1;
+  return n > 1 ? A.batch * A.heads * n * A.dk * A.dv * 4 : 0;
+}
+
 struct Layout {  // the workspace, in bytes from its start; 0 bytes: not needed
   int64_t seg_state, seg_decay, dq, dk, dv, r, c, last, states, joins, per_head, total;
   int64_t mark_tokens, marks;  // one stretch where the tokens are swept one by one
@@ -282,9 +294,9 @@ inline Layout layout_of(const ttc_linear_attention_args& A) {
     return p;
   };
   if (A.tokens > TOKEN_SWEEP) {
-    const int64_t n = segments_of(A).count, all = A.batch * A.heads * n;
-    W.seg_state = take(n > 1 ? all * A.dk * A.dv * 4 : 0);
-    W.seg_decay = take(n > 1 ? all * 4 : 0);
+    const int64_t n = segments_of(A).count;
+    W.seg_state = take(A.backward || !A.saved ? saved_bytes(A) : 0);
+    W.seg_decay = take(n > 1 ? A.batch * A.heads * n * 4 : 0);
   }
   W.dot_tiles = A.tokens > TOKEN_SWEEP ? 1 : token_tiles((int)A.dk);
   W.total = at;
@@ -356,38 +368,33 @@ inline Sweep sweep_of(const ttc_linear_attention_args& A) {
   return S;
 }
 
-// exact: the sweep's dots are wanted
-int run_sweep(const ttc_linear_attention_args& A, const Layout& W, const Sweep& S, bool exact, hipStream_t s) {
-  const bool bf16 = A.dtype == TTC_DTYPE_BF16;
-  if (A.tokens <= TOKEN_SWEEP) return launch_token_sweep(S, bf16, s);
-  if (A.batch == 0) return TTC_LQR_OK;
-  Segments G = segments_of(A);
-  char* ws = static_cast<char*>(A.workspace);
-  G.state = reinterpret_cast<float*>(ws + W.seg_state);
-  G.decay = reinterpret_cast<float*>(ws + W.seg_decay);
+int launch_chunks(const Sweep& S, const Segments& G, bool bf16, int mode, hipStream_t s) {
   const int vec = bf16 ? 8 : 4;
   auto wide = [&](const Side& x, int dim) {
-    return dim % vec == 0 && aligned16(x.p) && x.sb % vec == 0 && x.st % vec == 0 && x.sh % vec == 0 &&
-           x.st >= dim && x.st < (1 << 22);  // rows that do not overlap, a chunk's within 2^30 bytes
+    return dim % vec == 0 && aligned16(x.p) && x.sb % vec == 0 && x.st % vec == 0 && x.sh % vec == 0 && x.st >= dim &&
+           x.st < (1 << 22);  // rows that do not overlap, a chunk's within 2^30 bytes
   };
-  const Wides V{wide(S.q, S.kd) && wide(S.k, S.kd) && wide(S.v, S.vd) && (!S.x.p || wide(S.x, S.vd)),
+  const Wides V{(mode == STATE_ONLY || wide(S.q, S.kd)) && wide(S.k, S.kd) && wide(S.v, S.vd) &&
+                    (!S.x.p || wide(S.x, S.vd)),
                 S.vd % 4 == 0 && aligned16(S.out) && (int64_t)S.H * S.vd < (1 << 22)};
-  auto launch = [&](int mode) {
-    if (bf16)
-      return S.kd <= 32   ? launch_chunk_kd32<__bf16>(S, G, V, mode, s)
-             : S.kd <= 64 ? launch_chunk_kd64<__bf16>(S, G, V, mode, s)
-                          : launch_chunk_kd128<__bf16>(S, G, V, mode, s);
-    return S.kd <= 32   ? launch_chunk_kd32<float>(S, G, V, mode, s)
-           : S.kd <= 64 ? launch_chunk_kd64<float>(S, G, V, mode, s)
-                        : launch_chunk_kd128<float>(S, G, V, mode, s);
-  };
-  if (G.count > 1) {
-    if (const int rc = launch(STATE_ONLY)) return rc;
-    const int64_t per = ceil_div((int64_t)S.kd * S.vd, 256), blocks = A.batch * A.heads * per;
-    if (blocks > MAX_GRID) return TTC_LQR_EINVAL;
-    hipLaunchKernelGGL(segment_join_kernel, dim3((unsigned)blocks), dim3(256), 0, s, S, G, per);
-  }
-  return launch(exact ? EXACT : FAST);
+  if (bf16)
+    return S.kd <= 32   ? launch_chunk_kd32<__bf16>(S, G, V, mode, s)
+           : S.kd <= 64 ? launch_chunk_kd64<__bf16>(S, G, V, mode, s)
+                        : launch_chunk_kd128<__bf16>(S, G, V, mode, s);
+  return S.kd <= 32   ? launch_chunk_kd32<float>(S, G, V, mode, s)
+         : S.kd <= 64 ? launch_chunk_kd64<float>(S, G, V, mode, s)
+                      : launch_chunk_kd128<float>(S, G, V, mode, s);
+}
+
+// The states in front of the segments of sweep S, whose roles are those of the state [dk, dv] (S.sr = dv, S.sc = 1): read by
+// it and by the sweep with the roles of dk and dv swapped
+int segment_states(const Sweep& S, Segments& G, bool bf16, hipStream_t s) {
+  if (G.count <= 1) return TTC_LQR_OK;
+  if (const int rc = launch_chunks(S, G, bf16, STATE_ONLY, s)) return rc;
+  const int64_t per = ceil_div((int64_t)S.kd * S.vd, 256), blocks = S.B * S.H * per;
+  if (blocks > MAX_GRID) return TTC_LQR_EINVAL;
+  hipLaunchKernelGGL(segment_join_kernel, dim3((unsigned)blocks), dim3(256), 0, s, S, G, per);
+  return launched();
 }
 
 }  // namespace ttc
@@ -396,6 +403,12 @@ extern "C" size_t ttc_linear_attention_workspace_bytes(const ttc_linear_attentio
   using namespace ttc;
   if (!args || args_check(*args) != TTC_LQR_OK) return 0;
   return (size_t)layout_of(*args).total;
+}
+
+extern "C" size_t ttc_linear_attention_saved_bytes(const ttc_linear_attention_args* args) {
+  using namespace ttc;
+  if (!args || args_check(*args) != TTC_LQR_OK) return 0;
+  return (size_t)saved_bytes(*args);
 }
 
 extern "C" int ttc_linear_attention(const ttc_linear_attention_args* args, void* stream) {
@@ -407,34 +420,45 @@ extern "C" int ttc_linear_attention(const ttc_linear_attention_args* args, void*
   if (some && (!A.q || !A.k || !A.v || !A.log_gamma)) return TTC_LQR_EINVAL;
   const Layout W = layout_of(A);
   if (W.total > 0 && (!A.workspace || A.workspace_bytes < W.total)) return TTC_LQR_EINVAL;
+  if (A.saved && A.saved_bytes < saved_bytes(A)) return TTC_LQR_EINVAL;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const Side q = side_of(A.q, A.q_stride, A.heads, A.q_heads), k = side_of(A.k, A.k_stride, A.heads, A.k_heads),
              v = side_of(A.v, A.v_stride, A.heads, A.v_heads), none{};
+  char* ws = static_cast<char*>(A.workspace);
+  auto space = [&](int64_t at) { return reinterpret_cast<float*>(ws + at); };
+  const bool chunked = A.tokens > TOKEN_SWEEP && A.batch > 0;
+  Segments G = segments_of(A);
+  G.state = A.saved ? A.saved : space(W.seg_state);
+  G.decay = space(W.seg_decay);
+  int rc = TTC_LQR_OK;
+  // exact: the sweep's dots are wanted
+  auto sweep = [&](const Sweep& S, bool exact) {
+    if (!chunked) return launch_token_sweep(S, bf16, s);
+    G.sr = S.sr, G.sc = S.sc;
+    return launch_chunks(S, G, bf16, exact ? EXACT : FAST, s);
+  };
+  const int dk = (int)A.dk, dv = (int)A.dv;
   Sweep S = sweep_of(A);
+  S.q = q, S.k = k, S.v = v;
+  S.kd = dk, S.vd = dv;
+  S.sr = dv, S.sc = 1;
+  S.out_scale = (float)A.scale;
+  S.state_in = A.initial_state;
   if (!A.backward) {
     if (some && !A.o) return TTC_LQR_EINVAL;
-    S.q = q, S.k = k, S.v = v;
-    S.kd = (int)A.dk, S.vd = (int)A.dv;
-    S.out_scale = (float)A.scale;
-    S.state_in = A.initial_state;
     S.state_out = A.final_state;
-    S.sr = S.vd, S.sc = 1;
     S.out = A.o;
-    return run_sweep(A, W, S, false, s);
+    if (chunked && (rc = segment_states(S, G, bf16, s))) return rc;
+    return sweep(S, false);
   }
   if (some && !A.d_o) return TTC_LQR_EINVAL;
   const Side d_o = side_of(A.d_o, A.d_o_stride, A.heads, A.heads);
-  char* ws = static_cast<char*>(A.workspace);
-  auto space = [&](int64_t at) { return reinterpret_cast<float*>(ws + at); };
-  const int dk = (int)A.dk, dv = (int)A.dv;
   const bool gate = W.gate && some;
-  int rc = TTC_LQR_OK;
   if (some && (A.dq || gate)) {  // S transposed: [dv, dk]
+    if (chunked && !A.saved && (rc = segment_states(S, G, bf16, s))) return rc;
     S.q = d_o, S.k = v, S.v = k;
     S.x = gate ? q : none;
     S.kd = dv, S.vd = dk;
-    S.out_scale = (float)A.scale;
-    S.state_in = A.initial_state;
     S.state_out = gate && A.d_final_state ? space(W.last) : nullptr;
     S.sr = 1, S.sc = dv;
     S.dots = space(W.r);
@@ -442,13 +466,26 @@ extern "C" int ttc_linear_attention(const ttc_linear_attention_args* args, void*
     S.states = gate && W.marks > 1 ? space(W.states) : nullptr;
     S.out_f32 = shared_out(A.heads, A.q_heads) || !A.dq;
     S.out = S.out_f32 ? space(W.dq) : A.dq;
-    if ((rc = run_sweep(A, W, S, gate, s))) return rc;
+    if ((rc = sweep(S, gate))) return rc;
   }
   S = sweep_of(A);
   S.reverse = true;
+  S.q = k, S.k = q, S.v = d_o;
+  S.kd = dk, S.vd = dv;
+  S.sr = dv, S.sc = 1;
   S.key_scale = (float)A.scale;
   S.state_in = A.d_final_state;
-  if (some && (A.dk_out || gate)) {  // R transposed: [dv, dk]
+  const bool want_v = (some && A.dv_out) || A.d_initial_state, want_k = some && (A.dk_out || gate);
+  G.state = space(W.seg_state);
+  if (chunked && (want_v || want_k) && (rc = segment_states(S, G, bf16, s))) return rc;
+  if (want_v) {
+    Sweep V = S;
+    V.state_out = A.d_initial_state;
+    V.out_f32 = shared_out(A.heads, A.v_heads) && A.dv_out;
+    V.out = V.out_f32 ? space(W.dv) : A.dv_out;
+    if ((rc = sweep(V, false))) return rc;
+  }
+  if (want_k) {  // R transposed: [dv, dk]
     S.q = v, S.k = d_o, S.v = q;
     S.x = gate ? k : none;
     S.kd = dv, S.vd = dk;
@@ -460,19 +497,7 @@ extern "C" int ttc_linear_attention(const ttc_linear_attention_args* args, void*
     S.last = gate && A.d_final_state ? space(W.last) : nullptr;
     S.out_f32 = shared_out(A.heads, A.k_heads) || !A.dk_out;
     S.out = S.out_f32 ? space(W.dk) : A.dk_out;
-    if ((rc = run_sweep(A, W, S, gate, s))) return rc;
-  }
-  if ((some && A.dv_out) || A.d_initial_state) {
-    S.q = k, S.k = q, S.v = d_o;
-    S.x = none;
-    S.dots = S.states = S.joins = nullptr;
-    S.last = nullptr;
-    S.kd = dk, S.vd = dv;
-    S.sr = dv, S.sc = 1;
-    S.state_out = A.d_initial_state;
-    S.out_f32 = shared_out(A.heads, A.v_heads) && A.dv_out;
-    S.out = S.out_f32 ? space(W.dv) : A.dv_out;
-    if ((rc = run_sweep(A, W, S, false, s))) return rc;
+    if ((rc = sweep(S, gate))) return rc;
   }
   if (some) {
     const int64_t rows = A.batch * A.tokens;

@@ -65,7 +65,8 @@ __device__ __forceinline__ float gamma_at(const Sweep& A, int64_t i) {
 struct Segments {
   int count;          // segments a head
   int64_t chunks;     // chunks a segment
-  float* state;       // [batch, head, segment, kd, vd]: a segment's own contribution, then the state in front of it
+  float* state;       // [batch, head, segment, dk, dv]: a segment's own contribution, then the state in front of it
+  int sr, sc;         // the sweep's element (i, j) of it at i * sr + j * sc
   float* decay;       // [batch, head, segment]: its whole decay
 };
 

@@ -245,7 +245,7 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
     if (MODE != STATE_ONLY) {
       if (G.count > 1) {
         p = G.state + (bh * G.count + seg) * elems;
-        sr = A.vd, sc = 1;
+        sr = G.sr, sc = G.sc;
       } else if (A.state_in) {
         p = A.state_in + bh * elems;
       }

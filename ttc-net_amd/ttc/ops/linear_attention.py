@@ -24,7 +24,7 @@ __all__ = ["linear_attention", "linear_attention_step", "linear_attention_torch"
 MAX_DIM = 128         # TTC_LINEAR_ATTENTION_MAX_DIM
 RESET = -104.0        # TTC_RESET_LOG_GAMMA
 _CHUNK = 64
-_BLOCK = struct.Struct("12qd4q12qqqqq3qq4qqqq")
+_BLOCK = struct.Struct("12qd4q12qqqqq3qq4qqqqqq")
 _STEP_BLOCK = struct.Struct("10qd4q8qqqq")
 
 
@@ -66,14 +66,14 @@ def _gamma_strides(log_gamma):
 
 
 def _block(dtype, log_gamma, q, k, v, scale, initial, o, final, backward=0, d_o=None, d_final=None, dq=None, dk=None,
-           dv=None, d_gamma=None, d_initial=None, space=None):
+           dv=None, d_gamma=None, d_initial=None, saved=None, space=None):
     B, T = q.shape[:2]
     return _BLOCK.pack(DTYPES[dtype], DTYPES[log_gamma.dtype], log_gamma.dim() == 1, backward, B, T, log_gamma.shape[-1],
                        q.shape[2], k.shape[2], v.shape[2], q.shape[3], v.shape[3], scale, ptr(q), ptr(k), ptr(v),
                        ptr(log_gamma), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *_gamma_strides(log_gamma),
                        ptr(initial), ptr(o), ptr(final), ptr(d_o), *((0, 0, 0) if d_o is None else d_o.stride()[:3]),
-                       ptr(d_final), ptr(dq), ptr(dk), ptr(dv), ptr(d_gamma), ptr(d_initial), ptr(space),
-                       0 if space is None else space.numel())
+                       ptr(d_final), ptr(dq), ptr(dk), ptr(dv), ptr(d_gamma), ptr(d_initial), ptr(saved),
+                       0 if saved is None else 4 * saved.numel(), ptr(space), 0 if space is None else space.numel())
 
 
 def _run(*args, **kw):
@@ -86,27 +86,35 @@ def _run(*args, **kw):
     launch(lib.ttc_linear_attention, "ttc_linear_attention", block, q.device)
 
 
-def _forward(q, k, v, log_gamma, scale, initial, want_state):
+def _forward(q, k, v, log_gamma, scale, initial, want_state, train=False):
+    """``(o, final state or None, what the backward wants kept or None)``."""
     B, T = q.shape[:2]
     H = log_gamma.shape[-1]
     o = torch.empty(B, T, H, v.shape[-1], dtype=q.dtype, device=q.device)
     final = torch.empty(B, H, q.shape[-1], v.shape[-1], dtype=torch.float32, device=q.device) if want_state else None
-    _run(q.dtype, log_gamma, unit_rows(q), unit_rows(k), unit_rows(v), scale, initial, o, final)
-    return o, final
+    args = (q.dtype, log_gamma, unit_rows(q), unit_rows(k), unit_rows(v), scale, initial, o, final)
+    saved = None
+    if train:
+        size = lib.ttc_linear_attention_saved_bytes(_block(*args))
+        saved = torch.empty(size // 4, dtype=torch.float32, device=q.device) if size else None
+    _run(*args, saved=saved)
+    return o, final, saved
 
 
 class _LinearAttentionFunc(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, log_gamma, initial, scale, want_state):
-        ctx.save_for_backward(q, k, v, log_gamma, initial)
+        o, final, saved = _forward(q, k, v, log_gamma, scale, None if initial is None else initial.contiguous(),
+                                   want_state, True)
+        ctx.save_for_backward(q, k, v, log_gamma, initial, saved)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
-        return _forward(q, k, v, log_gamma, scale, None if initial is None else initial.contiguous(), want_state)
+        return o, final
 
     @staticmethod
     def backward(ctx, d_o, d_final):
-        q, k, v, log_gamma, initial = ctx.saved_tensors
+        q, k, v, log_gamma, initial, saved = ctx.saved_tensors
         needs = ctx.needs_input_grad[:5]
         if d_o is None and d_final is None:
             return (None,) * 7
@@ -121,7 +129,7 @@ class _LinearAttentionFunc(torch.autograd.Function):
         _run(q.dtype, log_gamma, unit_rows(q), unit_rows(k), unit_rows(v), ctx.scale,
              None if initial is None else initial.contiguous(), None, None, backward=1, d_o=unit_rows(d_o),
              d_final=None if d_final is None else d_final.contiguous(), dq=dq, dk=dk, dv=dv, d_gamma=d_gamma,
-             d_initial=d_initial)
+             d_initial=d_initial, saved=saved)
         return dq, dk, dv, d_gamma, d_initial, None, None
 
 
@@ -168,8 +176,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_gamm
     elif torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, log_gamma, initial_state)):
         o, final = _LinearAttentionFunc.apply(q, k, v, log_gamma, initial_state, scale, output_state)
     else:
-        o, final = _forward(q, k, v, log_gamma, scale, None if initial_state is None else initial_state.contiguous(),
-                            output_state)
+        o, final, _ = _forward(q, k, v, log_gamma, scale, None if initial_state is None else initial_state.contiguous(),
+                               output_state)
     return (o, final) if output_state else o
 
 

@@ -114,7 +114,8 @@ def _load():
     for name in ("ttc_rotary", "ttc_group_norm", "ttc_linear_attention", "ttc_linear_attention_step"):  # (block, stream)
         getattr(L, name).restype = ctypes.c_int
         getattr(L, name).argtypes = [ctypes.c_char_p, ctypes.c_void_p]
-    for name in ("ttc_group_norm_workspace_bytes", "ttc_linear_attention_workspace_bytes"):
+    for name in ("ttc_group_norm_workspace_bytes", "ttc_linear_attention_workspace_bytes",
+                 "ttc_linear_attention_saved_bytes"):
         getattr(L, name).restype = sz
         getattr(L, name).argtypes = [ctypes.c_char_p]
     for suffix in ("", "_bf16"):
