@@ -18,7 +18,34 @@ namespace ttc {
 
 struct Affine {  // weight and bias of type float or bf16, or none
   const void *w, *b;
-  bool bf16;
+  bool bf16, wide;  // wide: at 16-byte addresses
+  // V of each from channel c (a multiple of V) on, 1 and 0 beyond `end`
+  template <int V>
+  __device__ __forceinline__ void load(int64_t c, int64_t end, float (&wv)[V], float (&bv)[V]) const {
+    if (V > 1 && wide && w != nullptr && c + V <= end) {
+      auto vec = [&](const void* p, float (&out)[V]) {
+        if (bf16) {
+          struct alignas(V * 2) Values { __bf16 v[V]; };
+          const Values r = *reinterpret_cast<const Values*>(static_cast<const __bf16*>(p) + c);
+#pragma unroll
+          for (int j = 0; j < V; ++j) out[j] = to_f(r.v[j]);
+        } else {
+          struct alignas(V * 4 < 16 ? V * 4 : 16) Values { float v[V]; };
+          const Values r = *reinterpret_cast<const Values*>(static_cast<const float*>(p) + c);
+#pragma unroll
+          for (int j = 0; j < V; ++j) out[j] = r.v[j];
+        }
+      };
+      vec(w, wv);
+      vec(b, bv);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      wv[j] = c + j < end ? weight(c + j) : 1.0f;
+      bv[j] = c + j < end ? bias(c + j) : 0.0f;
+    }
+  }
   __device__ __forceinline__ float weight(int64_t c) const {
     if (w == nullptr) return 1.0f;
     return bf16 ? to_f(static_cast<const __bf16*>(w)[c]) : static_cast<const float*>(w)[c];
@@ -66,99 +93,135 @@ struct alignas(V * sizeof(T)) Vec {
 
 // ---- one position: rows of `cg` contiguous channels ---------------------------------------------------------
 
-// `lanes` (a power of two) lanes a row, NV vectors of V elements each
+// How the rows' kernels spread: `lanes` (a power of two) lanes a group, NV vectors of V elements each.  A thread keeps its
+// channels (group, lane) and walks down a slab of the n rows, so that weights stay in registers and the backward's sums over
+// n do; a workgroup covers 256 / lanes groups of a row of G, or several rows at once where G is smaller.
+struct Rows {
+  int64_t n;
+  int G, cg, lanes, gper, rper, gblocks, slab;  // gper groups and rper rows at once, slab rows in all
+};
+
 template <class T, int V, int NV, bool SILU, bool GATE>
 __global__ __launch_bounds__(256) void norm_row_kernel(const T* __restrict__ x, const T* __restrict__ gate, Affine aff,
-                                                       int64_t rows, int G, int cg, int lanes, float eps,
-                                                       T* __restrict__ y, float* __restrict__ mean_out,
+                                                       Rows R, float eps, T* __restrict__ y, float* __restrict__ mean_out,
                                                        float* __restrict__ rstd_out) {
-  const int lane = threadIdx.x % lanes;
-  const int64_t row = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
-  const bool live = row < rows;
-  const int64_t base = row * cg;
-  const int ch0 = (int)(row % G) * cg;
-  Vec<T, V> xv[NV], gv[NV];
-  float sum = 0.0f;
+  const int lanes = R.lanes, cg = R.cg, lane = threadIdx.x % lanes, unit = threadIdx.x / lanes;
+  const int gb = blockIdx.x % R.gblocks;
+  const int64_t sl = blockIdx.x / R.gblocks;
+  const int r = unit / R.gper, g = gb * R.gper + unit % R.gper;
+  if (r >= R.rper || g >= R.G) return;  // no barrier follows; a group's lanes leave together
+  const int64_t n1 = (sl + 1) * R.slab < R.n ? (sl + 1) * R.slab : R.n;
+  float w[NV][V], b[NV][V];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * lanes + lane) * V;
-    if (live && c < cg) {
-      xv[i] = *reinterpret_cast<const Vec<T, V>*>(x + base + c);
-      if (GATE) gv[i] = *reinterpret_cast<const Vec<T, V>*>(gate + base + c);
-#pragma unroll
-      for (int j = 0; j < V; ++j) sum += to_f(xv[i].v[j]);
-    }
+    aff.load<V>((int64_t)g * cg + c, (int64_t)g * cg + (c < cg ? cg : c), w[i], b[i]);
   }
-  const float mean = lane_sum(sum, lanes) / cg;
-  float sq = 0.0f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (live && (i * lanes + lane) * V < cg) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float d = to_f(xv[i].v[j]) - mean;
-        sq = fmaf(d, d, sq);
-      }
-    }
-  const float rstd = 1.0f / sqrtf(lane_sum(sq, lanes) / cg + eps);
-  if (!live) return;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * lanes + lane) * V;
-    if (c >= cg) break;
-    Vec<T, V> out;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float y0 = fmaf((to_f(xv[i].v[j]) - mean) * rstd, aff.weight(ch0 + c + j), aff.bias(ch0 + c + j));
-      out.v[j] = from_f<T>(out_of<SILU, GATE>(y0, GATE ? to_f(gv[i].v[j]) : 0.0f));
-    }
-    *reinterpret_cast<Vec<T, V>*>(y + base + c) = out;
-  }
-  if (lane == 0 && mean_out) {
-    mean_out[row] = mean;
-    rstd_out[row] = rstd;
-  }
-}
-
-// Backward: a thread keeps its channels (group, lane) and walks down a slab of the n rows, so the sums over n of
-// the weight's and bias's gradients stay in registers.  A workgroup covers 256 / lanes groups of a row of G, or
-// several rows at once where G is smaller (`gper` groups, `rper` rows).  partial: [parts, 2, c] fp32.
-template <class T, int V, int NV, bool SILU, bool GATE>
-__global__ __launch_bounds__(256) void norm_row_backward_kernel(
-    const T* __restrict__ x, const T* __restrict__ gate, const T* __restrict__ dy, Affine aff, int64_t n, int G, int cg,
-    int lanes, int gper, int rper, int gblocks, int slab, const float* __restrict__ mean_in,
-    const float* __restrict__ rstd_in, T* __restrict__ dx, T* __restrict__ dgate, float* __restrict__ partial) {
-  const int lane = threadIdx.x % lanes, unit = threadIdx.x / lanes;
-  const int gb = blockIdx.x % gblocks;
-  const int64_t sl = blockIdx.x / gblocks;
-  const int r = unit / gper, g = gb * gper + unit % gper;
-  if (r >= rper || g >= G) return;  // no barrier follows; a row's lanes leave together
-  const int64_t n0 = sl * slab, n1 = n0 + slab < n ? n0 + slab : n;
-  float w[NV][V], b[NV][V], dw[NV][V], db[NV][V];
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = (i * lanes + lane) * V + j;
-      w[i][j] = c < cg ? aff.weight(g * cg + c) : 0.0f;
-      b[i][j] = c < cg ? aff.bias(g * cg + c) : 0.0f;
-      dw[i][j] = db[i][j] = 0.0f;
-    }
   const float inv = 1.0f / cg;
-  for (int64_t m = n0 + r; m < n1; m += rper) {
-    const int64_t row = m * G + g, base = row * cg;
-    const float mean = mean_in[row], rstd = rstd_in[row];
-    float xh[NV][V], dh[NV][V], s1 = 0.0f, s2 = 0.0f;
-    Vec<T, V> xv[NV], dv[NV], gv[NV];
+  Vec<T, V> xn[NV], gn[NV];  // the next row's, on their way
+  auto fetch = [&](int64_t m) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * lanes + lane) * V;
       if (c < cg) {
-        xv[i] = *reinterpret_cast<const Vec<T, V>*>(x + base + c);
-        dv[i] = *reinterpret_cast<const Vec<T, V>*>(dy + base + c);
-        if (GATE) gv[i] = *reinterpret_cast<const Vec<T, V>*>(gate + base + c);
+        xn[i] = *reinterpret_cast<const Vec<T, V>*>(x + (m * R.G + g) * cg + c);
+        if (GATE) gn[i] = *reinterpret_cast<const Vec<T, V>*>(gate + (m * R.G + g) * cg + c);
       }
     }
+  };
+  const int64_t m0 = sl * R.slab + r;
+  if (m0 < n1) fetch(m0);
+  for (int64_t m = m0; m < n1; m += R.rper) {
+    Vec<T, V> xv[NV], gv[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) xv[i] = xn[i], gv[i] = gn[i];
+    if (m + R.rper < n1) fetch(m + R.rper);
+    const int64_t row = m * R.G + g, base = row * cg;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if ((i * lanes + lane) * V < cg) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum += to_f(xv[i].v[j]);
+      }
+    const float mean = lane_sum(sum, lanes) * inv;
+    float sq = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if ((i * lanes + lane) * V < cg) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float d = to_f(xv[i].v[j]) - mean;
+          sq = fmaf(d, d, sq);
+        }
+      }
+    const float rstd = 1.0f / sqrtf(lane_sum(sq, lanes) * inv + eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * lanes + lane) * V;
+      if (c >= cg) break;
+      Vec<T, V> out;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float y0 = fmaf((to_f(xv[i].v[j]) - mean) * rstd, w[i][j], b[i][j]);
+        out.v[j] = from_f<T>(out_of<SILU, GATE>(y0, GATE ? to_f(gv[i].v[j]) : 0.0f));
+      }
+      *reinterpret_cast<Vec<T, V>*>(y + base + c) = out;
+    }
+    if (lane == 0 && mean_out) {
+      mean_out[row] = mean;
+      rstd_out[row] = rstd;
+    }
+  }
+}
+
+// partial: [parts, 2, c] fp32, the sums over each thread row's part of the n rows
+template <class T, int V, int NV, bool SILU, bool GATE>
+__global__ __launch_bounds__(256) void norm_row_backward_kernel(const T* __restrict__ x, const T* __restrict__ gate,
+                                                                const T* __restrict__ dy, Affine aff, Rows R,
+                                                                const float* __restrict__ mean_in,
+                                                                const float* __restrict__ rstd_in, T* __restrict__ dx,
+                                                                T* __restrict__ dgate, float* __restrict__ partial) {
+  const int lanes = R.lanes, cg = R.cg, G = R.G, rper = R.rper, lane = threadIdx.x % lanes, unit = threadIdx.x / lanes;
+  const int gb = blockIdx.x % R.gblocks;
+  const int64_t sl = blockIdx.x / R.gblocks;
+  const int r = unit / R.gper, g = gb * R.gper + unit % R.gper;
+  if (r >= rper || g >= G) return;  // no barrier follows; a group's lanes leave together
+  const int64_t n0 = sl * R.slab, n1 = n0 + R.slab < R.n ? n0 + R.slab : R.n;
+  float w[NV][V], b[NV][V], dw[NV][V], db[NV][V];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * lanes + lane) * V;
+    aff.load<V>((int64_t)g * cg + c, (int64_t)g * cg + (c < cg ? cg : c), w[i], b[i]);
+#pragma unroll
+    for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.0f;
+  }
+  Vec<T, V> xn[NV], dn[NV], gn[NV];  // the next row's, on their way
+  float mean_n = 0.0f, rstd_n = 0.0f;
+  auto fetch = [&](int64_t m) {
+    const int64_t row = m * G + g;
+    mean_n = mean_in[row];
+    rstd_n = rstd_in[row];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * lanes + lane) * V;
+      if (c < cg) {
+        xn[i] = *reinterpret_cast<const Vec<T, V>*>(x + row * cg + c);
+        dn[i] = *reinterpret_cast<const Vec<T, V>*>(dy + row * cg + c);
+        if (GATE) gn[i] = *reinterpret_cast<const Vec<T, V>*>(gate + row * cg + c);
+      }
+    }
+  };
+  if (n0 + r < n1) fetch(n0 + r);
+  const float inv = 1.0f / cg;
+  for (int64_t m = n0 + r; m < n1; m += rper) {
+    const int64_t row = m * G + g, base = row * cg;
+    const float mean = mean_n, rstd = rstd_n;
+    float xh[NV][V], dh[NV][V], s1 = 0.0f, s2 = 0.0f;
+    Vec<T, V> xv[NV], dv[NV], gv[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) xv[i] = xn[i], dv[i] = dn[i], gv[i] = gn[i];
+    if (m + rper < n1) fetch(m + rper);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * lanes + lane) * V;
@@ -210,29 +273,32 @@ __global__ __launch_bounds__(256) void norm_row_backward_kernel(
   }
 }
 
-// Sums of [parts, 2, c] over the parts, in 64 bits: 16 channels a workgroup, 16 threads each
+// Sums of [parts, 2, c] over the parts, in 64 bits: 16 channels a workgroup, 64 threads each
 template <class W>
-__global__ __launch_bounds__(256) void norm_affine_sum_kernel(const float* __restrict__ partial, int64_t parts, int64_t c,
-                                                              W* __restrict__ dw, W* __restrict__ db) {
-  __shared__ double sw[16][17], sb[16][17];
+__global__ __launch_bounds__(1024) void norm_affine_sum_kernel(const float* __restrict__ partial, int64_t parts, int64_t c,
+                                                               W* __restrict__ dw, W* __restrict__ db) {
+  __shared__ double sw[64][17], sb[64][17];
   const int cx = threadIdx.x % 16, py = threadIdx.x / 16;
   const int64_t ch = (int64_t)blockIdx.x * 16 + cx;
   double w = 0.0, b = 0.0;
   if (ch < c)
-    for (int64_t p = py; p < parts; p += 16) {
+#pragma unroll 4
+    for (int64_t p = py; p < parts; p += 64) {
       w += partial[p * 2 * c + ch];
       b += partial[(p * 2 + 1) * c + ch];
     }
   sw[py][cx] = w;
   sb[py][cx] = b;
-  __syncthreads();
-  if (py == 0 && ch < c) {
-    for (int i = 1; i < 16; ++i) {
-      w += sw[i][cx];
-      b += sb[i][cx];
+  for (int m = 32; m >= 1; m >>= 1) {
+    __syncthreads();
+    if (py < m) {
+      sw[py][cx] += sw[py + m][cx];
+      sb[py][cx] += sb[py + m][cx];
     }
-    if (dw) dw[ch] = from_f<W>((float)w);
-    if (db) db[ch] = from_f<W>((float)b);
+  }
+  if (py == 0 && ch < c) {
+    if (dw) dw[ch] = from_f<W>((float)sw[0][cx]);
+    if (db) db[ch] = from_f<W>((float)sb[0][cx]);
   }
 }
 
@@ -357,9 +423,8 @@ __global__ __launch_bounds__(256) void norm_slab_apply_kernel(const T* __restric
     const int c = col * V + j, g = c / S.cg;
     m[j] = mean[n * S.G + g];
     k[j] = rstd[n * S.G + g];
-    w[j] = aff.weight(c);
-    b[j] = aff.bias(c);
   }
+  aff.load<V>((int64_t)col * V, S.C, w, b);
   const int64_t base = n * S.L * S.C + (int64_t)col * V;
 #pragma unroll 4
   for (int64_t l = l0 + r; l < l1; l += S.rper) {
@@ -400,9 +465,8 @@ __global__ __launch_bounds__(256) void norm_slab_back_stats_kernel(const T* __re
       const int c = col * V + j, g = c / S.cg;
       m[j] = mean[n * S.G + g];
       k[j] = rstd[n * S.G + g];
-      w[j] = aff.weight(c);
-      b[j] = aff.bias(c);
     }
+    aff.load<V>((int64_t)col * V, S.C, w, b);
     const int64_t base = n * S.L * S.C + (int64_t)col * V;
 #pragma unroll 4
     for (int64_t l = l0 + r; l < l1; l += S.rper) {
@@ -499,9 +563,8 @@ __global__ __launch_bounds__(256) void norm_slab_back_apply_kernel(const T* __re
     k[j] = rstd[g];
     c2[j] = sums[2 * g];
     c1[j] = sums[2 * g + 1];
-    w[j] = aff.weight(c);
-    b[j] = aff.bias(c);
   }
+  aff.load<V>((int64_t)col * V, S.C, w, b);
   const int64_t base = n * S.L * S.C + (int64_t)col * V;
 #pragma unroll 4
   for (int64_t l = l0 + r; l < l1; l += S.rper) {
@@ -524,8 +587,8 @@ __global__ __launch_bounds__(256) void norm_slab_back_apply_kernel(const T* __re
 
 struct NormPlan {
   bool rows;              // the one-position form
-  int V, lanes, NV;       // rows: lanes and vectors a group
-  int gper, rper, gblocks, slab;
+  int V, NV;
+  Rows R;
   int64_t slabs;
   Slab S;
   size_t floats;          // workspace
@@ -548,23 +611,27 @@ inline NormPlan norm_plan(const ttc_group_norm_args& A, bool wide) {
   P.rows = A.l == 1 && vecs <= 64 * 4;
   if (P.rows) {
     P.V = Vr;
-    P.lanes = 1;
-    while (P.lanes < 64 && P.lanes < vecs) P.lanes *= 2;
-    const int need = (int)ceil_div(vecs, P.lanes);
+    Rows& R = P.R;
+    R.n = A.n;
+    R.G = (int)A.groups;
+    R.cg = (int)cg;
+    R.lanes = 1;
+    while (R.lanes < 64 && R.lanes < vecs) R.lanes *= 2;
+    const int need = (int)ceil_div(vecs, R.lanes);
     P.NV = need <= 1 ? 1 : need <= 2 ? 2 : 4;
-    if (A.backward) {
-      const int units = 256 / P.lanes;
-      P.gper = A.groups < units ? (int)A.groups : units;
-      P.rper = units / P.gper;
-      P.gblocks = (int)ceil_div(A.groups, P.gper);
-      // 2,048 workgroups fill the GPU eight waves a SIMD deep; more rows each keep the partial sums small
-      const int64_t want = 2048 / P.gblocks > 0 ? 2048 / P.gblocks : 1;
-      int64_t slab = ceil_div(A.n, want);
-      slab = slab < P.rper ? P.rper : slab;
-      P.slab = (int)slab;
-      P.slabs = ceil_div(A.n, slab);
-      if (A.dweight || A.dbias) P.floats = (size_t)(P.slabs * P.rper * 2 * A.c);
-    }
+    const int units = 256 / R.lanes;
+    R.gper = A.groups < units ? (int)A.groups : units;
+    R.rper = units / R.gper;
+    R.gblocks = (int)ceil_div(A.groups, R.gper);
+    // Workgroups: 2,048 fill the GPU; half as many in the backward, whose partial sums grow with them
+    int64_t want = (A.backward ? 1024 : 2048) / R.gblocks;
+    if (want < 1) want = 1;
+    int64_t slab = ceil_div(A.n, want);
+    if (slab < R.rper) slab = R.rper;
+    if (slab > (1 << 30)) slab = 1 << 30;
+    R.slab = (int)slab;
+    P.slabs = ceil_div(A.n, slab);
+    if (A.backward && (A.dweight || A.dbias)) P.floats = (size_t)(P.slabs * R.rper * 2 * A.c);
     return P;
   }
   Slab& S = P.S;
@@ -577,7 +644,7 @@ inline NormPlan norm_plan(const ttc_group_norm_args& A, bool wide) {
   const int cper = S.cols < 256 ? S.cols : 256;
   S.rper = 256 / cper;
   S.cblocks = (int)ceil_div(S.cols, 256 / S.rper);
-  const int64_t want = ceil_div(2048, A.n * S.cblocks);
+  const int64_t want = ceil_div(1024, A.n * S.cblocks);
   int64_t slab = ceil_div(A.l, want);
   slab = slab < 4 * S.rper ? 4 * S.rper : slab;
   S.slab = slab < A.l ? slab : A.l;
@@ -589,34 +656,32 @@ inline NormPlan norm_plan(const ttc_group_norm_args& A, bool wide) {
 template <class T, int V, bool SILU, bool GATE>
 int norm_run(const ttc_group_norm_args& A, const NormPlan& P, hipStream_t s) {
   const T *x = static_cast<const T*>(A.x), *gate = static_cast<const T*>(A.gate), *dy = static_cast<const T*>(A.dy);
-  const Affine aff{A.weight, A.bias, A.weight_dtype == TTC_DTYPE_BF16};
+  const Affine aff{A.weight, A.bias, A.weight_dtype == TTC_DTYPE_BF16, aligned16(A.weight) && aligned16(A.bias)};
   const float eps = (float)A.eps;
   float* ws = static_cast<float*>(A.workspace);
-  const int G = (int)A.groups, cg = (int)(A.c / A.groups);
+  const int G = (int)A.groups;
   int64_t parts = 0;
   if (P.rows) {
     auto go = [&](auto nv) {
       constexpr int NV = decltype(nv)::value;
+      const int64_t blocks = P.slabs * P.R.gblocks;
+      if (blocks > MAX_GRID) return TTC_LQR_EINVAL;
+      const dim3 grid((unsigned)blocks);
       if (!A.backward) {
-        const int64_t rows = A.n * G, blocks = ceil_div(rows, 256 / P.lanes);
-        if (blocks > MAX_GRID) return TTC_LQR_EINVAL;
-        hipLaunchKernelGGL((norm_row_kernel<T, V, NV, SILU, GATE>), dim3((unsigned)blocks), dim3(256), 0, s, x, gate, aff,
-                           rows, G, cg, P.lanes, eps, static_cast<T*>(A.y), A.mean, A.rstd);
+        hipLaunchKernelGGL((norm_row_kernel<T, V, NV, SILU, GATE>), grid, dim3(256), 0, s, x, gate, aff, P.R, eps,
+                           static_cast<T*>(A.y), A.mean, A.rstd);
         return launched();
       }
-      const int64_t blocks = P.slabs * P.gblocks;
-      if (blocks > MAX_GRID) return TTC_LQR_EINVAL;
       float* part = A.dweight || A.dbias ? ws : nullptr;
-      hipLaunchKernelGGL((norm_row_backward_kernel<T, V, NV, SILU, GATE>), dim3((unsigned)blocks), dim3(256), 0, s, x,
-                         gate, dy, aff, A.n, G, cg, P.lanes, P.gper, P.rper, P.gblocks, P.slab, A.mean, A.rstd,
-                         static_cast<T*>(A.dx), static_cast<T*>(A.dgate), part);
+      hipLaunchKernelGGL((norm_row_backward_kernel<T, V, NV, SILU, GATE>), grid, dim3(256), 0, s, x, gate, dy, aff, P.R,
+                         A.mean, A.rstd, static_cast<T*>(A.dx), static_cast<T*>(A.dgate), part);
       return launched();
     };
     const int rc = P.NV == 1   ? go(std::integral_constant<int, 1>{})
                    : P.NV == 2 ? go(std::integral_constant<int, 2>{})
                                : go(std::integral_constant<int, 4>{});
     if (rc != TTC_LQR_OK) return rc;
-    parts = P.slabs * P.rper;
+    parts = P.slabs * P.R.rper;
   } else {
     const Slab& S = P.S;
     const int64_t blocks = A.n * S.slabs * S.cblocks;
@@ -644,10 +709,10 @@ int norm_run(const ttc_group_norm_args& A, const NormPlan& P, hipStream_t s) {
   if (A.dweight || A.dbias) {
     const dim3 grid((unsigned)ceil_div(A.c, 16));
     if (A.weight_dtype == TTC_DTYPE_BF16)
-      hipLaunchKernelGGL(norm_affine_sum_kernel<__bf16>, grid, dim3(256), 0, s, ws, parts, A.c,
+      hipLaunchKernelGGL(norm_affine_sum_kernel<__bf16>, grid, dim3(1024), 0, s, ws, parts, A.c,
                          static_cast<__bf16*>(A.dweight), static_cast<__bf16*>(A.dbias));
     else
-      hipLaunchKernelGGL(norm_affine_sum_kernel<float>, grid, dim3(256), 0, s, ws, parts, A.c,
+      hipLaunchKernelGGL(norm_affine_sum_kernel<float>, grid, dim3(1024), 0, s, ws, parts, A.c,
                          static_cast<float*>(A.dweight), static_cast<float*>(A.dbias));
   }
   return launched();
