@@ -13,26 +13,22 @@ def ptr(x) -> int:
     return 0 if x is None else x.data_ptr()
 
 
-def need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
-def check_types(name: str, *xs) -> None:
+def check_types(name: str, first, *xs) -> None:
     """All of one type that has kernels, all on one device."""
-    first = xs[0]
     if first.dtype not in DTYPES:
         raise TypeError(f"{name}: float32 and bfloat16 tensors are supported, got {first.dtype}")
-    for x in xs[1:]:
-        if x is not None and x.dtype != first.dtype:
-            raise TypeError(f"{name}: tensors of one type are needed, got {first.dtype} and {x.dtype}")
-    check_device(name, *xs)
+    for x in xs:
+        if x is not None:
+            if x.dtype != first.dtype:
+                raise TypeError(f"{name}: tensors of one type are needed, got {first.dtype} and {x.dtype}")
+            if x.device != first.device:
+                raise ValueError(f"{name}: tensors on one device are needed, got {first.device} and {x.device}")
 
 
-def check_device(name: str, *xs) -> None:
-    for x in xs[1:]:
-        if x is not None and x.device != xs[0].device:
-            raise ValueError(f"{name}: tensors on one device are needed, got {xs[0].device} and {x.device}")
+def check_device(name: str, first, *xs) -> None:
+    for x in xs:
+        if x is not None and x.device != first.device:
+            raise ValueError(f"{name}: tensors on one device are needed, got {first.device} and {x.device}")
 
 
 def unit_rows(x: torch.Tensor) -> torch.Tensor:
@@ -42,11 +38,12 @@ def unit_rows(x: torch.Tensor) -> torch.Tensor:
 
 def launch(fn, name: str, block: bytes, device: torch.device) -> None:
     """``fn(block, stream)`` on the device's current stream."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(block, torch._C._cuda_getCurrentRawStream(device.index))
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(block, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            rc = fn(block, torch._C._cuda_getCurrentRawStream(device.index))
+            rc = fn(block, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         check(rc, name)
 

@@ -11,7 +11,7 @@ import torch
 
 from .._dispatch import traced
 from ..solvers._lib import lib
-from ._call import DTYPES, check_device, check_types, launch, need, ptr, recorded_backward
+from ._call import DTYPES, check_device, check_types, launch, ptr, recorded_backward
 
 __all__ = ["group_norm", "group_norm_torch"]
 
@@ -48,7 +48,7 @@ def _block(x, groups, weight, bias, eps, activation, gate, mean, rstd, y, dy=Non
 
 
 def _forward(x, groups, weight, bias, eps, activation, gate, keep):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x)  # x is contiguous
     mean = rstd = None
     if keep:
         mean, rstd = torch.empty(2, x.shape[0], groups, dtype=torch.float32, device=x.device)
@@ -96,16 +96,23 @@ def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
     float32 or bfloat16 (``weight`` and ``bias`` of ``x``'s type or float32); statistics and arithmetic in 32 bits, biased
     variance of the centred values.  Differentiable in all tensors; a new contiguous tensor.
     """
-    need(x.dim() >= 2, "group_norm: x [n, ..., channels] is needed")
+    if x.dim() < 2:
+        raise ValueError("group_norm: x [n, ..., channels] is needed")
     C = x.shape[-1]
-    need(groups > 0 and C % groups == 0, f"group_norm: {C} channels do not divide into {groups} groups")
-    need(activation in _ACTIVATIONS, f"group_norm: unknown activation {activation!r}")
-    need(eps >= 0, f"group_norm: eps of at least 0 is needed, got {eps}")
-    need((weight is None) == (bias is None), "group_norm: weight and bias, or neither")
+    if groups <= 0 or C % groups:
+        raise ValueError(f"group_norm: {C} channels do not divide into {groups} groups")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"group_norm: unknown activation {activation!r}")
+    if not eps >= 0:
+        raise ValueError(f"group_norm: eps of at least 0 is needed, got {eps}")
+    if (weight is None) != (bias is None):
+        raise ValueError("group_norm: weight and bias, or neither")
     check_types("group_norm", x, gate)
-    need(gate is None or gate.shape == x.shape, "group_norm: a gate of x's shape is needed")
+    if gate is not None and gate.shape != x.shape:
+        raise ValueError("group_norm: a gate of x's shape is needed")
     if weight is not None:
-        need(weight.shape == (C,) and bias.shape == (C,), f"group_norm: weight and bias [{C}] are needed")
+        if weight.shape != (C,) or bias.shape != (C,):
+            raise ValueError(f"group_norm: weight and bias [{C}] are needed")
         if weight.dtype != bias.dtype or weight.dtype not in (x.dtype, torch.float32):
             raise TypeError(f"group_norm: weight and bias of type {x.dtype} or float32 are needed")
         check_device("group_norm", x, weight, bias)

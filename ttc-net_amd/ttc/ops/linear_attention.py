@@ -17,7 +17,7 @@ import torch
 
 from .._dispatch import traced
 from ..solvers._lib import lib
-from ._call import DTYPES, check_device, check_types, launch, need, ptr, recorded_backward, unit_rows
+from ._call import DTYPES, check_device, check_types, launch, ptr, recorded_backward, unit_rows
 
 __all__ = ["linear_attention", "linear_attention_step", "linear_attention_torch", "MAX_DIM"]
 
@@ -135,20 +135,25 @@ class _LinearAttentionFunc(torch.autograd.Function):
 
 def _check(name, q, k, v, log_gamma, dims):
     lead = "[batch, tokens, heads, dim]" if dims == 4 else "[batch, heads, dim]"
-    need(q.dim() == dims and k.dim() == dims and v.dim() == dims, f"{name}: q, k and v {lead} are needed")
-    need(k.shape[:-2] == q.shape[:-2] and v.shape[:-2] == q.shape[:-2] and k.shape[-1] == q.shape[-1],
-         f"{name}: q, k and v of one batch and number of tokens, q and k of one head size are needed")
-    need(1 <= q.shape[-1] <= MAX_DIM and 1 <= v.shape[-1] <= MAX_DIM,
-         f"{name}: head sizes of 1 to {MAX_DIM} are supported, got {q.shape[-1]} and {v.shape[-1]}")
+    if q.dim() != dims or k.dim() != dims or v.dim() != dims:
+        raise ValueError(f"{name}: q, k and v {lead} are needed")
+    *lead, qh, dk = q.shape
+    *k_lead, kh, k_dk = k.shape
+    *v_lead, vh, dv = v.shape
+    if k_lead != lead or v_lead != lead or k_dk != dk:
+        raise ValueError(f"{name}: q, k and v of one batch and number of tokens, q and k of one head size are needed")
+    if not (1 <= dk <= MAX_DIM and 1 <= dv <= MAX_DIM):
+        raise ValueError(f"{name}: head sizes of 1 to {MAX_DIM} are supported, got {dk} and {dv}")
     check_types(name, q, k, v)
     check_device(name, q, log_gamma)
     if log_gamma.dtype not in (torch.float32, q.dtype):
         raise TypeError(f"{name}: log_gamma of type float32 or {q.dtype} is needed, got {log_gamma.dtype}")
-    need(log_gamma.dim() == 1 or (log_gamma.dim() == dims - 1 and log_gamma.shape[:-1] == q.shape[:-2]),
-         f"{name}: log_gamma [heads] or one for each token and head is needed, got {tuple(log_gamma.shape)}")
-    H = log_gamma.shape[-1]
-    need(H > 0 and all(x.shape[-2] > 0 and H % x.shape[-2] == 0 for x in (q, k, v)),
-         f"{name}: the heads of q, k and v ({q.shape[-2]}, {k.shape[-2]}, {v.shape[-2]}) divide those of log_gamma ({H})")
+    *g_lead, H = log_gamma.shape
+    if g_lead and g_lead != lead:
+        raise ValueError(f"{name}: log_gamma [heads] or one for each token and head is needed, got "
+                         f"{tuple(log_gamma.shape)}")
+    if not (H and qh and kh and vh) or H % qh or H % kh or H % vh:
+        raise ValueError(f"{name}: the heads of q, k and v ({qh}, {kh}, {vh}) have to divide those of log_gamma ({H})")
     return H
 
 
@@ -168,8 +173,9 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_gamm
     H = _check("linear_attention", q, k, v, log_gamma, 4)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if initial_state is not None:
-        need(initial_state.shape == (q.shape[0], H, q.shape[-1], v.shape[-1]) and initial_state.dtype == torch.float32,
-             f"linear_attention: a float32 state {[q.shape[0], H, q.shape[-1], v.shape[-1]]} is needed")
+        shape = (q.shape[0], H, q.shape[-1], v.shape[-1])
+        if initial_state.shape != shape or initial_state.dtype != torch.float32:
+            raise ValueError(f"linear_attention: a float32 state {list(shape)} is needed")
         check_device("linear_attention", q, initial_state)
     if not q.is_cuda or traced(q, k, v, log_gamma, initial_state):
         o, final = linear_attention_torch(q, k, v, log_gamma, scale, initial_state)
@@ -194,20 +200,23 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     H = _check(name, q, k, v, log_gamma, 3)
     B, dk, dv = q.shape[0], q.shape[-1], v.shape[-1]
     scale = dk ** -0.5 if scale is None else float(scale)
-    need(state.dim() == 4 and state.shape[1:] == (H, dk, dv) and state.dtype == torch.float32 and state.is_contiguous(),
-         f"{name}: a contiguous float32 state [slots, {H}, {dk}, {dv}] is needed")
+    if state.shape[1:] != (H, dk, dv) or state.dtype != torch.float32 or not state.is_contiguous():
+        raise ValueError(f"{name}: a contiguous float32 state [slots, {H}, {dk}, {dv}] is needed")
     check_device(name, q, state, slots)
     if slots is None:
-        need(state.shape[0] == B, f"{name}: {B} sequences, {state.shape[0]} states")
+        if state.shape[0] != B:
+            raise ValueError(f"{name}: {B} sequences, {state.shape[0]} states")
     else:
-        need(slots.shape == (B,) and slots.dtype == torch.int32, f"{name}: int32 slots [{B}] are needed")
+        if slots.shape != (B,) or slots.dtype != torch.int32:
+            raise ValueError(f"{name}: int32 slots [{B}] are needed")
         slots = slots.contiguous()
-    if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v, log_gamma, state)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_gamma.requires_grad
+                                    or state.requires_grad):
         raise RuntimeError(f"{name} is not differentiable: call it under torch.no_grad(), or use linear_attention")
     if not q.is_cuda or traced(q, k, v, log_gamma, state, slots):
         return _step_torch(q, k, v, log_gamma, state, scale, slots)
     q, k, v = unit_rows(q), unit_rows(k), unit_rows(v)
-    o = torch.empty(B, H, dv, dtype=q.dtype, device=q.device)
+    o = q.new_empty((B, H, dv))
     gb, gh = (0, log_gamma.stride(0)) if log_gamma.dim() == 1 else log_gamma.stride()
     block = _STEP_BLOCK.pack(DTYPES[q.dtype], DTYPES[log_gamma.dtype], B, H, q.shape[1], k.shape[1], v.shape[1], dk, dv,
                              state.shape[0], scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_gamma.data_ptr(),

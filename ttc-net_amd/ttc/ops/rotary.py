@@ -13,7 +13,7 @@ import torch
 
 from .._dispatch import traced
 from ..solvers._lib import lib
-from ._call import DTYPES, check_device, check_types, launch, need, ptr, unit_rows
+from ._call import DTYPES, check_device, check_types, launch, ptr, unit_rows
 
 __all__ = ["rotary", "rotary_table", "rotary_torch"]
 
@@ -36,11 +36,15 @@ def rotary_table(length: int, dim: int, *, base: float = 10000.0, scaling: str =
       place (the pair's index); the table is multiplied by ``0.1 ln(factor) + 1``, which raises the scores of longer
       contexts.
     """
-    need(length >= 0 and dim >= 0 and dim % 2 == 0, f"rotary_table: length and an even dim are needed, got {length}, {dim}")
-    need(scaling in ("none", "linear", "base", "bands"), f"rotary_table: unknown scaling {scaling!r}")
-    need(base > 0 and (scaling == "none" or factor >= 1), "rotary_table: a positive base and a factor of at least 1 are needed")
+    if not (length >= 0 and dim >= 0 and dim % 2 == 0):
+        raise ValueError(f"rotary_table: length and an even dim are needed, got {length}, {dim}")
+    if scaling not in ("none", "linear", "base", "bands"):
+        raise ValueError(f"rotary_table: unknown scaling {scaling!r}")
+    if not (base > 0 and (scaling == "none" or factor >= 1)):
+        raise ValueError("rotary_table: a positive base and a factor of at least 1 are needed")
     if scaling == "base":
-        need(dim != 2 or factor == 1, "rotary_table: scaling 'base' needs more than one pair")
+        if dim == 2 and factor != 1:
+            raise ValueError("rotary_table: scaling 'base' needs more than one pair")
         if dim > 2:
             base = base * factor ** (dim / (dim - 2))
     pair = torch.arange(dim // 2, dtype=torch.float64, device=device)
@@ -49,8 +53,8 @@ def rotary_table(length: int, dim: int, *, base: float = 10000.0, scaling: str =
     if scaling == "linear":
         speed = speed / factor
     elif scaling == "bands":
-        need(original_length is not None and original_length > 0 and fast > slow > 0,
-             "rotary_table: scaling 'bands' needs original_length and fast > slow > 0")
+        if not (original_length is not None and original_length > 0 and fast > slow > 0):
+            raise ValueError("rotary_table: scaling 'bands' needs original_length and fast > slow > 0")
         at = lambda turns: dim * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
         low, high = max(math.floor(at(fast)), 0), min(math.ceil(at(slow)), dim - 1)
         kept = 1 - ((pair - low) / max(high - low, 1e-3)).clamp(0, 1)
@@ -89,7 +93,7 @@ def _launch(xs, table, positions, offset, layout, backward):
     q, k = xs
     B, T, H, D = q.shape
     xs = [None if x is None else unit_rows(x) for x in xs]
-    ys = [None if x is None else torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
+    ys = [None if x is None else x.new_empty(x.shape) for x in xs]
     strides = [0] * 6
     for i, x in enumerate(xs):
         if x is not None:
@@ -144,25 +148,30 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, table: torch.Tensor, positio
     ``(2 i, 2 i + 1)`` (``"interleaved"``).  ``q`` and ``k`` may be views with any strides over batch, tokens and heads;
     float32 or bfloat16, turned in 32 bits.  Differentiable in ``q`` and ``k``.
     """
-    need(q.dim() == 4 and (k is None or k.dim() == 4), "rotary: q and k [batch, tokens, heads, dim] are needed")
-    need(k is None or (k.shape[:2] == q.shape[:2] and k.shape[3] == q.shape[3]),
-         "rotary: q and k of one batch, number of tokens and head size are needed")
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        raise ValueError("rotary: q and k [batch, tokens, heads, dim] are needed")
+    if k is not None and (k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]):
+        raise ValueError("rotary: q and k of one batch, number of tokens and head size are needed")
     check_types("rotary", q, k)
     check_device("rotary", q, table, positions)
-    need(table.dim() == 3 and table.shape[2] == 2 and table.dtype == torch.float32 and table.is_contiguous(),
-         "rotary: a contiguous float32 table [length, rot / 2, 2] is needed")
-    need(2 * table.shape[1] <= q.shape[3], f"rotary: a table for {2 * table.shape[1]} components, heads of {q.shape[3]}")
-    need(layout in _LAYOUTS, f"rotary: unknown layout {layout!r}")
+    if table.dim() != 3 or table.shape[2] != 2 or table.dtype != torch.float32 or not table.is_contiguous():
+        raise ValueError("rotary: a contiguous float32 table [length, rot / 2, 2] is needed")
+    if 2 * table.shape[1] > q.shape[3]:
+        raise ValueError(f"rotary: a table for {2 * table.shape[1]} components, heads of {q.shape[3]}")
+    if layout not in _LAYOUTS:
+        raise ValueError(f"rotary: unknown layout {layout!r}")
     if positions is None:
-        need(0 <= offset and offset + q.shape[1] <= table.shape[0],
-             f"rotary: positions {offset} to {offset + q.shape[1] - 1}, a table of {table.shape[0]}")
+        if offset < 0 or offset + q.shape[1] > table.shape[0]:
+            raise ValueError(f"rotary: positions {offset} to {offset + q.shape[1] - 1}, a table of {table.shape[0]}")
     else:
-        need(positions.dtype in (torch.int32, torch.int64), "rotary: int32 or int64 positions are needed")
-        need(offset == 0, "rotary: either positions or an offset")
-        need(positions.shape in (q.shape[1:2], q.shape[:2]) or
-             (positions.dim() == 2 and positions.shape == (1, q.shape[1])),
-             f"rotary: positions [tokens] or [batch, tokens] are needed, got {tuple(positions.shape)}")
-        need(table.shape[0] > 0 or q.numel() == 0, "rotary: an empty table")
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise ValueError("rotary: int32 or int64 positions are needed")
+        if offset != 0:
+            raise ValueError("rotary: either positions or an offset")
+        if positions.shape != q.shape[:2] and positions.shape != q.shape[1:2] and positions.shape != (1, q.shape[1]):
+            raise ValueError(f"rotary: positions [tokens] or [batch, tokens] are needed, got {tuple(positions.shape)}")
+        if table.shape[0] == 0 and q.numel() > 0:
+            raise ValueError("rotary: an empty table")
     if not q.is_cuda or traced(q, k, table, positions):
         return rotary_torch(q, k, table, positions, offset=offset, layout=layout)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
