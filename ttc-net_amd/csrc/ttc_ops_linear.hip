@@ -110,7 +110,7 @@ int launch_token_sweep(const Sweep& A, bool bf16, hipStream_t s) {
   const int tiles = token_tiles(A.vd);
   const int64_t blocks = A.B * A.H * tiles;
   if (blocks == 0) return TTC_LQR_OK;
-  if (blocks > MAX_GRID) return TTC_LQR_EINVAL;
+  if (blocks > max_blocks(256)) return TTC_LQR_EINVAL;
   const bool wide = A.sc == 1 && A.vd % 4 == 0 && aligned16(A.state_in) && aligned16(A.state_out);
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, s, A, tiles, wide);
@@ -124,9 +124,10 @@ int launch_token_sweep(const Sweep& A, bool bf16, hipStream_t s) {
 }
 
 // Segments' own contributions to the states in front of them: state_in, then decay * state + contribution
-__global__ __launch_bounds__(256) void segment_join_kernel(Sweep A, Segments G, int64_t blocks_a_head) {
-  const int64_t bh = blockIdx.x / blocks_a_head, elems = (int64_t)A.kd * A.vd;
-  const int64_t i = blockIdx.x % blocks_a_head * 256 + threadIdx.x;
+__global__ __launch_bounds__(256) void segment_join_kernel(Sweep A, Segments G, int64_t blocks_a_head,
+                                                           int64_t first) {
+  const int64_t bh = (first + blockIdx.x) / blocks_a_head, elems = (int64_t)A.kd * A.vd;
+  const int64_t i = (first + blockIdx.x) % blocks_a_head * 256 + threadIdx.x;
   if (i >= elems) return;
   float run = A.state_in ? A.state_in[bh * elems + i / A.vd * A.sr + i % A.vd * A.sc] : 0.0f;
   float* p = G.state + bh * G.count * elems + i;
@@ -149,9 +150,9 @@ __global__ __launch_bounds__(256) void segment_join_kernel(Sweep A, Segments G, 
 
 // Gradients of shared heads: out [rows, heads / share, d] = sums over `share` heads of in [rows, heads, d]
 template <class T>
-__global__ __launch_bounds__(256) void share_sum_kernel(const float* __restrict__ in, T* __restrict__ out, int64_t n,
-                                                        int share, int d) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(256) void share_sum_kernel(const float* __restrict__ in, T* __restrict__ out, int64_t first,
+                                                        int64_t n, int share, int d) {
+  const int64_t i = (first + blockIdx.x) * 256 + threadIdx.x;
   if (i >= n) return;
   const int64_t head = i / d;
   const float* p = in + head * share * d + i % d;
@@ -348,11 +349,11 @@ inline Side side_of(const void* p, const int64_t* st, int64_t heads, int64_t own
 
 template <class T>
 int share_sum(const float* in, void* out, int64_t rows, int64_t own, int64_t heads, int64_t d, hipStream_t s) {
-  const int64_t n = rows * own * d, blocks = ceil_div(n, 256);
-  if (blocks > MAX_GRID) return TTC_LQR_EINVAL;
-  hipLaunchKernelGGL(share_sum_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, in, static_cast<T*>(out), n,
-                     (int)(heads / own), (int)d);
-  return launched();
+  const int64_t n = rows * own * d;
+  return in_launches(ceil_div(n, 256), 256, [&](int64_t first, dim3 grid) {
+    hipLaunchKernelGGL(share_sum_kernel<T>, grid, dim3(256), 0, s, in, static_cast<T*>(out), first, n,
+                       (int)(heads / own), (int)d);
+  });
 }
 
 inline Sweep sweep_of(const ttc_linear_attention_args& A) {
@@ -392,9 +393,9 @@ int segment_states(const Sweep& S, Segments& G, bool bf16, hipStream_t s) {
   if (G.count <= 1) return TTC_LQR_OK;
   if (const int rc = launch_chunks(S, G, bf16, STATE_ONLY, s)) return rc;
   const int64_t per = ceil_div((int64_t)S.kd * S.vd, 256), blocks = S.B * S.H * per;
-  if (blocks > MAX_GRID) return TTC_LQR_EINVAL;
-  hipLaunchKernelGGL(segment_join_kernel, dim3((unsigned)blocks), dim3(256), 0, s, S, G, per);
-  return launched();
+  return in_launches(blocks, 256, [&](int64_t first, dim3 grid) {
+    hipLaunchKernelGGL(segment_join_kernel, grid, dim3(256), 0, s, S, G, per, first);
+  });
 }
 
 }  // namespace ttc
@@ -510,7 +511,7 @@ extern "C" int ttc_linear_attention(const ttc_linear_attention_args* args, void*
   }
   if (W.gate) {  // of one decay for each head: zero where there are no tokens
     const int64_t stretches = A.batch * A.heads * W.marks;
-    if (stretches > MAX_GRID) return TTC_LQR_EINVAL;
+    if (stretches > max_blocks(64)) return TTC_LQR_EINVAL;
     S = sweep_of(A);
     S.mark_tokens = W.mark_tokens, S.marks = W.marks;
     S.joins = A.tokens > TOKEN_SWEEP ? space(W.joins) : nullptr;

@@ -641,7 +641,7 @@ template <class T, int KD, int VD, int MODE>
 int launch_mode(const Sweep& A, const Segments& G, const Wides& W, hipStream_t s) {
   using Z = ChunkShape<T, KD, VD>;
   const int64_t blocks = A.B * A.H * (MODE == STATE_ONLY ? G.count - 1 : G.count);
-  if (blocks > MAX_GRID) return TTC_LQR_EINVAL;
+  if (blocks > max_blocks(Z::NT)) return TTC_LQR_EINVAL;
   const dim3 grid((unsigned)blocks), block(Z::NT);
   if (W.in)
     hipLaunchKernelGGL((chunk_sweep_kernel<T, KD, VD, MODE, true>), grid, block, 0, s, A, G, W);

@@ -307,7 +307,7 @@ __global__ __launch_bounds__(1024) void norm_affine_sum_kernel(const float* __re
 // Slab kernels: a workgroup reads `slab` positions of one n, all channels in blocks of 256 / rper vectors; thread
 // (r, column) walks down positions r, r + rper, ...
 struct Slab {
-  int64_t L, slab, slabs;
+  int64_t L, slab, slabs, first;  // first: workgroup of this launch
   int C, G, cg, cols, rper, cblocks;  // cols: vectors of a row
 };
 
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(256) void norm_slab_stats_kernel(const T* __restric
   __shared__ float s1[256 * V], s2[256 * V];
   const int cper = 256 / S.rper;
   const int r = threadIdx.x / cper, cc = threadIdx.x % cper;
-  int64_t blk = blockIdx.x;
+  int64_t blk = S.first + blockIdx.x;
   const int cb = (int)(blk % S.cblocks);
   blk /= S.cblocks;
   const int64_t sl = blk % S.slabs, n = blk / S.slabs;
@@ -369,7 +369,7 @@ __global__ __launch_bounds__(256) void norm_slab_stats_kernel(const T* __restric
 __global__ __launch_bounds__(256) void norm_slab_join_kernel(const float* __restrict__ partial, Slab S, float eps,
                                                              float* __restrict__ mean_out, float* __restrict__ rstd_out) {
   __shared__ double sh[256];
-  const int64_t ng = blockIdx.x, n = ng / S.G;
+  const int64_t ng = S.first + blockIdx.x, n = ng / S.G;
   const int g = (int)(ng % S.G);
   const int64_t all = S.slabs * S.cg;
   const float* p = partial + n * S.slabs * 2 * S.C + g * S.cg;
@@ -410,7 +410,7 @@ __global__ __launch_bounds__(256) void norm_slab_apply_kernel(const T* __restric
                                                               const float* __restrict__ rstd, T* __restrict__ y) {
   const int cper = 256 / S.rper;
   const int r = threadIdx.x / cper, cc = threadIdx.x % cper;
-  int64_t blk = blockIdx.x;
+  int64_t blk = S.first + blockIdx.x;
   const int cb = (int)(blk % S.cblocks);
   blk /= S.cblocks;
   const int64_t sl = blk % S.slabs, n = blk / S.slabs;
@@ -449,7 +449,7 @@ __global__ __launch_bounds__(256) void norm_slab_back_stats_kernel(const T* __re
   __shared__ float s1[256 * V], s2[256 * V];
   const int cper = 256 / S.rper;
   const int r = threadIdx.x / cper, cc = threadIdx.x % cper;
-  int64_t blk = blockIdx.x;
+  int64_t blk = S.first + blockIdx.x;
   const int cb = (int)(blk % S.cblocks);
   blk /= S.cblocks;
   const int64_t sl = blk % S.slabs, n = blk / S.slabs;
@@ -511,7 +511,7 @@ __global__ __launch_bounds__(256) void norm_slab_back_stats_kernel(const T* __re
 __global__ __launch_bounds__(256) void norm_slab_back_join_kernel(const float* __restrict__ partial, Affine aff, Slab S,
                                                                   float* __restrict__ sums) {
   __shared__ double s1[256], s2[256];
-  const int64_t ng = blockIdx.x, n = ng / S.G;
+  const int64_t ng = S.first + blockIdx.x, n = ng / S.G;
   const int g = (int)(ng % S.G);
   const int64_t all = S.slabs * S.cg;
   const float* p = partial + n * S.slabs * 2 * S.C + g * S.cg;
@@ -547,7 +547,7 @@ __global__ __launch_bounds__(256) void norm_slab_back_apply_kernel(const T* __re
                                                                    const float* __restrict__ sums, T* __restrict__ dx) {
   const int cper = 256 / S.rper;
   const int r = threadIdx.x / cper, cc = threadIdx.x % cper;
-  int64_t blk = blockIdx.x;
+  int64_t blk = S.first + blockIdx.x;
   const int cb = (int)(blk % S.cblocks);
   blk /= S.cblocks;
   const int64_t sl = blk % S.slabs, n = blk / S.slabs;
@@ -665,7 +665,7 @@ int norm_run(const ttc_group_norm_args& A, const NormPlan& P, hipStream_t s) {
     auto go = [&](auto nv) {
       constexpr int NV = decltype(nv)::value;
       const int64_t blocks = P.slabs * P.R.gblocks;
-      if (blocks > MAX_GRID) return TTC_LQR_EINVAL;
+      if (blocks > max_blocks(256)) return TTC_LQR_EINVAL;
       const dim3 grid((unsigned)blocks);
       if (!A.backward) {
         hipLaunchKernelGGL((norm_row_kernel<T, V, NV, SILU, GATE>), grid, dim3(256), 0, s, x, gate, aff, P.R, eps,
@@ -683,27 +683,41 @@ int norm_run(const ttc_group_norm_args& A, const NormPlan& P, hipStream_t s) {
     if (rc != TTC_LQR_OK) return rc;
     parts = P.slabs * P.R.rper;
   } else {
-    const Slab& S = P.S;
-    const int64_t blocks = A.n * S.slabs * S.cblocks;
-    if (blocks > MAX_GRID || A.n * G > MAX_GRID) return TTC_LQR_EINVAL;
-    const dim3 grid((unsigned)blocks), block(256), join((unsigned)(A.n * G));
+    Slab S = P.S;
+    const int64_t blocks = A.n * S.slabs * S.cblocks, joins = A.n * G;
+    const dim3 block(256);
     float* extra = ws + A.n * S.slabs * 2 * A.c;
+    int rc = TTC_LQR_OK;
+    auto each = [&](int64_t n, auto go) {
+      if (rc == TTC_LQR_OK)
+        rc = in_launches(n, 256, [&](int64_t first, dim3 grid) {
+          S.first = first;
+          go(grid);
+        });
+    };
     if (!A.backward) {
       float* mean = A.mean ? A.mean : extra;
       float* rstd = A.mean ? A.rstd : extra + A.n * G;
-      hipLaunchKernelGGL((norm_slab_stats_kernel<T, V>), grid, block, 0, s, x, S, ws);
-      hipLaunchKernelGGL(norm_slab_join_kernel, join, block, 0, s, ws, S, eps, mean, rstd);
-      hipLaunchKernelGGL((norm_slab_apply_kernel<T, V, SILU, GATE>), grid, block, 0, s, x, gate, aff, S, mean, rstd,
-                         static_cast<T*>(A.y));
-      return launched();
+      each(blocks, [&](dim3 g) { hipLaunchKernelGGL((norm_slab_stats_kernel<T, V>), g, block, 0, s, x, S, ws); });
+      each(joins, [&](dim3 g) { hipLaunchKernelGGL(norm_slab_join_kernel, g, block, 0, s, ws, S, eps, mean, rstd); });
+      each(blocks, [&](dim3 g) {
+        hipLaunchKernelGGL((norm_slab_apply_kernel<T, V, SILU, GATE>), g, block, 0, s, x, gate, aff, S, mean, rstd,
+                           static_cast<T*>(A.y));
+      });
+      return rc;
     }
-    hipLaunchKernelGGL((norm_slab_back_stats_kernel<T, V, SILU, GATE>), grid, block, 0, s, x, gate, dy, aff, S, A.mean,
-                       A.rstd, static_cast<T*>(A.dgate), ws);
+    each(blocks, [&](dim3 g) {
+      hipLaunchKernelGGL((norm_slab_back_stats_kernel<T, V, SILU, GATE>), g, block, 0, s, x, gate, dy, aff, S, A.mean, A.rstd,
+                         static_cast<T*>(A.dgate), ws);
+    });
     if (A.dx) {
-      hipLaunchKernelGGL(norm_slab_back_join_kernel, join, block, 0, s, ws, aff, S, extra);
-      hipLaunchKernelGGL((norm_slab_back_apply_kernel<T, V, SILU, GATE>), grid, block, 0, s, x, gate, dy, aff, S, A.mean,
-                         A.rstd, extra, static_cast<T*>(A.dx));
+      each(joins, [&](dim3 g) { hipLaunchKernelGGL(norm_slab_back_join_kernel, g, block, 0, s, ws, aff, S, extra); });
+      each(blocks, [&](dim3 g) {
+        hipLaunchKernelGGL((norm_slab_back_apply_kernel<T, V, SILU, GATE>), g, block, 0, s, x, gate, dy, aff, S, A.mean,
+                           A.rstd, extra, static_cast<T*>(A.dx));
+      });
     }
+    if (rc != TTC_LQR_OK) return rc;
     parts = A.n * S.slabs;
   }
   if (A.dweight || A.dbias) {

@@ -30,8 +30,8 @@ template <class T, int V, bool INTER, int HEADS>
 __global__ __launch_bounds__(256) void rotary_kernel(const T* __restrict__ q, const T* __restrict__ k,
                                                      T* __restrict__ yq, T* __restrict__ yk,
                                                      const float* __restrict__ table, const void* __restrict__ pos,
-                                                     int pos_bytes, RotaryShape S, int64_t items) {
-  const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
+                                                     int pos_bytes, RotaryShape S, int64_t first, int64_t items) {
+  const int64_t item = (first + blockIdx.x) * 256 + threadIdx.x;
   if (item >= items) return;
   const int col = (int)(item % S.cols);
   const int64_t rest = item / S.cols;
@@ -115,14 +115,13 @@ int rotary_launch(const ttc_rotary_args& A, RotaryShape& S, hipStream_t s) {
   const int64_t tokens = A.batch * A.tokens, heads = S.H0 + S.H1;
   const int per = tokens * heads * S.cols >= (int64_t)4 * 256 * 1024 ? 4 : 1;
   S.groups = (int)ceil_div(heads, per);
-  const int64_t items = tokens * S.groups * S.cols, blocks = ceil_div(items, 256);
-  if (items == 0) return TTC_LQR_OK;
-  if (blocks > MAX_GRID) return TTC_LQR_EINVAL;
+  const int64_t items = tokens * S.groups * S.cols;
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, s, static_cast<const T*>(A.x[0]),
-                       static_cast<const T*>(A.x[1]), static_cast<T*>(A.y[0]), static_cast<T*>(A.y[1]), A.table,
-                       A.positions, (int)A.position_bytes, S, items);
-    return launched();
+    return in_launches(ceil_div(items, 256), 256, [&](int64_t first, dim3 grid) {
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, static_cast<const T*>(A.x[0]), static_cast<const T*>(A.x[1]),
+                         static_cast<T*>(A.y[0]), static_cast<T*>(A.y[1]), A.table, A.positions, (int)A.position_bytes,
+                         S, first, items);
+    });
   };
   if (inter) return per == 4 ? go(rotary_kernel<T, V, true, 4>) : go(rotary_kernel<T, V, true, 1>);
   return per == 4 ? go(rotary_kernel<T, V, false, 4>) : go(rotary_kernel<T, V, false, 1>);
