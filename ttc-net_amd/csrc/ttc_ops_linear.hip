@@ -4,43 +4,51 @@
 
 namespace ttc {
 
-// Token by token with the state in registers: a workgroup holds 32 columns of one head's state, a thread 4 of them for
-// RPT rows.  For one token it reads and writes the state once (8 bytes an element against 5 flops): bound by memory.
-template <class T, int RPT>
+// Token by token with the state in registers: a workgroup holds 4 LR columns of one head's state, a thread 4 of them for RPT
+// rows.  For one token it reads and writes the state once (8 bytes an element against 5 flops): bound by memory.
+template <class T, int RPT, int LR>
 __global__ __launch_bounds__(256) void token_sweep_kernel(Sweep A, int tiles, bool wide) {
-  __shared__ float part[2][4][32];
+  constexpr int COLS = 4 * LR, STEP = 256 / LR;  // columns of a workgroup, rows between a thread's
+  __shared__ float part[2][4][COLS];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int tile = (int)(blockIdx.x % tiles);
   const int64_t bh = blockIdx.x / tiles, b = bh / A.H;
   const int h = (int)(bh % A.H);
-  const int e0 = tile * 32 + (lane & 7) * 4, r0 = wave * 8 + (lane >> 3);
+  const int e0 = tile * COLS + lane % LR * 4, r0 = wave * (64 / LR) + lane / LR;
   const int64_t slot = A.slots ? A.slots[b] : b;
   T* out = static_cast<T*>(A.out) + (b * A.T * A.H + h) * (int64_t)A.vd;
   float* outf = static_cast<float*>(A.out) + (b * A.T * A.H + h) * (int64_t)A.vd;
   if (slot < 0 || slot >= A.nslots) {  // a row without a state
     for (int64_t t = 0; t < A.T; ++t)
-      for (int j = threadIdx.x; j < 32 && tile * 32 + j < A.vd; j += 256) {
-        const int64_t at = t * A.H * (int64_t)A.vd + tile * 32 + j;
+      for (int j = threadIdx.x; j < COLS && tile * COLS + j < A.vd; j += 256) {
+        const int64_t at = t * A.H * (int64_t)A.vd + tile * COLS + j;
         if (A.out_f32) outf[at] = 0.0f; else out[at] = from_f<T>(0.0f);
       }
     return;
   }
   const int64_t base = (slot * A.H + h) * (int64_t)A.kd * A.vd;
+  // Loads come from the nearest place that exists and are dropped afterwards: in branches, each would wait for the last
   float S[RPT][4];
+  const bool held[4] = {e0 < A.vd, e0 + 1 < A.vd, e0 + 2 < A.vd, e0 + 3 < A.vd};
+  auto row_at = [&](int i) { return r0 + STEP * i < A.kd ? r0 + STEP * i : A.kd - 1; };
+  auto col_at = [&](int j) { return held[j] ? e0 + j : A.vd - 1; };
+  if (A.state_in == nullptr) {
 #pragma unroll
-  for (int i = 0; i < RPT; ++i) {
-    const int r = r0 + 32 * i;
-    if (A.state_in == nullptr || r >= A.kd) {
+    for (int i = 0; i < RPT; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) S[i][j] = 0.0f;
-    } else if (wide) {
-      const float4 f = e0 < A.vd ? *reinterpret_cast<const float4*>(A.state_in + base + r * A.sr + e0)
-                                 : make_float4(0.f, 0.f, 0.f, 0.f);
-      S[i][0] = f.x, S[i][1] = f.y, S[i][2] = f.z, S[i][3] = f.w;
-    } else {
+  } else if (wide) {
+    float4 f[RPT];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) S[i][j] = e0 + j < A.vd ? A.state_in[base + r * A.sr + (e0 + j) * A.sc] : 0.0f;
-    }
+    for (int i = 0; i < RPT; ++i)
+      f[i] = *reinterpret_cast<const float4*>(A.state_in + base + row_at(i) * A.sr + (held[0] ? e0 : 0));
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) S[i][0] = f[i].x, S[i][1] = f[i].y, S[i][2] = f[i].z, S[i][3] = f[i].w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < RPT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) S[i][j] = A.state_in[base + row_at(i) * A.sr + col_at(j) * A.sc];
   }
   const T *q = A.q.at<T>(b, h), *k = A.k.at<T>(b, h), *v = A.v.at<T>(b, h);
   const T* x = A.x.p ? A.x.at<T>(b, h) : nullptr;
@@ -48,37 +56,40 @@ __global__ __launch_bounds__(256) void token_sweep_kernel(Sweep A, int tiles, bo
   for (int64_t n = 0; n < A.T; ++n) {
     const int64_t t = A.reverse ? A.T - 1 - n : n;
     const float lg = !A.reverse ? gamma_at(A, g + t * A.gt) : n == 0 ? 0.0f : gamma_at(A, g + (t + 1) * A.gt);
-    const float decay = expf(lg);
-    float vv[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
+    float vv[4], kk[RPT], qq[RPT], acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) vv[j] = e0 + j < A.vd ? to_f(v[t * A.v.st + e0 + j]) : 0.0f;
+    for (int j = 0; j < 4; ++j) vv[j] = to_f(v[t * A.v.st + col_at(j)]);
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
-      const int r = r0 + 32 * i;
-      if (r < A.kd) {
-        const float kk = to_f(k[t * A.k.st + r]) * A.key_scale, qq = to_f(q[t * A.q.st + r]);
+      kk[i] = to_f(k[t * A.k.st + row_at(i)]);
+      qq[i] = to_f(q[t * A.q.st + row_at(i)]);
+    }
+    const float decay = expf(lg);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          S[i][j] = lg < RESET ? kk * vv[j] : fmaf(S[i][j], decay, kk * vv[j]);
-          acc[j] = fmaf(qq, S[i][j], acc[j]);
-        }
+    for (int i = 0; i < RPT; ++i) {
+      const bool row = r0 + STEP * i < A.kd;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float add = kk[i] * A.key_scale * vv[j];
+        S[i][j] = lg < RESET ? add : fmaf(S[i][j], decay, add);
+        acc[j] = row ? fmaf(qq[i], S[i][j], acc[j]) : acc[j];
       }
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
-      for (int m = 8; m <= 32; m <<= 1) acc[j] += __shfl_xor(acc[j], m, 64);
-      if (lane < 8) part[n & 1][wave][lane * 4 + j] = acc[j];
+      for (int m = LR; m <= 32; m <<= 1) acc[j] += __shfl_xor(acc[j], m, 64);
+      if (lane < LR) part[n & 1][wave][lane * 4 + j] = acc[j];
     }
     __syncthreads();  // the next token writes the other buffer, and meets this barrier before it comes back to this one
-    if (threadIdx.x < 32) {
-      const int j = threadIdx.x, e = tile * 32 + j;
+    if (threadIdx.x < COLS) {
+      const int j = threadIdx.x, e = tile * COLS + j;
       float o = (part[n & 1][0][j] + part[n & 1][1][j] + part[n & 1][2][j] + part[n & 1][3][j]) * A.out_scale;
       const int64_t at = t * A.H * (int64_t)A.vd + e;
       if (e < A.vd && A.out) {
         if (A.out_f32) outf[at] = o; else out[at] = from_f<T>(o);
       }
-      if (x) {
+      if (x) {  // COLS is 32
         const float d = lane_sum(e < A.vd ? o * to_f(x[t * A.x.st + e]) : 0.0f, 32);
         if (j == 0) A.dots[(tile * A.B * A.H + bh) * A.T + t] = d;
       }
@@ -89,7 +100,7 @@ __global__ __launch_bounds__(256) void token_sweep_kernel(Sweep A, int tiles, bo
   const float last = expf(lg);
 #pragma unroll
   for (int i = 0; i < RPT; ++i) {
-    const int r = r0 + 32 * i;
+    const int r = r0 + STEP * i;
     if (r >= A.kd) continue;
 #pragma unroll
     for (int j = 0; j < 4; ++j) S[i][j] = !A.reverse ? S[i][j] : lg < RESET ? 0.0f : S[i][j] * last;
@@ -104,10 +115,11 @@ __global__ __launch_bounds__(256) void token_sweep_kernel(Sweep A, int tiles, bo
   }
 }
 
-inline int token_tiles(int vd) { return (vd + 31) / 32; }
+inline int token_tiles(int vd) { return (vd + 31) / 32; }  // of the sweeps that give dots
 
-int launch_token_sweep(const Sweep& A, bool bf16, hipStream_t s) {
-  const int tiles = token_tiles(A.vd);
+template <class T, int LR>
+int launch_token_tile(const Sweep& A, hipStream_t s) {
+  const int tiles = (A.vd + 4 * LR - 1) / (4 * LR);
   const int64_t blocks = A.B * A.H * tiles;
   if (blocks == 0) return TTC_LQR_OK;
   if (blocks > max_blocks(256)) return TTC_LQR_EINVAL;
@@ -116,11 +128,17 @@ int launch_token_sweep(const Sweep& A, bool bf16, hipStream_t s) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, s, A, tiles, wide);
     return launched();
   };
-  if (bf16)
-    return A.kd <= 32 ? go(token_sweep_kernel<__bf16, 1>) : A.kd <= 64 ? go(token_sweep_kernel<__bf16, 2>)
-                                                                       : go(token_sweep_kernel<__bf16, 4>);
-  return A.kd <= 32 ? go(token_sweep_kernel<float, 1>) : A.kd <= 64 ? go(token_sweep_kernel<float, 2>)
-                                                                    : go(token_sweep_kernel<float, 4>);
+  constexpr int R = LR / 8;  // passes over 32 rows
+  return A.kd <= 32   ? go(token_sweep_kernel<T, R, LR>)
+         : A.kd <= 64 ? go(token_sweep_kernel<T, 2 * R, LR>)
+                      : go(token_sweep_kernel<T, 4 * R, LR>);
+}
+
+int launch_token_sweep(const Sweep& A, bool bf16, hipStream_t s) {
+  // Whole rows of a state a workgroup where there are enough heads to fill the GPU that way, 32 columns otherwise
+  const bool rows = A.x.p == nullptr && A.vd > 64 && A.B * A.H >= 1024;
+  if (bf16) return rows ? launch_token_tile<__bf16, 32>(A, s) : launch_token_tile<__bf16, 8>(A, s);
+  return rows ? launch_token_tile<float, 32>(A, s) : launch_token_tile<float, 8>(A, s);
 }
 
 // Segments' own contributions to the states in front of them: state_in, then decay * state + contribution
