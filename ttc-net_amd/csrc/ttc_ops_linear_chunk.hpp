@@ -239,6 +239,19 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
 #pragma unroll
         for (int i = 0; i < 4; ++i) S[d][e][i] = f((float)S[d][e][i], 16 * d + r + i, c + 16 * e);
   };
+  // a state in memory (NULL: zero): loads and stores bounded, since those in branches would wait for each other
+  auto state_of = [&](const float* p) { return bounded(p, p ? A.kd * A.vd * 4 : 0); };
+  auto entry = [&](int r, int c, int sr, int sc) { return r < A.kd && c < A.vd ? (r * sr + c * sc) * 4 : BEYOND; };
+  auto load_f = [&](__amdgpu_buffer_rsrc_t from, int off) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(from, off, 0, 0));
+  };
+  auto put_state = [&](float* p, int sr, int sc) {
+    const auto to = state_of(p);
+    each([&](float s, int r, int c) {
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s), to, entry(r, c, sr, sc), 0, 0);
+      return s;
+    });
+  };
   {
     const float* p = nullptr;
     int sr = A.sr, sc = A.sc;
@@ -250,13 +263,15 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
         p = A.state_in + bh * elems;
       }
     }
-    each([&](float, int r, int c) { return p && r < A.kd && c < A.vd ? p[r * sr + c * sc] : 0.0f; });
+    const auto from = state_of(p);
+    each([&](float, int r, int c) { return load_f(from, entry(r, c, sr, sc)); });
   }
   // <S, p>, the wave's part of it: the decays' gradient at a boundary
   auto meet = [&](const float* p, int sr, int sc, float w, int64_t mark) {
     float d = 0.0f;
+    const auto from = state_of(p);
     each([&](float s, int r, int c) {
-      if (r < A.kd && c < A.vd) d = fmaf(s, p[r * sr + c * sc], d);
+      d = fmaf(s, load_f(from, entry(r, c, sr, sc)), d);  // both are 0 where there is no row or column
       return s;
     });
     d = lane_sum(d, 64);
@@ -385,33 +400,29 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
     Four xs[DOTS ? Z::TT : 1][Z::ET];
     if constexpr (DOTS) {
       if (x) {
+        const auto xrows = bounded(x + low * A.x.st, left * (int)A.x.st * (int)sizeof(T));
 #pragma unroll
         for (int t = 0; t < Z::TT; ++t) {
           const int r = place(16 * t + n);
-          const T* p = x + (low + r) * A.x.st;
 #pragma unroll
           for (int e = 0; e < Z::ET; ++e) {
             const int c = e0 + 16 * e + 4 * g;
+            if constexpr (WIDE) {
+              const int off = c < A.vd ? (r * (int)A.x.st + c) * (int)sizeof(T) : BEYOND;
+              if constexpr (sizeof(T) == 2)
+                xs[t][e] = __builtin_bit_cast(Four, __builtin_amdgcn_raw_buffer_load_b64(xrows, off, 0, 0));
+              else
+                xs[t][e] = __builtin_bit_cast(Four, __builtin_amdgcn_raw_buffer_load_b128(xrows, off, 0, 0));
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) xs[t][e].v[i] = from_f<T>(0.0f);
-            if (r < left) {
-              if (WIDE) {
-                if (c < A.vd) xs[t][e] = *reinterpret_cast<const Four*>(p + c);
-              } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  if (c + i < A.vd) xs[t][e].v[i] = p[c + i];
-              }
+              for (int i = 0; i < 4; ++i)
+                xs[t][e].v[i] = r < left && c + i < A.vd ? x[(low + r) * A.x.st + c + i] : from_f<T>(0.0f);
             }
           }
         }
       }
       if (A.states && !A.reverse && at > 0 && at % A.mark_tokens == 0) {  // the state in front of a boundary
-        float* p = A.states + (bh * A.marks + at / A.mark_tokens) * elems;
-        each([&](float s, int r, int c) {
-          if (r < A.kd && c < A.vd) p[r * A.vd + c] = s;
-          return s;
-        });
+        put_state(A.states + (bh * A.marks + at / A.mark_tokens) * elems, A.vd, 1);
       }
     }
 
@@ -630,11 +641,7 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
       each([&](float s, int, int) { return kept(last, s); });
     }
   }
-  if (p)
-    each([&](float s, int r, int c) {
-      if (r < A.kd && c < A.vd) p[r * sr + c * sc] = s;
-      return s;
-    });
+  if (p) put_state(p, sr, sc);
 }
 
 template <class T, int KD, int VD, int MODE>
