@@ -4,17 +4,20 @@
 
 namespace ttc {
 
-// Token by token with the state in registers: a workgroup holds 4 LR columns of one head's state, a thread 4 of them for RPT
-// rows.  For one token it reads and writes the state once (8 bytes an element against 5 flops): bound by memory.
-template <class T, int RPT, int LR>
+// Token by token with the state in registers: a workgroup holds 32 columns of one head's state, a thread 4 of them for RPT
+// rows.  For one token it reads and writes the state once (8 bytes an element against 5 flops): bound by memory.  192
+// sequences x 16 states of 128 x 128 in a pool: 86 us for 406 MB, 4.7 TB/s where a copy of 1 GiB reaches 5.2; one sequence of
+// 8 states of 64 x 64: 4.6 us, of which the loads' latency is most.  Whole rows of 128 columns a workgroup take the same
+// (61.8 us against 61.1 for states in a row), and leave too few workgroups for few sequences (6.7 us against 4.7).
+template <class T, int RPT>
 __global__ __launch_bounds__(256) void token_sweep_kernel(Sweep A, int tiles, bool wide) {
-  constexpr int COLS = 4 * LR, STEP = 256 / LR;  // columns of a workgroup, rows between a thread's
+  constexpr int COLS = 32, STEP = 32;  // columns of a workgroup, rows between a thread's
   __shared__ float part[2][4][COLS];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int tile = (int)(blockIdx.x % tiles);
   const int64_t bh = blockIdx.x / tiles, b = bh / A.H;
   const int h = (int)(bh % A.H);
-  const int e0 = tile * COLS + lane % LR * 4, r0 = wave * (64 / LR) + lane / LR;
+  const int e0 = tile * COLS + (lane & 7) * 4, r0 = wave * 8 + (lane >> 3);
   const int64_t slot = A.slots ? A.slots[b] : b;
   T* out = static_cast<T*>(A.out) + (b * A.T * A.H + h) * (int64_t)A.vd;
   float* outf = static_cast<float*>(A.out) + (b * A.T * A.H + h) * (int64_t)A.vd;
@@ -78,8 +81,8 @@ __global__ __launch_bounds__(256) void token_sweep_kernel(Sweep A, int tiles, bo
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
-      for (int m = LR; m <= 32; m <<= 1) acc[j] += __shfl_xor(acc[j], m, 64);
-      if (lane < LR) part[n & 1][wave][lane * 4 + j] = acc[j];
+      for (int m = 8; m <= 32; m <<= 1) acc[j] += __shfl_xor(acc[j], m, 64);
+      if (lane < 8) part[n & 1][wave][lane * 4 + j] = acc[j];
     }
     __syncthreads();  // the next token writes the other buffer, and meets this barrier before it comes back to this one
     if (threadIdx.x < COLS) {
@@ -89,7 +92,7 @@ __global__ __launch_bounds__(256) void token_sweep_kernel(Sweep A, int tiles, bo
       if (e < A.vd && A.out) {
         if (A.out_f32) outf[at] = o; else out[at] = from_f<T>(o);
       }
-      if (x) {  // COLS is 32
+      if (x) {
         const float d = lane_sum(e < A.vd ? o * to_f(x[t * A.x.st + e]) : 0.0f, 32);
         if (j == 0) A.dots[(tile * A.B * A.H + bh) * A.T + t] = d;
       }
@@ -115,11 +118,10 @@ __global__ __launch_bounds__(256) void token_sweep_kernel(Sweep A, int tiles, bo
   }
 }
 
-inline int token_tiles(int vd) { return (vd + 31) / 32; }  // of the sweeps that give dots
+inline int token_tiles(int vd) { return (vd + 31) / 32; }
 
-template <class T, int LR>
-int launch_token_tile(const Sweep& A, hipStream_t s) {
-  const int tiles = (A.vd + 4 * LR - 1) / (4 * LR);
+int launch_token_sweep(const Sweep& A, bool bf16, hipStream_t s) {
+  const int tiles = token_tiles(A.vd);
   const int64_t blocks = A.B * A.H * tiles;
   if (blocks == 0) return TTC_LQR_OK;
   if (blocks > max_blocks(256)) return TTC_LQR_EINVAL;
@@ -128,20 +130,15 @@ int launch_token_tile(const Sweep& A, hipStream_t s) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, s, A, tiles, wide);
     return launched();
   };
-  constexpr int R = LR / 8;  // passes over 32 rows
-  return A.kd <= 32   ? go(token_sweep_kernel<T, R, LR>)
-         : A.kd <= 64 ? go(token_sweep_kernel<T, 2 * R, LR>)
-                      : go(token_sweep_kernel<T, 4 * R, LR>);
+  if (bf16)
+    return A.kd <= 32 ? go(token_sweep_kernel<__bf16, 1>) : A.kd <= 64 ? go(token_sweep_kernel<__bf16, 2>)
+                                                                       : go(token_sweep_kernel<__bf16, 4>);
+  return A.kd <= 32 ? go(token_sweep_kernel<float, 1>) : A.kd <= 64 ? go(token_sweep_kernel<float, 2>)
+                                                                    : go(token_sweep_kernel<float, 4>);
 }
 
-int launch_token_sweep(const Sweep& A, bool bf16, hipStream_t s) {
-  // Whole rows of a state a workgroup where there are enough heads to fill the GPU that way, 32 columns otherwise
-  const bool rows = A.x.p == nullptr && A.vd > 64 && A.B * A.H >= 1024;
-  if (bf16) return rows ? launch_token_tile<__bf16, 32>(A, s) : launch_token_tile<__bf16, 8>(A, s);
-  return rows ? launch_token_tile<float, 32>(A, s) : launch_token_tile<float, 8>(A, s);
-}
-
-// Segments' own contributions to the states in front of them: state_in, then decay * state + contribution
+// Segments' own contributions to the states in front of them: state_in, then decay * state + contribution.  A thread walks
+// along one element of the state; 8 loads in flight (32 segments x 16 heads of 128 x 128: 15 us for 67 MB)
 __global__ __launch_bounds__(256) void segment_join_kernel(Sweep A, Segments G, int64_t blocks_a_head,
                                                            int64_t first) {
   const int64_t bh = (first + blockIdx.x) / blocks_a_head, elems = (int64_t)A.kd * A.vd;
@@ -166,7 +163,7 @@ __global__ __launch_bounds__(256) void segment_join_kernel(Sweep A, Segments G, 
   }
 }
 
-// Gradients of shared heads: out [rows, heads / share, d] = sums over `share` heads of in [rows, heads, d]
+// Gradients of shared heads, one pass over memory (3 x 509 x 12 heads of 48 to 4: 4.8 us, most of it the launch): out [rows, heads / share, d] = sums over `share` heads of in [rows, heads, d]
 template <class T>
 __global__ __launch_bounds__(256) void share_sum_kernel(const float* __restrict__ in, T* __restrict__ out, int64_t first,
                                                         int64_t n, int share, int d) {
@@ -181,7 +178,8 @@ __global__ __launch_bounds__(256) void share_sum_kernel(const float* __restrict_
 
 // dg_t = sum_{u >= t} (r_u - c_u) + what the boundary behind passes on: one wave per sequence, head and stretch between
 // boundaries, from its end, 8 tokens a lane at a time, in 64 bits (the sum's terms cancel).  A reset's own gradient is 0,
-// and nothing after it reaches tokens before it.
+// and nothing after it reaches tokens before it.  2,048 tokens x 128 heads: 8.6 us, bound by the latency of the loads and
+// of the sums across lanes.
 constexpr int GATE_TOKENS = 8;
 __global__ __launch_bounds__(64) void gate_kernel(Sweep A, const float* __restrict__ r, const float* __restrict__ c,
                                                   int tiles, int waves, const float* __restrict__ last,
@@ -273,11 +271,14 @@ __global__ __launch_bounds__(64) void gate_head_kernel(const double* __restrict_
 
 // ---- host ----------------------------------------------------------------------------------------------------
 
-// Up to this many tokens are swept one by one; more in chunks
+// Up to this many tokens are swept one by one; more in chunks.  8 heads of 128: 2, 4, 8 and 16 tokens take 5.8, 7.7, 12.0 and
+// 20.5 us one by one, 12.2 us in a chunk; 1,024 heads 26.5, 33.5, 48.0 and 78.9 us against 36
 constexpr int64_t TOKEN_SWEEP = 4;
 
-// Segments of a chunked sweep: enough workgroups to fill the GPU's 256 CUs twice; a segment's keys and values are read once
-// more for the state behind it, so heads that fill the GPU by themselves are not split
+// Segments of a chunked sweep: enough workgroups to fill the GPU's 256 CUs twice, as many as the registers of the largest
+// kernels let run; a segment's keys and values are read once more for the state behind it, so heads that fill the GPU by
+// themselves are not split.  Workgroups aimed at for 16,381 tokens x 16 heads of 128, and 2,048 x 128 heads of 64 forward
+// and backward: 256 182 and 560 us, 384 163 and 440, 512 142 and 367, 768 177 and 419, 1,024 171 and 377
 inline Segments segments_of(const ttc_linear_attention_args& A) {
   Segments G{};
   const int64_t chunks = ceil_div(A.tokens, chunk_tokens(A.dtype == TTC_DTYPE_BF16)), heads = A.batch * A.heads;

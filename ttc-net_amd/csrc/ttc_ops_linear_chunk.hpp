@@ -11,6 +11,15 @@
 //        the operand (rows 4 g + i and 16 + 4 g + i of 32 are the 8 a lane gives, on the other side too)
 //   S += K' (w V)   K' and V' by transposing reads of shared memory (bf16) or element by element (fp32).
 //
+// Bound.  At 64 x 64 with three workgroups a CU a chunk's 32 KB take 4,000 cycles, the rate of a copy; the matrix cores need
+// 700 of them, the vector ALU (weights, splits, conversions) about 2,000, shared memory 1,400.  At 128 x 128 registers leave
+// two workgroups a CU (a wave holds 32 columns of the state, 64 registers), whose phases between barriers do not cover each
+// other: 11,700 cycles for 64 KB.  16 columns a wave need twice the operand reads (2,048 tokens x 512 heads: 360 us, with
+// 32 columns 313).  Measured: 16,381 tokens x 16 heads of 128, bf16: 91 us (269 MB), after 52 us for the states between its
+// 32 segments (134 MB) and 15 us to join them; 2,048 x 128 heads of 64 (134 MB): FAST 48 us, EXACT 68, the segments' states
+// 24.  fp32 is bound by its matrix instructions: 2,048 tokens x 512 heads of 128 in 827 us, 101 TFLOP/s (a large library
+// product: 153).
+//
 // Numerics.  The sums G are held in 64 bits while they are formed and as pairs of fp32 after, so that differences of
 // large sums keep their digits; a decay of 0 is 2^-4096.  In bf16, w V is split into three bf16 parts (exact in fp32's 24
 // digits), so the state has fp32's accuracy; P and the state's copy in front of a chunk are rounded to bf16 for a bf16
