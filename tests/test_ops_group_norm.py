@@ -18,7 +18,7 @@ K = 96
 SHAPES = [  # x's shape, groups: rows of one to many lanes, odd sizes, one position and many
     ((1, 4), 1), ((3, 1), 1), ((5, 64), 8), ((16, 256), 2), ((7, 120), 6), ((2, 2048), 1), ((3, 4100), 2), ((9, 10), 10),
     ((4, 1, 48), 3), ((2, 5, 32), 4), ((1, 300, 24), 2), ((2, 9, 7, 15), 5), ((3, 65, 320), 32), ((1, 2, 4096), 2),
-    ((300, 96), 12), ((2, 1021, 12), 6)]
+    ((300, 96), 12), ((2, 1021, 12), 6), ((1, 9000, 6), 2), ((2, 5000, 32), 2)]
 
 
 def make(shape, dtype, device, seed, shift=0.0, scale=1.0):
@@ -184,7 +184,7 @@ def test_c_entry_refuses():
     from ttc.ops.group_norm import _BLOCK
     names = ["dtype", "wdtype", "n", "l", "c", "groups", "act", "backward", "eps", "x", "gate", "weight", "bias", "mean",
              "rstd", "y", "dy", "dx", "dgate", "dweight", "dbias", "ws", "size"]
-    base = dict.fromkeys(names, 0) | dict(n=2, l=3, c=8, groups=2, eps=1e-5, x=64, y=64, ws=64, size=1 << 20)
+    base = dict.fromkeys(names, 0) | dict(n=2, l=9000, c=8, groups=2, eps=1e-5, x=64, y=64, ws=64, size=1 << 20)
     pack = lambda **kw: _BLOCK.pack(*(base | kw).values())  # noqa: E731
     need = lib.ttc_group_norm_workspace_bytes(pack())
     assert need > 0 and lib.ttc_group_norm_workspace_bytes(pack(n=0)) == 0

@@ -11,7 +11,9 @@
 //    registers (up to 4 vectors of 16 bytes each), so x is read once and the variance is that of the centred values.
 //    8,192 x 2,048 in 32 groups, gated, bf16: forward 30 us (100 MB, 3.4 TB/s), backward 39 us (168 MB, 4.3 TB/s) and
 //    8 us for the sums of the weights' gradients; 16 x 2,048: 4.2 us;
-//  * any l: slabs of positions, each reduced over whole rows of c channels (coalesced); sums per channel are taken
+//  * a group that fits in a workgroup's registers, forward: one workgroup a group, x read once.  2 x 1,021 x 192 in 6 groups,
+//    bf16: 12 us, most of it latency (slabs 18);
+//  * any l, and every backward over several positions: slabs of positions, each reduced over whole rows of c channels (coalesced); sums per channel are taken
 //    about the slab's first position (a large common mean costs no digits) and joined as (mean, sum of squares)
 //    pairs; a second pass reads x again and writes y.  8 x 4,096 x 320 in 32 groups, fp32 (42 MB an array): forward
 //    13 + 8 + 17 us (statistics, join, output), backward 18 + 5 + 21 + 5 us; the caches hold x between the passes.
@@ -314,6 +316,72 @@ struct Slab {
   int C, G, cg, cols, rper, cblocks;  // cols: vectors of a row
 };
 
+// Groups that fit in a workgroup's registers, forward: one workgroup a group, x read once, one launch instead of three.
+// The group's l rows of cg channels are counted in vectors; thread t holds vectors t, t + 1024, ...
+constexpr int WHOLE = 8;  // vectors a thread
+template <class T, int V, bool SILU, bool GATE>
+__global__ __launch_bounds__(1024) void norm_whole_kernel(const T* __restrict__ x, const T* __restrict__ gate, Affine aff,
+                                                          Slab S, float eps, T* __restrict__ y, float* __restrict__ mean_out,
+                                                          float* __restrict__ rstd_out) {
+  __shared__ float part[16];
+  const int64_t ng = S.first + blockIdx.x, n = ng / S.G;
+  const int g = (int)(ng % S.G), cols = S.cg / V;
+  const int vecs = (int)S.L * cols;
+  const T *xg = x + n * S.L * S.C + g * S.cg, *gg = GATE ? gate + n * S.L * S.C + g * S.cg : nullptr;
+  T* yg = y + n * S.L * S.C + g * S.cg;
+  auto sum = [&](float v) {
+    v = lane_sum(v, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float r = 0.0f;
+    for (int i = 0; i < (int)blockDim.x / 64; ++i) r += part[i];
+    return r;
+  };
+  Vec<T, V> xv[WHOLE];
+  int64_t at[WHOLE];
+  float a = 0.0f;
+#pragma unroll
+  for (int k = 0; k < WHOLE; ++k) {  // loads from the last vector where there is none: in branches each would wait
+    const int i = (int)threadIdx.x + k * (int)blockDim.x, j = i < vecs ? i : vecs - 1;
+    at[k] = (int64_t)(j / cols) * S.C + j % cols * V;
+    xv[k] = *reinterpret_cast<const Vec<T, V>*>(xg + at[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < WHOLE; ++k)
+#pragma unroll
+    for (int j = 0; j < V; ++j) a += (int)threadIdx.x + k * (int)blockDim.x < vecs ? to_f(xv[k].v[j]) : 0.0f;
+  const float total = (float)S.L * S.cg, mean = sum(a) / total;
+  float q = 0.0f;
+#pragma unroll
+  for (int k = 0; k < WHOLE; ++k)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float d = to_f(xv[k].v[j]) - mean;
+      q = (int)threadIdx.x + k * (int)blockDim.x < vecs ? fmaf(d, d, q) : q;
+    }
+  const float rstd = 1.0f / sqrtf(sum(q) / total + eps);
+#pragma unroll
+  for (int k = 0; k < WHOLE; ++k) {
+    const int i = (int)threadIdx.x + k * (int)blockDim.x;
+    if (i >= vecs) break;
+    float w[V], b[V];
+    const int64_t c = (int64_t)g * S.cg + i % cols * V;
+    aff.load<V>(c, S.C, w, b);
+    Vec<T, V> gt, out;
+    if (GATE) gt = *reinterpret_cast<const Vec<T, V>*>(gg + at[k]);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      out.v[j] = from_f<T>(
+          out_of<SILU, GATE>(fmaf((to_f(xv[k].v[j]) - mean) * rstd, w[j], b[j]), GATE ? to_f(gt.v[j]) : 0.0f));
+    *reinterpret_cast<Vec<T, V>*>(yg + at[k]) = out;
+  }
+  if (threadIdx.x == 0 && mean_out) {
+    mean_out[ng] = mean;
+    rstd_out[ng] = rstd;
+  }
+}
+
 // (mean, M2) of `count` values per (n, slab, channel) -> partial [n, slabs, 2, c]
 template <class T, int V>
 __global__ __launch_bounds__(256) void norm_slab_stats_kernel(const T* __restrict__ x, Slab S,
@@ -591,6 +659,7 @@ __global__ __launch_bounds__(256) void norm_slab_back_apply_kernel(const T* __re
 struct NormPlan {
   bool rows;              // the one-position form
   int V, NV;
+  int whole;              // threads a group of the form in registers; 0: slabs
   Rows R;
   int64_t slabs;
   Slab S;
@@ -647,6 +716,19 @@ inline NormPlan norm_plan(const ttc_group_norm_args& A, bool wide) {
   const int cper = S.cols < 256 ? S.cols : 256;
   S.rper = 256 / cper;
   S.cblocks = (int)ceil_div(S.cols, 256 / S.rper);
+  if (!A.backward) {
+    const int Vw = wide && cg % full == 0 ? full : 1;
+    const int64_t v = ceil_div(cg, Vw) <= 1024 * WHOLE && A.l <= 1024 * WHOLE ? A.l * (cg / Vw) : 1024 * WHOLE + 1;
+    // Rows of less than 64 bytes a group are read in halves of what memory gives: large arrays of them take the slabs (64 x
+    // 1,024 x 512 in 32 groups, bf16: 53 us, whole 70; 16 x 1,024 x 512: 28, whole 23; 64 x 256 x 1,024 in 8 groups: 42, whole 24)
+    const bool narrow = cg * (A.dtype == TTC_DTYPE_F32 ? 4 : 2) < 64;
+    if (v <= 1024 * WHOLE && (!narrow || A.n * A.l * A.c <= 1 << 24)) {
+      P.V = Vw;
+      P.whole = (int)(ceil_div(ceil_div(v, WHOLE), 64) * 64);
+      if (P.whole < 256) P.whole = 256;
+      return P;
+    }
+  }
   const int64_t want = ceil_div(1024, A.n * S.cblocks);
   int64_t slab = ceil_div(A.l, want);
   slab = slab < 4 * S.rper ? 4 * S.rper : slab;
@@ -689,7 +771,6 @@ int norm_run(const ttc_group_norm_args& A, const NormPlan& P, hipStream_t s) {
     Slab S = P.S;
     const int64_t blocks = A.n * S.slabs * S.cblocks, joins = A.n * G;
     const dim3 block(256);
-    float* extra = ws + A.n * S.slabs * 2 * A.c;
     int rc = TTC_LQR_OK;
     auto each = [&](int64_t n, auto go) {
       if (rc == TTC_LQR_OK)
@@ -698,6 +779,15 @@ int norm_run(const ttc_group_norm_args& A, const NormPlan& P, hipStream_t s) {
           go(grid);
         });
     };
+    if (P.whole) {
+      rc = in_launches(joins, P.whole, [&](int64_t first, dim3 grid) {
+        S.first = first;
+        hipLaunchKernelGGL((norm_whole_kernel<T, V, SILU, GATE>), grid, dim3(P.whole), 0, s, x, gate, aff, S, eps,
+                           static_cast<T*>(A.y), A.mean, A.rstd);
+      });
+      return rc;
+    }
+    float* extra = ws + A.n * S.slabs * 2 * A.c;
     if (!A.backward) {
       float* mean = A.mean ? A.mean : extra;
       float* rstd = A.mean ? A.rstd : extra + A.n * G;
