@@ -188,6 +188,10 @@ def test_c_entry_refuses():
     pack = lambda **kw: _BLOCK.pack(*(base | kw).values())  # noqa: E731
     need = lib.ttc_group_norm_workspace_bytes(pack())
     assert need > 0 and lib.ttc_group_norm_workspace_bytes(pack(n=0)) == 0
+    for c in range(1, 9):  # fewer channels than a vector
+        for dtype in (0, 1):
+            assert lib.ttc_group_norm_workspace_bytes(pack(c=c, groups=1, l=90000, dtype=dtype)) > 0
+            assert lib.ttc_group_norm_workspace_bytes(pack(c=c, groups=c, l=2, dtype=dtype, backward=1)) > 0
     assert lib.ttc_group_norm_workspace_bytes(None) == 0 and lib.ttc_group_norm_workspace_bytes(pack(groups=3)) == 0
     for kw, code in [(dict(dtype=3), 2), (dict(wdtype=-1), 2), (dict(groups=3), 1), (dict(groups=0), 1), (dict(n=-1), 1),
                      (dict(l=-1), 1), (dict(c=-8), 1), (dict(act=2), 1), (dict(eps=-1.0), 1), (dict(eps=float("nan")), 1),

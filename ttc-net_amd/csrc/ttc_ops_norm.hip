@@ -678,6 +678,7 @@ inline NormPlan norm_plan(const ttc_group_norm_args& A, bool wide) {
   NormPlan P{};
   const int full = A.dtype == TTC_DTYPE_F32 ? 4 : 8;
   const int64_t cg = A.c / A.groups;
+  wide = wide && A.c % full == 0;
   const int Vr = wide && cg % full == 0 ? full : 1;
   const int64_t vecs = ceil_div(cg, Vr);
   P.rows = A.l == 1 && vecs <= 64 * 4;
