@@ -6,16 +6,16 @@
 //   dx = rstd (dxhat - mean(dxhat) - xhat mean(dxhat xhat)),  dw = sum dy0 xhat,  db = sum dy0,
 //   dgate = dy y0 act'(gate).
 //
-// Bound: memory.  Two forms:
+// Bound: memory.  Three forms:
 //  * one position (l = 1: a norm over each head of a token): a group is contiguous, up to 64 lanes hold it in
 //    registers (up to 4 vectors of 16 bytes each), so x is read once and the variance is that of the centred values.
 //    8,192 x 2,048 in 32 groups, gated, bf16: forward 30 us (100 MB, 3.4 TB/s), backward 39 us (168 MB, 4.3 TB/s) and
 //    8 us for the sums of the weights' gradients; 16 x 2,048: 4.2 us;
-//  * a group that fits in a workgroup's registers, forward: one workgroup a group, x read once.  2 x 1,021 x 192 in 6 groups,
-//    bf16: 12 us, most of it latency (slabs 18);
-//  * any l, and every backward over several positions: slabs of positions, each reduced over whole rows of c channels (coalesced); sums per channel are taken
-//    about the slab's first position (a large common mean costs no digits) and joined as (mean, sum of squares)
-//    pairs; a second pass reads x again and writes y.  8 x 4,096 x 320 in 32 groups, fp32 (42 MB an array): forward
+//  * a group that fits in a workgroup's registers, forward: one workgroup a group, x read once.
+//    2 x 1,021 x 192 in 6 groups, bf16: 12 us, most of it latency (slabs 18);
+//  * any other, and every backward over several positions: slabs of positions, each reduced over whole rows of c
+//    channels (coalesced); sums per channel are taken about the slab's first position (a large common mean costs no
+//    digits) and joined as (mean, sum of squares) pairs; a second pass reads x again and writes y.  8 x 4,096 x 320 in 32 groups, fp32 (42 MB an array): forward
 //    13 + 8 + 17 us (statistics, join, output), backward 18 + 5 + 21 + 5 us; the caches hold x between the passes.
 #include "ttc_ops_common.hpp"
 
