@@ -16,15 +16,17 @@
 // two workgroups a CU (a wave holds 32 columns of the state, 64 registers), whose phases between barriers do not cover each
 // other: 11,700 cycles for 64 KB.  16 columns a wave need twice the operand reads (2,048 tokens x 512 heads: 360 us, with
 // 32 columns 313).  Measured: 16,381 tokens x 16 heads of 128, bf16: 91 us (269 MB), after 52 us for the states between its
-// 32 segments (134 MB) and 15 us to join them; 2,048 x 128 heads of 64 (134 MB): FAST 48 us, EXACT 68, the segments' states
-// 24.  fp32 is bound by its matrix instructions: 2,048 tokens x 512 heads of 128 in 827 us, 101 TFLOP/s (a large library
+// 32 segments (134 MB) and 15 us to join them; 2,048 x 128 heads of 64 (134 MB): FAST 48 us, EXACT 61 with
+// its fourth input, the segments' states 24.  fp32 is bound by its matrix instructions: 2,048 tokens x 512 heads of 128 in 827 us, 101 TFLOP/s (a large library
 // product: 153).
 //
 // Numerics.  The sums G are held in 64 bits while they are formed and as pairs of fp32 after, so that differences of
 // large sums keep their digits; a decay of 0 is 2^-4096.  In bf16, w V is split into three bf16 parts (exact in fp32's 24
 // digits), so the state has fp32's accuracy; P and the state's copy in front of a chunk are rounded to bf16 for a bf16
-// output (FAST), and split into three parts too where the sum feeds the decays' gradient (EXACT), a long sum of
-// cancelling terms.  Weights that are 0 select: what is masked has no effect, whatever it holds.  Where a chunk's keys or
+// output (FAST).  The decays' gradient is a long sum of cancelling terms, so the dots x . o it is made of are not taken from
+// such an o (EXACT): P's part is sum_s P_ts (v_s . x_t), whose products are exact as they are, in fp32; the state's copy
+// is split into three parts.  (P split into three for an exact o instead: 2,048 x 128 heads of 64 68 us; training on
+// 8 x 2,048 x 32 heads of 128 1,170 us, so 1,058.)  Weights that are 0 select: what is masked has no effect, whatever it holds.  Where a chunk's keys or
 // values are not all finite, its sums over tokens are formed term by term instead, without the masked ones.
 #pragma once
 #include "ttc_ops_linear.hpp"
@@ -174,7 +176,7 @@ __device__ __forceinline__ float kept(float w, float x) { return w == 0.0f ? 0.0
 template <class T, int KD, int VD>
 struct ChunkShape {
   static constexpr int WAVES = sweep_waves(VD), NT = WAVES * 64, ET = VD / 16 / WAVES;  // a wave's columns: 16 ET
-  static constexpr int C = chunk_tokens(sizeof(T) == 2), TT = C / 16, KB = C / 32, DB = KD / 32, DT = KD / 16;
+  static constexpr int C = chunk_tokens(sizeof(T) == 2), TT = C / 16, KB = C / 32, DB = KD / 32, DT = KD / 16, VB = VD / 32;
   static constexpr int VEC = 16 / sizeof(T), QS = KD + Operand<T>::ROW_PAD, KS = KD + Operand<T>::COL_PAD,
                        VS = VD + Operand<T>::COL_PAD;
   static constexpr int KV = (C * KD / VEC + NT - 1) / NT, VV = (C * VD / VEC + NT - 1) / NT;  // 16-byte loads a thread
@@ -204,13 +206,18 @@ template <class T, int KD, int VD, int MODE, bool WIDE>
 __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_kernel(Sweep A, Segments G, Wides W) {
   using Z = ChunkShape<T, KD, VD>;
   using Op = Operand<T>;
-  using PT = std::conditional_t<MODE == EXACT, float, T>;  // the weighted scores in shared memory
-  constexpr bool DOTS = MODE == EXACT || (MODE == FAST && sizeof(T) == 4);
-  constexpr int C = Z::C, NT = Z::NT, VEC = Z::VEC, QS = Z::QS, KS = Z::KS, VS = Z::VS, PS = C + 16 / (int)sizeof(PT);
-  __shared__ __attribute__((aligned(16))) T Qs[MODE == STATE_ONLY ? 1 : C * QS];
-  __shared__ __attribute__((aligned(16))) T Ks[C * KS];
-  __shared__ __attribute__((aligned(16))) T Vs[C * VS];
-  __shared__ __attribute__((aligned(16))) PT Ps[MODE == STATE_ONLY ? 1 : C * PS];
+  // the dots x . o: from products of scores and of v . x (PAIRED), or from fp32's o as it is (DIRECT)
+  constexpr bool PAIRED = MODE == EXACT, DIRECT = MODE == FAST && sizeof(T) == 4, DOTS = PAIRED || DIRECT;
+  // With x there too, 128 x 128 stays below half of the 160 KB a CU has only if columns are padded as rows are and the last
+  // rows end without a pad.  (Without the pads' end FAST at 128 x 128 spills 24 registers.)
+  constexpr int C = Z::C, NT = Z::NT, VEC = Z::VEC, QS = Z::QS, XS = VD + Op::ROW_PAD,
+                KS = PAIRED && KD + VD > 192 ? QS : Z::KS, VS = PAIRED && KD + VD > 192 ? XS : Z::VS,
+                PS = C + 16 / (int)sizeof(T), TAIL = PAIRED ? 16 / (int)sizeof(T) : 0;
+  __shared__ __attribute__((aligned(16))) T Qs[MODE == STATE_ONLY ? 1 : C * QS - TAIL];
+  __shared__ __attribute__((aligned(16))) T Ks[C * KS - TAIL];
+  __shared__ __attribute__((aligned(16))) T Vs[C * VS - TAIL];
+  __shared__ __attribute__((aligned(16))) T Xs[PAIRED ? C * XS - TAIL : 1];
+  __shared__ __attribute__((aligned(16))) T Ps[MODE == STATE_ONLY ? 1 : C * PS - TAIL];  // the weighted scores
   __shared__ __attribute__((aligned(16))) float Hi[2][C], Lo[2][C], In[2][C], Up[2][C];
   __shared__ float Whole[2], Dot[DOTS ? Z::WAVES : 1][C];
   __shared__ int Odd[Z::WAVES];
@@ -288,8 +295,8 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
   };
   if (DOTS && A.joins && A.reverse && seg == 0 && A.last) meet(A.last + bh * elems, A.sr, A.sc, 1.0f, A.marks);
 
-  u32x4 qr[Z::KV], kr[Z::KV], vr[Z::VV];
-  int ko[Z::KV], qo[Z::KV], vo[Z::VV];  // offsets of this thread's 16 bytes from the chunk's lowest address
+  u32x4 qr[Z::KV], kr[Z::KV], vr[Z::VV], xr[Z::VV];
+  int ko[Z::KV], qo[Z::KV], vo[Z::VV], xo[Z::VV];  // offsets of this thread's 16 bytes from the chunk's lowest address
   auto offsets = [&](int64_t st, int dim, auto& o, auto width) {
     constexpr int D = decltype(width)::value;
 #pragma unroll
@@ -302,6 +309,7 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
     offsets(A.k.st, A.kd, ko, std::integral_constant<int, KD>{});
     if constexpr (MODE != STATE_ONLY) offsets(A.q.st, A.kd, qo, std::integral_constant<int, KD>{});
     offsets(A.v.st, A.vd, vo, std::integral_constant<int, VD>{});
+    if constexpr (PAIRED) offsets(A.x.st, A.vd, xo, std::integral_constant<int, VD>{});
   }
   auto fetch_side = [&](const T* p, int64_t st, int dim, int64_t at, auto& r, const auto& o, auto width) {
     constexpr int D = decltype(width)::value;
@@ -323,6 +331,7 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
     fetch_side(k, A.k.st, A.kd, at, kr, ko, std::integral_constant<int, KD>{});
     if constexpr (MODE != STATE_ONLY) fetch_side(q, A.q.st, A.kd, at, qr, qo, std::integral_constant<int, KD>{});
     fetch_side(v, A.v.st, A.vd, at, vr, vo, std::integral_constant<int, VD>{});
+    if constexpr (PAIRED) fetch_side(x, A.x.st, A.vd, at, xr, xo, std::integral_constant<int, VD>{});
   };
   // One wave: a chunk's decays, one a lane (before a token in reverse order, that of the one after it), as they are stored
   constexpr int GATES = Z::WAVES - 1;
@@ -352,7 +361,7 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
       if (lane == C - 1) Whole[buf] = in;
     }
   };
-  auto put_dots = [&](int64_t at) {  // after the barrier behind the chunk
+  auto put_dots = [&](int64_t at) {  // after the barrier behind what a chunk's waves left
     if constexpr (DOTS) {
       if (x && tid < C && place(tid) < left_of(at)) {
         float d = 0.0f;
@@ -390,10 +399,11 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
     stage(Ks, KS, kr, std::integral_constant<int, KD>{}, true);
     if constexpr (MODE != STATE_ONLY) stage(Qs, QS, qr, std::integral_constant<int, KD>{}, false);
     stage(Vs, VS, vr, std::integral_constant<int, VD>{}, true);
+    if constexpr (PAIRED) stage(Xs, XS, xr, std::integral_constant<int, VD>{}, false);
     const bool odd_here = __ballot(!Op::finite(most)) != 0;
     if (lane == 0) Odd[wave] = odd_here;
     __syncthreads();
-    if (at > u0) put_dots(at - C);
+    if (DIRECT && at > u0) put_dots(at - C);
     bool odd = false;
 #pragma unroll
     for (int w = 0; w < Z::WAVES; ++w) odd = odd || Odd[w];
@@ -406,8 +416,8 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
       gate = gate_bits(at + 2 * C);
     }
     struct alignas(4 * sizeof(T)) Four { T v[4]; };
-    Four xs[DOTS ? Z::TT : 1][Z::ET];
-    if constexpr (DOTS) {
+    Four xs[DIRECT ? Z::TT : 1][Z::ET];
+    if constexpr (DIRECT) {
       if (x) {
         const auto xrows = bounded(x + low * A.x.st, left * (int)A.x.st * (int)sizeof(T));
 #pragma unroll
@@ -418,10 +428,7 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
             const int c = e0 + 16 * e + 4 * g;
             if constexpr (WIDE) {
               const int off = c < A.vd ? (r * (int)A.x.st + c) * (int)sizeof(T) : BEYOND;
-              if constexpr (sizeof(T) == 2)
-                xs[t][e] = __builtin_bit_cast(Four, __builtin_amdgcn_raw_buffer_load_b64(xrows, off, 0, 0));
-              else
-                xs[t][e] = __builtin_bit_cast(Four, __builtin_amdgcn_raw_buffer_load_b128(xrows, off, 0, 0));
+              xs[t][e] = __builtin_bit_cast(Four, __builtin_amdgcn_raw_buffer_load_b128(xrows, off, 0, 0));
             } else {
 #pragma unroll
               for (int i = 0; i < 4; ++i)
@@ -430,12 +437,15 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
           }
         }
       }
+    }
+    if constexpr (DOTS) {
       if (A.states && !A.reverse && at > 0 && at % A.mark_tokens == 0) {  // the state in front of a boundary
         put_state(A.states + (bh * A.marks + at / A.mark_tokens) * elems, A.vd, 1);
       }
     }
 
     f32x4 O[Z::TT][Z::ET];
+    float dots[PAIRED ? Z::TT : 1] = {};  // this lane's part of x . o of token 16 t + n
     if constexpr (MODE != STATE_ONLY) {
       // scores, tile by tile over the waves: (ti, si <= ti), and zeros where a later product's 32 tokens reach past ti
       int turn = 0;
@@ -450,6 +460,13 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
             for (int d = 0; d < Z::DB; ++d)
               p = Op::mma(Op::row(&Ks[(16 * si + n) * KS + 32 * d + 8 * g]), Op::row(&Qs[(16 * ti + n) * QS + 32 * d + 8 * g]),
                           p);
+            f32x4 vx = {0.f, 0.f, 0.f, 0.f};
+            if constexpr (PAIRED) {
+#pragma unroll
+              for (int d = 0; d < Z::VB; ++d)
+                vx = Op::mma(Op::row(&Vs[(16 * si + n) * VS + 32 * d + 8 * g]), Op::row(&Xs[(16 * ti + n) * XS + 32 * d + 8 * g]),
+                             vx);
+            }
             const float th = Hi[buf][16 * ti + n], tl = Lo[buf][16 * ti + n];
             const f32x4 sh = *reinterpret_cast<const f32x4*>(&Hi[buf][16 * si + 4 * g]),
                         sl = *reinterpret_cast<const f32x4*>(&Lo[buf][16 * si + 4 * g]);
@@ -457,12 +474,13 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
             for (int i = 0; i < 4; ++i) {
               const float w = exp2_of((th - sh[i]) + (tl - sl[i])) * (A.key_scale * A.out_scale);
               p[i] = si < ti || 4 * g + i <= n ? kept(w, p[i]) : 0.0f;
+              if constexpr (PAIRED) dots[ti] += (si < ti || 4 * g + i <= n) && w != 0.0f ? p[i] * vx[i] : 0.0f;
             }
           }
-          struct alignas(4 * sizeof(PT)) Scores { PT v[4]; };
+          struct alignas(4 * sizeof(T)) Scores { T v[4]; };
           Scores f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) f.v[i] = from_f<PT>(p[i]);
+          for (int i = 0; i < 4; ++i) f.v[i] = from_f<T>(p[i]);
           *reinterpret_cast<Scores*>(&Ps[(16 * ti + n) * PS + 16 * si + 4 * g]) = f;
         }
       // the state's part
@@ -499,8 +517,21 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
 #pragma unroll
             for (int i = 0; i < 4; ++i) O[t][e][i] = kept(w, O[t][e][i]);
         }
+        if constexpr (PAIRED) {
+          float dot = dots[t];
+#pragma unroll
+          for (int e = 0; e < Z::ET; ++e) {
+            const Four f = *reinterpret_cast<const Four*>(&Xs[(16 * t + n) * XS + e0 + 16 * e + 4 * g]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dot = fmaf(O[t][e][i], to_f(f.v[i]), dot);
+          }
+          dot += __shfl_xor(dot, 16, 64);
+          dot += __shfl_xor(dot, 32, 64);
+          if (g == 0) Dot[wave][16 * t + n] = dot;
+        }
       }
       __syncthreads();
+      if constexpr (PAIRED) put_dots(at);
     }
 
     typename Op::Frag vf[Z::KB][Z::ET];
@@ -515,18 +546,9 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
         for (int t = 0; t < Z::TT; ++t)
 #pragma unroll
           for (int s = 0; s <= t / 2; ++s) {
-            const PT* p = &Ps[(16 * t + n) * PS + 32 * s + 4 * g];
-            auto by = [&](const auto& f) {
+            const typename Op::Frag f = Op::row_split(&Ps[(16 * t + n) * PS + 32 * s + 4 * g]);
 #pragma unroll
-              for (int e = 0; e < Z::ET; ++e) O[t][e] = Op::mma(vf[s][e], f, O[t][e]);
-            };
-            if constexpr (MODE == EXACT) {
-              float y[8];
-              Operand<float>::values(Operand<float>::row_split(p), y);
-              by(Op::wide(y));
-            } else {
-              by(Op::row_split(p));
-            }
+            for (int e = 0; e < Z::ET; ++e) O[t][e] = Op::mma(vf[s][e], f, O[t][e]);
           }
       } else {
 #pragma unroll
@@ -575,14 +597,14 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
             if (A.out_f32) put(static_cast<float*>(A.out), place(16 * t + n), c, r);
             else put(static_cast<T*>(A.out), place(16 * t + n), c, r);
           }
-          if constexpr (DOTS) {
+          if constexpr (DIRECT) {
             if (x) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) dot = fmaf(r[i], to_f(xs[t][e].v[i]), dot);
             }
           }
         }
-        if constexpr (DOTS) {
+        if constexpr (DIRECT) {
           if (x) {
             dot += __shfl_xor(dot, 16, 64);
             dot += __shfl_xor(dot, 32, 64);
@@ -635,7 +657,7 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
     }
     __syncthreads();
   }
-  put_dots(u1 - C);
+  if (DIRECT) put_dots(u1 - C);
 
   float* p = nullptr;
   int sr = A.sr, sc = A.sc;
