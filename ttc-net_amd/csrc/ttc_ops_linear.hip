@@ -275,14 +275,22 @@ __global__ __launch_bounds__(64) void gate_head_kernel(const double* __restrict_
 // 20.5 us one by one, 12.2 us in a chunk; 1,024 heads 26.5, 33.5, 48.0 and 78.9 us against 36
 constexpr int64_t TOKEN_SWEEP = 4;
 
-// Segments of a chunked sweep: enough workgroups to fill the GPU's 256 CUs twice, as many as the registers of the largest
-// kernels let run; a segment's keys and values are read once more for the state behind it, so heads that fill the GPU by
-// themselves are not split.  Workgroups aimed at for 16,381 tokens x 16 heads of 128, and 2,048 x 128 heads of 64 forward
-// and backward: 256 182 and 560 us, 384 163 and 440, 512 142 and 367, 768 177 and 419, 1,024 171 and 377
+// Segments of a chunked sweep: enough workgroups to fill the GPU's 256 CUs as often as registers let them run beside each
+// other, twice, three times up to 64 x 64, four where keys or values have up to 32; a segment's keys and values are read once
+// more for the state behind it, so heads that fill the GPU by themselves are not split.  Workgroups aimed at, training in bf16:
+//                                            384      512     768   1,024   1,536
+//   8 x 2,048 tokens x 32 heads of 128 x 128 1,245  1,060   1,222   1,123           (16,381 x 16 forward 165 146 184 176)
+//   the same, 64 x 128                         818    678     779     706
+//   4 x 2,048 tokens x 32 heads of 64 x 64     337    278     265     282
+//   3 x 4,096 tokens x 32 heads of 64 x 64            404     338     406     376
+//   4 x 4,096 tokens x 32 heads of 64 x 32            450     364     357     394
+//   8 x 4,096 tokens x 32 heads of 32 x 32            791     573     513     598
+//   4 x 4,096 tokens x 32 heads of 32 x 128           617     727     619     667   (128 x 32 625 626 605 613)
 inline Segments segments_of(const ttc_linear_attention_args& A) {
   Segments G{};
   const int64_t chunks = ceil_div(A.tokens, chunk_tokens(A.dtype == TTC_DTYPE_BF16)), heads = A.batch * A.heads;
-  int64_t count = heads > 0 ? 512 / heads : 1;
+  const int64_t fill = 256 * (A.dk <= 32 || A.dv <= 32 ? 4 : A.dk <= 64 && A.dv <= 64 ? 3 : 2);
+  int64_t count = heads > 0 ? fill / heads : 1;
   if (count > chunks / 2) count = chunks / 2;
   if (count < 1) count = 1;
   G.chunks = ceil_div(chunks, count);

@@ -16,18 +16,19 @@
 // two workgroups a CU (a wave holds 32 columns of the state, 64 registers), whose phases between barriers do not cover each
 // other: 11,700 cycles for 64 KB.  16 columns a wave need twice the operand reads (2,048 tokens x 512 heads: 360 us, with
 // 32 columns 313).  Measured: 16,381 tokens x 16 heads of 128, bf16: 91 us (269 MB), after 52 us for the states between its
-// 32 segments (134 MB) and 15 us to join them; 2,048 x 128 heads of 64 (134 MB): FAST 48 us, EXACT 61 with
-// its fourth input, the segments' states 24.  fp32 is bound by its matrix instructions: 2,048 tokens x 512 heads of 128 in 827 us, 101 TFLOP/s (a large library
-// product: 153).
+// 32 segments (134 MB) and 15 us to join them; 2,048 x 128 heads of 64 (134 MB): FAST 44 us, EXACT 58 with its fourth input,
+// the segments' states 25.  fp32 is bound by its matrix instructions: 2,048 tokens x 512 heads of 128 in 827 us, 101 TFLOP/s
+// (a large library product: 153).
 //
 // Numerics.  The sums G are held in 64 bits while they are formed and as pairs of fp32 after, so that differences of
 // large sums keep their digits; a decay of 0 is 2^-4096.  In bf16, w V is split into three bf16 parts (exact in fp32's 24
 // digits), so the state has fp32's accuracy; P and the state's copy in front of a chunk are rounded to bf16 for a bf16
 // output (FAST).  The decays' gradient is a long sum of cancelling terms, so the dots x . o it is made of are not taken from
 // such an o (EXACT): P's part is sum_s P_ts (v_s . x_t), whose products are exact as they are, in fp32; the state's copy
-// is split into three parts.  (P split into three for an exact o instead: 2,048 x 128 heads of 64 68 us; training on
-// 8 x 2,048 x 32 heads of 128 1,170 us, so 1,058.)  Weights that are 0 select: what is masked has no effect, whatever it holds.  Where a chunk's keys or
-// values are not all finite, its sums over tokens are formed term by term instead, without the masked ones.
+// is split into three parts.  (P split into three for an exact o instead: 2,048 x 128 heads of 64 68 us, so 61; training on
+// 8 x 2,048 x 32 heads of 128 1,170 us, so 1,058.)  Weights that are 0 select: what is masked has no effect, whatever it
+// holds.  Where a chunk's keys or values are not all finite, its sums over tokens are formed term by term instead, without
+// the masked ones.
 #pragma once
 #include "ttc_ops_linear.hpp"
 
@@ -242,8 +243,8 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
   auto left_of = [&](int64_t at) { return (int)(A.T - low_of(at) < C ? A.T - low_of(at) : C); };
   auto place = [&](int r) { return A.reverse ? C - 1 - r : r; };
 
-  // S: lane's rows 16 d + 4 g + i, columns e0 + 16 e + n.  The lane's place is hidden from the compiler, which would otherwise keep
-  // 32 addresses in registers over the whole loop.
+  // S: lane's rows 16 d + 4 g + i, columns e0 + 16 e + n.  The lane's place is hidden from the compiler, which
+  // would otherwise keep 32 addresses in registers over the whole loop.
   f32x4 S[Z::DT][Z::ET];
   auto each = [&](auto f) {
     int r = 4 * g, c = e0 + n;
@@ -458,14 +459,14 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
           if (si <= ti) {
 #pragma unroll
             for (int d = 0; d < Z::DB; ++d)
-              p = Op::mma(Op::row(&Ks[(16 * si + n) * KS + 32 * d + 8 * g]), Op::row(&Qs[(16 * ti + n) * QS + 32 * d + 8 * g]),
-                          p);
+              p = Op::mma(Op::row(&Ks[(16 * si + n) * KS + 32 * d + 8 * g]),
+                          Op::row(&Qs[(16 * ti + n) * QS + 32 * d + 8 * g]), p);
             f32x4 vx = {0.f, 0.f, 0.f, 0.f};
             if constexpr (PAIRED) {
 #pragma unroll
               for (int d = 0; d < Z::VB; ++d)
-                vx = Op::mma(Op::row(&Vs[(16 * si + n) * VS + 32 * d + 8 * g]), Op::row(&Xs[(16 * ti + n) * XS + 32 * d + 8 * g]),
-                             vx);
+                vx = Op::mma(Op::row(&Vs[(16 * si + n) * VS + 32 * d + 8 * g]),
+                             Op::row(&Xs[(16 * ti + n) * XS + 32 * d + 8 * g]), vx);
             }
             const float th = Hi[buf][16 * ti + n], tl = Lo[buf][16 * ti + n];
             const f32x4 sh = *reinterpret_cast<const f32x4*>(&Hi[buf][16 * si + 4 * g]),
