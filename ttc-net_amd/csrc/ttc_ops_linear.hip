@@ -163,7 +163,8 @@ __global__ __launch_bounds__(256) void segment_join_kernel(Sweep A, Segments G, 
   }
 }
 
-// Gradients of shared heads, one pass over memory (3 x 509 x 12 heads of 48 to 4: 4.8 us, most of it the launch): out [rows, heads / share, d] = sums over `share` heads of in [rows, heads, d]
+// Gradients of shared heads, one pass over memory (3 x 509 x 12 heads of 48 to 4: 4.8 us, most of it the launch):
+// out [rows, heads / share, d] = sums over `share` heads of in [rows, heads, d]
 template <class T>
 __global__ __launch_bounds__(256) void share_sum_kernel(const float* __restrict__ in, T* __restrict__ out, int64_t first,
                                                         int64_t n, int share, int d) {
