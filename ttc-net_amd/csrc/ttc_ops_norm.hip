@@ -436,42 +436,58 @@ __global__ __launch_bounds__(256) void norm_slab_stats_kernel(const T* __restric
   }
 }
 
-// joins them: one workgroup per (n, group)
-__global__ __launch_bounds__(256) void norm_slab_join_kernel(const float* __restrict__ partial, Slab S, float eps,
-                                                             float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-  __shared__ double sh[256];
+// The partials of a group, one workgroup per (n, group) and up to 1,024 threads: f(slab, channel, both values), 4 at a time
+// in flight, with no division in the loop
+template <class F>
+__device__ __forceinline__ void each_partial(const float* p, const Slab& S, F f) {
+  const int NT = blockDim.x, dsl = NT / S.cg, dc = NT % S.cg;
+  int64_t sl = (int)threadIdx.x / S.cg;
+  int c = (int)threadIdx.x % S.cg;
+  while (sl < S.slabs) {
+    float u[4], w[4];
+    int64_t at[4];
+    int ch[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      at[i] = sl, ch[i] = c;
+      const float* from = p + (sl < S.slabs ? sl : S.slabs - 1) * 2 * S.C + c;
+      u[i] = from[0], w[i] = from[S.C];
+      sl += dsl, c += dc;
+      if (c >= S.cg) c -= S.cg, ++sl;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (at[i] < S.slabs) f(at[i], ch[i], u[i], w[i]);
+  }
+}
+// sums of a and q over the workgroup, in thread 0
+__device__ __forceinline__ void block_sum(double& a, double& q) {
+  __shared__ double sa[16], sq[16];
+  for (int m = 32; m >= 1; m >>= 1) a += __shfl_xor(a, m, 64), q += __shfl_xor(q, m, 64);
+  if (threadIdx.x % 64 == 0) sa[threadIdx.x / 64] = a, sq[threadIdx.x / 64] = q;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    for (int i = 1; i < (int)blockDim.x / 64; ++i) a += sa[i], q += sq[i];
+}
+
+// joins them, about the first one's mean
+__global__ __launch_bounds__(1024) void norm_slab_join_kernel(const float* __restrict__ partial, Slab S, float eps,
+                                                              float* __restrict__ mean_out, float* __restrict__ rstd_out) {
   const int64_t ng = S.first + blockIdx.x, n = ng / S.G;
   const int g = (int)(ng % S.G);
-  const int64_t all = S.slabs * S.cg;
   const float* p = partial + n * S.slabs * 2 * S.C + g * S.cg;
-  auto sum = [&](double v) {
-    sh[threadIdx.x] = v;
-    __syncthreads();
-    for (int m = 128; m >= 1; m >>= 1) {
-      if ((int)threadIdx.x < m) sh[threadIdx.x] += sh[threadIdx.x + m];
-      __syncthreads();
-    }
-    const double r = sh[0];
-    __syncthreads();
-    return r;
-  };
-  auto count = [&](int64_t sl) { return (double)(sl + 1 < S.slabs ? S.slab : S.L - sl * S.slab); };
-  double acc = 0.0;
-  for (int64_t i = threadIdx.x; i < all; i += 256) {
-    const int64_t sl = i / S.cg, c = i % S.cg;
-    acc += count(sl) * p[sl * 2 * S.C + c];
-  }
-  const double total = (double)S.L * S.cg, mean = sum(acc) / total;
-  acc = 0.0;
-  for (int64_t i = threadIdx.x; i < all; i += 256) {
-    const int64_t sl = i / S.cg, c = i % S.cg;
-    const double d = p[sl * 2 * S.C + c] - mean;
-    acc += p[(sl * 2 + 1) * S.C + c] + count(sl) * d * d;
-  }
-  const double var = sum(acc) / total;
+  const double pivot = p[0], whole = (double)S.slab, rest = (double)(S.L - (S.slabs - 1) * S.slab);
+  double a = 0.0, q = 0.0;
+  each_partial(p, S, [&](int64_t sl, int, float m, float m2) {
+    const double count = sl + 1 < S.slabs ? whole : rest, d = m - pivot;
+    a += count * d;
+    q += m2 + count * d * d;
+  });
+  block_sum(a, q);
   if (threadIdx.x == 0) {
-    mean_out[ng] = (float)mean;
-    rstd_out[ng] = (float)(1.0 / sqrt(var + eps));
+    const double total = (double)S.L * S.cg, off = a / total, var = q / total - off * off;
+    mean_out[ng] = (float)(pivot + off);
+    rstd_out[ng] = (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + eps));
   }
 }
 
@@ -579,34 +595,21 @@ __global__ __launch_bounds__(256) void norm_slab_back_stats_kernel(const T* __re
 }
 
 // means over each group of dxhat xhat and dxhat -> sums [n, g, 2]
-__global__ __launch_bounds__(256) void norm_slab_back_join_kernel(const float* __restrict__ partial, Affine aff, Slab S,
-                                                                  float* __restrict__ sums) {
-  __shared__ double s1[256], s2[256];
+__global__ __launch_bounds__(1024) void norm_slab_back_join_kernel(const float* __restrict__ partial, Affine aff, Slab S,
+                                                                   float* __restrict__ sums) {
   const int64_t ng = S.first + blockIdx.x, n = ng / S.G;
   const int g = (int)(ng % S.G);
-  const int64_t all = S.slabs * S.cg;
-  const float* p = partial + n * S.slabs * 2 * S.C + g * S.cg;
   double a = 0.0, q = 0.0;
-  for (int64_t i = threadIdx.x; i < all; i += 256) {
-    const int64_t sl = i / S.cg, c = i % S.cg;
+  each_partial(partial + n * S.slabs * 2 * S.C + g * S.cg, S, [&](int64_t, int c, float u, float v) {
     const double w = aff.weight(g * S.cg + c);
-    a += w * p[sl * 2 * S.C + c];
-    q += w * p[(sl * 2 + 1) * S.C + c];
-  }
-  s1[threadIdx.x] = a;
-  s2[threadIdx.x] = q;
-  __syncthreads();
-  for (int m = 128; m >= 1; m >>= 1) {
-    if ((int)threadIdx.x < m) {
-      s1[threadIdx.x] += s1[threadIdx.x + m];
-      s2[threadIdx.x] += s2[threadIdx.x + m];
-    }
-    __syncthreads();
-  }
+    a += w * u;
+    q += w * v;
+  });
+  block_sum(a, q);
   if (threadIdx.x == 0) {
     const double total = (double)S.L * S.cg;
-    sums[2 * ng] = (float)(s1[0] / total);
-    sums[2 * ng + 1] = (float)(s2[0] / total);
+    sums[2 * ng] = (float)(a / total);
+    sums[2 * ng + 1] = (float)(q / total);
   }
 }
 
@@ -771,11 +774,12 @@ int norm_run(const ttc_group_norm_args& A, const NormPlan& P, hipStream_t s) {
   } else {
     Slab S = P.S;
     const int64_t blocks = A.n * S.slabs * S.cblocks, joins = A.n * G;
-    const dim3 block(256);
+    const int64_t parts_a_group = S.slabs * S.cg;
+    const dim3 block(256), joiners(parts_a_group >= 1024 ? 1024 : (unsigned)(ceil_div(parts_a_group, 64) * 64));
     int rc = TTC_LQR_OK;
     auto each = [&](int64_t n, auto go) {
       if (rc == TTC_LQR_OK)
-        rc = in_launches(n, 256, [&](int64_t first, dim3 grid) {
+        rc = in_launches(n, 1024, [&](int64_t first, dim3 grid) {
           S.first = first;
           go(grid);
         });
@@ -793,7 +797,7 @@ int norm_run(const ttc_group_norm_args& A, const NormPlan& P, hipStream_t s) {
       float* mean = A.mean ? A.mean : extra;
       float* rstd = A.mean ? A.rstd : extra + A.n * G;
       each(blocks, [&](dim3 g) { hipLaunchKernelGGL((norm_slab_stats_kernel<T, V>), g, block, 0, s, x, S, ws); });
-      each(joins, [&](dim3 g) { hipLaunchKernelGGL(norm_slab_join_kernel, g, block, 0, s, ws, S, eps, mean, rstd); });
+      each(joins, [&](dim3 g) { hipLaunchKernelGGL(norm_slab_join_kernel, g, joiners, 0, s, ws, S, eps, mean, rstd); });
       each(blocks, [&](dim3 g) {
         hipLaunchKernelGGL((norm_slab_apply_kernel<T, V, SILU, GATE>), g, block, 0, s, x, gate, aff, S, mean, rstd,
                            static_cast<T*>(A.y));
@@ -805,7 +809,7 @@ int norm_run(const ttc_group_norm_args& A, const NormPlan& P, hipStream_t s) {
                          static_cast<T*>(A.dgate), ws);
     });
     if (A.dx) {
-      each(joins, [&](dim3 g) { hipLaunchKernelGGL(norm_slab_back_join_kernel, g, block, 0, s, ws, aff, S, extra); });
+      each(joins, [&](dim3 g) { hipLaunchKernelGGL(norm_slab_back_join_kernel, g, joiners, 0, s, ws, aff, S, extra); });
       each(blocks, [&](dim3 g) {
         hipLaunchKernelGGL((norm_slab_back_apply_kernel<T, V, SILU, GATE>), g, block, 0, s, x, gate, dy, aff, S, A.mean,
                            A.rstd, extra, static_cast<T*>(A.dx));
