@@ -12,11 +12,12 @@
 //    8,192 x 2,048 in 32 groups, gated, bf16: forward 30 us (100 MB, 3.4 TB/s), backward 39 us (168 MB, 4.3 TB/s) and
 //    8 us for the sums of the weights' gradients; 16 x 2,048: 4.2 us;
 //  * a group that fits in a workgroup's registers, forward: one workgroup a group, x read once.
-//    2 x 1,021 x 192 in 6 groups, bf16: 12 us, most of it latency (slabs 18);
+//    2 x 1,021 x 192 in 6 groups, bf16: 12 us, most of it latency (slabs 16 in three launches);
 //  * any other, and every backward over several positions: slabs of positions, each reduced over whole rows of c
 //    channels (coalesced); sums per channel are taken about the slab's first position (a large common mean costs no
-//    digits) and joined as (mean, sum of squares) pairs; a second pass reads x again and writes y.  8 x 4,096 x 320 in 32 groups, fp32 (42 MB an array): forward
-//    13 + 8 + 17 us (statistics, join, output), backward 18 + 5 + 21 + 5 us; the caches hold x between the passes.
+//    digits) and joined as (mean, sum of squares) pairs; a second pass reads x again and writes y.  8 x 4,096 x 320 in 32
+//    groups, fp32 (42 MB an array): forward 14 + 5 + 17 us (statistics, join, output), backward 18 + 5 + 21 + 5 us; the
+//    caches hold x between the passes.  7,269 x 768 in 12 groups, bf16 (11 MB): forward 7 + 6 + 10 us.
 #include "ttc_ops_common.hpp"
 
 namespace ttc {
@@ -314,6 +315,7 @@ __global__ __launch_bounds__(1024) void norm_affine_sum_kernel(const float* __re
 struct Slab {
   int64_t L, slab, slabs, first;  // first: workgroup of this launch
   int C, G, cg, cols, rper, cblocks;  // cols: vectors of a row
+  int per;  // channels of a forward's partial: a vector's where none reaches into two groups
 };
 
 // Groups that fit in a workgroup's registers, forward: one workgroup a group, x read once, one launch instead of three.
@@ -382,7 +384,7 @@ __global__ __launch_bounds__(1024) void norm_whole_kernel(const T* __restrict__ 
   }
 }
 
-// (mean, M2) of `count` values per (n, slab, channel) -> partial [n, slabs, 2, c]
+// (mean, M2) of `count` values per (n, slab, channel or vector of a group) -> partial [n, slabs, 2, c / per]
 template <class T, int V>
 __global__ __launch_bounds__(256) void norm_slab_stats_kernel(const T* __restrict__ x, Slab S,
                                                               float* __restrict__ partial) {
@@ -423,15 +425,30 @@ __global__ __launch_bounds__(256) void norm_slab_stats_kernel(const T* __restric
   __syncthreads();
   if (r == 0 && col < S.cols) {
     const float cnt = (float)(l1 - l0);
-    float* out = partial + ((n * S.slabs + sl) * 2) * S.C + (int64_t)col * V;
+    const int row = S.C / S.per;
+    float* out = partial + ((n * S.slabs + sl) * 2) * row + (S.per > 1 ? (int64_t)col : (int64_t)col * V);
+    float mean = 0.0f, m2 = 0.0f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       for (int i = 1; i < S.rper; ++i) {
         a[j] += s1[j * 256 + i * cper + cc];
         q[j] += s2[j * 256 + i * cper + cc];
       }
-      out[j] = k[j] + a[j] / cnt;
-      out[S.C + j] = fmaxf(q[j] - a[j] * (a[j] / cnt), 0.0f);
+      q[j] = fmaxf(q[j] - a[j] * (a[j] / cnt), 0.0f);
+      a[j] = k[j] + a[j] / cnt;
+      mean += (a[j] - a[0]) * (1.0f / V);
+    }
+    if (S.per > 1) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = a[j] - a[0] - mean;
+        m2 += q[j] + cnt * d * d;
+      }
+      out[0] = a[0] + mean;
+      out[row] = m2;
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) out[j] = a[j], out[row + j] = q[j];
     }
   }
 }
@@ -439,10 +456,11 @@ __global__ __launch_bounds__(256) void norm_slab_stats_kernel(const T* __restric
 // The partials of a group, one workgroup per (n, group) and up to 1,024 threads: f(slab, channel, both values), 4 at a time
 // in flight, with no division in the loop
 template <class F>
-__device__ __forceinline__ void each_partial(const float* p, const Slab& S, F f) {
-  const int NT = blockDim.x, dsl = NT / S.cg, dc = NT % S.cg;
-  int64_t sl = (int)threadIdx.x / S.cg;
-  int c = (int)threadIdx.x % S.cg;
+__device__ __forceinline__ void each_partial(const float* partial, const Slab& S, int64_t n, int g, int per, F f) {
+  const int row = S.C / per, cg = S.cg / per, NT = blockDim.x, dsl = NT / cg, dc = NT % cg;
+  const float* p = partial + n * S.slabs * 2 * row + g * cg;
+  int64_t sl = (int)threadIdx.x / cg;
+  int c = (int)threadIdx.x % cg;
   while (sl < S.slabs) {
     float u[4], w[4];
     int64_t at[4];
@@ -450,10 +468,10 @@ __device__ __forceinline__ void each_partial(const float* p, const Slab& S, F f)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       at[i] = sl, ch[i] = c;
-      const float* from = p + (sl < S.slabs ? sl : S.slabs - 1) * 2 * S.C + c;
-      u[i] = from[0], w[i] = from[S.C];
+      const float* from = p + (sl < S.slabs ? sl : S.slabs - 1) * 2 * row + c;
+      u[i] = from[0], w[i] = from[row];
       sl += dsl, c += dc;
-      if (c >= S.cg) c -= S.cg, ++sl;
+      if (c >= cg) c -= cg, ++sl;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -475,10 +493,10 @@ __global__ __launch_bounds__(1024) void norm_slab_join_kernel(const float* __res
                                                               float* __restrict__ mean_out, float* __restrict__ rstd_out) {
   const int64_t ng = S.first + blockIdx.x, n = ng / S.G;
   const int g = (int)(ng % S.G);
-  const float* p = partial + n * S.slabs * 2 * S.C + g * S.cg;
-  const double pivot = p[0], whole = (double)S.slab, rest = (double)(S.L - (S.slabs - 1) * S.slab);
+  const double pivot = partial[n * S.slabs * 2 * (S.C / S.per) + g * (S.cg / S.per)];
+  const double whole = (double)S.slab * S.per, rest = (double)(S.L - (S.slabs - 1) * S.slab) * S.per;
   double a = 0.0, q = 0.0;
-  each_partial(p, S, [&](int64_t sl, int, float m, float m2) {
+  each_partial(partial, S, n, g, S.per, [&](int64_t sl, int, float m, float m2) {
     const double count = sl + 1 < S.slabs ? whole : rest, d = m - pivot;
     a += count * d;
     q += m2 + count * d * d;
@@ -600,7 +618,7 @@ __global__ __launch_bounds__(1024) void norm_slab_back_join_kernel(const float* 
   const int64_t ng = S.first + blockIdx.x, n = ng / S.G;
   const int g = (int)(ng % S.G);
   double a = 0.0, q = 0.0;
-  each_partial(partial + n * S.slabs * 2 * S.C + g * S.cg, S, [&](int64_t, int c, float u, float v) {
+  each_partial(partial, S, n, g, 1, [&](int64_t, int c, float u, float v) {
     const double w = aff.weight(g * S.cg + c);
     a += w * u;
     q += w * v;
@@ -717,16 +735,18 @@ inline NormPlan norm_plan(const ttc_group_norm_args& A, bool wide) {
   S.G = (int)A.groups;
   S.cg = (int)cg;
   S.cols = (int)(A.c / P.V);
+  S.per = !A.backward && cg % P.V == 0 ? P.V : 1;
   const int cper = S.cols < 256 ? S.cols : 256;
   S.rper = 256 / cper;
   S.cblocks = (int)ceil_div(S.cols, 256 / S.rper);
   if (!A.backward) {
     const int Vw = wide && cg % full == 0 ? full : 1;
     const int64_t v = ceil_div(cg, Vw) <= 1024 * WHOLE && A.l <= 1024 * WHOLE ? A.l * (cg / Vw) : 1024 * WHOLE + 1;
-    // Rows of less than 64 bytes a group are read in halves of what memory gives: large arrays of them take the slabs (64 x
-    // 1,024 x 512 in 32 groups, bf16: 53 us, whole 70; 16 x 1,024 x 512: 28, whole 23; 64 x 256 x 1,024 in 8 groups: 42, whole 24)
+    // Rows of less than 64 bytes a group are read in halves of what memory gives: large arrays of them take the slabs (1,024 x
+    // 512 in 32 groups, bf16, 64 of them: slabs 55 us, whole 85; 32: 33, 37; 16: 24, 25 in one launch; wider rows, 64 x 256 x
+    // 1,024 in 8 groups: 32, whole 25)
     const bool narrow = cg * (A.dtype == TTC_DTYPE_F32 ? 4 : 2) < 64;
-    if (v <= 1024 * WHOLE && (!narrow || A.n * A.l * A.c <= 1 << 24)) {
+    if (v <= 1024 * WHOLE && (!narrow || A.n * A.l * A.c <= 1 << 23)) {
       P.V = Vw;
       P.whole = (int)(ceil_div(ceil_div(v, WHOLE), 64) * 64);
       if (P.whole < 256) P.whole = 256;
@@ -774,7 +794,7 @@ int norm_run(const ttc_group_norm_args& A, const NormPlan& P, hipStream_t s) {
   } else {
     Slab S = P.S;
     const int64_t blocks = A.n * S.slabs * S.cblocks, joins = A.n * G;
-    const int64_t parts_a_group = S.slabs * S.cg;
+    const int64_t parts_a_group = S.slabs * (S.cg / S.per);
     const dim3 block(256), joiners(parts_a_group >= 1024 ? 1024 : (unsigned)(ceil_div(parts_a_group, 64) * 64));
     int rc = TTC_LQR_OK;
     auto each = [&](int64_t n, auto go) {
