@@ -151,6 +151,19 @@ def test_gradients_against_differences(device, shape, groups):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,groups", [((37, 5, 24), 3), ((3, 11, 36), 4), ((1, 5000, 64), 2), ((1, 9000, 15), 3)])
+def test_few_and_many_values_a_group(device, dtype, shape, groups):
+    """Groups of a few lanes, the last workgroup not full; groups of many slabs, of whole vectors and not."""
+    for gate in (False, True):
+        x, w, b, g = tensors(shape, dtype, device, gate, True)
+        check_forward(x, groups, w, b, 1e-5, "silu", g)
+    if dtype == torch.float32:
+        x, w, b, _ = tensors(shape, dtype, device, False, True, shift=1000.0)
+        check_forward(x, groups, w, b, 1e-5, "none", None)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_needed_gradients_only(device):
     x, w, b, g = tensors((5, 3, 24), torch.float32, device, True, True)
     full = [t.clone().requires_grad_() for t in (x, w, b, g)]

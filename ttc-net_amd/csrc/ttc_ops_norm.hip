@@ -11,7 +11,7 @@
 //    registers (up to 4 vectors of 16 bytes each), so x is read once and the variance is that of the centred values.
 //    8,192 x 2,048 in 32 groups, gated, bf16: forward 30 us (100 MB, 3.4 TB/s), backward 39 us (168 MB, 4.3 TB/s) and
 //    8 us for the sums of the weights' gradients; 16 x 2,048: 4.2 us;
-//  * a group that fits in a workgroup's registers, forward: one workgroup a group, x read once.
+//  * a group that fits in a workgroup's registers, forward: up to 64 lanes or one workgroup a group, x read once.
 //    2 x 1,021 x 192 in 6 groups, bf16: 12 us, most of it latency (slabs 16 in three launches);
 //  * any other, and every backward over several positions: slabs of positions, each reduced over whole rows of c
 //    channels (coalesced); sums per channel are taken about the slab's first position (a large common mean costs no
@@ -318,21 +318,26 @@ struct Slab {
   int per;  // channels of a forward's partial: a vector's where none reaches into two groups
 };
 
-// Groups that fit in a workgroup's registers, forward: one workgroup a group, x read once, one launch instead of three.
-// The group's l rows of cg channels are counted in vectors; thread t holds vectors t, t + 1024, ...
-constexpr int WHOLE = 8;  // vectors a thread
-template <class T, int V, bool SILU, bool GATE>
+// Groups that fit in registers, forward: x read once, one launch instead of three.  The group's l rows of cg channels are
+// counted in vectors; thread t of its `team` holds vectors t, t + team, ...  A team is a workgroup, or up to 64 lanes of a
+// workgroup of 256 that holds several groups (NV = 2): 38,176 groups of 5 x 8 in bf16 7 us, a workgroup each 150.
+constexpr int WHOLE = 8, SMALL = 2;  // vectors a thread
+template <class T, int V, bool SILU, bool GATE, int NV>
 __global__ __launch_bounds__(1024) void norm_whole_kernel(const T* __restrict__ x, const T* __restrict__ gate, Affine aff,
-                                                          Slab S, float eps, T* __restrict__ y, float* __restrict__ mean_out,
-                                                          float* __restrict__ rstd_out) {
+                                                          Slab S, int team, int64_t groups, float eps, T* __restrict__ y,
+                                                          float* __restrict__ mean_out, float* __restrict__ rstd_out) {
   __shared__ float part[16];
-  const int64_t ng = S.first + blockIdx.x, n = ng / S.G;
+  const int t = (int)threadIdx.x % team;
+  const int64_t mine = (S.first + blockIdx.x) * ((int)blockDim.x / team) + (int)threadIdx.x / team;
+  const bool live = mine < groups;  // the others repeat the last group and write nothing
+  const int64_t ng = live ? mine : groups - 1, n = ng / S.G;
   const int g = (int)(ng % S.G), cols = S.cg / V;
   const int vecs = (int)S.L * cols;
   const T *xg = x + n * S.L * S.C + g * S.cg, *gg = GATE ? gate + n * S.L * S.C + g * S.cg : nullptr;
   T* yg = y + n * S.L * S.C + g * S.cg;
   auto sum = [&](float v) {
-    v = lane_sum(v, 64);
+    v = lane_sum(v, NV == SMALL ? team : 64);
+    if (NV == SMALL) return v;
     __syncthreads();
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     __syncthreads();
@@ -340,33 +345,33 @@ __global__ __launch_bounds__(1024) void norm_whole_kernel(const T* __restrict__ 
     for (int i = 0; i < (int)blockDim.x / 64; ++i) r += part[i];
     return r;
   };
-  Vec<T, V> xv[WHOLE];
-  int64_t at[WHOLE];
+  Vec<T, V> xv[NV];
+  int64_t at[NV];
   float a = 0.0f;
 #pragma unroll
-  for (int k = 0; k < WHOLE; ++k) {  // loads from the last vector where there is none: in branches each would wait
-    const int i = (int)threadIdx.x + k * (int)blockDim.x, j = i < vecs ? i : vecs - 1;
+  for (int k = 0; k < NV; ++k) {  // loads from the last vector where there is none: in branches each would wait
+    const int i = t + k * team, j = i < vecs ? i : vecs - 1;
     at[k] = (int64_t)(j / cols) * S.C + j % cols * V;
     xv[k] = *reinterpret_cast<const Vec<T, V>*>(xg + at[k]);
   }
 #pragma unroll
-  for (int k = 0; k < WHOLE; ++k)
+  for (int k = 0; k < NV; ++k)
 #pragma unroll
-    for (int j = 0; j < V; ++j) a += (int)threadIdx.x + k * (int)blockDim.x < vecs ? to_f(xv[k].v[j]) : 0.0f;
+    for (int j = 0; j < V; ++j) a += t + k * team < vecs ? to_f(xv[k].v[j]) : 0.0f;
   const float total = (float)S.L * S.cg, mean = sum(a) / total;
   float q = 0.0f;
 #pragma unroll
-  for (int k = 0; k < WHOLE; ++k)
+  for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const float d = to_f(xv[k].v[j]) - mean;
-      q = (int)threadIdx.x + k * (int)blockDim.x < vecs ? fmaf(d, d, q) : q;
+      q = t + k * team < vecs ? fmaf(d, d, q) : q;
     }
   const float rstd = 1.0f / sqrtf(sum(q) / total + eps);
 #pragma unroll
-  for (int k = 0; k < WHOLE; ++k) {
-    const int i = (int)threadIdx.x + k * (int)blockDim.x;
-    if (i >= vecs) break;
+  for (int k = 0; k < NV; ++k) {
+    const int i = t + k * team;
+    if (i >= vecs || !live) break;
     float w[V], b[V];
     const int64_t c = (int64_t)g * S.cg + i % cols * V;
     aff.load<V>(c, S.C, w, b);
@@ -378,7 +383,7 @@ __global__ __launch_bounds__(1024) void norm_whole_kernel(const T* __restrict__ 
           out_of<SILU, GATE>(fmaf((to_f(xv[k].v[j]) - mean) * rstd, w[j], b[j]), GATE ? to_f(gt.v[j]) : 0.0f));
     *reinterpret_cast<Vec<T, V>*>(yg + at[k]) = out;
   }
-  if (threadIdx.x == 0 && mean_out) {
+  if (t == 0 && live && mean_out) {
     mean_out[ng] = mean;
     rstd_out[ng] = rstd;
   }
@@ -680,7 +685,7 @@ __global__ __launch_bounds__(256) void norm_slab_back_apply_kernel(const T* __re
 struct NormPlan {
   bool rows;              // the one-position form
   int V, NV;
-  int whole;              // threads a group of the form in registers; 0: slabs
+  int whole;              // threads a group of the form in registers, up to 64: several groups a workgroup; 0: slabs
   Rows R;
   int64_t slabs;
   Slab S;
@@ -746,6 +751,12 @@ inline NormPlan norm_plan(const ttc_group_norm_args& A, bool wide) {
     // 512 in 32 groups, bf16, 64 of them: slabs 55 us, whole 85; 32: 33, 37; 16: 24, 25 in one launch; wider rows, 64 x 256 x
     // 1,024 in 8 groups: 32, whole 25)
     const bool narrow = cg * (A.dtype == TTC_DTYPE_F32 ? 4 : 2) < 64;
+    if (v <= 64 * SMALL) {  // teams beside each other read whole rows between them
+      P.V = Vw;
+      P.whole = 1;
+      while (P.whole * SMALL < v) P.whole *= 2;
+      return P;
+    }
     if (v <= 1024 * WHOLE && (!narrow || A.n * A.l * A.c <= 1 << 23)) {
       P.V = Vw;
       P.whole = (int)(ceil_div(ceil_div(v, WHOLE), 64) * 64);
@@ -805,10 +816,16 @@ int norm_run(const ttc_group_norm_args& A, const NormPlan& P, hipStream_t s) {
         });
     };
     if (P.whole) {
-      rc = in_launches(joins, P.whole, [&](int64_t first, dim3 grid) {
+      const bool small = P.whole <= 64;
+      const int threads = small ? 256 : P.whole;
+      rc = in_launches(ceil_div(joins, threads / P.whole), threads, [&](int64_t first, dim3 grid) {
         S.first = first;
-        hipLaunchKernelGGL((norm_whole_kernel<T, V, SILU, GATE>), grid, dim3(P.whole), 0, s, x, gate, aff, S, eps,
-                           static_cast<T*>(A.y), A.mean, A.rstd);
+        auto go = [&](auto nv) {
+          hipLaunchKernelGGL((norm_whole_kernel<T, V, SILU, GATE, decltype(nv)::value>), grid, dim3(threads), 0, s, x, gate,
+                             aff, S, P.whole, joins, eps, static_cast<T*>(A.y), A.mean, A.rstd);
+        };
+        if (small) go(std::integral_constant<int, SMALL>{});
+        else go(std::integral_constant<int, WHOLE>{});
       });
       return rc;
     }
