@@ -1,0 +1,28 @@
+"""What the sequence operators (``ttc.ops``) promise beyond their formulas: how often a value is rounded, what masked places
+can reach, whose derivative a gradient is, and which calls are taken at all.  Tolerances stand at each test."""
+import math
+
+import pytest
+import torch
+
+from _ops_oracle import EPS, HALF, linear64, within
+from test_ops_linear_attention import DEVICES, grads, inputs, magnitudes, make, roundings
+from ttc.ops import linear_attention
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("case", [(2, 200, 2, 2, 2, 2, 64, 64), (1, 150, 2, 2, 1, 1, 128, 128), (2, 130, 3, 3, 3, 1, 32, 20),
+                                  (1, 700, 1, 1, 1, 1, 128, 33), (2, 3, 2, 2, 2, 2, 16, 40)])
+def test_outputs_in_16_bits_are_rounded_once(device, case):
+    """Scores and states keep 16 digits or more on the way (the first 8 of a value, then 8 of the rest, which is below 2^-7
+    of it: 2^-15 for each term), and the output, a gradient of a head that is not shared included, is rounded once."""
+    x = inputs(*case, torch.bfloat16, device, True)
+    B, T, H, dk, dv = case[0], case[1], case[2], case[6], case[7]
+    d_o, d_state = make((B, T, H, dv), torch.bfloat16, device, 9), make((B, H, dk, dv), torch.float32, device, 10)
+    got = grads(x, d_o, d_state, 0.4)
+    got["o"] = linear_attention(x["q"], x["k"], x["v"], x["g"], scale=0.4, initial_state=x["state"])
+    want = linear64(x["q"], x["k"], x["v"], x["g"], 0.4, x["state"], d_o, d_state)
+    size = magnitudes(x, 0.4, d_o, d_state)
+    for name in ("o", "q", "k", "v"):
+        once = HALF[torch.bfloat16] * 1.01 * want[name].abs()
+        within(got[name], want[name], once + size[name] * (roundings(x, T) * EPS + 2.0 ** -15) + 1e-30)

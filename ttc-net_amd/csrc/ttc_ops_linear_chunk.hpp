@@ -22,13 +22,13 @@
 //
 // Numerics.  The sums G are held in 64 bits while they are formed and as pairs of fp32 after, so that differences of
 // large sums keep their digits; a decay of 0 is 2^-4096.  In bf16, w V is split into three bf16 parts (exact in fp32's 24
-// digits), so the state has fp32's accuracy; P and the state's copy in front of a chunk are rounded to bf16 for a bf16
-// output (FAST).  The decays' gradient is a long sum of cancelling terms, so the dots x . o it is made of are not taken from
-// such an o (EXACT): P's part is sum_s P_ts (v_s . x_t), whose products are exact as they are, in fp32; the state's copy
-// is split into three parts.  (P split into three for an exact o instead: 2,048 x 128 heads of 64 68 us, so 61; training on
-// 8 x 2,048 x 32 heads of 128 1,170 us, so 1,058.)  Weights that are 0 select: what is masked has no effect, whatever it
-// holds.  Where a chunk's keys or values are not all finite, its sums over tokens are formed term by term instead, without
-// the masked ones.
+// digits), so the state has fp32's accuracy; P, and in FAST the state's copy in front of a chunk, into two (16 digits), so that a
+// bf16 output is rounded to 8 digits once.  (Both in one part of 8 digits: the prompt above takes 143 us as a whole, so 155,
+// training on 4 x 2,048 tokens x 32 heads of 64 264, so 288, and the outputs' error is 2.35e-3 of their norm instead of 1.66e-3.)
+// The decays' gradient is a long sum of cancelling terms, so the dots x . o it is made of are not taken from such an o (EXACT):
+// P's part is sum_s P_ts (v_s . x_t), whose products are exact as they are, in fp32; the state's copy is split into three
+// parts.  Weights that are 0 select: what is masked has no effect, whatever it holds.  Where a chunk's keys or values are not all
+// finite, its sums over tokens are formed term by term instead, without the masked ones.
 #pragma once
 #include "ttc_ops_linear.hpp"
 
@@ -53,6 +53,9 @@ struct Operand<__bf16> {
   struct Wide {  // a value as the exact sum of three bf16 numbers
     Frag h, m, l;
   };
+  struct Pair {  // its first 16 digits as the sum of two
+    Frag h, l;
+  };
   // rows read along them: 4 banks apart (mod 32); rows read across them, 8 rows at once, 8 banks apart
   static constexpr int ROW_PAD = 8, COL_PAD = 16;
   static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
@@ -64,6 +67,8 @@ struct Operand<__bf16> {
   static __device__ __forceinline__ f32x4 mma(Frag a, const Wide& b, f32x4 c) {
     return mma(a, b.h, mma(a, b.m, mma(a, b.l, c)));
   }
+  static __device__ __forceinline__ f32x4 mma(const Pair& a, Frag b, f32x4 c) { return mma(a.h, b, mma(a.l, b, c)); }
+  static __device__ __forceinline__ f32x4 mma(Frag a, const Pair& b, f32x4 c) { return mma(a, b.h, mma(a, b.l, c)); }
   static __device__ __forceinline__ Frag row(const __bf16* p) { return *reinterpret_cast<const Frag*>(p); }
   // elements p[0..3] and p[16..19]
   static __device__ __forceinline__ Frag row_split(const __bf16* p) {
@@ -80,12 +85,43 @@ struct Operand<__bf16> {
     const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)(a + 16 * stride));
     return __builtin_bit_cast(Frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
   }
-  static __device__ __forceinline__ Frag narrow(const float (&x)[8]) {
-    Frag r;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) r[j] = (__bf16)x[j];
-    return r;
+  // two values cut to bf16, and what that leaves of each
+  static __device__ __forceinline__ uint32_t cut(float x, float y, float& dx, float& dy) {
+    const uint32_t a = __float_as_uint(x) & 0xffff0000u, b = __float_as_uint(y) & 0xffff0000u;
+    dx = x - __uint_as_float(a);
+    dy = y - __uint_as_float(b);
+    return __builtin_amdgcn_perm(b, a, 0x07060302);
   }
+  static __device__ __forceinline__ Pair pair(const float (&x)[8]) {
+    u32x4 h;
+    Frag l;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float d, e;
+      h[j] = cut(x[2 * j], x[2 * j + 1], d, e);
+      l[2 * j] = (__bf16)d;
+      l[2 * j + 1] = (__bf16)e;
+    }
+    return Pair{__builtin_bit_cast(Frag, h), l};
+  }
+  // Scores in tiles of 16 x 16 (SCORE_PARTS such arrays, `part` elements apart): 4 neighbours of a row at p, and those of
+  // two neighbouring tiles as an operand (zeros for the second one where there is none)
+  static constexpr int SCORE_PARTS = 2;
+  static __device__ __forceinline__ void put_scores(__bf16* p, int part, f32x4 x) {
+    float d[4];
+    const u32x2 h = {cut(x[0], x[1], d[0], d[1]), cut(x[2], x[3], d[2], d[3])};
+    *reinterpret_cast<u32x2*>(p) = h;
+    *reinterpret_cast<bf16x4*>(p + part) = bf16x4{(__bf16)d[0], (__bf16)d[1], (__bf16)d[2], (__bf16)d[3]};
+  }
+  static __device__ __forceinline__ Pair scores(const __bf16* p, int part, bool second) {
+    auto both = [&](const __bf16* q) {
+      const bf16x4 a = *reinterpret_cast<const bf16x4*>(q);
+      const bf16x4 b = second ? *reinterpret_cast<const bf16x4*>(q + 256) : bf16x4{};
+      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    return Pair{both(p), both(p + part)};
+  }
+  static __device__ __forceinline__ float score(const __bf16* p, int part) { return to_f(p[0]) + to_f(p[part]); }
   static __device__ __forceinline__ Wide wide(const float (&x)[8]) {
     u32x4 h, m, l;
 #pragma unroll
@@ -130,6 +166,7 @@ struct Operand<float> {
     float v[8];
   };
   using Wide = Frag;
+  using Pair = Frag;
   static constexpr int ROW_PAD = 4, COL_PAD = 4;
   static __device__ __forceinline__ f32x4 mma(const Frag& a, const Frag& b, f32x4 c) {
 #pragma unroll
@@ -149,7 +186,15 @@ struct Operand<float> {
     for (int j = 0; j < 8; ++j) r.v[j] = a[(j < 4 ? j : 12 + j) * stride];
     return r;
   }
-  static __device__ __forceinline__ Frag narrow(const float (&x)[8]) { return wide(x); }
+  static __device__ __forceinline__ Frag pair(const float (&x)[8]) { return wide(x); }
+  static constexpr int SCORE_PARTS = 1;
+  static __device__ __forceinline__ void put_scores(float* p, int, f32x4 x) { *reinterpret_cast<f32x4*>(p) = x; }
+  static __device__ __forceinline__ Frag scores(const float* p, int, bool second) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p),
+                b = second ? *reinterpret_cast<const f32x4*>(p + 256) : f32x4{0.f, 0.f, 0.f, 0.f};
+    return Frag{{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
+  }
+  static __device__ __forceinline__ float score(const float* p, int) { return p[0]; }
   static __device__ __forceinline__ Frag wide(const float (&x)[8]) {
     Frag r;
 #pragma unroll
@@ -209,16 +254,19 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
   using Op = Operand<T>;
   // the dots x . o: from products of scores and of v . x (PAIRED), or from fp32's o as it is (DIRECT)
   constexpr bool PAIRED = MODE == EXACT, DIRECT = MODE == FAST && sizeof(T) == 4, DOTS = PAIRED || DIRECT;
-  // With x there too, 128 x 128 stays below half of the 160 KB a CU has only if columns are padded as rows are and the last
-  // rows end without a pad.  (Without the pads' end FAST at 128 x 128 spills 24 registers.)
-  constexpr int C = Z::C, NT = Z::NT, VEC = Z::VEC, QS = Z::QS, XS = VD + Op::ROW_PAD,
-                KS = PAIRED && KD + VD > 192 ? QS : Z::KS, VS = PAIRED && KD + VD > 192 ? XS : Z::VS,
-                PS = C + 16 / (int)sizeof(T), TAIL = PAIRED ? 16 / (int)sizeof(T) : 0;
+  // With x there too, 128 x 128 stays below half of the 160 KB a CU has only if columns are padded as rows are, the last
+  // rows end without a pad, and x has none: its rows' 16 bytes change places instead (x_at).
+  constexpr bool TIGHT = PAIRED && KD + VD > 192;
+  constexpr int C = Z::C, NT = Z::NT, VEC = Z::VEC, QS = Z::QS, XS = TIGHT ? VD : VD + Op::ROW_PAD, KS = TIGHT ? QS : Z::KS,
+                VS = TIGHT ? VD + Op::ROW_PAD : Z::VS, TAIL = PAIRED ? 16 / (int)sizeof(T) : 0;
+  constexpr int PART = Z::TT * (Z::TT + 1) / 2 * 256;  // the scores' tiles (ti, si <= ti)
+  auto score_at = [](int ti, int si, int row, int col) { return ((ti * (ti + 1) / 2 + si) * 16 + row) * 16 + col; };
+  auto x_at = [](int row, int c) { return row * XS + (TIGHT ? c ^ (row % 16 * VEC) : c); };
   __shared__ __attribute__((aligned(16))) T Qs[MODE == STATE_ONLY ? 1 : C * QS - TAIL];
   __shared__ __attribute__((aligned(16))) T Ks[C * KS - TAIL];
   __shared__ __attribute__((aligned(16))) T Vs[C * VS - TAIL];
-  __shared__ __attribute__((aligned(16))) T Xs[PAIRED ? C * XS - TAIL : 1];
-  __shared__ __attribute__((aligned(16))) T Ps[MODE == STATE_ONLY ? 1 : C * PS - TAIL];  // the weighted scores
+  __shared__ __attribute__((aligned(16))) T Xs[PAIRED ? C * XS - (TIGHT ? 0 : TAIL) : 1];
+  __shared__ __attribute__((aligned(16))) T Ps[MODE == STATE_ONLY ? 1 : Op::SCORE_PARTS * PART];  // the weighted scores
   __shared__ __attribute__((aligned(16))) float Hi[2][C], Lo[2][C], In[2][C], Up[2][C];
   __shared__ float Whole[2], Dot[DOTS ? Z::WAVES : 1][C];
   __shared__ int Odd[Z::WAVES];
@@ -388,19 +436,20 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
     g = lane >> 4, n = lane & 15;
     // the chunk's tokens to shared memory, and whether all keys and values are finite
     uint32_t most = 0;
-    auto stage = [&](T* to, int stride, auto& r, auto width, bool look) {
+    auto stage = [&](T* to, auto place_of, auto& r, auto width, bool look) {
       constexpr int D = decltype(width)::value;
 #pragma unroll
       for (int j = 0; j < (int)(sizeof(r) / sizeof(r[0])); ++j) {
         const int i = tid + j * NT, row = i / (D / VEC), c = i % (D / VEC) * VEC;
         if (look) Op::largest(r[j], most);
-        if (C * D / VEC % NT == 0 || row < C) *reinterpret_cast<u32x4*>(&to[row * stride + c]) = r[j];
+        if (C * D / VEC % NT == 0 || row < C) *reinterpret_cast<u32x4*>(&to[place_of(row, c)]) = r[j];
       }
     };
-    stage(Ks, KS, kr, std::integral_constant<int, KD>{}, true);
-    if constexpr (MODE != STATE_ONLY) stage(Qs, QS, qr, std::integral_constant<int, KD>{}, false);
-    stage(Vs, VS, vr, std::integral_constant<int, VD>{}, true);
-    if constexpr (PAIRED) stage(Xs, XS, xr, std::integral_constant<int, VD>{}, false);
+    auto rows_of = [](auto stride) { return [](int row, int c) { return row * decltype(stride)::value + c; }; };
+    stage(Ks, rows_of(std::integral_constant<int, KS>{}), kr, std::integral_constant<int, KD>{}, true);
+    if constexpr (MODE != STATE_ONLY) stage(Qs, rows_of(std::integral_constant<int, QS>{}), qr, std::integral_constant<int, KD>{}, false);
+    stage(Vs, rows_of(std::integral_constant<int, VS>{}), vr, std::integral_constant<int, VD>{}, true);
+    if constexpr (PAIRED) stage(Xs, x_at, xr, std::integral_constant<int, VD>{}, false);
     const bool odd_here = __ballot(!Op::finite(most)) != 0;
     if (lane == 0) Odd[wave] = odd_here;
     __syncthreads();
@@ -448,41 +497,35 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
     f32x4 O[Z::TT][Z::ET];
     float dots[PAIRED ? Z::TT : 1] = {};  // this lane's part of x . o of token 16 t + n
     if constexpr (MODE != STATE_ONLY) {
-      // scores, tile by tile over the waves: (ti, si <= ti), and zeros where a later product's 32 tokens reach past ti
+      // scores, tile by tile over the waves
       int turn = 0;
 #pragma unroll
       for (int ti = 0; ti < Z::TT; ++ti)
 #pragma unroll
-        for (int si = 0; si <= (ti | 1); ++si, ++turn) {
+        for (int si = 0; si <= ti; ++si, ++turn) {
           if (turn % Z::WAVES != wave) continue;
           f32x4 p = {0.f, 0.f, 0.f, 0.f};
-          if (si <= ti) {
 #pragma unroll
-            for (int d = 0; d < Z::DB; ++d)
-              p = Op::mma(Op::row(&Ks[(16 * si + n) * KS + 32 * d + 8 * g]),
-                          Op::row(&Qs[(16 * ti + n) * QS + 32 * d + 8 * g]), p);
-            f32x4 vx = {0.f, 0.f, 0.f, 0.f};
-            if constexpr (PAIRED) {
+          for (int d = 0; d < Z::DB; ++d)
+            p = Op::mma(Op::row(&Ks[(16 * si + n) * KS + 32 * d + 8 * g]),
+                        Op::row(&Qs[(16 * ti + n) * QS + 32 * d + 8 * g]), p);
+          f32x4 vx = {0.f, 0.f, 0.f, 0.f};
+          if constexpr (PAIRED) {
 #pragma unroll
-              for (int d = 0; d < Z::VB; ++d)
-                vx = Op::mma(Op::row(&Vs[(16 * si + n) * VS + 32 * d + 8 * g]),
-                             Op::row(&Xs[(16 * ti + n) * XS + 32 * d + 8 * g]), vx);
-            }
-            const float th = Hi[buf][16 * ti + n], tl = Lo[buf][16 * ti + n];
-            const f32x4 sh = *reinterpret_cast<const f32x4*>(&Hi[buf][16 * si + 4 * g]),
-                        sl = *reinterpret_cast<const f32x4*>(&Lo[buf][16 * si + 4 * g]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float w = exp2_of((th - sh[i]) + (tl - sl[i])) * (A.key_scale * A.out_scale);
-              p[i] = si < ti || 4 * g + i <= n ? kept(w, p[i]) : 0.0f;
-              if constexpr (PAIRED) dots[ti] += (si < ti || 4 * g + i <= n) && w != 0.0f ? p[i] * vx[i] : 0.0f;
-            }
+            for (int d = 0; d < Z::VB; ++d)
+              vx = Op::mma(Op::row(&Vs[(16 * si + n) * VS + 32 * d + 8 * g]), Op::row(&Xs[x_at(16 * ti + n, 32 * d + 8 * g)]),
+                           vx);
           }
-          struct alignas(4 * sizeof(T)) Scores { T v[4]; };
-          Scores f;
+          const float th = Hi[buf][16 * ti + n], tl = Lo[buf][16 * ti + n];
+          const f32x4 sh = *reinterpret_cast<const f32x4*>(&Hi[buf][16 * si + 4 * g]),
+                      sl = *reinterpret_cast<const f32x4*>(&Lo[buf][16 * si + 4 * g]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) f.v[i] = from_f<T>(p[i]);
-          *reinterpret_cast<Scores*>(&Ps[(16 * ti + n) * PS + 16 * si + 4 * g]) = f;
+          for (int i = 0; i < 4; ++i) {
+            const float w = exp2_of((th - sh[i]) + (tl - sl[i])) * (A.key_scale * A.out_scale);
+            p[i] = si < ti || 4 * g + i <= n ? kept(w, p[i]) : 0.0f;
+            if constexpr (PAIRED) dots[ti] += (si < ti || 4 * g + i <= n) && w != 0.0f ? p[i] * vx[i] : 0.0f;
+          }
+          Op::put_scores(&Ps[score_at(ti, si, n, 4 * g)], PART, p);
         }
       // the state's part
 #pragma unroll
@@ -491,13 +534,13 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
         for (int e = 0; e < Z::ET; ++e) O[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int d = 0; d < Z::DB; ++d) {
-        std::conditional_t<MODE == EXACT, typename Op::Wide, typename Op::Frag> s[Z::ET];
+        std::conditional_t<MODE == EXACT, typename Op::Wide, typename Op::Pair> s[Z::ET];
 #pragma unroll
         for (int e = 0; e < Z::ET; ++e) {
           float y[8];
 #pragma unroll
           for (int i = 0; i < 4; ++i) y[i] = S[2 * d][e][i], y[4 + i] = S[2 * d + 1][e][i];
-          if constexpr (MODE == EXACT) s[e] = Op::wide(y); else s[e] = Op::narrow(y);
+          if constexpr (MODE == EXACT) s[e] = Op::wide(y); else s[e] = Op::pair(y);
         }
 #pragma unroll
         for (int t = 0; t < Z::TT; ++t) {
@@ -522,7 +565,7 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
           float dot = dots[t];
 #pragma unroll
           for (int e = 0; e < Z::ET; ++e) {
-            const Four f = *reinterpret_cast<const Four*>(&Xs[(16 * t + n) * XS + e0 + 16 * e + 4 * g]);
+            const Four f = *reinterpret_cast<const Four*>(&Xs[x_at(16 * t + n, e0 + 16 * e + 4 * g)]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) dot = fmaf(O[t][e][i], to_f(f.v[i]), dot);
           }
@@ -547,7 +590,7 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
         for (int t = 0; t < Z::TT; ++t)
 #pragma unroll
           for (int s = 0; s <= t / 2; ++s) {
-            const typename Op::Frag f = Op::row_split(&Ps[(16 * t + n) * PS + 32 * s + 4 * g]);
+            const typename Op::Pair f = Op::scores(&Ps[score_at(t, 2 * s, n, 4 * g)], PART, 2 * s < t);
 #pragma unroll
             for (int e = 0; e < Z::ET; ++e) O[t][e] = Op::mma(vf[s][e], f, O[t][e]);
           }
@@ -558,7 +601,7 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
           for (int s = 0; s < C; ++s) {
             const float w = exp2_of((Hi[buf][tt] - Hi[buf][s]) + (Lo[buf][tt] - Lo[buf][s]));
             if (s > tt || w == 0.0f) continue;
-            const float p = to_f(Ps[tt * PS + s]);
+            const float p = Op::score(&Ps[score_at(t, s / 16, n, s % 16)], PART);
 #pragma unroll
             for (int e = 0; e < Z::ET; ++e)
 #pragma unroll
