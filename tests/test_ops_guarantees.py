@@ -7,7 +7,7 @@ import torch
 
 from _ops_oracle import EPS, HALF, linear64, within
 from test_ops_linear_attention import DEVICES, grads, inputs, magnitudes, make, roundings
-from ttc.ops import linear_attention
+from ttc.ops import linear_attention, linear_attention_step
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -26,3 +26,21 @@ def test_outputs_in_16_bits_are_rounded_once(device, case):
     for name in ("o", "q", "k", "v"):
         once = HALF[torch.bfloat16] * 1.01 * want[name].abs()
         within(got[name], want[name], once + size[name] * (roundings(x, T) * EPS + 2.0 ** -15) + 1e-30)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("slots", [False, True])
+def test_a_state_that_a_backward_needs_is_not_overwritten_unnoticed(device, slots):
+    x = inputs(2, 20, 2, 2, 2, 2, 16, 24, torch.float32, device, True)
+    index = torch.tensor([1, 0], dtype=torch.int32, device=device) if slots else None
+    q = x["q"].clone().requires_grad_()
+    o = linear_attention(q, x["k"], x["v"], x["g"], initial_state=x["state"])
+    before = x["state"]._version
+    linear_attention_step(x["q"][:, 0], x["k"][:, 0], x["v"][:, 0], x["g"][:, 0], x["state"], slots=index)
+    assert x["state"]._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(o.sum(), q)
+    with torch.inference_mode():  # where tensors have no versions
+        state = x["state"].clone()
+        linear_attention_step(x["q"][:, 0], x["k"][:, 0], x["v"][:, 0], x["g"][:, 0], state, slots=index)
+    assert not torch.equal(state, x["state"])

@@ -223,6 +223,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
                              *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], gb, gh, state.data_ptr(), ptr(slots),
                              o.data_ptr())
     launch(lib.ttc_linear_attention_step, "ttc_linear_attention_step", block, q.device)
+    torch.autograd.graph.increment_version(state)  # whoever saved it for a backward has to find out
     return o
 
 
