@@ -44,3 +44,33 @@ def test_a_state_that_a_backward_needs_is_not_overwritten_unnoticed(device, slot
         state = x["state"].clone()
         linear_attention_step(x["q"][:, 0], x["k"][:, 0], x["v"][:, 0], x["g"][:, 0], state, slots=index)
     assert not torch.equal(state, x["state"])
+
+
+def from_token(t, got, x, scale, d_o, d_state):
+    """Outputs and gradients of tokens t on, and the final state, are those of the recurrence."""
+    o, final = linear_attention(x["q"], x["k"], x["v"], x["g"], scale=scale, initial_state=x["state"], output_state=True)
+    want = linear64(x["q"], x["k"], x["v"], x["g"], scale, x["state"], d_o, d_state)
+    size, n, dt = magnitudes(x, scale, d_o, d_state), roundings(x, o.shape[1]) * EPS, o.dtype
+    near = n + (2.0 ** -15 if dt != torch.float32 else 0)
+    within(final, want["state"], size["state"] * n + 1e-30)
+    for name, out in (("o", o), ("q", got["q"]), ("k", got["k"]), ("v", got["v"])):
+        within(out[:, t:], want[name][:, t:], HALF[dt] * 1.01 * want[name][:, t:].abs() + size[name][:, t:] * near + 1e-30)
+    d = (x["q"].detach().double().cpu().abs() * size["q"]).sum(-1) + (x["k"].detach().double().cpu().abs() * size["k"]).sum(-1)
+    end = (size["state"] * d_state.detach().double().cpu().abs()).sum((-1, -2))[:, None]
+    within(got["g"][:, t:], want["g"][:, t:], (d.flip(1).cumsum(1).flip(1) + end)[:, t:] * n + EPS * want["g"][:, t:].abs())
+
+
+@pytest.mark.parametrize("device", DEVICES[1:])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("value", [100.0, math.inf, math.nan])
+def test_a_reset_behind_decays_that_overflow(device, dtype, value):
+    """In the next chunk (32 tokens in 32 bits, 64 in 16) of the same part of a long input, which has two chunks here: nothing
+    of what came before is left."""
+    C = 64 if dtype == torch.bfloat16 else 32
+    x = inputs(1, 512, 2, 2, 2, 2, 32, 48, dtype, device, True)
+    x["g"][:, C // 2, 0], reset = value, C + C // 2
+    x["g"][:, reset, 0] = -math.inf
+    d_o = make((1, 512, 2, 48), dtype, device, 9)
+    d_o[:, :reset, 0] = 0
+    d_state = make((1, 2, 32, 48), torch.float32, device, 10)
+    from_token(reset, grads(x, d_o, d_state, 0.3), x, 0.3, d_o, d_state)

@@ -663,7 +663,7 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
     for (int d = 0; d < Z::DT; ++d)
 #pragma unroll
       for (int e = 0; e < Z::ET; ++e) S[d][e] = whole == 0.0f ? f32x4{0.f, 0.f, 0.f, 0.f} : S[d][e] * whole;
-    whole_decay *= whole;
+    whole_decay = whole == 0.0f ? 0.0f : kept(whole_decay, whole);  // a reset stays one beside decays that are not finite
     if (!odd) {
 #pragma unroll
       for (int s = 0; s < Z::KB; ++s) {
