@@ -74,3 +74,22 @@ def test_a_reset_behind_decays_that_overflow(device, dtype, value):
     d_o[:, :reset, 0] = 0
     d_state = make((1, 2, 32, 48), torch.float32, device, 10)
     from_token(reset, grads(x, d_o, d_state, 0.3), x, 0.3, d_o, d_state)
+
+
+@pytest.mark.parametrize("device", DEVICES[1:])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T", [4, 64, 200])
+def test_a_reset_just_below_the_limit(device, dtype, T):
+    """-105 drops the state as -inf does, where later tokens grow by more than it took away too."""
+    x = inputs(1, T, 2, 2, 2, 2, 32, 48, dtype, device, True)
+    x["g"][:, 2, 0] = -105.0
+    x["g"][:, 3:20, 0] = 3.0 if T > 4 else 40.0
+    x["k"][:, 2:20, 0] = 0  # so that nothing but what leaks is left in the state
+    x["state"] *= 1e30
+    d_o, d_state = make((1, T, 2, 48), dtype, device, 9), make((1, 2, 32, 48), torch.float32, device, 10)
+    got = grads(x, d_o, d_state, 0.3)
+    from_token(0, got, x, 0.3, d_o, d_state)
+    cut = dict(x, g=x["g"].clone())
+    cut["g"][:, 2, 0] = -math.inf
+    for name, d in grads(cut, d_o, d_state, 0.3).items():
+        assert torch.equal(d, got[name]), name

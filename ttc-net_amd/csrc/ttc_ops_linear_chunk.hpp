@@ -392,8 +392,8 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
     return A.gamma_bf16 ? (uint32_t) static_cast<const uint16_t*>(A.gamma)[i] : static_cast<const uint32_t*>(A.gamma)[i];
   };
   auto gates = [&](uint32_t bits, int buf) {
-    double y = (double)__uint_as_float(A.gamma_bf16 ? bits << 16 : bits) * 1.4426950408889634;
-    y = y < -4096.0 ? -4096.0 : y;
+    const float lg = __uint_as_float(A.gamma_bf16 ? bits << 16 : bits);
+    double y = lg < RESET ? -4096.0 : (double)lg * 1.4426950408889634;
 #pragma unroll
     for (int m = 1; m < C; m <<= 1) {
       const double z = __shfl_up(y, m, 64);
