@@ -93,3 +93,26 @@ def test_a_reset_just_below_the_limit(device, dtype, T):
     cut["g"][:, 2, 0] = -math.inf
     for name, d in grads(cut, d_o, d_state, 0.3).items():
         assert torch.equal(d, got[name]), name
+
+
+def with_lost_token(T, bad, reset, dtype, device, value, parts):
+    """Inputs of which one token is lost (all of `parts` not finite, in the first head) and a later one resets."""
+    x = inputs(1, T, 2, 2, 2, 2, 32, 48, dtype, device, True)
+    for name in parts:
+        x[name][0, bad, 0] = value
+    x["g"][0, reset, 0] = -math.inf
+    d_o, d_state = make((1, T, 2, 48), dtype, device, 9), make((1, 2, 32, 48), torch.float32, device, 10)
+    d_o[:, :reset, 0] = 0
+    return x, d_o, d_state
+
+
+@pytest.mark.parametrize("device", DEVICES[1:])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,bad,reset", [(4, 1, 2), (12, 3, 4), (64, 20, 29), (200, 70, 90), (130, 128, 129)])
+@pytest.mark.parametrize("value,parts", [(math.nan, "g"), (math.inf, "g"), (math.nan, "qkvg")])
+def test_a_lost_token_stays_in_its_text(device, dtype, T, bad, reset, value, parts):
+    """A decay that is not finite has no effect past a reset, in one chunk too; nor has a token that is NaN altogether."""
+    x, d_o, d_state = with_lost_token(T, bad, reset, dtype, device, value, parts)
+    o = linear_attention(x["q"], x["k"], x["v"], x["g"], initial_state=x["state"])
+    assert not torch.isfinite(o[0, bad, 0]).all() and torch.isfinite(o[0, :bad]).all() and torch.isfinite(o[0, :, 1]).all()
+    from_token(reset, grads(x, d_o, d_state, 0.3), x, 0.3, d_o, d_state)

@@ -21,7 +21,7 @@
 // (a large library product: 153).
 //
 // Numerics.  The sums G are held in 64 bits while they are formed and as pairs of fp32 after, so that differences of
-// large sums keep their digits; a decay of 0 is 2^-4096.  In bf16, w V is split into three bf16 parts (exact in fp32's 24
+// large sums keep their digits; they start anew at a reset.  In bf16, w V is split into three bf16 parts (exact in fp32's 24
 // digits), so the state has fp32's accuracy; P, and in FAST the state's copy in front of a chunk, into two (16 digits), so that a
 // bf16 output is rounded to 8 digits once.  (Both in one part of 8 digits: the prompt above takes 143 us as a whole, so 155,
 // training on 4 x 2,048 tokens x 32 heads of 64 264, so 288, and the outputs' error is 2.35e-3 of their norm instead of 1.66e-3.)
@@ -392,21 +392,29 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
     return A.gamma_bf16 ? (uint32_t) static_cast<const uint16_t*>(A.gamma)[i] : static_cast<const uint32_t*>(A.gamma)[i];
   };
   auto gates = [&](uint32_t bits, int buf) {
-    const float lg = __uint_as_float(A.gamma_bf16 ? bits << 16 : bits);
-    double y = lg < RESET ? -4096.0 : (double)lg * 1.4426950408889634;
+    // Sums start anew at a reset, so that nothing in front of it is in those behind it.  What Hi and Lo hold is 2^15 lower for
+    // each reset so far, and infinite where a sum is lost (a NaN, or growth beyond e^128, which fp32 does not hold), so that
+    // Hi_t - Hi_s gives a weight of 0 across a reset, whatever s holds: sums between resets lie within 64 x 185.
+    const float lg = __uint_as_float(A.gamma_bf16 ? bits << 16 : bits), inf = __builtin_inff();
+    const bool cut = lane < C && lg < RESET;
+    const uint64_t cuts = __ballot(cut), so_far = cuts & (((uint64_t)2 << lane) - 1);
+    const int start = so_far == 0 ? 0 : 63 - __builtin_clzll(so_far);
+    double y = cut ? 0.0 : lg <= 128.0f ? (double)lg * 1.4426950408889634 : (double)inf;
 #pragma unroll
     for (int m = 1; m < C; m <<= 1) {
       const double z = __shfl_up(y, m, 64);
-      if (lane >= m) y += z;
+      if (lane - m >= start) y += z;
     }
     const double rest = __shfl(y, C - 1, 64) - y;
     if (lane < C) {
-      const float hi = (float)y, lo = (float)(y - (double)hi), uh = (float)rest, ul = (float)(rest - (double)uh);
+      const double low = y - 32768.0 * __builtin_popcountll(so_far);
+      const float uh = (float)rest, ul = (float)(rest - (double)uh), hi = (float)low;
+      const float lo = hi < inf ? (float)(low - (double)hi) : 0.0f;
       Hi[buf][lane] = hi;
       Lo[buf][lane] = lo;
-      const float in = exp2_of(hi) * exp2_of(lo);
+      const float in = so_far != 0 ? 0.0f : exp2_of(hi) * exp2_of(lo);
       In[buf][lane] = in * A.out_scale;
-      Up[buf][lane] = exp2_of(uh) * exp2_of(ul) * A.key_scale;
+      Up[buf][lane] = so_far != cuts ? 0.0f : hi < inf ? exp2_of(uh) * exp2_of(ul) * A.key_scale : inf;
       if (lane == C - 1) Whole[buf] = in;
     }
   };
