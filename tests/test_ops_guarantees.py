@@ -7,7 +7,10 @@ import torch
 
 from _ops_oracle import EPS, HALF, linear64, within
 from test_ops_linear_attention import DEVICES, grads, inputs, magnitudes, make, roundings
-from ttc.ops import linear_attention, linear_attention_step
+from ttc.ops import group_norm, linear_attention, linear_attention_step
+from ttc.ops._call import recorded_backward
+from ttc.ops.group_norm import group_norm_torch
+from ttc.ops.linear_attention import linear_attention_torch
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -116,3 +119,57 @@ def test_a_lost_token_stays_in_its_text(device, dtype, T, bad, reset, value, par
     o = linear_attention(x["q"], x["k"], x["v"], x["g"], initial_state=x["state"])
     assert not torch.isfinite(o[0, bad, 0]).all() and torch.isfinite(o[0, :bad]).all() and torch.isfinite(o[0, :, 1]).all()
     from_token(reset, grads(x, d_o, d_state, 0.3), x, 0.3, d_o, d_state)
+
+
+class Recorded(torch.autograd.Function):
+    """A form whose backward is recorded_backward, as that of the kernels' Functions where it is itself recorded."""
+
+    @staticmethod
+    def forward(ctx, form, *xs):
+        ctx.form = form
+        ctx.save_for_backward(*xs)
+        return form(*xs)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        return (None, *recorded_backward(ctx.form, ctx.saved_tensors, ctx.needs_input_grad[1:], grads,
+                                         torch.is_grad_enabled()))
+
+
+def related(name, x, w):
+    """An operator's inputs that are computed from one another."""
+    if name == "norm":  # the gate from what is normalised, the weights from a mean of it
+        return x, x.mean((0, 1)), x.sum((0, 1)) * 0.1, x @ w
+    heads = lambda t: t.unflatten(-1, (2, 8))  # noqa: E731
+    if name == "same":  # queries and keys are one tensor, values and decays functions of it
+        q = heads(x)
+        return q, q, torch.tanh(heads(x @ w)), -torch.sigmoid(x[..., :2]), None
+    q = heads(x @ w)
+    return q, torch.tanh(q), q * q, -torch.sigmoid(q[..., 0]), q.mean(1).unsqueeze(-1) * q.mean(1).unsqueeze(-2)
+
+
+FORMS = {"norm": (lambda x, w, b, g: group_norm(x, 2, w, b, activation="silu", gate=g),
+                  lambda x, w, b, g: group_norm_torch(x, 2, w, b, activation="silu", gate=g))}
+FORMS["same"] = FORMS["chain"] = (lambda q, k, v, g, s: linear_attention(q, k, v, g, scale=0.3, initial_state=s),
+                                  lambda q, k, v, g, s: linear_attention_torch(q, k, v, g, 0.3, s)[0])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("name", ["norm", "same", "chain"])
+def test_recorded_gradients_are_partial(device, name):
+    """An input's gradient leaves out what reaches the output through other inputs, with create_graph too: first and second
+    derivatives are those of the torch operators.  Both are 32-bit sums of at most 20 x 16 terms over three stages with slopes
+    below 8: 2^10 EPS of the largest value."""
+    x = make((2, 20, 16), torch.float32, device, 30)
+    w = make((16, 16), torch.float32, device, 31, 0.25)
+    op, form = FORMS[name]
+
+    def derivatives(f):
+        leaf = x.clone().requires_grad_()
+        first, = torch.autograd.grad(f(*related(name, leaf, w)).sin().sum(), leaf, create_graph=True)
+        return first.detach(), torch.autograd.grad(first.sin().sum(), leaf)[0]
+
+    want = derivatives(form)
+    for f in (op, lambda *xs: Recorded.apply(form, *xs)):
+        for d, e in zip(derivatives(f), want):
+            assert float((d - e).abs().max()) <= 2 ** 10 * EPS * max(1.0, float(e.abs().max()))

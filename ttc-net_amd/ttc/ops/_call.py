@@ -52,8 +52,9 @@ def recorded_backward(form, inputs, needs, grads, create_graph: bool):
     """Gradients of ``form(*inputs)`` (torch operators; a tensor or a tuple) for the inputs flagged in ``needs``, with
     operators that can be differentiated or observed again."""
     with torch.enable_grad():
-        if not create_graph:
-            inputs = [x if x is None else x.detach().requires_grad_(n) for x, n in zip(inputs, needs)]
+        # Partial derivatives: with respect to aliases, since one input may be computed from another, or be the same tensor
+        inputs = [x if x is None else x.view_as(x) if create_graph else x.detach().requires_grad_(n)
+                  for x, n in zip(inputs, needs)]
         out = form(*inputs)
         pairs = [(o, g) for o, g in zip(out if isinstance(out, tuple) else (out,), grads) if g is not None]
         wrt = [x for x, n in zip(inputs, needs) if n]
