@@ -7,6 +7,7 @@ import torch
 
 from _ops_oracle import EPS, HALF, linear64, within
 from test_ops_linear_attention import DEVICES, grads, inputs, magnitudes, make, roundings
+from ttc.layers.front_end import front_end, front_end_torch
 from ttc.ops import group_norm, linear_attention, linear_attention_step
 from ttc.ops._call import recorded_backward
 from ttc.ops.group_norm import group_norm_torch
@@ -173,3 +174,20 @@ def test_recorded_gradients_are_partial(device, name):
     for f in (op, lambda *xs: Recorded.apply(form, *xs)):
         for d, e in zip(derivatives(f), want):
             assert float((d - e).abs().max()) <= 2 ** 10 * EPS * max(1.0, float(e.abs().max()))
+
+
+@pytest.mark.gpu
+def test_recorded_gradients_of_the_front_end_are_partial():
+    """The bias computed from the projection: the kernel's first derivatives under create_graph and the second ones against
+    the operators', both 32-bit sums of at most 80 terms with slopes below 8: 2^10 EPS of the largest."""
+    dims = (2, 6, 5, 3, 4)
+    x = make((3, 73), torch.float32, "cuda", 40)
+
+    def derivatives(f):
+        leaf = x.clone().requires_grad_()
+        y = f(leaf, leaf.mean(0)[:12] - 1.0, dims)
+        first, = torch.autograd.grad(sum(t.sin().sum() for t in y), leaf, create_graph=True)
+        return first.detach(), torch.autograd.grad(first.sin().sum(), leaf)[0]
+
+    for d, e in zip(derivatives(front_end), derivatives(front_end_torch)):
+        assert float((d - e).abs().max()) <= 2 ** 10 * EPS * max(1.0, float(e.abs().max()))

@@ -71,8 +71,9 @@ class _FrontEndFunc(torch.autograd.Function):
         recorded = torch.is_grad_enabled()
         if recorded or _traced(proj, bias, *grads):  # differentiable operators, seen one by one
             with torch.enable_grad():
-                if not recorded:
-                    proj, bias = (t if t is None else t.detach().requires_grad_() for t in (proj, bias))
+                # partial derivatives: with respect to aliases, since the bias may be computed from the projection
+                proj, bias = (t if t is None else t.view_as(t) if recorded else t.detach().requires_grad_()
+                              for t in (proj, bias))
                 out = front_end_torch(proj, bias, ctx.dims)
                 pairs = [(o, g) for o, g in zip(out, grads) if g is not None]
                 wrt = [t for t, need in ((proj, need_proj), (bias, need_bias)) if need]
