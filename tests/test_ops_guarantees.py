@@ -191,3 +191,25 @@ def test_recorded_gradients_of_the_front_end_are_partial():
 
     for d, e in zip(derivatives(front_end), derivatives(front_end_torch)):
         assert float((d - e).abs().max()) <= 2 ** 10 * EPS * max(1.0, float(e.abs().max()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,bad,reset", [(10, 5, 6), (64, 20, 29), (200, 70, 90), (130, 128, 129)])
+@pytest.mark.parametrize("value,parts", [(math.nan, "v"), (math.inf, "k"), (math.nan, "q"), (math.nan, "g"), (math.inf, "g"),
+                                         (math.nan, "qkvg"), (100.0, "g")])
+def test_torch_form_drops_what_is_masked(dtype, T, bad, reset, value, parts):
+    """The CPU's form as the kernels: no effect on earlier tokens, on other heads or past a reset, outputs or gradients."""
+    x, d_o, d_state = with_lost_token(T, bad, reset, dtype, "cpu", value, parts)
+    o = linear_attention(x["q"], x["k"], x["v"], x["g"], scale=0.3, initial_state=x["state"])
+    clean = linear64(x["q"][:, :bad], x["k"][:, :bad], x["v"][:, :bad], x["g"][:, :bad], 0.3, x["state"])["o"]
+    early = {n: x[n][:, :bad] for n in "qkvg"} | {"state": x["state"]}
+    size = magnitudes(early, 0.3)["o"]
+    within(o[:, :bad], clean, HALF[dtype] * 1.01 * clean.abs() + size * roundings(x, T) * EPS + 1e-30)
+    assert torch.isfinite(o[:, :, 1]).all() and (value == 100.0 or not torch.isfinite(o[0, bad, 0]).all())
+    from_token(reset, grads(x, d_o, d_state, 0.3), x, 0.3, d_o, d_state)
+
+
+def test_torch_form_drops_a_state_that_is_not_finite():
+    x, d_o, d_state = with_lost_token(70, 3, 5, torch.float32, "cpu", 0.0, "v")
+    x["state"][0, 0, 3, 4] = math.nan
+    from_token(5, grads(x, d_o, d_state, 0.3), x, 0.3, d_o, d_state)

@@ -28,19 +28,39 @@ _BLOCK = struct.Struct("12qd4q12qqqqq3qq4qqqqqq")
 _STEP_BLOCK = struct.Struct("10qd4q8qqqq")
 
 
+def _token_by_token(q, k, v, g, S):
+    """A chunk as its recurrence: a token meets nothing but the state, and a reset selects."""
+    out = []
+    for t in range(q.shape[2]):
+        cut = g[:, :, t] < RESET
+        S = torch.where(cut[..., None, None], torch.zeros_like(S), S)
+        S = S * g[:, :, t].masked_fill(cut, 0.0).exp()[..., None, None] + k[:, :, t].unsqueeze(-1) * v[:, :, t].unsqueeze(-2)
+        out.append((S * q[:, :, t].unsqueeze(-1)).sum(-2))
+    return torch.stack(out, 2), S
+
+
 def linear_attention_torch(q, k, v, log_gamma, scale, initial_state=None):
     """:func:`linear_attention` as torch operators: ``(o, final state)``.  Chunks of 64 tokens, products within a chunk,
-    the state from chunk to chunk."""
+    the state from chunk to chunk.  A product with a weight of 0 does not drop what is not finite: a chunk that holds such
+    values goes token by token.  Where nothing can look at them (operators that are observed; a CUDA tensor, for which the host
+    would have to wait) it does not, and they can reach every output of their chunk and head and of those after it."""
+    look = not (q.is_cuda or traced(q, k, v, log_gamma, initial_state))
+    finite = lambda *xs: all(bool(x.detach().sum().isfinite()) for x in xs)  # noqa: E731  (or else sums that overflow)
     B, T = q.shape[:2]
     H, dk, dv = log_gamma.shape[-1], q.shape[-1], v.shape[-1]
     wide = lambda x: x.float().repeat_interleave(H // x.shape[2], dim=2).transpose(1, 2)  # noqa: E731
     qs, ks, vs = wide(q) * scale, wide(k), wide(v)
     g = log_gamma.float().expand(B, T, H).transpose(1, 2)
     S = q.new_zeros((B, H, dk, dv), dtype=torch.float32) if initial_state is None else initial_state
+    whole = look and finite(q, k, v) and bool((log_gamma < torch.inf).all())
     nothing = (qs * ks).sum(-1, keepdim=True) * vs * g.unsqueeze(-1)  # of no tokens: empty, and depends on everything
     out = [nothing] if T == 0 else []
     for at in range(0, T, _CHUNK):
         qc, kc, vc, gc = (x[:, :, at:at + _CHUNK] for x in (qs, ks, vs, g))
+        if look and not (finite(S) and (whole or finite(qc, kc, vc) and bool((gc < torch.inf).all()))):
+            o, S = _token_by_token(qc, kc, vc, gc, S)
+            out.append(o)
+            continue
         n = gc.shape[-1]
         reset = gc < RESET  # drops the state: no weight crosses it
         part = reset.long().cumsum(-1)
@@ -168,7 +188,9 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_gamm
     share ``q`` and ``k``).  ``scale``: ``dk ** -0.5`` by default.  States are float32 ``[batch, heads, dk, dv]``.
 
     A ``log_gamma`` below -104 (``exp`` is 0 in 32 bits; ``-inf`` included) drops the state, so that several texts can
-    follow each other in one sequence: nothing before it has any effect on what follows.  Differentiable in all tensors.
+    follow each other in one sequence: nothing before it has any effect on what follows, whatever it holds.  Of CUDA calls
+    that are observed operator by operator (compiled, under a transform, gradients with ``create_graph``) that holds for
+    finite values only.  Differentiable in all tensors.
     """
     H = _check("linear_attention", q, k, v, log_gamma, 4)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
