@@ -213,3 +213,30 @@ def test_torch_form_drops_a_state_that_is_not_finite():
     x, d_o, d_state = with_lost_token(70, 3, 5, torch.float32, "cpu", 0.0, "v")
     x["state"][0, 0, 3, 4] = math.nan
     from_token(5, grads(x, d_o, d_state, 0.3), x, 0.3, d_o, d_state)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("observed", [False, True])
+def test_autocast_does_not_narrow_the_arithmetic(device, observed):
+    """32-bit inputs have 32-bit results under autocast as outside of it, in the kernels' form and the operators'."""
+    x = inputs(1, 90, 2, 2, 2, 2, 32, 48, torch.float32, device, True)
+    run = lambda s: linear_attention(x["q"], x["k"], x["v"], x["g"], scale=0.3, initial_state=s, output_state=True)  # noqa: E731
+    with torch.autocast(device, torch.bfloat16):
+        o, final = torch.func.vmap(run)(x["state"][None]) if observed else run(x["state"])
+    o, final = (o[0], final[0]) if observed else (o, final)
+    want, size = linear64(x["q"], x["k"], x["v"], x["g"], 0.3, x["state"]), magnitudes(x, 0.3)
+    assert o.dtype == final.dtype == torch.float32
+    within(o, want["o"], size["o"] * roundings(x, 90) * EPS)
+    within(final, want["state"], size["state"] * roundings(x, 90) * EPS)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("narrow", [False, True])
+def test_compiles_as_one_graph(device, narrow):
+    """Operators and their order are those of the torch form: 4 EPS of the largest value."""
+    x = inputs(1, 20, 2, 2, 2, 2, 8, 8, torch.float32, device, True)
+    f = lambda q, s: linear_attention(q, x["k"], x["v"], x["g"], scale=0.3, initial_state=s)  # noqa: E731
+    want = linear_attention_torch(x["q"], x["k"], x["v"], x["g"], 0.3, x["state"])[0]
+    with torch.autocast(device, torch.bfloat16, enabled=narrow):
+        got = torch.compile(f, fullgraph=True, backend="eager")(x["q"], x["state"])
+    assert float((got - want).abs().max()) <= 4 * EPS * float(want.abs().max())

@@ -44,6 +44,13 @@ def linear_attention_torch(q, k, v, log_gamma, scale, initial_state=None):
     the state from chunk to chunk.  A product with a weight of 0 does not drop what is not finite: a chunk that holds such
     values goes token by token.  Where nothing can look at them (operators that are observed; a CUDA tensor, for which the host
     would have to wait) it does not, and they can reach every output of their chunk and head and of those after it."""
+    if q.device.type in ("cpu", "cuda"):
+        with torch.autocast(q.device.type, enabled=False):  # products in 32 bits, whatever a model's own are in
+            return _in_chunks(q, k, v, log_gamma, scale, initial_state)
+    return _in_chunks(q, k, v, log_gamma, scale, initial_state)
+
+
+def _in_chunks(q, k, v, log_gamma, scale, initial_state):
     look = not (q.is_cuda or traced(q, k, v, log_gamma, initial_state))
     finite = lambda *xs: all(bool(x.detach().sum().isfinite()) for x in xs)  # noqa: E731  (or else sums that overflow)
     B, T = q.shape[:2]
