@@ -7,6 +7,7 @@ import torch
 
 from _ops_oracle import EPS, HALF, linear64, within
 from test_ops_linear_attention import DEVICES, grads, inputs, magnitudes, make, roundings
+from ttc import LinearAttentionLayer
 from ttc.layers.front_end import front_end, front_end_torch
 from ttc.ops import group_norm, linear_attention, linear_attention_step
 from ttc.ops._call import recorded_backward
@@ -240,3 +241,18 @@ def test_compiles_as_one_graph(device, narrow):
     with torch.autocast(device, torch.bfloat16, enabled=narrow):
         got = torch.compile(f, fullgraph=True, backend="eager")(x["q"], x["state"])
     assert float((got - want).abs().max()) <= 4 * EPS * float(want.abs().max())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_layer_without_positions_has_no_longest_input(device):
+    """One call on 9 tokens against two on 5 and 4 and against single steps; some hundred 32-bit terms of about 1: 1e-5."""
+    torch.manual_seed(3)
+    layer = LinearAttentionLayer(16, 2, 8, 8, rotary_dim=0, max_positions=4).to(device)
+    x = make((1, 9, 16), torch.float32, device, 50)
+    with torch.no_grad():
+        y, state = layer(x, output_state=True)
+        first, S = layer(x[:, :5], output_state=True)
+        rest, S2 = layer(x[:, 5:], S, offset=5, output_state=True)
+        steps = torch.cat([layer.step(x[:, t], S, torch.tensor([t], device=device)) for t in range(5, 9)])
+    assert float((torch.cat([first, rest], 1) - y).abs().max()) < 1e-5 and float((S2 - state).abs().max()) < 1e-5
+    assert float((steps - y[0, 5:]).abs().max()) < 1e-5 and float((S - state).abs().max()) < 1e-5

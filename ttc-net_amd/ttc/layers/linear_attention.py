@@ -24,7 +24,7 @@ __all__ = ["LinearAttentionLayer"]
 
 class LinearAttentionLayer(nn.Module):
     """``dim``: width of the model; ``key_dim``, ``value_dim``: a head's sizes (up to 128); ``kv_heads`` divides
-    ``num_heads`` (shared keys and values); ``rotary_dim``: how much of a key is turned (``key_dim`` by default, 0: none);
+    ``num_heads`` (shared keys and values); ``rotary_dim``: how much of a key is turned (``key_dim`` by default, 0: none, so that positions have no limit);
     ``max_positions``: of the table of angles; ``memory``: the heads' decays start, spread evenly over their logarithm, at
     memories of this many tokens; ``rotary``: further arguments of :func:`ttc.ops.rotary_table`."""
 
@@ -62,6 +62,11 @@ class LinearAttentionLayer(nn.Module):
         log_gamma = -F.softplus(g.float() + self.bias_gamma.float())
         return heads(q, self.key_dim), heads(k, self.key_dim), heads(v, self.value_dim), z, log_gamma
 
+    def _turn(self, q, k, positions=None, offset=0):
+        if self.angles.shape[1] == 0:  # rotary_dim = 0: no positions, so any number of tokens
+            return q, k
+        return rotary(q, k, self.angles, positions, offset=offset, layout=self.layout)
+
     def _finish(self, o, z):
         rows = group_norm(o.reshape(-1, self.num_heads * self.value_dim), self.num_heads, self.norm_weight, self.norm_bias,
                           eps=self.eps, activation="silu", gate=z.reshape(-1, self.num_heads * self.value_dim))
@@ -76,7 +81,7 @@ class LinearAttentionLayer(nn.Module):
         """``x [batch, tokens, dim]``, whose first token has position ``offset`` and follows ``state``; with
         ``output_state`` also the state behind the last token."""
         q, k, v, z, log_gamma = self._project(x)
-        q, k = rotary(q, k, self.angles, offset=offset, layout=self.layout)
+        q, k = self._turn(q, k, offset=offset)
         out = linear_attention(q, k, v, log_gamma, initial_state=state, output_state=output_state)
         o, state = out if output_state else (out, None)
         y = self._finish(o, z)
@@ -88,6 +93,5 @@ class LinearAttentionLayer(nn.Module):
         """``x [batch, dim]``, one token of each sequence at ``positions [batch]``; ``state`` (:meth:`new_state`) is
         updated in place, row ``b``'s at ``slots[b]`` (int32; outside: the row is skipped) or ``b``."""
         q, k, v, z, log_gamma = self._project(x)
-        q, k = (t.squeeze(1) for t in rotary(q.unsqueeze(1), k.unsqueeze(1), self.angles, positions.unsqueeze(1),
-                                             layout=self.layout))
+        q, k = (t.squeeze(1) for t in self._turn(q.unsqueeze(1), k.unsqueeze(1), positions.unsqueeze(1)))
         return self._finish(linear_attention_step(q, k, v, log_gamma, state, slots=slots), z)
