@@ -9,7 +9,7 @@ from _ops_oracle import EPS, HALF, linear64, within
 from test_ops_linear_attention import DEVICES, grads, inputs, magnitudes, make, roundings
 from ttc import LinearAttentionLayer
 from ttc.layers.front_end import front_end, front_end_torch
-from ttc.ops import group_norm, linear_attention, linear_attention_step
+from ttc.ops import group_norm, linear_attention, linear_attention_step, rotary, rotary_table
 from ttc.ops._call import recorded_backward
 from ttc.ops.group_norm import group_norm_torch
 from ttc.ops.linear_attention import linear_attention_torch
@@ -256,3 +256,21 @@ def test_a_layer_without_positions_has_no_longest_input(device):
         steps = torch.cat([layer.step(x[:, t], S, torch.tensor([t], device=device)) for t in range(5, 9)])
     assert float((torch.cat([first, rest], 1) - y).abs().max()) < 1e-5 and float((S2 - state).abs().max()) < 1e-5
     assert float((steps - y[0, 5:]).abs().max()) < 1e-5 and float((S - state).abs().max()) < 1e-5
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_a_table_that_is_learnt_has_a_gradient(device, layout):
+    """d cos = sum (x_a d_a + x_b d_b), d sin = sum (x_a d_b - x_b d_a) over the 2 x 3 heads at a position: 12 products and
+    their sums of values below 5, 32 EPS x 25 x 12."""
+    q, k = make((2, 6, 2, 8), torch.float32, device, 60), make((2, 6, 1, 8), torch.float32, device, 61)
+    dq, dk = make(q.shape, torch.float32, device, 62), make(k.shape, torch.float32, device, 63)
+    table = rotary_table(9, 6, device=device).requires_grad_()
+    got, = torch.autograd.grad(rotary(q, k, table, offset=2, layout=layout), table, (dq, dk))
+    want = torch.zeros(9, 3, 2, dtype=torch.float64)
+    for x, d in ((q, dq), (k, dk)):
+        x, d = x.double().cpu()[..., :6], d.double().cpu()[..., :6]
+        a, b = (slice(0, 3), slice(3, 6)) if layout == "half" else (slice(0, 6, 2), slice(1, 6, 2))
+        want[2:8, :, 0] += (x[..., a] * d[..., a] + x[..., b] * d[..., b]).sum((0, 2))
+        want[2:8, :, 1] += (x[..., a] * d[..., b] - x[..., b] * d[..., a]).sum((0, 2))
+    within(got, want, torch.tensor(32 * EPS * 25 * 12))

@@ -146,7 +146,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, table: torch.Tensor, positio
     position ``offset + t``.  A given position outside the table makes that token's turned components NaN (nothing is read
     outside, and nothing waits for the device to find out).  ``layout``: pairs ``(i, i + rot / 2)`` (``"half"``) or
     ``(2 i, 2 i + 1)`` (``"interleaved"``).  ``q`` and ``k`` may be views with any strides over batch, tokens and heads;
-    float32 or bfloat16, turned in 32 bits.  Differentiable in ``q`` and ``k``.
+    float32 or bfloat16, turned in 32 bits.  Differentiable in ``q`` and ``k``; with a ``table`` that requires a gradient the torch operators run
+    instead of the kernel, and it has one too.
     """
     if q.dim() != 4 or (k is not None and k.dim() != 4):
         raise ValueError("rotary: q and k [batch, tokens, heads, dim] are needed")
@@ -172,7 +173,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, table: torch.Tensor, positio
             raise ValueError(f"rotary: positions [tokens] or [batch, tokens] are needed, got {tuple(positions.shape)}")
         if table.shape[0] == 0 and q.numel() > 0:
             raise ValueError("rotary: an empty table")
-    if not q.is_cuda or traced(q, k, table, positions):
+    learnt = table.requires_grad and torch.is_grad_enabled()  # the kernel's backward has no gradient for the table
+    if not q.is_cuda or learnt or traced(q, k, table, positions):
         return rotary_torch(q, k, table, positions, offset=offset, layout=layout)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _RotaryFunc.apply(q, k, table, positions, offset, layout)
