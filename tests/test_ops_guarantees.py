@@ -274,3 +274,20 @@ def test_a_table_that_is_learnt_has_a_gradient(device, layout):
         want[2:8, :, 0] += (x[..., a] * d[..., a] + x[..., b] * d[..., b]).sum((0, 2))
         want[2:8, :, 1] += (x[..., a] * d[..., b] - x[..., b] * d[..., a]).sum((0, 2))
     within(got, want, torch.tensor(32 * EPS * 25 * 12))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("where", ["meta", "cpu"])
+def test_a_layer_without_storage_gets_its_angles(device, where):
+    """Made on the meta device or emptied, then filled from a checkpoint, which holds no angles."""
+    args = dict(dim=16, num_heads=2, key_dim=8, value_dim=8, max_positions=64, rotary=dict(scaling="linear", factor=2.0))
+    torch.manual_seed(3)
+    layer = LinearAttentionLayer(**args)
+    with torch.device(where):
+        other = LinearAttentionLayer(**args)
+    other = other.to_empty(device=device)
+    other.load_state_dict(layer.state_dict())
+    assert other.angles.device.type == device and torch.equal(other.angles.cpu(), layer.angles)
+    x = make((1, 5, 16), torch.float32, device, 51)
+    assert torch.equal(other(x), layer.to(device)(x))
+    assert torch.equal(other.bfloat16().angles, layer.angles) and other.to("meta").angles.is_meta

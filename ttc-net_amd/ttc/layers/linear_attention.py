@@ -46,13 +46,17 @@ class LinearAttentionLayer(nn.Module):
         # softplus(bias_gamma) = 1 / memory where the projection gives 0
         rate = torch.exp(torch.linspace(math.log(1 / memory[1]), math.log(1 / memory[0]), num_heads))
         self.bias_gamma = nn.Parameter(torch.log(torch.expm1(rate)))
-        table = rotary_table(max_positions, key_dim if rotary_dim is None else rotary_dim, **(rotary or {}))
-        self.register_buffer("angles", table, persistent=False)
+        self._table = dict(rotary or {}, length=max_positions, dim=key_dim if rotary_dim is None else rotary_dim)
+        self.register_buffer("angles", rotary_table(**self._table), persistent=False)
 
     def _apply(self, fn, recurse=True):
         angles = self.angles
         super()._apply(fn, recurse)
-        if self.angles.dtype != torch.float32:  # .to(bfloat16) and the like: angles stay in 32 bits
+        # No checkpoint holds the angles: whatever is done to the parameters (another type, to_empty), they keep their values
+        # in 32 bits, or get them where the layer was made without any
+        if angles.is_meta and not self.angles.is_meta:
+            self.angles = rotary_table(**dict(self._table, device=self.angles.device))
+        elif self.angles is not angles:
             self.angles = angles.to(self.angles.device)
         return self
 
