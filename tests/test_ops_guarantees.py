@@ -291,3 +291,29 @@ def test_a_layer_without_storage_gets_its_angles(device, where):
     x = make((1, 5, 16), torch.float32, device, 51)
     assert torch.equal(other(x), layer.to(device)(x))
     assert torch.equal(other.bfloat16().angles, layer.angles) and other.to("meta").angles.is_meta
+
+
+@pytest.mark.gpu
+def test_more_heads_than_one_launch_holds():
+    """2^26 and 2^24 (sequence, head) pairs and more, one by one and in chunks: what the pieces of the batch give, bit for bit."""
+    B, H = 2 ** 13, 2 ** 13 + 1
+    q, k, v, d_o = (make((B, 1, 1, 1), torch.bfloat16, "cuda", 70 + i) * make((1, 1, H, 1), torch.bfloat16, "cuda", 75 + i)
+                    for i in range(4))
+    g = -torch.rand(1, 1, H, device="cuda").expand(B, 1, H).contiguous()
+
+    def run(rows):
+        leaves = [t[rows].detach().requires_grad_() for t in (q, k, v, g)]
+        o = linear_attention(*leaves)
+        return (o.detach(), *torch.autograd.grad(o, leaves, d_o[rows]))
+
+    whole = run(slice(None))
+    for at in range(0, B, 1024):
+        for a, b in zip(whole, run(slice(at, at + 1024))):
+            assert torch.equal(a[at:at + 1024], b)
+    del whole, q, k, v, d_o, g
+    B, H = 2 ** 12 + 1, 2 ** 12
+    q, k, v = (make((B, 5, 1, d), torch.bfloat16, "cuda", 80 + d) for d in (8, 8, 33))
+    g = -torch.rand(H, device="cuda")
+    whole = linear_attention(q, k, v, g)
+    for at in range(0, B, 512):
+        assert torch.equal(whole[at:at + 512], linear_attention(*(t[at:at + 512] for t in (q, k, v)), g))

@@ -49,12 +49,13 @@ inline bool countable(std::initializer_list<int64_t> sizes) {
 // A launch of 2^32 threads or more does not run whole: the workgroups that one launch can have
 inline int64_t max_blocks(int threads) { return ((int64_t)1 << 32) / threads - 1; }
 
-// go(first workgroup, workgroups) for as many launches as that takes
+// go(first workgroup, workgroups) for as many launches as that takes, each of a multiple of `unit` workgroups
 template <class F>
-int in_launches(int64_t blocks, int threads, F go) {
-  for (int64_t first = 0; first < blocks; first += max_blocks(threads)) {
+int in_launches(int64_t blocks, int threads, F go, int64_t unit = 1) {
+  const int64_t most = max_blocks(threads) / unit * unit;
+  for (int64_t first = 0; first < blocks; first += most) {
     const int64_t left = blocks - first;
-    go(first, dim3((unsigned)(left < max_blocks(threads) ? left : max_blocks(threads))));
+    go(first, dim3((unsigned)(left < most ? left : most)));
     if (const int rc = launched()) return rc;
   }
   return TTC_LQR_OK;

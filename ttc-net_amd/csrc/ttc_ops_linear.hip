@@ -15,7 +15,7 @@ __global__ __launch_bounds__(256) void token_sweep_kernel(Sweep A, int tiles, bo
   __shared__ float part[2][4][COLS];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int tile = (int)(blockIdx.x % tiles);
-  const int64_t bh = blockIdx.x / tiles, b = bh / A.H;
+  const int64_t bh = A.first + blockIdx.x / tiles, b = bh / A.H;
   const int h = (int)(bh % A.H);
   const int e0 = tile * COLS + (lane & 7) * 4, r0 = wave * 8 + (lane >> 3);
   const int64_t slot = A.slots ? A.slots[b] : b;
@@ -123,12 +123,13 @@ inline int token_tiles(int vd) { return (vd + 31) / 32; }
 int launch_token_sweep(const Sweep& A, bool bf16, hipStream_t s) {
   const int tiles = token_tiles(A.vd);
   const int64_t blocks = A.B * A.H * tiles;
-  if (blocks == 0) return TTC_LQR_OK;
-  if (blocks > max_blocks(256)) return TTC_LQR_EINVAL;
   const bool wide = A.sc == 1 && A.vd % 4 == 0 && aligned16(A.state_in) && aligned16(A.state_out);
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, s, A, tiles, wide);
-    return launched();
+    return in_launches(blocks, 256, [&](int64_t first, dim3 grid) {
+      Sweep part = A;
+      part.first = first / tiles;
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, part, tiles, wide);
+    }, tiles);
   };
   if (bf16)
     return A.kd <= 32 ? go(token_sweep_kernel<__bf16, 1>) : A.kd <= 64 ? go(token_sweep_kernel<__bf16, 2>)
@@ -185,11 +186,11 @@ constexpr int GATE_TOKENS = 8;
 __global__ __launch_bounds__(64) void gate_kernel(Sweep A, const float* __restrict__ r, const float* __restrict__ c,
                                                   int tiles, int waves, const float* __restrict__ last,
                                                   const float* __restrict__ dlast, int64_t elems, void* d_gamma,
-                                                  double* __restrict__ per_head) {
+                                                  double* __restrict__ per_head, int64_t first) {
   const int lane = threadIdx.x;
-  const int64_t bh = blockIdx.x / A.marks, mark = blockIdx.x % A.marks, b = bh / A.H, BHT = A.B * A.H * A.T;
+  const int64_t stretch = first + blockIdx.x, bh = stretch / A.marks, mark = stretch % A.marks, b = bh / A.H, BHT = A.B * A.H * A.T;
   const int h = (int)(bh % A.H);
-  const int64_t first = mark * A.mark_tokens, behind = first + A.mark_tokens < A.T ? first + A.mark_tokens : A.T;
+  const int64_t begin = mark * A.mark_tokens, behind = begin + A.mark_tokens < A.T ? begin + A.mark_tokens : A.T;
   double carry = 0.0, total = 0.0;
   if (A.joins) {
     if (mark + 1 < A.marks || dlast)
@@ -198,14 +199,14 @@ __global__ __launch_bounds__(64) void gate_kernel(Sweep A, const float* __restri
     for (int64_t i = lane; i < elems; i += 64) carry += (double)last[bh * elems + i] * dlast[bh * elems + i];
     for (int m = 32; m >= 1; m >>= 1) carry += __shfl_xor(carry, m, 64);
   }
-  for (int64_t end = behind; end > first; end -= 64 * GATE_TOKENS) {
+  for (int64_t end = behind; end > begin; end -= 64 * GATE_TOKENS) {
     const int64_t hi = end - lane * GATE_TOKENS;  // this lane: tokens hi - 1 down to hi - 8
     double sum[GATE_TOKENS], run = 0.0;
     bool cut[GATE_TOKENS], cuts = false;
     float rs[GATE_TOKENS], cs[GATE_TOKENS];
 #pragma unroll
     for (int i = 0; i < GATE_TOKENS; ++i) {  // all loads at once, from the stretch's first token where there is none
-      const int64_t t = hi - 1 - i < first ? first : hi - 1 - i;
+      const int64_t t = hi - 1 - i < begin ? begin : hi - 1 - i;
       rs[i] = r[bh * A.T + t];
       cs[i] = c[bh * A.T + t];
       cut[i] = gamma_at(A, b * A.gb + h * A.gh + t * A.gt) < RESET;
@@ -214,10 +215,10 @@ __global__ __launch_bounds__(64) void gate_kernel(Sweep A, const float* __restri
     for (int i = 0; i < GATE_TOKENS; ++i) {
       const int64_t t = hi - 1 - i;
       double d = (double)rs[i] - cs[i];
-      if (tiles > 1 && t >= first)
+      if (tiles > 1 && t >= begin)
         for (int j = 1; j < tiles; ++j) d += (double)r[j * BHT + bh * A.T + t] - c[j * BHT + bh * A.T + t];
-      cut[i] = cut[i] && t >= first;
-      if (t >= first) run += d;
+      cut[i] = cut[i] && t >= begin;
+      if (t >= begin) run += d;
       if (cut[i]) run = 0.0, cuts = true;
       sum[i] = run;
     }
@@ -244,7 +245,7 @@ __global__ __launch_bounds__(64) void gate_kernel(Sweep A, const float* __restri
       const int64_t t = hi - 1 - i;
       open = open && !cut[i];
       const double d = cut[i] ? 0.0 : open ? sum[i] + before : sum[i];
-      if (t < first) continue;
+      if (t < begin) continue;
       total += d;
       if (per_head == nullptr) {
         const int64_t at = (b * A.T + t) * A.H + h;
@@ -255,7 +256,7 @@ __global__ __launch_bounds__(64) void gate_kernel(Sweep A, const float* __restri
   }
   if (per_head) {
     for (int m = 32; m >= 1; m >>= 1) total += __shfl_xor(total, m, 64);
-    if (lane == 0) per_head[blockIdx.x] = total;
+    if (lane == 0) per_head[stretch] = total;
   }
 }
 
@@ -539,15 +540,16 @@ extern "C" int ttc_linear_attention(const ttc_linear_attention_args* args, void*
   }
   if (W.gate) {  // of one decay for each head: zero where there are no tokens
     const int64_t stretches = A.batch * A.heads * W.marks;
-    if (stretches > max_blocks(64)) return TTC_LQR_EINVAL;
     S = sweep_of(A);
     S.mark_tokens = W.mark_tokens, S.marks = W.marks;
     S.joins = A.tokens > TOKEN_SWEEP ? space(W.joins) : nullptr;
     const int waves = sweep_waves(dk);  // of the sweep of dk
     double* per_head = A.gamma_per_head ? reinterpret_cast<double*>(space(W.per_head)) : nullptr;
-    if (stretches > 0)
-      hipLaunchKernelGGL(gate_kernel, dim3((unsigned)stretches), dim3(64), 0, s, S, space(W.r), space(W.c), W.dot_tiles,
-                         waves, space(W.last), some ? A.d_final_state : nullptr, (int64_t)dk * dv, A.d_log_gamma, per_head);
+    rc = in_launches(stretches, 64, [&](int64_t first, dim3 grid) {
+      hipLaunchKernelGGL(gate_kernel, grid, dim3(64), 0, s, S, space(W.r), space(W.c), W.dot_tiles, waves, space(W.last),
+                         some ? A.d_final_state : nullptr, (int64_t)dk * dv, A.d_log_gamma, per_head, first);
+    });
+    if (rc) return rc;
     if (per_head)
       hipLaunchKernelGGL(gate_head_kernel, dim3((unsigned)A.heads), dim3(64), 0, s, per_head, A.batch, (int)A.heads, W.marks,
                          S.gamma_bf16, A.d_log_gamma);

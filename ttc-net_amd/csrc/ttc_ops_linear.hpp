@@ -39,6 +39,7 @@ struct Sweep {
   bool gamma_bf16, reverse, out_f32;
   int kd, vd, H;
   int64_t B, T;
+  int64_t first;               // head, of all sequences' heads in a row, that this launch begins with
   float key_scale, out_scale;  // of the state's products; of the output
   const float* state_in;       // [slot, head, ...]: element (i, j) at i * sr + j * sc
   float* state_out;

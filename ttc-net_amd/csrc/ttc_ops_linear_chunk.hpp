@@ -276,7 +276,7 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
   int lane = tid & 63, g = lane >> 4, n = lane & 15;
   const int segs = MODE == STATE_ONLY ? G.count - 1 : G.count;  // the last one's own contribution is not needed
   const int seg = (int)(blockIdx.x % segs);
-  const int64_t bh = blockIdx.x / segs, b = bh / A.H, elems = (int64_t)A.kd * A.vd;
+  const int64_t bh = A.first + blockIdx.x / segs, b = bh / A.H, elems = (int64_t)A.kd * A.vd;
   const int h = (int)(bh % A.H);
   const T *q = MODE == STATE_ONLY ? nullptr : A.q.at<T>(b, h), *k = A.k.at<T>(b, h), *v = A.v.at<T>(b, h);
   const T* x = DOTS && A.x.p ? A.x.at<T>(b, h) : nullptr;
@@ -730,14 +730,15 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
 template <class T, int KD, int VD, int MODE>
 int launch_mode(const Sweep& A, const Segments& G, const Wides& W, hipStream_t s) {
   using Z = ChunkShape<T, KD, VD>;
-  const int64_t blocks = A.B * A.H * (MODE == STATE_ONLY ? G.count - 1 : G.count);
-  if (blocks > max_blocks(Z::NT)) return TTC_LQR_EINVAL;
-  const dim3 grid((unsigned)blocks), block(Z::NT);
-  if (W.in)
-    hipLaunchKernelGGL((chunk_sweep_kernel<T, KD, VD, MODE, true>), grid, block, 0, s, A, G, W);
-  else
-    hipLaunchKernelGGL((chunk_sweep_kernel<T, KD, VD, MODE, false>), grid, block, 0, s, A, G, W);
-  return launched();
+  const int segs = MODE == STATE_ONLY ? G.count - 1 : G.count;
+  return in_launches(A.B * A.H * segs, Z::NT, [&](int64_t first, dim3 grid) {
+    Sweep part = A;
+    part.first = first / segs;
+    if (W.in)
+      hipLaunchKernelGGL((chunk_sweep_kernel<T, KD, VD, MODE, true>), grid, dim3(Z::NT), 0, s, part, G, W);
+    else
+      hipLaunchKernelGGL((chunk_sweep_kernel<T, KD, VD, MODE, false>), grid, dim3(Z::NT), 0, s, part, G, W);
+  }, segs);
 }
 
 template <class T, int KD, int VD>
