@@ -317,3 +317,14 @@ def test_more_heads_than_one_launch_holds():
     whole = linear_attention(q, k, v, g)
     for at in range(0, B, 512):
         assert torch.equal(whole[at:at + 512], linear_attention(*(t[at:at + 512] for t in (q, k, v)), g))
+
+
+@pytest.mark.gpu
+def test_rows_of_2_31_elements():
+    """2^24 heads of 128, the most there are: all have the decay of the first one, and so its outputs."""
+    H = 2 ** 24
+    q, k, v = (make((1, 5, 1, d), torch.bfloat16, "cuda", 90 + i) for i, d in enumerate((8, 8, 128)))
+    o = linear_attention(q, k, v, torch.full((1,), -0.3, device="cuda").expand(H))
+    want = linear_attention(q, k, v, torch.full((1,), -0.3, device="cuda"))
+    for t in range(5):
+        assert bool((o[0, t] == want[0, t, 0]).all())

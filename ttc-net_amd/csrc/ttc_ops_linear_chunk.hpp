@@ -621,11 +621,11 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
       const int64_t first = ((b * A.T + low) * A.H + h) * A.vd;
       auto put = [&](auto* y, int r, int c, const f32x4& o) {
         using Y = std::remove_pointer_t<decltype(y)>;
-        const int row = A.H * A.vd;
         Y f[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) f[i] = from_f<Y>(o[i]);
         if (W.out) {
+          const int row = A.H * A.vd;  // below 2^22 here: the host sees to it
           const auto rows = bounded(y + first, ((left - 1) * row + A.vd) * (int)sizeof(Y));
           const int off = c < A.vd ? (r * row + c) * (int)sizeof(Y) : BEYOND;
           if constexpr (sizeof(Y) == 4)
@@ -635,7 +635,7 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
         } else if (r < left) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (c + i < A.vd) y[first + (int64_t)r * row + c + i] = f[i];
+            if (c + i < A.vd) y[first + (int64_t)r * A.H * A.vd + c + i] = f[i];
         }
       };
 #pragma unroll
