@@ -216,3 +216,51 @@ def test_c_entry_refuses():
     assert lib.ttc_group_norm(None, None) == 1
     for kw in (dict(n=0), dict(l=0), dict(c=0, groups=1)):
         assert lib.ttc_group_norm(pack(**kw), None) == 0
+
+
+def term_bounds(x, groups, w, b, eps, act, gate, dy):
+    """Bounds of dx, dweight, dbias and dgate from their terms' absolute values in 64 bits.  In units of EPS: a normalised
+    value is off by K (|xhat| + |x| rstd), what depends on it by that times the weight and slopes below 1.1 (K (1 + |y0|) in
+    all), a product by each factor's error times the other; a sum adds at most N of its terms one after the other in 32 bits
+    (4 positions and 256 rows of a workgroup, 64 values of a lane and 6 joins), the rest in 64."""
+    N = 300
+    n, c = x.shape[0], x.shape[-1]
+    d = lambda t: t.detach().double()  # noqa: E731
+    grouped = lambda t: t.reshape(n, -1, groups, c // groups)  # noqa: E731
+    mean_of = lambda t: grouped(t).mean((1, 3), keepdim=True)  # noqa: E731
+    back = lambda t: (t + torch.zeros_like(grouped(d(x)))).reshape(x.shape)  # noqa: E731
+    rstd = back((mean_of((d(x) - back(mean_of(d(x)))) ** 2) + eps).rsqrt())
+    xh = (d(x) - back(mean_of(d(x)))) * rstd
+    raw = xh.abs() + d(x).abs() * rstd
+    weight, bias = (1.0, 0.0) if w is None else (d(w).abs(), d(b).abs())
+    y0 = 1 + weight * raw + bias
+    on = 1.1 if gate is None else 1.1 + d(gate).abs()
+    d0 = d(dy).abs() * on
+    e0 = d0 * y0                        # what d0 is off by, in units of K EPS
+    dh, eh = d0 * weight, e0 * weight
+    s1 = back(mean_of((N + K) * dh + K * eh))
+    s2 = back(mean_of((N + K) * dh * xh.abs() + K * (dh * raw + eh * xh.abs())))
+    rows = lambda t: t.reshape(-1, c).sum(0)  # noqa: E731
+    return {"x": EPS * rstd * (K * (dh + eh) + s1 + xh.abs() * s2 + K * raw * back(mean_of(dh * xh.abs()))),
+            "w": EPS * rows((N + K) * d0 * xh.abs() + K * (d0 * raw + e0 * xh.abs())), "b": EPS * rows((N + K) * d0 + K * e0),
+            "gate": EPS * K * 1.1 * d(dy).abs() * y0}
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("act,gate", [("none", False), ("silu", False), ("silu", True)])
+@pytest.mark.parametrize("shape,groups", [((300, 96), 12), ((2, 5000, 32), 2), ((1, 9000, 6), 2), ((50000, 24), 3),
+                                          ((20000, 7), 1), ((3, 4100), 1), ((700, 3, 40), 5), ((9, 2048), 2)])
+def test_gradients_term_by_term(device, dtype, act, gate, shape, groups):
+    """Sums over many rows, several rows a thread and slabs, with bounds that a wrong or missing part of a sum passes."""
+    x, w, b, g = tensors(shape, dtype, device, gate, True)
+    dy = make(shape, dtype, device, 9)
+    xs = {n: t.requires_grad_() for n, t in (("x", x), ("w", w), ("b", b), ("gate", g)) if t is not None}
+    got = dict(zip(xs, torch.autograd.grad(group_norm(x, groups, w, b, eps=1e-3, activation=act, gate=g), list(xs.values()), dy)))
+    wide = {n: t.detach().double().requires_grad_() for n, t in xs.items()}
+    y = group_norm64(wide["x"], groups, wide["w"], wide["b"], 1e-3, act, wide.get("gate"))
+    want = dict(zip(wide, torch.autograd.grad(y, list(wide.values()), dy.double())))
+    bound = term_bounds(x, groups, w, b, 1e-3, act, g, dy)
+    for name in xs:
+        assert float(bound[name].max()) < 0.05 * float(want[name].abs().max()), name
+        within(got[name], want[name], bound[name] + HALF[dtype] * 1.01 * want[name].abs())
