@@ -11,13 +11,6 @@
 
 namespace ttc {
 
-// 16 bytes of T: what a lane loads or stores at once
-template <class T>
-struct alignas(16) Pack {
-  static constexpr int N = 16 / sizeof(T);
-  T v[N];
-};
-
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__bf16 x) { return (float)x; }
 template <class T>
