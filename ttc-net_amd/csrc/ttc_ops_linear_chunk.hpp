@@ -23,8 +23,8 @@
 // Numerics.  The sums G are held in 64 bits while they are formed and as pairs of fp32 after, so that differences of
 // large sums keep their digits; they start anew at a reset.  In bf16, w V is split into three bf16 parts (exact in fp32's 24
 // digits), so the state has fp32's accuracy; P, and in FAST the state's copy in front of a chunk, into two (16 digits), so that a
-// bf16 output is rounded to 8 digits once.  (Both in one part of 8 digits: the prompt above takes 143 us as a whole, so 155,
-// training on 4 x 2,048 tokens x 32 heads of 64 264, so 288, and the outputs' error is 2.35e-3 of their norm instead of 1.66e-3.)
+// bf16 output is rounded to 8 digits once.  (Both in one part of 8 digits: the prompt above takes 143 us as a whole, so 154,
+// training on 4 x 2,048 tokens x 32 heads of 64 264, so 277, and the outputs' error is 2.35e-3 of their norm instead of 1.66e-3.)
 // The decays' gradient is a long sum of cancelling terms, so the dots x . o it is made of are not taken from such an o (EXACT):
 // P's part is sum_s P_ts (v_s . x_t), whose products are exact as they are, in fp32; the state's copy is split into three
 // parts.  Weights that are 0 select: what is masked has no effect, whatever it holds.  Where a chunk's keys or values are not all
@@ -260,7 +260,11 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
   constexpr int C = Z::C, NT = Z::NT, VEC = Z::VEC, QS = Z::QS, XS = TIGHT ? VD : VD + Op::ROW_PAD, KS = TIGHT ? QS : Z::KS,
                 VS = TIGHT ? VD + Op::ROW_PAD : Z::VS, TAIL = PAIRED ? 16 / (int)sizeof(T) : 0;
   constexpr int PART = Z::TT * (Z::TT + 1) / 2 * 256;  // the scores' tiles (ti, si <= ti)
-  auto score_at = [](int ti, int si, int row, int col) { return ((ti * (ti + 1) / 2 + si) * 16 + row) * 16 + col; };
+  // The rows of 4 neighbours that are read or written at once lie in different banks (training on 4 x 2,048 tokens x 32 heads
+  // of 64: 277 us, in order 291); at 128 x 128 with x they are in order, for the registers (1,104 us, so 1,135: 24 spills, so 18)
+  auto score_at = [](int ti, int si, int row, int col) {
+    return ((ti * (ti + 1) / 2 + si) * 16 + row) * 16 + (col ^ (row & (TIGHT ? 0 : sizeof(T) == 2 ? 8 : 12)));
+  };
   auto x_at = [](int row, int c) { return row * XS + (TIGHT ? c ^ (row % 16 * VEC) : c); };
   __shared__ __attribute__((aligned(16))) T Qs[MODE == STATE_ONLY ? 1 : C * QS - TAIL];
   __shared__ __attribute__((aligned(16))) T Ks[C * KS - TAIL];
