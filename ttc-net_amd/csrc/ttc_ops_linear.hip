@@ -6,7 +6,7 @@ namespace ttc {
 
 // Token by token with the state in registers: a workgroup holds 32 columns of one head's state, a thread 4 of them for RPT
 // rows.  For one token it reads and writes the state once (8 bytes an element against 5 flops): bound by memory.  192
-// sequences x 16 states of 128 x 128 in a pool: 86 us for 406 MB, 4.7 TB/s where a copy of 1 GiB reaches 5.2; one sequence of
+// sequences x 16 states of 128 x 128 in a pool: 87 us for 406 MB, 4.7 TB/s where a copy of 1 GiB reaches 5.2; one sequence of
 // 8 states of 64 x 64: 4.6 us, of which the loads' latency is most.  Whole rows of 128 columns a workgroup take the same
 // (61.8 us against 61.1 for states in a row), and leave too few workgroups for few sequences (6.7 us against 4.7).
 template <class T, int RPT>
@@ -188,7 +188,8 @@ __global__ __launch_bounds__(64) void gate_kernel(Sweep A, const float* __restri
                                                   const float* __restrict__ dlast, int64_t elems, void* d_gamma,
                                                   double* __restrict__ per_head, int64_t first) {
   const int lane = threadIdx.x;
-  const int64_t stretch = first + blockIdx.x, bh = stretch / A.marks, mark = stretch % A.marks, b = bh / A.H, BHT = A.B * A.H * A.T;
+  const int64_t stretch = first + blockIdx.x, bh = stretch / A.marks, mark = stretch % A.marks, b = bh / A.H;
+  const int64_t BHT = A.B * A.H * A.T;
   const int h = (int)(bh % A.H);
   const int64_t begin = mark * A.mark_tokens, behind = begin + A.mark_tokens < A.T ? begin + A.mark_tokens : A.T;
   double carry = 0.0, total = 0.0;
@@ -273,21 +274,27 @@ __global__ __launch_bounds__(64) void gate_head_kernel(const double* __restrict_
 
 // ---- host ----------------------------------------------------------------------------------------------------
 
-// Up to this many tokens are swept one by one; more in chunks.  8 heads of 128: 2, 4, 8 and 16 tokens take 5.8, 7.7, 12.0 and
-// 20.5 us one by one, 12.2 us in a chunk; 1,024 heads 26.5, 33.5, 48.0 and 78.9 us against 36
+// Up to this many tokens are swept one by one; more in chunks.  8 heads of 128: 2, 4, 8 and 16 tokens take 5.8, 7.8, 12.0 and
+// 20.6 us one by one, 13.1 us in a chunk; 1,024 heads 25.4, 35.6, 53.5 and 89.9 us against 39
 constexpr int64_t TOKEN_SWEEP = 4;
 
-// Segments of a chunked sweep: enough workgroups to fill the GPU's 256 CUs as often as registers let them run beside each
-// other, twice, three times up to 64 x 64, four where keys or values have up to 32; a segment's keys and values are read once
-// more for the state behind it, so heads that fill the GPU by themselves are not split.  Workgroups aimed at, training in bf16:
+// Segments of a chunked sweep: enough workgroups to fill the GPU's 256 CUs twice, three times up to 64 x 64, four where keys or
+// values have up to 32; a segment's keys and values are read once more for the state behind it, so heads that fill the GPU by
+// themselves are not split.  Registers let two workgroups of 128 x 128 run beside each other and three of 64 x 64; with 32 on
+// one side it is shared memory (128 x 32: two or three of two waves), and the rule is what the table shows.  Head counts that
+// do not divide the number leave some of it empty (400 heads of 64 x 64: one segment each).  Workgroups aimed at, us, bf16:
 //                                            384      512     768   1,024   1,536
-//   8 x 2,048 tokens x 32 heads of 128 x 128 1,245  1,060   1,222   1,123           (16,381 x 16 forward 165 146 184 176)
-//   the same, 64 x 128                         818    678     779     706
-//   4 x 2,048 tokens x 32 heads of 64 x 64     337    278     265     282
-//   3 x 4,096 tokens x 32 heads of 64 x 64            404     338     406     376
-//   4 x 4,096 tokens x 32 heads of 64 x 32            450     364     357     394
-//   8 x 4,096 tokens x 32 heads of 32 x 32            791     573     513     598
-//   4 x 4,096 tokens x 32 heads of 32 x 128           617     727     619     667   (128 x 32 625 626 605 613)
+//   8 x 2,048 tokens x 32 heads of 128 x 128 1,373  1,097   1,290   1,138   1,279   (16,381 x 16 forward 177 150 187 171 193)
+//   the same, 64 x 128 (128 x 64)              866    714     819     740     834   (887 722 846 723 832)
+//   4 x 2,048 tokens x 32 heads of 64 x 64     353    285     276     286     289
+//   3 x 4,096 tokens x 32 heads of 64 x 64     498    422     351     427     380
+//   8 x 2,048 tokens x 50 heads of 64 x 64     771    770     768     863     710
+//   4 x 4,096 tokens x 32 heads of 64 x 32     625    481     390     385     424
+//   8 x 4,096 tokens x 32 heads of 32 x 32   1,303    842     615     540     639
+//   4 x 4,096 tokens x 32 heads of 32 x 128    784    640     763     645     694   (128 x 32 845 664 797 661 721)
+// and in fp32 (8 x 2,048 x 32 of 128 x 128 2,070 2,085 2,231 2,199 2,286)
+//   4 x 2,048 tokens x 32 heads of 64 x 64     612    489     456     477     486   (3 x 4,096 x 32 904 753 644 774 679)
+//   8 x 4,096 tokens x 32 heads of 32 x 32   1,710  1,327     952     787     733   (32 x 128 1,526 1,214 1,146 1,145 1,077)
 inline Segments segments_of(const ttc_linear_attention_args& A) {
   Segments G{};
   const int64_t chunks = ceil_div(A.tokens, chunk_tokens(A.dtype == TTC_DTYPE_BF16)), heads = A.batch * A.heads;

@@ -86,7 +86,7 @@ template <class T>
 int launch_chunk_kd128(const Sweep& A, const Segments& G, const Wides& W, int mode, hipStream_t s);
 
 // Tokens of a chunk: in bf16 64, so that the state's own work is spread over more of them (2,048 tokens of 512 heads of
-// 128: 313 us, with 32 tokens 332); in fp32, whose tiles are twice as large, 32
+// 128: 372 us, with 32 tokens 397); in fp32, whose tiles are twice as large, 32
 constexpr int chunk_tokens(bool bf16) { return bf16 ? 64 : 32; }
 
 }  // namespace ttc

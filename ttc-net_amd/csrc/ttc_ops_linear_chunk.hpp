@@ -11,24 +11,29 @@
 //        the operand (rows 4 g + i and 16 + 4 g + i of 32 are the 8 a lane gives, on the other side too)
 //   S += K' (w V)   K' and V' by transposing reads of shared memory (bf16) or element by element (fp32).
 //
-// Bound.  At 64 x 64 with three workgroups a CU a chunk's 32 KB take 4,000 cycles, the rate of a copy; the matrix cores need
-// 700 of them, the vector ALU (weights, splits, conversions) about 2,000, shared memory 1,400.  At 128 x 128 registers leave
-// two workgroups a CU (a wave holds 32 columns of the state, 64 registers), whose phases between barriers do not cover each
-// other: 11,700 cycles for 64 KB.  16 columns a wave need twice the operand reads (2,048 tokens x 512 heads: 360 us, with
-// 32 columns 313).  Measured: 16,381 tokens x 16 heads of 128, bf16: 91 us (269 MB), after 52 us for the states between its
-// 32 segments (134 MB) and 15 us to join them; 2,048 x 128 heads of 64 (134 MB): FAST 44 us, EXACT 58 with its fourth input,
-// the segments' states 25.  fp32 is bound by its matrix instructions: 2,048 tokens x 512 heads of 128 in 827 us, 101 TFLOP/s
-// (a large library product: 153).
+// Bound.  No unit is full: the phases between two barriers do not cover each other.  Of a sweep's cycles
+//                                                    vector ALU  matrix cores  shared memory (its bank conflicts)  us
+//   64 x 64, 2,048 x 128 heads in 768 parts, FAST        45 %         12 %          29 % (9)    59 MB read, 34 written  50
+//   the same, EXACT (a fourth input)                     39           12            29 (9)      76, 36                  62
+//   the same, STATE_ONLY                                 34            8            10 (0)      35, 11                  25
+//   128 x 128, 16,381 x 16 heads in 512 parts, FAST      43           22            23 (7)      118, 68                102
+//   the same, STATE_ONLY                                 42           20            10 (0)      69, 33                  52
+// (read and written: as counted behind the XCDs' caches, less than the inputs where the last level holds some).  At 64 x 64
+// three workgroups share a CU; at 128 x 128 registers leave two (a wave holds 32 columns of the state, 64 registers), and
+// EXACT spills 18 of them.  16 columns a wave need twice the operand reads (2,048 tokens x 512 heads, with scores of 8
+// digits: 360 us, with 32 columns 313).  2,048 tokens x 512 heads of 128 that fill the GPU unsplit: 372 us.  fp32 is bound by
+// its matrix instructions: the same in 806 us, 104 TFLOP/s (a large library product: 153).
 //
 // Numerics.  The sums G are held in 64 bits while they are formed and as pairs of fp32 after, so that differences of
 // large sums keep their digits; they start anew at a reset.  In bf16, w V is split into three bf16 parts (exact in fp32's 24
-// digits), so the state has fp32's accuracy; P, and in FAST the state's copy in front of a chunk, into two (16 digits), so that a
-// bf16 output is rounded to 8 digits once.  (Both in one part of 8 digits: the prompt above takes 143 us as a whole, so 154,
-// training on 4 x 2,048 tokens x 32 heads of 64 264, so 277, and the outputs' error is 2.35e-3 of their norm instead of 1.66e-3.)
-// The decays' gradient is a long sum of cancelling terms, so the dots x . o it is made of are not taken from such an o (EXACT):
-// P's part is sum_s P_ts (v_s . x_t), whose products are exact as they are, in fp32; the state's copy is split into three
-// parts.  Weights that are 0 select: what is masked has no effect, whatever it holds.  Where a chunk's keys or values are not all
-// finite, its sums over tokens are formed term by term instead, without the masked ones.
+// digits), so the state has fp32's accuracy; P, and in FAST the state's copy in front of a chunk, into two (16 digits), so that
+// a bf16 output is rounded to 8 digits once.  (Both in one part of 8 digits: the call on 16,381 x 16 heads of 128 takes 143 us,
+// so 154, 2,048 tokens x 512 heads of 128 313, so 372, training on 4 x 2,048 tokens x 32 heads of 64 264, so 277, and the
+// outputs' error is 2.35e-3 of their norm instead of 1.66e-3.)  The decays' gradient is a long sum of cancelling terms, so the
+// dots x . o it is made of are not taken from such an o (EXACT): P's part is sum_s P_ts (v_s . x_t), whose products are exact
+// as they are, in fp32; the state's copy is split into three parts.  Weights that are 0 select: what is masked has no effect,
+// whatever it holds.  Where a chunk's keys or values are not all finite, its sums over tokens are formed term by term instead,
+// without the masked ones.
 #pragma once
 #include "ttc_ops_linear.hpp"
 
@@ -260,8 +265,9 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
   constexpr int C = Z::C, NT = Z::NT, VEC = Z::VEC, QS = Z::QS, XS = TIGHT ? VD : VD + Op::ROW_PAD, KS = TIGHT ? QS : Z::KS,
                 VS = TIGHT ? VD + Op::ROW_PAD : Z::VS, TAIL = PAIRED ? 16 / (int)sizeof(T) : 0;
   constexpr int PART = Z::TT * (Z::TT + 1) / 2 * 256;  // the scores' tiles (ti, si <= ti)
-  // The rows of 4 neighbours that are read or written at once lie in different banks (training on 4 x 2,048 tokens x 32 heads
-  // of 64: 277 us, in order 291); at 128 x 128 with x they are in order, for the registers (1,104 us, so 1,135: 24 spills, so 18)
+  // The rows of 4 neighbours that are read or written at once lie in different banks (training on 4 x 2,048 tokens x 32
+  // heads of 64: 277 us, in order 291); at 128 x 128 with x they are in order, which needs fewer registers (8 x 2,048 x 32
+  // heads: 1,098 us and 18 spills, otherwise 1,135 and 24)
   auto score_at = [](int ti, int si, int row, int col) {
     return ((ti * (ti + 1) / 2 + si) * 16 + row) * 16 + (col ^ (row & (TIGHT ? 0 : sizeof(T) == 2 ? 8 : 12)));
   };
@@ -459,7 +465,8 @@ __global__ __launch_bounds__((ChunkShape<T, KD, VD>::NT), 2) void chunk_sweep_ke
     };
     auto rows_of = [](auto stride) { return [](int row, int c) { return row * decltype(stride)::value + c; }; };
     stage(Ks, rows_of(std::integral_constant<int, KS>{}), kr, std::integral_constant<int, KD>{}, true);
-    if constexpr (MODE != STATE_ONLY) stage(Qs, rows_of(std::integral_constant<int, QS>{}), qr, std::integral_constant<int, KD>{}, false);
+    if constexpr (MODE != STATE_ONLY)
+      stage(Qs, rows_of(std::integral_constant<int, QS>{}), qr, std::integral_constant<int, KD>{}, false);
     stage(Vs, rows_of(std::integral_constant<int, VS>{}), vr, std::integral_constant<int, VD>{}, true);
     if constexpr (PAIRED) stage(Xs, x_at, xr, std::integral_constant<int, VD>{}, false);
     const bool odd_here = __ballot(!Op::finite(most)) != 0;
