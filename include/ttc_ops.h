@@ -1,6 +1,6 @@
 /* ttc_ops.h -- C ABI of libttc_lqr.so's sequence operators, for models that hold the test-time control
- * layer: rotary positions, group norm with an activation or a gate, linear attention with a decay for
- * each head (status codes: ttc_lqr.h).
+ * layer: rotary positions, group norm with an activation or a gate, causal convolution, linear attention with a
+ * decay for each head, the gated delta rule (status codes: ttc_lqr.h).
  *
  * Each call takes one argument block on the host (every field 8 bytes: numbers, device pointers, strides in
  * elements).  The calls read it before they return, allocate nothing, enqueue their work on `stream` (a
@@ -40,6 +40,67 @@ typedef struct {
 } ttc_rotary_args;
 
 int ttc_rotary(const ttc_rotary_args* args, void* stream);
+
+/* Positions with several axes (time, height and width of a picture's or video's token): pair i takes its position from the
+ * axis in whose section it lies, the first section[0] pairs from axis 0 and so on, and (c, s) from the table's entry of that
+ * position and pair i; a position outside the table gives NaN in its axis's pairs.  rot / 2 is the sections' sum (at most
+ * dim / 2), the table [length, rot / 2, 2]; axes: 1 to TTC_ROTARY_MAX_AXES; everything else as above. */
+#define TTC_ROTARY_MAX_AXES 4
+typedef struct {
+  int64_t dtype, batch, tokens, dim, interleaved, backward, axes;
+  int64_t section[TTC_ROTARY_MAX_AXES];
+  int64_t heads[2];
+  const void* x[2];
+  int64_t stride[2][3]; /* batch, token, head */
+  void* y[2];
+  const float* table;
+  int64_t length;
+  const void* positions;
+  int64_t position_bytes, position_stride[3]; /* batch, token, axis */
+} ttc_rotary_axes_args;
+
+int ttc_rotary_axes(const ttc_rotary_axes_args* args, void* stream);
+
+/* ---- Causal convolution of each channel, channels last ----
+ * y_t = act(bias + sum_j weight[c, j] w_{t + j}) with w the initial state's taps - 1 rows (NULL: zeros) followed by x, so that
+ * tap taps - 1 meets x_t itself.  activation 0: none, 1: silu.  x [batch, tokens, channels] with unit stride along the
+ * channels; weight [channels, taps] and bias [channels] (NULL: none) of type weight_dtype (fp32, or dtype); taps: 1 to
+ * TTC_CAUSAL_CONV_MAX_TAPS.  y contiguous; final_state (NULL: not wanted): the last taps - 1 rows of w, contiguous
+ * [batch, taps - 1, channels] as initial_state, both of x's type.
+ * The backward takes d_y (unit stride along the channels) and d_final_state (NULL: zero) and writes dx, d_initial_state
+ * (contiguous, x's type), dweight and dbias (weight_dtype); NULL: not wanted.
+ * workspace: ttc_causal_conv_workspace_bytes() of the same block (0: none needed). */
+#define TTC_CAUSAL_CONV_MAX_TAPS 8
+typedef struct {
+  int64_t dtype, weight_dtype, batch, tokens, channels, taps, activation, backward;
+  const void* x;
+  int64_t x_stride[2]; /* batch, token */
+  const void *weight, *bias, *initial_state;
+  void *y, *final_state;
+  const void* d_y;
+  int64_t d_y_stride[2];
+  const void* d_final_state;
+  void *dx, *dweight, *dbias, *d_initial_state;
+  void* workspace;
+  int64_t workspace_bytes;
+} ttc_causal_conv_args;
+
+size_t ttc_causal_conv_workspace_bytes(const ttc_causal_conv_args* args);
+int ttc_causal_conv(const ttc_causal_conv_args* args, void* stream);
+
+/* One token of each sequence, its state updated in place: x [batch, channels] with unit stride along the channels, y
+ * contiguous.  state [slots, taps - 1, channels] of x's type, contiguous; slot_index as in ttc_linear_attention_step. */
+typedef struct {
+  int64_t dtype, weight_dtype, batch, channels, taps, activation, slots;
+  const void* x;
+  int64_t x_stride;
+  const void *weight, *bias;
+  void* state;
+  const int32_t* slot_index;
+  void* y;
+} ttc_causal_conv_step_args;
+
+int ttc_causal_conv_step(const ttc_causal_conv_step_args* args, void* stream);
 
 /* ---- Group norm with an activation or a gate, channels last ----
  * x [n, l, c] contiguous; statistics over the l positions and the c / groups channels of a group, biased

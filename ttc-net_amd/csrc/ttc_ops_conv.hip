@@ -1,0 +1,448 @@
+// ttc_ops_conv.hip -- causal convolution of each channel over a few tokens, forward, backward and single tokens.
+//
+//   w = [state; x] (taps - 1 rows more than x),  p_t = bias + sum_j c_j w_{t + j},  y_t = act(p_t)
+// and with e_t = dy_t act'(p_t), zero outside [0, T),
+//   dw_i = sum_j c_j e_{i - j} (+ the final state's gradient),  dc_j = sum_t e_t w_{t + j},  dbias = sum_t e_t.
+// A thread holds 16 bytes of neighbouring channels and walks along a run of tokens with the last `taps` rows in registers,
+// so that a row is read from memory once (and once more from the caches at the start of each run).
+#include "ttc_ops_common.hpp"
+
+namespace ttc {
+
+constexpr int MAX_TAPS = TTC_CAUSAL_CONV_MAX_TAPS;
+
+struct Conv {
+  const void *x, *weight, *bias, *state;
+  int64_t xb, xt, B, T, C;
+  bool weight_bf16;
+  void *y, *final_state;
+  const void *dy, *dfinal;
+  int64_t yb, yt;
+  void *dx, *dstate;
+  float* part;  // [row of workgroups, taps + 1, C]: sums of the weights' and the bias's gradients
+  int64_t run, runs;  // tokens a thread, such runs a sequence
+  int64_t cols;       // vectors of a row
+};
+
+template <class T, int V>
+struct alignas(V * sizeof(T)) Vec {
+  T v[V];
+};
+
+template <class T, int V>
+__device__ __forceinline__ void get(const T* p, float (&f)[V]) {
+  const Vec<T, V> a = *reinterpret_cast<const Vec<T, V>*>(p);
+#pragma unroll
+  for (int i = 0; i < V; ++i) f[i] = to_f(a.v[i]);
+}
+
+template <class T, int V>
+__device__ __forceinline__ void put(T* p, const float (&f)[V]) {
+  Vec<T, V> a;
+#pragma unroll
+  for (int i = 0; i < V; ++i) a.v[i] = from_f<T>(f[i]);
+  *reinterpret_cast<Vec<T, V>*>(p) = a;
+}
+
+__device__ __forceinline__ float param(const void* p, bool bf16, int64_t i) {
+  return bf16 ? to_f(static_cast<const __bf16*>(p)[i]) : static_cast<const float*>(p)[i];
+}
+
+template <int K, int V>
+__device__ __forceinline__ void weights(const void* weight, const void* bias, bool bf16, int64_t c, float (&w)[K][V],
+                                        float (&b)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+#pragma unroll
+    for (int j = 0; j < K; ++j) w[j][i] = param(weight, bf16, (c + i) * K + j);
+    b[i] = bias ? param(bias, bf16, c + i) : 0.0f;
+  }
+}
+
+// row i of w = [state; x], for 0 <= i < T + K - 1
+template <class T, int K, int V>
+__device__ __forceinline__ void wide_row(const Conv& A, int64_t b, int64_t i, int64_t c, float (&f)[V]) {
+  if (i >= K - 1) {
+    get<T, V>(static_cast<const T*>(A.x) + b * A.xb + (i - (K - 1)) * A.xt + c, f);
+  } else if (A.state) {
+    get<T, V>(static_cast<const T*>(A.state) + (b * (K - 1) + i) * A.C + c, f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = 0.0f;
+  }
+}
+
+template <int K, int V>
+__device__ __forceinline__ void taps_of(const float (&w)[K][V], const float (&b)[V], const float (&row)[K][V], float (&p)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    p[i] = b[i];
+#pragma unroll
+    for (int j = 0; j < K; ++j) p[i] = fmaf(w[j][i], row[j][i], p[i]);
+  }
+}
+
+constexpr int FORWARD_RUN = 8;  // tokens a thread
+
+// All rows of a run are asked for at once.
+template <class T, int K, int V, bool SILU>
+__global__ __launch_bounds__(256) void conv_kernel(Conv A, int64_t first, int64_t items) {
+  const int64_t item = (first + blockIdx.x) * 256 + threadIdx.x;
+  if (item >= items) return;
+  const int64_t c = item % A.cols * V, rest = item / A.cols, run = rest % A.runs, b = rest / A.runs;
+  const int64_t t0 = run * FORWARD_RUN, last = A.T + K - 2;  // of w's rows
+  float w[K][V], bias[V], rows[FORWARD_RUN + K - 1][V];
+#pragma unroll
+  for (int i = 0; i < FORWARD_RUN + K - 1; ++i) wide_row<T, K, V>(A, b, t0 + i < last ? t0 + i : last, c, rows[i]);
+  weights<K, V>(A.weight, A.bias, A.weight_bf16, c, w, bias);
+#pragma unroll
+  for (int i = 0; i < FORWARD_RUN; ++i) {
+    if (t0 + i >= A.T) break;
+    float now[K][V], p[V];
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+#pragma unroll
+      for (int k = 0; k < V; ++k) now[j][k] = rows[i + j][k];
+    taps_of<K, V>(w, bias, now, p);
+    if (SILU) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) p[k] *= sigmoid(p[k]);
+    }
+    put<T, V>(static_cast<T*>(A.y) + (b * A.T + t0 + i) * A.C + c, p);
+  }
+  if (K > 1 && A.final_state && run == A.runs - 1) {
+#pragma unroll
+    for (int i = 0; i < K - 1; ++i) {
+      float f[V];
+      wide_row<T, K, V>(A, b, A.T + i, c, f);
+      put<T, V>(static_cast<T*>(A.final_state) + (b * (K - 1) + i) * A.C + c, f);
+    }
+  }
+}
+
+// Four runs a workgroup, 64 vectors of channels each: the weights' sums are joined in shared memory.  A run covers `run` of
+// the T + K - 1 rows of w and the tokens of the same numbers; the K - 1 tokens in front of it, whose e its rows' gradients
+// need, are computed again.
+template <class T, int K, int V, bool SILU>
+__global__ __launch_bounds__(256) void conv_backward_kernel(Conv A, int64_t first) {
+  __shared__ float sums[3][64][V + 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t tiles = (A.cols + 63) / 64, block = first + blockIdx.x, tile = block % tiles, rest = block / tiles;
+  const int64_t quads = (A.runs + 3) / 4, b = rest / quads, run = rest % quads * 4 + wave;
+  const int64_t col = tile * 64 + lane, c = col * V, N = A.T + K - 1;
+  const bool here = col < A.cols && run < A.runs;
+  float dw[K + 1][V];
+#pragma unroll
+  for (int j = 0; j <= K; ++j)
+#pragma unroll
+    for (int i = 0; i < V; ++i) dw[j][i] = 0.0f;
+  if (here) {
+    float w[K][V], bias[V], rows[K][V], e[K][V];  // rows t .. t + K - 1 of w; e of tokens t - K + 1 .. t
+    weights<K, V>(A.weight, A.bias, A.weight_bf16, c, w, bias);
+    const int64_t t0 = run * A.run, t1 = t0 + A.run < N ? t0 + A.run : N, lead = t0 - (K - 1) > 0 ? t0 - (K - 1) : 0;
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) e[j][i] = rows[j][i] = 0.0f;
+#pragma unroll
+    for (int j = 1; j < K; ++j)
+      if (lead + j - 1 < N) wide_row<T, K, V>(A, b, lead + j - 1, c, rows[j]);
+    const T* dy = static_cast<const T*>(A.dy) + b * A.yb + c;
+    for (int64_t t = lead; t < t1; ++t) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+#pragma unroll
+        for (int j = 0; j + 1 < K; ++j) rows[j][i] = rows[j + 1][i], e[j][i] = e[j + 1][i];
+        e[K - 1][i] = 0.0f;
+      }
+      if (t < A.T) {
+        float p[V], d[V];
+        wide_row<T, K, V>(A, b, t + K - 1, c, rows[K - 1]);
+        get<T, V>(dy + t * A.yt, d);
+        if (SILU) {
+          taps_of<K, V>(w, bias, rows, p);
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float s = sigmoid(p[i]);
+            d[i] *= s * fmaf(p[i], 1.0f - s, 1.0f);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          e[K - 1][i] = d[i];
+          if (t >= t0) {
+#pragma unroll
+            for (int j = 0; j < K; ++j) dw[j][i] = fmaf(d[i], rows[j][i], dw[j][i]);
+            dw[K][i] += d[i];
+          }
+        }
+      }
+      if (t < t0) continue;
+      float g[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        g[i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < K; ++j)  // of tokens that exist: a tap may be infinite
+          g[i] = t - j >= 0 && t - j < A.T ? fmaf(w[j][i], e[K - 1 - j][i], g[i]) : g[i];
+      }
+      if (t >= A.T && A.dfinal) {
+        float f[V];
+        get<T, V>(static_cast<const T*>(A.dfinal) + (b * (K - 1) + t - A.T) * A.C + c, f);
+#pragma unroll
+        for (int i = 0; i < V; ++i) g[i] += f[i];
+      }
+      if (t >= K - 1) {
+        if (A.dx) put<T, V>(static_cast<T*>(A.dx) + (b * A.T + t - (K - 1)) * A.C + c, g);
+      } else if (A.dstate) {
+        put<T, V>(static_cast<T*>(A.dstate) + (b * (K - 1) + t) * A.C + c, g);
+      }
+    }
+  }
+  if (A.part == nullptr) return;
+#pragma unroll
+  for (int j = 0; j <= K; ++j) {
+    if (wave > 0) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) sums[wave - 1][lane][i] = dw[j][i];
+    }
+    __syncthreads();
+    if (wave == 0 && col < A.cols) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float a = dw[j][i];
+#pragma unroll
+        for (int m = 0; m < 3; ++m) a += sums[m][lane][i];
+        A.part[(rest * (K + 1) + j) * A.C + c + i] = a;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// The workgroups' sums: a workgroup takes 64 neighbouring entries of [taps + 1, C], its waves every fourth row of parts
+__global__ __launch_bounds__(256) void conv_join_kernel(const float* __restrict__ part, int64_t parts, int64_t C, int K,
+                                                        bool bf16, void* dweight, void* dbias) {
+  __shared__ float sums[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t n = C * (K + 1), i = (int64_t)blockIdx.x * 64 + lane;
+  float a = 0.0f;
+  if (i < n)
+    for (int64_t p = wave; p < parts; p += 4) a += part[p * n + i];
+  sums[wave][lane] = a;
+  __syncthreads();
+  if (wave > 0 || i >= n) return;
+  a = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+  const int64_t j = i / C, c = i % C;
+  void* to = j == K ? dbias : dweight;
+  const int64_t at = j == K ? c : c * K + j;
+  if (to == nullptr) return;
+  if (bf16) static_cast<__bf16*>(to)[at] = from_f<__bf16>(a);
+  else static_cast<float*>(to)[at] = a;
+}
+
+// One token: a thread's channels of a row's state, moved on by one.  A state's rows are read before any is written.
+template <class T, int K, int V, bool SILU>
+__global__ __launch_bounds__(256) void conv_step_kernel(Conv A, const int32_t* __restrict__ slots, int64_t nslots,
+                                                        int64_t first, int64_t items) {
+  const int64_t item = (first + blockIdx.x) * 256 + threadIdx.x;
+  if (item >= items) return;
+  const int64_t c = item % A.cols * V, b = item / A.cols, slot = slots ? slots[b] : b;
+  T* y = static_cast<T*>(A.y) + b * A.C + c;
+  float w[K][V], bias[V], rows[K][V], p[V];
+  if (slot < 0 || slot >= nslots) {  // a row without a state
+#pragma unroll
+    for (int i = 0; i < V; ++i) p[i] = 0.0f;
+    put<T, V>(y, p);
+    return;
+  }
+  T* state = static_cast<T*>(A.final_state) + slot * (K - 1) * A.C + c;
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j) get<T, V>(state + j * A.C, rows[j]);
+  get<T, V>(static_cast<const T*>(A.x) + b * A.xb + c, rows[K - 1]);
+  weights<K, V>(A.weight, A.bias, A.weight_bf16, c, w, bias);
+  taps_of<K, V>(w, bias, rows, p);
+  if (SILU) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) p[i] *= sigmoid(p[i]);
+  }
+  put<T, V>(y, p);
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j) put<T, V>(state + j * A.C, rows[j + 1]);
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------
+
+// f(tap count as a constant)
+template <class F>
+int with_taps(int64_t taps, F f) {
+  switch (taps) {
+    case 1: return f(std::integral_constant<int, 1>{});
+    case 2: return f(std::integral_constant<int, 2>{});
+    case 3: return f(std::integral_constant<int, 3>{});
+    case 4: return f(std::integral_constant<int, 4>{});
+    case 5: return f(std::integral_constant<int, 5>{});
+    case 6: return f(std::integral_constant<int, 6>{});
+    case 7: return f(std::integral_constant<int, 7>{});
+    default: return f(std::integral_constant<int, 8>{});
+  }
+}
+
+inline int conv_check(int64_t dtype, int64_t weight_dtype, std::initializer_list<int64_t> sizes, int64_t taps,
+                      int64_t activation) {
+  for (int64_t v : sizes)
+    if (v < 0) return TTC_LQR_EINVAL;
+  if (taps < 1 || taps > MAX_TAPS || activation < 0 || activation > 1 || !countable(sizes)) return TTC_LQR_EINVAL;
+  if (dtype != TTC_DTYPE_F32 && dtype != TTC_DTYPE_BF16) return TTC_LQR_EUNSUPPORTED;
+  if (weight_dtype != TTC_DTYPE_F32 && weight_dtype != dtype) return TTC_LQR_EUNSUPPORTED;
+  return TTC_LQR_OK;
+}
+
+constexpr int64_t MAX_CHANNELS = 1 << 26;  // the sums' join is one launch
+
+inline int conv_check(const ttc_causal_conv_args& A) {
+  if (A.tokens < 0 || A.tokens > ((int64_t)1 << 58) || A.channels > MAX_CHANNELS) return TTC_LQR_EINVAL;
+  return conv_check(A.dtype, A.weight_dtype, {A.batch, A.tokens + MAX_TAPS, A.channels, MAX_TAPS + 1}, A.taps, A.activation);
+}
+
+// Rows of w a thread walks along backwards: the K - 1 tokens in front of a run are computed again, so runs of up to 64; as
+// many runs as give each of 256 CUs four workgroups where there are fewer tokens
+inline int64_t backward_run(const ttc_causal_conv_args& A, int64_t cols) {
+  const int64_t tiles = ceil_div(cols, 64) * (A.batch > 0 ? A.batch : 1), N = A.tokens + A.taps - 1;
+  const int64_t run = N * tiles / (4 * 1024);
+  return run < 8 ? 8 : run > 64 ? 64 : run;
+}
+
+template <class T>
+int64_t conv_vector(const ttc_causal_conv_args& A) {
+  constexpr int V = 16 / sizeof(T);
+  bool wide = A.channels % V == 0 && A.x_stride[0] % V == 0 && A.x_stride[1] % V == 0 && aligned16(A.x) && aligned16(A.y) &&
+              aligned16(A.initial_state) && aligned16(A.final_state);
+  if (A.backward)
+    wide = wide && A.d_y_stride[0] % V == 0 && A.d_y_stride[1] % V == 0 && aligned16(A.d_y) && aligned16(A.dx) &&
+           aligned16(A.d_final_state) && aligned16(A.d_initial_state);
+  return wide ? V : 1;
+}
+
+// Sums of the weights' gradients: one row of them for each four runs of a sequence.  Of the block alone, whatever its
+// pointers: those of 16-byte vectors are fewer.
+inline int64_t conv_parts(const ttc_causal_conv_args& A, int64_t cols) {
+  return A.batch * ceil_div(ceil_div(A.tokens + A.taps - 1, backward_run(A, cols)), 4);
+}
+
+inline int64_t conv_bytes(const ttc_causal_conv_args& A) {
+  if (!A.backward || (!A.dweight && !A.dbias)) return 0;
+  const int64_t V = A.dtype == TTC_DTYPE_BF16 ? 8 : 4;
+  const int64_t a = conv_parts(A, ceil_div(A.channels, V)), b = conv_parts(A, A.channels);
+  return (a > b ? a : b) * (A.taps + 1) * A.channels * 4;
+}
+
+template <class T, int V>
+int conv_run(const ttc_causal_conv_args& A, hipStream_t s) {
+  Conv P{};
+  P.x = A.x, P.weight = A.weight, P.bias = A.bias, P.state = A.initial_state;
+  P.xb = A.x_stride[0], P.xt = A.x_stride[1];
+  P.B = A.batch, P.T = A.tokens, P.C = A.channels;
+  P.weight_bf16 = A.weight_dtype == TTC_DTYPE_BF16;
+  P.cols = A.channels / V;
+  if (!A.backward) {
+    P.y = A.y, P.final_state = A.final_state;
+    P.runs = A.tokens > 0 ? ceil_div(A.tokens, FORWARD_RUN) : 1;
+    const int64_t items = A.batch * P.runs * P.cols;
+    return with_taps(A.taps, [&](auto taps) {
+      constexpr int K = decltype(taps)::value;
+      return in_launches(ceil_div(items, 256), 256, [&](int64_t first, dim3 grid) {
+        if (A.activation) hipLaunchKernelGGL((conv_kernel<T, K, V, true>), grid, dim3(256), 0, s, P, first, items);
+        else hipLaunchKernelGGL((conv_kernel<T, K, V, false>), grid, dim3(256), 0, s, P, first, items);
+      });
+    });
+  }
+  P.dy = A.d_y, P.dfinal = A.d_final_state;
+  P.yb = A.d_y_stride[0], P.yt = A.d_y_stride[1];
+  P.dx = A.dx, P.dstate = A.d_initial_state;
+  P.part = A.dweight || A.dbias ? static_cast<float*>(A.workspace) : nullptr;
+  P.run = backward_run(A, P.cols);
+  P.runs = ceil_div(A.tokens + A.taps - 1, P.run);
+  const int64_t parts = conv_parts(A, P.cols);
+  const int rc = with_taps(A.taps, [&](auto taps) {
+    constexpr int K = decltype(taps)::value;
+    return in_launches(parts * ceil_div(P.cols, 64), 256, [&](int64_t first, dim3 grid) {
+      if (A.activation) hipLaunchKernelGGL((conv_backward_kernel<T, K, V, true>), grid, dim3(256), 0, s, P, first);
+      else hipLaunchKernelGGL((conv_backward_kernel<T, K, V, false>), grid, dim3(256), 0, s, P, first);
+    });
+  });
+  if (rc || !P.part) return rc;
+  hipLaunchKernelGGL(conv_join_kernel, dim3((unsigned)ceil_div(A.channels * (A.taps + 1), 64)), dim3(256), 0, s, P.part, parts,
+                     A.channels, (int)A.taps, P.weight_bf16, A.dweight, A.dbias);
+  return launched();
+}
+
+template <class T>
+int conv_typed(const ttc_causal_conv_args& A, hipStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  return conv_vector<T>(A) == V ? conv_run<T, V>(A, s) : conv_run<T, 1>(A, s);
+}
+
+template <class T, int V>
+int conv_step_run(const ttc_causal_conv_step_args& A, hipStream_t s) {
+  Conv P{};
+  P.x = A.x, P.weight = A.weight, P.bias = A.bias;
+  P.xb = A.x_stride;
+  P.C = A.channels;
+  P.weight_bf16 = A.weight_dtype == TTC_DTYPE_BF16;
+  P.y = A.y, P.final_state = A.state;
+  P.cols = A.channels / V;
+  const int64_t items = A.batch * P.cols;
+  return with_taps(A.taps, [&](auto taps) {
+    constexpr int K = decltype(taps)::value;
+    return in_launches(ceil_div(items, 256), 256, [&](int64_t first, dim3 grid) {
+      if (A.activation)
+        hipLaunchKernelGGL((conv_step_kernel<T, K, V, true>), grid, dim3(256), 0, s, P, A.slot_index, A.slots, first, items);
+      else
+        hipLaunchKernelGGL((conv_step_kernel<T, K, V, false>), grid, dim3(256), 0, s, P, A.slot_index, A.slots, first, items);
+    });
+  });
+}
+
+template <class T>
+int conv_step_typed(const ttc_causal_conv_step_args& A, hipStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  const bool wide = A.channels % V == 0 && A.x_stride % V == 0 && aligned16(A.x) && aligned16(A.y) && aligned16(A.state);
+  return wide ? conv_step_run<T, V>(A, s) : conv_step_run<T, 1>(A, s);
+}
+
+}  // namespace ttc
+
+extern "C" size_t ttc_causal_conv_workspace_bytes(const ttc_causal_conv_args* args) {
+  using namespace ttc;
+  if (!args || conv_check(*args) != TTC_LQR_OK) return 0;
+  return (size_t)conv_bytes(*args);
+}
+
+extern "C" int ttc_causal_conv(const ttc_causal_conv_args* args, void* stream) {
+  using namespace ttc;
+  if (!args) return TTC_LQR_EINVAL;
+  const ttc_causal_conv_args& A = *args;
+  if (const int rc = conv_check(A)) return rc;
+  if (A.channels == 0 || (!A.backward && (A.batch == 0 || A.tokens + A.taps == 1))) return TTC_LQR_OK;
+  if (!A.weight || (A.tokens > 0 && !A.x)) return TTC_LQR_EINVAL;
+  if (!A.backward && A.tokens > 0 && !A.y) return TTC_LQR_EINVAL;
+  if (A.backward && A.tokens > 0 && !A.d_y) return TTC_LQR_EINVAL;
+  const int64_t bytes = conv_bytes(A);
+  if (bytes > 0 && (!A.workspace || A.workspace_bytes < bytes)) return TTC_LQR_EINVAL;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return A.dtype == TTC_DTYPE_F32 ? conv_typed<float>(A, s) : conv_typed<__bf16>(A, s);
+}
+
+extern "C" int ttc_causal_conv_step(const ttc_causal_conv_step_args* args, void* stream) {
+  using namespace ttc;
+  if (!args) return TTC_LQR_EINVAL;
+  const ttc_causal_conv_step_args& A = *args;
+  if (const int rc = conv_check(A.dtype, A.weight_dtype, {A.batch, A.channels, MAX_TAPS}, A.taps, A.activation)) return rc;
+  if (A.slots < 0 || !countable({A.slots, A.channels, MAX_TAPS}) || (!A.slot_index && A.slots != A.batch))
+    return TTC_LQR_EINVAL;
+  if (A.batch == 0 || A.channels == 0) return TTC_LQR_OK;
+  if (!A.x || !A.weight || !A.y || (A.slots > 0 && A.taps > 1 && !A.state)) return TTC_LQR_EINVAL;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return A.dtype == TTC_DTYPE_F32 ? conv_step_typed<float>(A, s) : conv_step_typed<__bf16>(A, s);
+}

@@ -12,22 +12,26 @@ namespace ttc {
 
 struct RotaryShape {
   int64_t T, length, first;
-  int64_t pos_b, pos_t, xs[2][3];
+  int64_t pos_b, pos_t, pos_a, xs[2][3];
+  int axes, end[TTC_ROTARY_MAX_AXES];  // the pairs in front of each axis's end
   int H0, H1, dim, half, cols, groups;  // cols: vectors of a head, groups: head groups of a token
   float sign;
 };
 
+__device__ __forceinline__ int64_t position_at(const void* pos, int bytes, int64_t i) {
+  return bytes == 8 ? static_cast<const int64_t*>(pos)[i] : static_cast<const int32_t*>(pos)[i];
+}
+
 __device__ __forceinline__ int64_t position_of(const void* pos, int bytes, const RotaryShape& S, int64_t b, int64_t t) {
   if (pos == nullptr) return S.first + t;
-  const int64_t i = b * S.pos_b + t * S.pos_t;
-  return bytes == 8 ? static_cast<const int64_t*>(pos)[i] : static_cast<const int32_t*>(pos)[i];
+  return position_at(pos, bytes, b * S.pos_b + t * S.pos_t);
 }
 
 // One thread: one vector column of one token, HEADS heads of it.  V elements a vector (1 where sizes or
 // addresses do not allow 16 bytes).  Half layout: columns [0, half / V) are the pairs (column and its partner half
 // a rotation on); interleaved: columns [0, 2 half / V) hold whole pairs, or with V = 1 one pair each.  The columns
 // after them are copied.
-template <class T, int V, bool INTER, int HEADS>
+template <class T, int V, bool INTER, int HEADS, bool AXES>
 __global__ __launch_bounds__(256) void rotary_kernel(const T* __restrict__ q, const T* __restrict__ k,
                                                      T* __restrict__ yq, T* __restrict__ yk,
                                                      const float* __restrict__ table, const void* __restrict__ pos,
@@ -46,7 +50,25 @@ __global__ __launch_bounds__(256) void rotary_kernel(const T* __restrict__ q, co
   const int at = turn ? col * W : 2 * S.half + (col - pair_cols) * V;  // its first element
   constexpr int PAIRS = INTER ? W / 2 : V;
   float c[PAIRS], s[PAIRS];
-  if (turn) {
+  if (turn && AXES) {
+    // Every axis's position at once, then each pair's entry.  A vector's pairs lie in one section or in several: 8 bytes a
+    // pair from the cache, where one read of 16 bytes for two pairs of the same axis saves nothing (HEADS heads share it)
+    const int pair = INTER ? at / 2 : at;
+    int64_t p[TTC_ROTARY_MAX_AXES];
+#pragma unroll
+    for (int a = 0; a < TTC_ROTARY_MAX_AXES; ++a)
+      p[a] = position_at(pos, pos_bytes, b * S.pos_b + t * S.pos_t + (a < S.axes ? a : 0) * S.pos_a);
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+      int64_t own = p[0];
+#pragma unroll
+      for (int a = 1; a < TTC_ROTARY_MAX_AXES; ++a) own = pair + i >= S.end[a - 1] ? p[a] : own;
+      const bool in = own >= 0 && own < S.length;
+      const float2 cs = *reinterpret_cast<const float2*>(table + ((in ? own : 0) * S.half + pair + i) * 2);
+      c[i] = in ? cs.x : __builtin_nanf("");
+      s[i] = in ? cs.y * S.sign : __builtin_nanf("");
+    }
+  } else if (turn) {
     const int64_t p = position_of(pos, pos_bytes, S, b, t);
     const int pair = INTER ? at / 2 : at;
     const bool in = p >= 0 && p < S.length;
@@ -106,8 +128,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(const T* __restrict__ q, co
   }
 }
 
-template <class T, int V>
-int rotary_launch(const ttc_rotary_args& A, RotaryShape& S, hipStream_t s) {
+template <bool AXES, class T, int V, class Args>
+int rotary_launch(const Args& A, RotaryShape& S, hipStream_t s) {
   const bool inter = A.interleaved != 0;
   const int w = inter && V == 1 ? 2 : V;
   S.cols = (int)((inter ? 2 * S.half / w : S.half / V) + (S.dim - 2 * S.half) / V);
@@ -124,12 +146,12 @@ int rotary_launch(const ttc_rotary_args& A, RotaryShape& S, hipStream_t s) {
                          S, first, items);
     });
   };
-  if (inter) return per == 4 ? go(rotary_kernel<T, V, true, 4>) : go(rotary_kernel<T, V, true, 1>);
-  return per == 4 ? go(rotary_kernel<T, V, false, 4>) : go(rotary_kernel<T, V, false, 1>);
+  if (inter) return per == 4 ? go(rotary_kernel<T, V, true, 4, AXES>) : go(rotary_kernel<T, V, true, 1, AXES>);
+  return per == 4 ? go(rotary_kernel<T, V, false, 4, AXES>) : go(rotary_kernel<T, V, false, 1, AXES>);
 }
 
-template <class T>
-int rotary_typed(const ttc_rotary_args& A, RotaryShape& S, hipStream_t s) {
+template <bool AXES, class T, class Args>
+int rotary_typed(const Args& A, RotaryShape& S, hipStream_t s) {
   constexpr int V = 16 / sizeof(T);
   bool wide = S.dim % V == 0 && (A.interleaved ? 2 * S.half : S.half) % V == 0 && aligned16(A.table);
   for (int i = 0; i < 2; ++i) {
@@ -137,7 +159,44 @@ int rotary_typed(const ttc_rotary_args& A, RotaryShape& S, hipStream_t s) {
     wide = wide && aligned16(A.x[i]) && aligned16(A.y[i]);
     for (int j = 0; j < 3; ++j) wide = wide && A.stride[i][j] % V == 0;
   }
-  return wide ? rotary_launch<T, V>(A, S, s) : rotary_launch<T, 1>(A, S, s);
+  return wide ? rotary_launch<AXES, T, V>(A, S, s) : rotary_launch<AXES, T, 1>(A, S, s);
+}
+
+// what both entries check of their blocks; rot: of the table's entries
+template <class Args>
+int rotary_check(const Args& A, int64_t rot) {
+  const int64_t lim = 1 << 24;  // heads and head sizes are held in 32 bits
+  if (A.batch < 0 || A.tokens < 0 || A.heads[0] < 0 || A.heads[1] < 0 || A.heads[0] > lim || A.heads[1] > lim ||
+      A.dim < 0 || A.dim > lim || rot < 0 || rot > A.dim || rot % 2 || A.length < 0 ||
+      !countable({A.batch, A.tokens, A.heads[0] + A.heads[1], A.dim}) || !countable({A.length, rot}))
+    return TTC_LQR_EINVAL;
+  return A.dtype != TTC_DTYPE_F32 && A.dtype != TTC_DTYPE_BF16 ? TTC_LQR_EUNSUPPORTED : TTC_LQR_OK;
+}
+
+// and of a call that has something to turn
+template <bool AXES, class Args>
+int rotary_run(const Args& A, int64_t rot, RotaryShape& S, hipStream_t s) {
+  for (int i = 0; i < 2; ++i)
+    if (A.heads[i] > 0 && (!A.x[i] || !A.y[i])) return TTC_LQR_EINVAL;
+  if (rot > 0 && (A.length == 0 || !A.table)) return TTC_LQR_EINVAL;
+  if (A.positions && A.position_bytes != 4 && A.position_bytes != 8) return TTC_LQR_EINVAL;
+  S.T = A.tokens;
+  S.length = A.length;
+  S.pos_b = A.position_stride[0];
+  S.pos_t = A.position_stride[1];
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 3; ++j) S.xs[i][j] = A.stride[i][j];
+  S.H0 = (int)A.heads[0];
+  S.H1 = (int)A.heads[1];
+  S.dim = (int)A.dim;
+  S.half = (int)(rot / 2);
+  S.sign = A.backward ? -1.0f : 1.0f;
+  return A.dtype == TTC_DTYPE_F32 ? rotary_typed<AXES, float>(A, S, s) : rotary_typed<AXES, __bf16>(A, S, s);
+}
+
+template <class Args>
+bool rotary_empty(const Args& A) {
+  return A.batch == 0 || A.tokens == 0 || A.heads[0] + A.heads[1] == 0 || A.dim == 0;
 }
 
 }  // namespace ttc
@@ -146,31 +205,31 @@ extern "C" int ttc_rotary(const ttc_rotary_args* args, void* stream) {
   using namespace ttc;
   if (!args) return TTC_LQR_EINVAL;
   const ttc_rotary_args& A = *args;
-  const int64_t lim = 1 << 24;  // heads and head sizes are held in 32 bits
-  if (A.batch < 0 || A.tokens < 0 || A.heads[0] < 0 || A.heads[1] < 0 || A.heads[0] > lim || A.heads[1] > lim ||
-      A.dim < 0 || A.dim > lim || A.rot < 0 || A.rot > A.dim || A.rot % 2 || A.length < 0 ||
-      !countable({A.batch, A.tokens, A.heads[0] + A.heads[1], A.dim}) || !countable({A.length, A.rot}))
-    return TTC_LQR_EINVAL;
-  if (A.dtype != TTC_DTYPE_F32 && A.dtype != TTC_DTYPE_BF16) return TTC_LQR_EUNSUPPORTED;
-  if (A.batch == 0 || A.tokens == 0 || A.heads[0] + A.heads[1] == 0 || A.dim == 0) return TTC_LQR_OK;
-  for (int i = 0; i < 2; ++i)
-    if (A.heads[i] > 0 && (!A.x[i] || !A.y[i])) return TTC_LQR_EINVAL;
-  if (A.rot > 0 && A.length > 0 && !A.table) return TTC_LQR_EINVAL;
-  if (A.rot > 0 && A.length == 0) return TTC_LQR_EINVAL;
-  if (A.positions && A.position_bytes != 4 && A.position_bytes != 8) return TTC_LQR_EINVAL;
-  RotaryShape S;
-  S.T = A.tokens;
-  S.length = A.length;
+  if (const int rc = rotary_check(A, A.rot)) return rc;
+  if (rotary_empty(A)) return TTC_LQR_OK;
+  RotaryShape S{};
   S.first = A.first;
-  S.pos_b = A.position_stride[0];
-  S.pos_t = A.position_stride[1];
-  for (int i = 0; i < 2; ++i)
-    for (int j = 0; j < 3; ++j) S.xs[i][j] = A.stride[i][j];
-  S.H0 = (int)A.heads[0];
-  S.H1 = (int)A.heads[1];
-  S.dim = (int)A.dim;
-  S.half = (int)(A.rot / 2);
-  S.sign = A.backward ? -1.0f : 1.0f;
-  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  return A.dtype == TTC_DTYPE_F32 ? rotary_typed<float>(A, S, s) : rotary_typed<__bf16>(A, S, s);
+  return rotary_run<false>(A, A.rot, S, reinterpret_cast<hipStream_t>(stream));
+}
+
+extern "C" int ttc_rotary_axes(const ttc_rotary_axes_args* args, void* stream) {
+  using namespace ttc;
+  if (!args) return TTC_LQR_EINVAL;
+  const ttc_rotary_axes_args& A = *args;
+  if (A.axes < 1 || A.axes > TTC_ROTARY_MAX_AXES) return TTC_LQR_EINVAL;
+  RotaryShape S{};
+  int64_t pairs = 0;
+  for (int a = 0; a < TTC_ROTARY_MAX_AXES; ++a) {  // pairs behind the last axis's end do not turn
+    if (a < A.axes) {
+      if (A.section[a] < 0 || A.section[a] > (1 << 24)) return TTC_LQR_EINVAL;
+      pairs += A.section[a];
+    }
+    S.end[a] = (int)pairs;
+  }
+  if (const int rc = rotary_check(A, 2 * pairs)) return rc;
+  if (rotary_empty(A)) return TTC_LQR_OK;
+  if (pairs > 0 && !A.positions) return TTC_LQR_EINVAL;
+  S.axes = (int)A.axes;
+  S.pos_a = A.position_stride[2];
+  return rotary_run<true>(A, 2 * pairs, S, reinterpret_cast<hipStream_t>(stream));
 }

@@ -1,8 +1,11 @@
-"""Sequence operators for models that hold the test-time control layer: rotary positions, linear attention with a
-decay for each head, group norm with an activation or a gate.  Hand-written gfx950 kernels for CUDA tensors
+"""Sequence operators for models that hold the test-time control layer: rotary positions (with one
+axis or several), causal convolution over a few tokens, linear attention with a decay for each head, group norm with an
+activation or a gate.  Hand-written gfx950 kernels for CUDA tensors
 (``include/ttc_ops.h``), the same formulas as torch operators for CPU tensors."""
+from .causal_conv import causal_conv, causal_conv_step
 from .group_norm import group_norm
 from .linear_attention import linear_attention, linear_attention_step
-from .rotary import rotary, rotary_table
+from .rotary import grid_positions, rotary, rotary_axes, rotary_table
 
-__all__ = ["group_norm", "linear_attention", "linear_attention_step", "rotary", "rotary_table"]
+__all__ = ["causal_conv", "causal_conv_step", "grid_positions", "group_norm", "linear_attention", "linear_attention_step",
+           "rotary", "rotary_axes", "rotary_table"]
