@@ -182,6 +182,51 @@ typedef struct {
 
 int ttc_linear_attention_step(const ttc_linear_attention_step_args* args, void* stream);
 
+/* ---- The gated delta rule ----
+ * Linear attention whose state forgets, before it takes up v_t at k_t, what it holds there: with strengths b = beta,
+ *   S_t = e^{g_t} (I - b_t k_t k_t') S_{t-1} + b_t k_t v_t',   o_t = scale S_t' q_t.
+ * normalize: q and k stand for q / sqrt(|q|^2 + eps) and k / sqrt(|k|^2 + eps).  Keys longer than sqrt(2 / b) make the state
+ * grow.  beta [batch, tokens, heads]: any strides, of type beta_dtype (fp32, or dtype), like log_gamma (which has all three
+ * dimensions here).  Everything else as in ttc_linear_attention; resets (TTC_RESET_LOG_GAMMA) too.
+ * saved: NULL, or ttc_delta_rule_saved_bytes() that the forward fills and the backward of the same inputs needs.
+ * workspace: ttc_delta_rule_workspace_bytes() of the same block (whether `saved` is there counts). */
+typedef struct {
+  int64_t dtype, gamma_dtype, beta_dtype, normalize, backward;
+  int64_t batch, tokens, heads, q_heads, k_heads, v_heads, dk, dv;
+  double scale, eps;
+  const void *q, *k, *v, *log_gamma, *beta;
+  int64_t q_stride[3], k_stride[3], v_stride[3], gamma_stride[3], beta_stride[3]; /* batch, token, head */
+  const float* initial_state;
+  void* o;
+  float* final_state;
+  const void* d_o;
+  int64_t d_o_stride[3];
+  const float* d_final_state;
+  void *dq, *dk_out, *dv_out, *d_log_gamma, *d_beta;
+  float* d_initial_state;
+  void* saved;
+  int64_t saved_bytes;
+  void* workspace;
+  int64_t workspace_bytes;
+} ttc_delta_rule_args;
+
+size_t ttc_delta_rule_workspace_bytes(const ttc_delta_rule_args* args);
+size_t ttc_delta_rule_saved_bytes(const ttc_delta_rule_args* args);
+int ttc_delta_rule(const ttc_delta_rule_args* args, void* stream);
+
+/* One token of each sequence, its state updated in place: as ttc_linear_attention_step. */
+typedef struct {
+  int64_t dtype, gamma_dtype, beta_dtype, normalize, batch, heads, q_heads, k_heads, v_heads, dk, dv, slots;
+  double scale, eps;
+  const void *q, *k, *v, *log_gamma, *beta;
+  int64_t q_stride[2], k_stride[2], v_stride[2], gamma_stride[2], beta_stride[2]; /* batch, head */
+  float* state;
+  const int32_t* slot_index;
+  void* o;
+} ttc_delta_rule_step_args;
+
+int ttc_delta_rule_step(const ttc_delta_rule_step_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

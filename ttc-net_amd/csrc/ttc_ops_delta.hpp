@@ -1,0 +1,55 @@
+// ttc_ops_delta.hpp -- the gated delta rule: what its kernels share.
+//
+//   S_t = e^{g_t} (I - b_t k_t k_t') S_{t-1} + b_t k_t v_t',   o_t = scale S_t' q_t
+// With e_t = v_t - e^{g_t} S_{t-1}' k_t, what the state does not yet hold at k_t, this is linear attention with the values
+// b_t e_t.  In a chunk of C tokens behind the state S, with G_t the sum of its decays up to token t,
+//   N_ts = e^{G_t - G_s} k_t . k_s (s < t),   P_ts = scale e^{G_t - G_s} q_t . k_s (s <= t),
+//   (I + N b) E = V - e^G K S,   O = scale e^G Q S + P b E,   S <- e^{G_C} S + (e^{G_C - G} K)' b E,
+// where the triangle's inverse needs no state: all chunks' at once (prepare), then the states from chunk to chunk (sweep).
+// Backward, with R the gradient of the state behind a chunk and dO given,
+//   Z = b (P' dO + e^{G_C - G} K R),   dV = (I + N b)^-T Z,   R <- e^{G_C} R + (scale e^G Q)' dO - (e^G K)' dV
+// is such a sweep from the end; what remains needs S, R, E and dV of a chunk alone, all chunks at once (gradients).
+#pragma once
+#include "ttc_ops_linear.hpp"
+
+namespace ttc {
+
+// What prepare leaves for each chunk of each head
+enum { IN, UP, BETA, RK, RQ, DEC, HI, LO, PART, ROWS };  // C values each:
+// IN    e^{G_t}, 0 behind a reset                  UP    e^{G_C - G_t}, 0 in front of one
+// RK    1 / |k_t| (1 unless keys are normalised)   RQ    1 / |q_t|
+// DEC   e^{g_t}, -1 at a reset                     PART  resets so far
+// HI, LO  the two parts of log2(e) G_t, whose sum starts anew at a reset; infinite where it is lost (a NaN, growth beyond e^128)
+
+struct Delta {
+  Side q, k, v, d_o;
+  const void *gamma, *beta;
+  int64_t gb, gt, gh, bb, bt, bh;
+  bool gamma_bf16, beta_bf16, normalize;
+  bool wide_q, wide_k, wide_v, wide_d, wide_o;  // 16-byte loads; stores of 4 elements at once
+  int kd, vd, vdp, H, colblocks;                // vdp: columns of the arrays below, 32, 64 or 128
+  int64_t B, T, chunks, first;                  // first: head (or chunk) of all that this launch begins with
+  float scale, eps;
+  const float* state_in;  // [B, H, kd, vd]
+  float* state_out;
+  void* o;
+  // [B, H, chunks, ...]
+  float *inverse, *scores;  // lower triangles of 16 x 16 tiles (the diagonal ones whole): (I + N b)^-1, P b
+  float* rows;              // [ROWS, C]
+  int* odd;                 // keys or inverse not finite
+  float *S, *R;             // [KD, vdp]: states in front of the chunks, gradients behind them (NULL: not kept)
+  float *E, *dV;            // [C, vdp]
+  // outputs of the gradients' kernel; fp32 for heads that share
+  void *dq, *dk, *dv, *dgamma, *dbeta;
+  bool dq_f32, dk_f32;
+};
+
+template <class T>
+int launch_delta_kd32(const Delta& A, int what, hipStream_t s);
+template <class T>
+int launch_delta_kd64(const Delta& A, int what, hipStream_t s);
+template <class T>
+int launch_delta_kd128(const Delta& A, int what, hipStream_t s);
+enum { PREPARE, SWEEP, SWEEP_BACK, GRADIENTS };
+
+}  // namespace ttc

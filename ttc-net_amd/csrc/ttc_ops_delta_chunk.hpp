@@ -1,0 +1,992 @@
+// ttc_ops_delta_chunk.hpp -- the gated delta rule in chunks on the matrix cores (formulas: ttc_ops_delta.hpp).
+//
+// A sweep's wave holds 16 ET columns of the state in registers, all rows, and needs nothing of the other waves: the columns of
+// S, E, O, R and dV never meet.  Products are laid out so that no accumulator moves before it is an operand:
+//   K S         lane: column n, 4 neighbouring tokens       -> with V, rows of the next product's right side
+//   E = T Y     T's rows straight from memory as operands; E as it lies in the accumulators is the next right side
+//   O' = S' Q' + E' (P b)'   lane: token n, 4 neighbouring columns -> stored 4 at once
+//   S += K' (w E)            K' by transposing reads of shared memory (bf16) or element by element (fp32)
+// Tokens that are not finite: where E (dV) of a wave's columns is not, the wave goes through that chunk token by token, so that
+// no token has an effect on earlier ones and none passes a reset.
+//
+// Numerics.  In bf16 every operand that is not an input is split into bf16 parts: three (24 digits) on the way of the states,
+// E, dV and the dots that the decays' and strengths' gradients are made of, two (16 digits) where the result is a bf16 output.
+#pragma once
+#include "ttc_ops_delta.hpp"
+#include "ttc_ops_mfma.hpp"
+
+namespace ttc {
+
+template <class T, int KD>
+struct DeltaShape {
+  static constexpr int C = chunk_tokens(sizeof(T) == 2), TT = C / 16, KB = C / 32, DB = KD / 32, DT = KD / 16;
+  static constexpr int VEC = 16 / sizeof(T), TILES = TT * (TT + 1) / 2;
+  static constexpr int QS = KD + Operand<T>::ROW_PAD, KS = KD + Operand<T>::COL_PAD;
+};
+constexpr int tile_of(int t, int s) { return t * (t + 1) / 2 + s; }
+
+// A chunk's rows of D elements: 16-byte loads, all in flight at once, then to shared memory.  Rows that do not exist and
+// elements behind `dim` are 0.
+template <class T, int D, int C, int NT>
+struct Stage {
+  static constexpr int VEC = 16 / sizeof(T), N = (C * D / VEC + NT - 1) / NT;
+  u32x4 r[N];
+  __device__ __forceinline__ void fetch(const T* p, int64_t st, int dim, int left, bool wide, int tid) {
+    if (wide) {
+      const auto rows = bounded(p, left * (int)st * (int)sizeof(T));  // rows do not overlap: st >= dim
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int i = tid + j * NT, row = i / (D / VEC), c = i % (D / VEC) * VEC;
+        r[j] = __builtin_amdgcn_raw_buffer_load_b128(
+            rows, row < C && c < dim ? (row * (int)st + c) * (int)sizeof(T) : BEYOND, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int i = tid + j * NT, row = i / (D / VEC), c = i % (D / VEC) * VEC;
+        const u32x4 zero = {0, 0, 0, 0};
+        r[j] = row < C && row < left ? load_any(p + row * st, c, dim) : zero;
+      }
+    }
+  }
+  template <int STRIDE>
+  __device__ __forceinline__ void put(T* to, int tid) const {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int i = tid + j * NT, row = i / (D / VEC), c = i % (D / VEC) * VEC;
+      if (C * D / VEC % NT == 0 || row < C) *reinterpret_cast<u32x4*>(&to[row * STRIDE + c]) = r[j];
+    }
+  }
+  __device__ __forceinline__ void largest(uint32_t& m) const {
+#pragma unroll
+    for (int j = 0; j < N; ++j) Operand<T>::largest(r[j], m);
+  }
+};
+
+__device__ __forceinline__ float gate_value(const void* p, bool bf16, int64_t i) {
+  return bf16 ? to_f(static_cast<const __bf16*>(p)[i]) : static_cast<const float*>(p)[i];
+}
+
+// A token's place among the decays, and e^{G_t - G_s}: 0 across a reset, whatever the sums hold
+struct Place {
+  float hi, lo, part;
+};
+__device__ __forceinline__ float weight_of(const Place& t, const Place& s) {
+  return t.part == s.part ? exp2_of((t.hi - s.hi) + (t.lo - s.lo)) : 0.0f;
+}
+
+__device__ __forceinline__ bool all_finite(const f32x4& x) {
+  bool ok = true;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) ok = ok && (__float_as_uint(x[i]) & 0x7f800000u) != 0x7f800000u;
+  return ok;
+}
+
+// ---- prepare: decays, lengths, scores and the triangle's inverse, one workgroup a chunk ----------------------------
+
+// acc + a b of 16 x 16 blocks in fp32
+__device__ __forceinline__ f32x4 block_mma(const float* a, const float* b, int stride, f32x4 acc, int lane) {
+  const int g = lane >> 4, n = lane & 15;
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[n * stride + 4 * s + g], b[(4 * s + g) * stride + n], acc, 0, 0, 0);
+  return acc;
+}
+
+template <class T, int KD>
+__global__ __launch_bounds__(256) void delta_prepare_kernel(Delta A) {
+  using Z = DeltaShape<T, KD>;
+  using Op = Operand<T>;
+  constexpr int C = Z::C, TT = Z::TT, QS = Z::QS, LS = C + 4, SUB = 256 / C;
+  __shared__ __attribute__((aligned(16))) T Ks[C * QS], Qs[C * QS];
+  __shared__ __attribute__((aligned(16))) float Lm[C * LS], Tm[C * LS];
+  __shared__ __attribute__((aligned(16))) float Row[ROWS][C];
+  __shared__ int Odd[4];
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, n = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t unit = A.first + blockIdx.x, bh = unit / A.chunks, t0 = unit % A.chunks * C, b = bh / A.H;
+  const int h = (int)(bh % A.H), left = A.T - t0 < C ? (int)(A.T - t0) : C;
+  {
+    Stage<T, KD, C, 256> k, q;
+    k.fetch(A.k.at<T>(b, h) + t0 * A.k.st, A.k.st, A.kd, left, A.wide_k, tid);
+    q.fetch(A.q.at<T>(b, h) + t0 * A.q.st, A.q.st, A.kd, left, A.wide_q, tid);
+    if (wave == 3) {
+      const int64_t t = t0 + lane;
+      const bool here = lane < left;
+      const float lg = here ? gate_value(A.gamma, A.gamma_bf16, b * A.gb + h * A.gh + t * A.gt) : 0.0f;
+      const float strength = here ? gate_value(A.beta, A.beta_bf16, b * A.bb + h * A.bh + t * A.bt) : 0.0f;
+      const float inf = __builtin_inff();
+      const bool cut = lane < C && lg < RESET;
+      const uint64_t cuts = __ballot(cut), so_far = cuts & (((uint64_t)2 << lane) - 1);
+      const int start = so_far == 0 ? 0 : 63 - __builtin_clzll(so_far);
+      double y = cut ? 0.0 : lg <= 128.0f ? (double)lg * 1.4426950408889634 : (double)inf;
+#pragma unroll
+      for (int m = 1; m < C; m <<= 1) {
+        const double z = __shfl_up(y, m, 64);
+        if (lane - m >= start) y += z;
+      }
+      const double rest = __shfl(y, C - 1, 64) - y;
+      if (lane < C) {
+        const float uh = (float)rest, ul = (float)(rest - (double)uh), hi = (float)y;
+        const float lo = hi < inf ? (float)(y - (double)hi) : 0.0f;
+        Row[HI][lane] = hi;
+        Row[LO][lane] = lo;
+        Row[PART][lane] = (float)__builtin_popcountll(so_far);
+        Row[IN][lane] = so_far != 0 ? 0.0f : exp2_of(hi) * exp2_of(lo);
+        Row[UP][lane] = so_far != cuts ? 0.0f : hi < inf ? exp2_of(uh) * exp2_of(ul) : inf;
+        Row[DEC][lane] = cut ? -1.0f : expf(lg);
+        Row[BETA][lane] = strength;
+      }
+    }
+    k.template put<QS>(Ks, tid);
+    q.template put<QS>(Qs, tid);
+    uint32_t most = 0;
+    k.largest(most);
+    const bool odd = __ballot(!Op::finite(most)) != 0;
+    if (lane == 0) Odd[wave] = odd;
+  }
+  __syncthreads();
+  {
+    const int row = tid / SUB, sub = tid % SUB;
+    float kk = 1.0f, qq = 1.0f;
+    if (A.normalize) {
+      kk = qq = 0.0f;
+      for (int c = sub; c < KD; c += SUB) {
+        const float x = to_f(Ks[row * QS + c]), y = to_f(Qs[row * QS + c]);
+        kk = fmaf(x, x, kk);
+        qq = fmaf(y, y, qq);
+      }
+      kk = 1.0f / sqrtf(lane_sum(kk, SUB) + A.eps);
+      qq = 1.0f / sqrtf(lane_sum(qq, SUB) + A.eps);
+    }
+    if (sub == 0) {
+      Row[RK][row] = row < left ? kk : 0.0f;
+      Row[RQ][row] = row < left ? qq : 0.0f;
+    }
+  }
+  __syncthreads();
+  const int64_t tiles_at = unit * Z::TILES * 256;
+  for (int i = tid; i < ROWS * C / 4; i += 256)
+    reinterpret_cast<f32x4*>(A.rows + unit * ROWS * C)[i] = reinterpret_cast<const f32x4*>(&Row[0][0])[i];
+  int turn = 0;
+#pragma unroll
+  for (int ti = 0; ti < TT; ++ti)
+#pragma unroll
+    for (int si = 0; si <= ti; ++si, ++turn) {
+      if (turn % 4 != wave) continue;
+      f32x4 kk = {0.f, 0.f, 0.f, 0.f}, qk = kk;  // lane: token t = n, 4 neighbouring s
+#pragma unroll
+      for (int d = 0; d < Z::DB; ++d) {
+        const typename Op::Frag f = Op::row(&Ks[(16 * si + n) * QS + 32 * d + 8 * g]);
+        kk = Op::mma(f, Op::row(&Ks[(16 * ti + n) * QS + 32 * d + 8 * g]), kk);
+        qk = Op::mma(f, Op::row(&Qs[(16 * ti + n) * QS + 32 * d + 8 * g]), qk);
+      }
+      const int t = 16 * ti + n, s = 16 * si + 4 * g;
+      const Place at_t = {Row[HI][t], Row[LO][t], Row[PART][t]};
+      const float rk = Row[RK][t], rq = Row[RQ][t] * A.scale;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float w = weight_of(at_t, Place{Row[HI][s + i], Row[LO][s + i], Row[PART][s + i]}), by = Row[RK][s + i] * Row[BETA][s + i];
+        kk[i] = s + i < t ? kept(w, kk[i] * rk * by) : 0.0f;
+        qk[i] = s + i <= t ? kept(w, qk[i] * rq * by) : 0.0f;
+      }
+      *reinterpret_cast<f32x4*>(&Lm[t * LS + s]) = kk;
+      *reinterpret_cast<f32x4*>(A.scores + tiles_at + tile_of(ti, si) * 256 + n * 16 + 4 * g) = qk;
+    }
+  __syncthreads();
+  // the diagonal blocks' inverses: a lane's column by forward substitution
+  if (wave == 0 && lane < C) {
+    const float* L = Lm + (lane & ~15) * (LS + 1);
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float a = i == n ? 1.0f : 0.0f;
+#pragma unroll
+      for (int j = 0; j < i; ++j) a = fmaf(-L[i * LS + j], x[j], a);
+      x[i] = a;
+      Tm[((lane & ~15) + i) * LS + lane] = a;
+    }
+  }
+  __syncthreads();
+  // [[a, 0], [c, b]]^-1 = [[a^-1, 0], [-b^-1 c a^-1, b^-1]]: blocks of 16, then of 32.  c a^-1 goes where nothing else is: above
+  // the diagonal
+  const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+  auto put = [&](int r, int c, const f32x4& x, float sign) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) Tm[(16 * r + 4 * g + i) * LS + 16 * c + n] = sign * x[i];
+  };
+  auto block = [&](const float* m, int r, int c) { return m + 16 * r * LS + 16 * c; };
+  if (wave < TT / 2)
+    put(2 * wave, 2 * wave + 1, block_mma(block(Lm, 2 * wave + 1, 2 * wave), block(Tm, 2 * wave, 2 * wave), LS, none, lane), 1.0f);
+  __syncthreads();
+  if (wave < TT / 2)
+    put(2 * wave + 1, 2 * wave, block_mma(block(Tm, 2 * wave + 1, 2 * wave + 1), block(Tm, 2 * wave, 2 * wave + 1), LS, none, lane),
+        -1.0f);
+  if constexpr (TT == 4) {
+    const int r = wave >> 1, c = wave & 1;
+    __syncthreads();
+    f32x4 x = none;
+    for (int k = c; k < 2; ++k) x = block_mma(block(Lm, 2 + r, k), block(Tm, k, c), LS, x, lane);
+    put(r, 2 + c, x, 1.0f);
+    __syncthreads();
+    x = none;
+    for (int k = 0; k <= r; ++k) x = block_mma(block(Tm, 2 + r, 2 + k), block(Tm, k, 2 + c), LS, x, lane);
+    put(2 + r, c, x, -1.0f);
+  }
+  __syncthreads();
+  bool ok = true;
+#pragma unroll
+  for (int ti = 0; ti < TT; ++ti)
+#pragma unroll
+    for (int si = 0; si <= ti; ++si) {
+      if (tile_of(ti, si) % 4 != wave) continue;
+      const f32x4 x = *reinterpret_cast<const f32x4*>(&Tm[(16 * ti + n) * LS + 16 * si + 4 * g]);
+      ok = ok && all_finite(x);
+      *reinterpret_cast<f32x4*>(A.inverse + tiles_at + tile_of(ti, si) * 256 + n * 16 + 4 * g) = x;
+    }
+  const bool bad = __ballot(!ok) != 0;
+  if (lane == 0) Odd[wave] |= bad;
+  __syncthreads();
+  if (tid == 0) A.odd[unit] = Odd[0] | Odd[1] | Odd[2] | Odd[3];
+}
+
+// ---- sweeps ----------------------------------------------------------------------------------------------------
+
+// Lower triangle of tiles in memory as operands.  ROW: row 16 t + n, columns 32 s + 4 g .. and 16 + 4 g ..; otherwise its
+// transpose's: column 16 t + n, rows 32 s + ...
+template <bool ROW, int TT>
+__device__ __forceinline__ void triangle(const float* tiles, int t, int s, int lane, float (&x)[8]) {
+  const int g = lane >> 4, n = lane & 15;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int other = 2 * s + half, r = ROW ? t : other, c = ROW ? other : t;
+    if (c > r || r >= TT) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[4 * half + i] = 0.0f;
+    } else if (ROW) {
+      const f32x4 f = *reinterpret_cast<const f32x4*>(tiles + tile_of(r, c) * 256 + n * 16 + 4 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[4 * half + i] = f[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[4 * half + i] = tiles[tile_of(r, c) * 256 + (4 * g + i) * 16 + n];
+    }
+  }
+}
+
+// 8 values of two accumulators: rows 4 g + i of both
+__device__ __forceinline__ void eight(const f32x4& a, const f32x4& b, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+}
+
+template <class T, int KD, int WAVES, int ET, bool BACK>
+__global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
+  using Z = DeltaShape<T, KD>;
+  using Op = Operand<T>;
+  using Wide = typename Op::Wide;
+  using Frag = typename Op::Frag;
+  constexpr int C = Z::C, TT = Z::TT, KB = Z::KB, NT = WAVES * 64, COLS = 16 * ET * WAVES, QS = BACK ? Z::KS : Z::QS, KS = Z::KS,
+                VS = COLS + Op::COL_PAD;
+  __shared__ __attribute__((aligned(16))) T Ks[C * KS], Qs[C * QS], Vs[C * VS];  // Vs: V, or dO
+  __shared__ __attribute__((aligned(16))) float Row[ROWS][C];
+  int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int lane = tid & 63, g = lane >> 4, n = lane & 15;
+  const int c0 = (int)(blockIdx.x % A.colblocks) * COLS, e0 = wave * 16 * ET;  // the workgroup's columns, the wave's of those
+  const int64_t bh = A.first + blockIdx.x / A.colblocks, b = bh / A.H;
+  const int h = (int)(bh % A.H);
+  const T *q = A.q.at<T>(b, h), *k = A.k.at<T>(b, h), *v = (BACK ? A.d_o : A.v).at<T>(b, h) + c0;
+  const int64_t vst = BACK ? A.d_o.st : A.v.st;
+  const bool wide_v = BACK ? A.wide_d : A.wide_v;
+
+  f32x4 S[Z::DT][ET];  // the state (BACK: its gradient): rows 16 d + 4 g + i, columns e0 + 16 e + n
+  auto each = [&](auto f) {
+    int r = 4 * g, c = c0 + e0 + n;
+    asm volatile("" : "+v"(r), "+v"(c));  // otherwise the addresses stay in registers over the whole loop
+#pragma unroll
+    for (int d = 0; d < Z::DT; ++d)
+#pragma unroll
+      for (int e = 0; e < ET; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) S[d][e][i] = f((float)S[d][e][i], 16 * d + r + i, c + 16 * e);
+  };
+  {
+    const float* p = A.state_in ? A.state_in + bh * A.kd * A.vd : nullptr;
+    const auto from = bounded(p, p ? A.kd * A.vd * 4 : 0);
+    each([&](float, int r, int c) {
+      return __builtin_bit_cast(
+          float, __builtin_amdgcn_raw_buffer_load_b32(from, r < A.kd && c < A.vd ? (r * A.vd + c) * 4 : BEYOND, 0, 0));
+    });
+  }
+  Stage<T, KD, C, NT> kr, qr;
+  Stage<T, COLS, C, NT> vr;
+  Stage<float, C, ROWS, NT> rr;
+  auto chunk_of = [&](int64_t i) { return BACK ? A.chunks - 1 - i : i; };
+  auto fetch = [&](int64_t i) {
+    const int64_t ch = chunk_of(i), t0 = ch * C;
+    const int left = A.T - t0 < C ? (int)(A.T - t0) : C;
+    kr.fetch(k + t0 * A.k.st, A.k.st, A.kd, left, A.wide_k, tid);
+    qr.fetch(q + t0 * A.q.st, A.q.st, A.kd, left, A.wide_q, tid);
+    vr.fetch(v + t0 * vst, vst, A.vd - c0, left, wide_v, tid);
+    rr.fetch(A.rows + (bh * A.chunks + ch) * ROWS * C, C, C, ROWS, true, tid);
+  };
+  fetch(0);
+  for (int64_t i = 0; i < A.chunks; ++i) {
+    asm volatile("" : "+v"(lane), "+v"(tid));
+    g = lane >> 4, n = lane & 15;
+    const int64_t ch = chunk_of(i), t0 = ch * C, unit = bh * A.chunks + ch;
+    const int left = A.T - t0 < C ? (int)(A.T - t0) : C;
+    kr.template put<KS>(Ks, tid);
+    qr.template put<QS>(Qs, tid);
+    vr.template put<VS>(Vs, tid);
+    rr.template put<C>(&Row[0][0], tid);
+    __syncthreads();
+    const float *inverse = A.inverse + unit * Z::TILES * 256, *scores = A.scores + unit * Z::TILES * 256;
+    bool odd = A.odd[unit] != 0;
+    if (i + 1 < A.chunks) fetch(i + 1);
+    const float whole = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(Row[IN][C - 1])));
+    float* kept_state = BACK ? A.R : A.S;
+    if (kept_state) {
+      float* p = kept_state + unit * KD * A.vdp;
+      each([&](float s, int r, int c) {
+        p[r * A.vdp + c] = s;
+        return s;
+      });
+    }
+    auto row4 = [&](int which, int t) { return *reinterpret_cast<const f32x4*>(&Row[which][t]); };  // of 4 neighbouring tokens
+
+    // X = K S: lane's tokens 16 t + 4 g + i, columns e0 + 16 e + n.  Forward's O' = S' Q': lane's token n, 4 columns
+    f32x4 X[TT][ET], O[BACK ? 1 : TT][ET];
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+      for (int e = 0; e < ET; ++e) {
+        X[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (!BACK) O[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+    for (int d = 0; d < Z::DB; ++d) {
+      Wide s[ET];
+#pragma unroll
+      for (int e = 0; e < ET; ++e) {
+        float y[8];
+        eight(S[2 * d][e], S[2 * d + 1][e], y);
+        s[e] = Op::wide(y);
+      }
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        const Frag f = Op::row_split(&Ks[(16 * t + n) * KS + 32 * d + 4 * g]);
+#pragma unroll
+        for (int e = 0; e < ET; ++e) X[t][e] = Op::mma(f, s[e], X[t][e]);
+        if constexpr (!BACK) {
+          const Frag w = Op::row_split(&Qs[(16 * t + n) * QS + 32 * d + 4 * g]);
+#pragma unroll
+          for (int e = 0; e < ET; ++e) O[t][e] = Op::mma(Op::first(s[e]), w, O[t][e]);
+        }
+      }
+    }
+    // what the triangle is solved for: V - e^G K S, or b (e^{G_C - G} K R + P' dO)
+    Frag vf[KB][ET];
+#pragma unroll
+    for (int s = 0; s < KB; ++s)
+#pragma unroll
+      for (int e = 0; e < ET; ++e) vf[s][e] = Op::column(&Vs[32 * s * VS], VS, e0 + 16 * e, lane);
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      const f32x4 w = row4(BACK ? UP : IN, 16 * t + 4 * g), rk = row4(RK, 16 * t + 4 * g), be = row4(BETA, 16 * t + 4 * g);
+#pragma unroll
+      for (int e = 0; e < ET; ++e) {
+        float y[8];
+        if constexpr (!BACK) Op::values(vf[t / 2][e], y);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          X[t][e][j] = BACK ? kept(w[j], rk[j] * be[j] * X[t][e][j]) : y[t % 2 * 4 + j] - kept(w[j], rk[j] * X[t][e][j]);
+      }
+      if constexpr (BACK) {
+#pragma unroll
+        for (int s = t / 2; s < KB; ++s) {
+          float y[8];
+          triangle<false, TT>(scores, t, s, lane, y);
+          const Wide f = Op::wide(y);
+#pragma unroll
+          for (int e = 0; e < ET; ++e) X[t][e] = Op::mma(f, vf[s][e], X[t][e]);
+        }
+      }
+    }
+    // E (dV): the inverse's (its transpose's) rows times that
+    f32x4 E[TT][ET];
+    {
+      Wide y[KB][ET];
+#pragma unroll
+      for (int s = 0; s < KB; ++s)
+#pragma unroll
+        for (int e = 0; e < ET; ++e) {
+          float x[8];
+          eight(X[2 * s][e], X[2 * s + 1][e], x);
+          y[s][e] = Op::wide(x);
+        }
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+#pragma unroll
+        for (int e = 0; e < ET; ++e) E[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = BACK ? t / 2 : 0; s < (BACK ? KB : t / 2 + 1); ++s) {
+          float x[8];
+          triangle<!BACK, TT>(inverse, t, s, lane, x);
+          const Wide f = Op::wide(x);
+#pragma unroll
+          for (int e = 0; e < ET; ++e) E[t][e] = Op::mma(f, y[s][e], E[t][e]);
+        }
+      }
+    }
+    bool fine = true;
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+      for (int e = 0; e < ET; ++e) fine = fine && all_finite(E[t][e]);
+    odd = odd || __ballot(!fine) != 0;
+    float* kept_rows = (BACK ? A.dV : A.E) ? (BACK ? A.dV : A.E) + unit * C * A.vdp + c0 + e0 : nullptr;
+    const int64_t first = ((b * A.T + t0) * A.H + h) * A.vd;  // of the output
+    const int row = A.H * A.vd;
+    if (!odd) {
+      if (kept_rows) {
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+#pragma unroll
+          for (int e = 0; e < ET; ++e)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) kept_rows[(16 * t + 4 * g + j) * A.vdp + 16 * e + n] = E[t][e][j];
+      }
+      if constexpr (!BACK) {
+        typename Op::Pair y[KB][ET];
+#pragma unroll
+        for (int s = 0; s < KB; ++s)
+#pragma unroll
+          for (int e = 0; e < ET; ++e) {
+            float x[8];
+            eight(E[2 * s][e], E[2 * s + 1][e], x);
+            y[s][e] = Op::pair(x);
+          }
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+          const float w = Row[IN][16 * t + n], rq = Row[RQ][16 * t + n] * A.scale;
+#pragma unroll
+          for (int e = 0; e < ET; ++e)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) O[t][e][j] = kept(w, rq * O[t][e][j]);
+#pragma unroll
+          for (int s = 0; s <= t / 2; ++s) {
+            float x[8];
+            triangle<true, TT>(scores, t, s, lane, x);
+            const typename Op::Pair f = Op::pair(x);
+#pragma unroll
+            for (int e = 0; e < ET; ++e) O[t][e] = Op::mma(y[s][e], f, O[t][e]);
+          }
+#pragma unroll
+          for (int e = 0; e < ET; ++e) {  // a lane holds 4 neighbouring columns of one token
+            const int r = 16 * t + n, c = c0 + e0 + 16 * e + 4 * g;
+            T f[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[j] = from_f<T>(O[t][e][j]);
+            T* to = static_cast<T*>(A.o) + first;
+            if (A.wide_o) {
+              const auto rows = bounded(to, ((left - 1) * row + A.vd) * (int)sizeof(T));
+              const int off = c < A.vd ? (r * row + c) * (int)sizeof(T) : BEYOND;
+              if constexpr (sizeof(T) == 4)
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f), rows, off, 0, 0);
+              else
+                __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f), rows, off, 0, 0);
+            } else if (r < left) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (c + j < A.vd) to[(int64_t)r * row + c + j] = f[j];
+            }
+          }
+        }
+      }
+      // the state behind the chunk, or its gradient in front of it
+#pragma unroll
+      for (int d = 0; d < Z::DT; ++d)
+#pragma unroll
+        for (int e = 0; e < ET; ++e) S[d][e] = whole == 0.0f ? f32x4{0.f, 0.f, 0.f, 0.f} : S[d][e] * whole;
+#pragma unroll
+      for (int s = 0; s < KB; ++s) {
+        Wide we[ET], wd[BACK ? ET : 1];
+        float w[8], wq[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int t = 32 * s + (j < 4 ? 0 : 16) + 4 * g + j % 4;
+          const float rk = Row[RK][t];
+          w[j] = BACK ? -rk : rk * Row[BETA][t];
+          wq[j] = Row[RQ][t] * A.scale;
+        }
+        const f32x4 ua = row4(BACK ? IN : UP, 32 * s + 4 * g), ub = row4(BACK ? IN : UP, 32 * s + 16 + 4 * g);
+#pragma unroll
+        for (int e = 0; e < ET; ++e) {
+          float x[8];
+          eight(E[2 * s][e], E[2 * s + 1][e], x);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = kept(j < 4 ? ua[j % 4] : ub[j % 4], w[j] * x[j]);
+          we[e] = Op::wide(x);
+          if constexpr (BACK) {
+            Op::values(vf[s][e], x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = kept(j < 4 ? ua[j % 4] : ub[j % 4], wq[j] * x[j]);
+            wd[e] = Op::wide(x);
+          }
+        }
+#pragma unroll
+        for (int d = 0; d < Z::DT; ++d) {
+          const Frag f = Op::column(&Ks[32 * s * KS], KS, 16 * d, lane);
+#pragma unroll
+          for (int e = 0; e < ET; ++e) S[d][e] = Op::mma(f, we[e], S[d][e]);
+          if constexpr (BACK) {
+            const Frag x = Op::column(&Qs[32 * s * QS], QS, 16 * d, lane);
+#pragma unroll
+            for (int e = 0; e < ET; ++e) S[d][e] = Op::mma(x, wd[e], S[d][e]);
+          }
+        }
+      }
+    } else {  // token by token: a column needs nothing but its own entries
+      for (int a = 0; a < left; ++a) {
+        const int t = BACK ? left - 1 - a : a;
+        const float rk = Row[RK][t], rq = Row[RQ][t] * A.scale, be = Row[BETA][t], dec = Row[DEC][t];
+        float in[ET], x[ET], o[ET];
+#pragma unroll
+        for (int e = 0; e < ET; ++e) in[e] = to_f(Vs[t * VS + e0 + 16 * e + n]), x[e] = o[e] = 0.0f;
+        auto decay = [&](float s) { return dec < 0.0f ? 0.0f : kept(dec, s); };
+#pragma unroll
+        for (int d = 0; d < Z::DT; ++d)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int r = 16 * d + 4 * g + j;
+            const float kk = to_f(Ks[t * KS + r]), qq = to_f(Qs[t * QS + r]);
+#pragma unroll
+            for (int e = 0; e < ET; ++e) {
+              S[d][e][j] = BACK ? fmaf(rq * qq, in[e], S[d][e][j]) : decay(S[d][e][j]);
+              x[e] = r < A.kd ? fmaf(kk, S[d][e][j], x[e]) : x[e];
+            }
+          }
+#pragma unroll
+        for (int e = 0; e < ET; ++e) {
+          x[e] += __shfl_xor(x[e], 16, 64);
+          x[e] += __shfl_xor(x[e], 32, 64);
+          x[e] = BACK ? be * (rk * x[e]) : in[e] - rk * x[e];  // dV, or E
+          if (kept_rows && g == 0) kept_rows[t * A.vdp + 16 * e + n] = x[e];
+        }
+#pragma unroll
+        for (int d = 0; d < Z::DT; ++d)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int r = 16 * d + 4 * g + j;
+            const float kk = to_f(Ks[t * KS + r]), qq = to_f(Qs[t * QS + r]);
+#pragma unroll
+            for (int e = 0; e < ET; ++e) {
+              if constexpr (BACK) {
+                S[d][e][j] = r < A.kd ? decay(fmaf(-rk * kk, x[e], S[d][e][j])) : 0.0f;
+              } else {
+                S[d][e][j] = r < A.kd ? fmaf(rk * kk, be * x[e], S[d][e][j]) : 0.0f;
+                o[e] = r < A.kd ? fmaf(qq, S[d][e][j], o[e]) : o[e];
+              }
+            }
+          }
+        if constexpr (!BACK) {
+#pragma unroll
+          for (int e = 0; e < ET; ++e) {
+            o[e] += __shfl_xor(o[e], 16, 64);
+            o[e] += __shfl_xor(o[e], 32, 64);
+            const int c = c0 + e0 + 16 * e + n;
+            if (g == 0 && c < A.vd) static_cast<T*>(A.o)[first + (int64_t)t * row + c] = from_f<T>(rq * o[e]);
+          }
+        }
+      }
+      if (kept_rows && left < C) {  // rows that do not exist
+        for (int t = left; t < C; ++t)
+#pragma unroll
+          for (int e = 0; e < ET; ++e)
+            if (g == 0) kept_rows[t * A.vdp + 16 * e + n] = 0.0f;
+      }
+    }
+    __syncthreads();
+  }
+  if (A.state_out) {
+    float* p = A.state_out + bh * A.kd * A.vd;
+    const auto to = bounded(p, A.kd * A.vd * 4);
+    each([&](float s, int r, int c) {
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s), to, r < A.kd && c < A.vd ? (r * A.vd + c) * 4 : BEYOND, 0, 0);
+      return s;
+    });
+  }
+}
+
+// ---- gradients: of queries, keys, decays and strengths, one workgroup a chunk ----------------------------------------
+//
+//   L = dO E',  M = dV E',  A = b e^{G_t - G_s} L (s <= t),  B = -b e^{G_t - G_s} M (s < t)
+//   dq_t = sum_s A_ts k_s + e^{G_t} S dO_t,   dk_s = sum_t A_ts q_t + sum_t B_ts k_t + sum_t B_st k_t + b e^{G_C - G_s} R E_s
+//          - e^{G_s} S dV_s       (q with its scale, both at their lengths)
+// and with x_ts = P_ts L_ts - N_ts M_ts, f_s = e^{G_C - G_s} k_s . R E_s,
+//   db_s = sum_t x_ts + f_s,   dg_t = the sum over all terms of the loss's gradient that decay across token t: pairs s < t <= t',
+//   the state in front (into tokens from t on), the state behind (from tokens before t), and the state through the chunk.
+// Waves share the score tiles, then each takes 16 columns of the keys.  Lanes hold one token and 4 neighbouring columns.
+template <class T, int KD, int VD>
+__global__ __launch_bounds__((KD / 16 * 64), 2) void delta_gradients_kernel(Delta A) {
+  using Z = DeltaShape<T, KD>;
+  using Op = Operand<T>;
+  using Wide = typename Op::Wide;
+  using Frag = typename Op::Frag;
+  constexpr int C = Z::C, TT = Z::TT, KB = Z::KB, WAVES = KD / 16, NT = WAVES * 64, KS = Z::KS, VB = VD / 32;
+  constexpr int DS = VD + Op::ROW_PAD, ES = VD + 4, TILE = Z::TILES * 256;
+  __shared__ __attribute__((aligned(16))) T Ks[C * KS], Qs[C * KS], Ds[C * DS];
+  __shared__ __attribute__((aligned(16))) float Big[2 * C * ES > 2 * TILE ? 2 * C * ES : 2 * TILE];  // E and dV, then A and B
+  __shared__ __attribute__((aligned(16))) float Row[ROWS][C];
+  __shared__ float Part[TT][3][C];      // by tile: sums over s of b P L and of b N M (by si), over t of x (by ti)
+  __shared__ float Dot[WAVES][3][C];    // by wave: q . S dO, k . S dV, k . R E
+  __shared__ float Through[WAVES], Qd[C], Kd[C];
+  __shared__ int Odd[WAVES];
+  float *Es = Big, *Vs = Big + C * ES;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, n = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t unit = A.first + blockIdx.x, bh = unit / A.chunks, t0 = unit % A.chunks * C, b = bh / A.H;
+  const int h = (int)(bh % A.H), left = A.T - t0 < C ? (int)(A.T - t0) : C;
+  {
+    Stage<T, KD, C, NT> k, q;
+    Stage<T, VD, C, NT> d;
+    Stage<float, C, ROWS, NT> r;
+    Stage<float, VD, C, NT> e;
+    k.fetch(A.k.at<T>(b, h) + t0 * A.k.st, A.k.st, A.kd, left, A.wide_k, tid);
+    q.fetch(A.q.at<T>(b, h) + t0 * A.q.st, A.q.st, A.kd, left, A.wide_q, tid);
+    d.fetch(A.d_o.at<T>(b, h) + t0 * A.d_o.st, A.d_o.st, A.vd, left, A.wide_d, tid);
+    r.fetch(A.rows + unit * ROWS * C, C, C, ROWS, true, tid);
+    uint32_t most = 0, mf = 0;
+    k.template put<KS>(Ks, tid);
+    q.template put<KS>(Qs, tid);
+    d.template put<DS>(Ds, tid);
+    r.template put<C>(&Row[0][0], tid);
+    k.largest(most);
+    q.largest(most);
+    d.largest(most);
+    e.fetch(A.E + unit * C * A.vdp, A.vdp, A.vdp, C, true, tid);
+    e.template put<ES>(Es, tid);
+    e.largest(mf);
+    e.fetch(A.dV + unit * C * A.vdp, A.vdp, A.vdp, C, true, tid);
+    e.template put<ES>(Vs, tid);
+    e.largest(mf);
+    const bool odd = __ballot(!Op::finite(most) || !Operand<float>::finite(mf)) != 0;
+    if (lane == 0) Odd[wave] = odd;
+  }
+  __syncthreads();
+  bool odd = A.odd[unit] != 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) odd = odd || Odd[w];
+  auto wide_row = [&](const float* p) {  // 8 neighbours
+    const f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + 4);
+    float f[8];
+    eight(x, y, f);
+    return Op::wide(f);
+  };
+
+  // values' gradients, where each head has its own
+  if (A.dv) {
+    T* to = static_cast<T*>(A.dv) + ((b * A.T + t0) * A.H + h) * A.vd;
+    for (int i = tid; i < left * A.vd; i += NT) {
+      const int t = i / A.vd, c = i % A.vd;
+      to[(int64_t)t * A.H * A.vd + c] = from_f<T>(Vs[t * ES + c]);
+    }
+  }
+
+  // score tiles (lane: token t = n, 4 neighbouring s)
+  constexpr int MINE = (Z::TILES + WAVES - 1) / WAVES;
+  f32x4 At[MINE], Bt[MINE];
+  int turn = 0;
+#pragma unroll
+  for (int ti = 0; ti < TT; ++ti)
+#pragma unroll
+    for (int si = 0; si <= ti; ++si, ++turn) {
+      if (turn % WAVES != wave) continue;
+      f32x4 kk = {0.f, 0.f, 0.f, 0.f}, qk = kk, lt = kk, mt = kk;
+#pragma unroll
+      for (int d = 0; d < Z::DB; ++d) {
+        const Frag f = Op::row(&Ks[(16 * si + n) * KS + 32 * d + 8 * g]);
+        kk = Op::mma(f, Op::row(&Ks[(16 * ti + n) * KS + 32 * d + 8 * g]), kk);
+        qk = Op::mma(f, Op::row(&Qs[(16 * ti + n) * KS + 32 * d + 8 * g]), qk);
+      }
+#pragma unroll
+      for (int d = 0; d < VB; ++d) {
+        const Wide f = wide_row(&Es[(16 * si + n) * ES + 32 * d + 8 * g]);
+        lt = Op::mma(f, Op::row(&Ds[(16 * ti + n) * DS + 32 * d + 8 * g]), lt);
+        mt = Op::mma(f, wide_row(&Vs[(16 * ti + n) * ES + 32 * d + 8 * g]), mt);
+      }
+      const int t = 16 * ti + n, s = 16 * si + 4 * g;
+      const Place at_t = {Row[HI][t], Row[LO][t], Row[PART][t]};
+      const float rk = Row[RK][t], rq = Row[RQ][t] * A.scale;
+      float sum_p = 0.0f, sum_n = 0.0f, by_s[4];
+      f32x4 at, bt;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float w = weight_of(at_t, Place{Row[HI][s + i], Row[LO][s + i], Row[PART][s + i]}), be = Row[BETA][s + i], rs = Row[RK][s + i];
+        const float pl = s + i <= t ? kept(w, rq * rs * qk[i] * lt[i]) : 0.0f;
+        const float nm = s + i < t ? kept(w, rk * rs * kk[i] * mt[i]) : 0.0f;
+        sum_p = s + i <= t && w != 0.0f ? fmaf(be, pl, sum_p) : sum_p;
+        sum_n = s + i < t && w != 0.0f ? fmaf(be, nm, sum_n) : sum_n;
+        by_s[i] = pl - nm;
+        at[i] = s + i <= t ? kept(w, be * lt[i]) : 0.0f;
+        bt[i] = s + i < t ? kept(w, -be * mt[i]) : 0.0f;
+      }
+      At[turn / WAVES] = at, Bt[turn / WAVES] = bt;
+      sum_p += __shfl_xor(sum_p, 16, 64);
+      sum_p += __shfl_xor(sum_p, 32, 64);
+      sum_n += __shfl_xor(sum_n, 16, 64);
+      sum_n += __shfl_xor(sum_n, 32, 64);
+      if (g == 0) Part[si][0][t] = sum_p, Part[si][1][t] = sum_n;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int m = 1; m <= 8; m <<= 1) by_s[i] += __shfl_xor(by_s[i], m, 64);
+        if (n == 0) Part[ti][2][s + i] = by_s[i];
+      }
+    }
+
+  // the state's parts: S dO, S dV and R E (rows r0 + n of S and R, lane's token n, columns r0 + 4 g + i)
+  const int r0 = wave * 16;
+  f32x4 dq[TT], dk[TT];
+  {
+    f32x4 sv[TT], re[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) dq[t] = sv[t] = re[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const float *Sp = A.S + (unit * KD + r0 + n) * A.vdp + 8 * g, *Rp = A.R + (unit * KD + r0 + n) * A.vdp + 8 * g;
+    float through = 0.0f;
+#pragma unroll
+    for (int d = 0; d < VB; ++d) {
+      const f32x4 sa = *reinterpret_cast<const f32x4*>(Sp + 32 * d), sb = *reinterpret_cast<const f32x4*>(Sp + 32 * d + 4);
+      const f32x4 ra = *reinterpret_cast<const f32x4*>(Rp + 32 * d), rb = *reinterpret_cast<const f32x4*>(Rp + 32 * d + 4);
+      float s8[8], r8[8];
+      eight(sa, sb, s8);
+      eight(ra, rb, r8);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) through = fmaf(s8[i], r8[i], through);
+      const Wide s = Op::wide(s8), r = Op::wide(r8);
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        dq[t] = Op::mma(s, Op::row(&Ds[(16 * t + n) * DS + 32 * d + 8 * g]), dq[t]);
+        sv[t] = Op::mma(s, wide_row(&Vs[(16 * t + n) * ES + 32 * d + 8 * g]), sv[t]);
+        re[t] = Op::mma(r, wide_row(&Es[(16 * t + n) * ES + 32 * d + 8 * g]), re[t]);
+      }
+    }
+    through = lane_sum(through, 64);
+    if (lane == 0) Through[wave] = through;
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      const int tt = 16 * t + n;
+      const float in = Row[IN][tt], up = Row[UP][tt], be = Row[BETA][tt], rq = Row[RQ][tt] * A.scale, rk = Row[RK][tt];
+      float c = 0.0f, d = 0.0f, f = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float qq = rq * to_f(Qs[tt * KS + r0 + 4 * g + i]), kk = rk * to_f(Ks[tt * KS + r0 + 4 * g + i]);
+        dq[t][i] = kept(in, dq[t][i]);
+        sv[t][i] = kept(in, sv[t][i]);
+        re[t][i] = kept(up, re[t][i]);
+        if (r0 + 4 * g + i < A.kd) {
+          c = in == 0.0f ? c : fmaf(qq, dq[t][i], c);
+          d = in == 0.0f ? d : fmaf(kk, sv[t][i], d);
+          f = up == 0.0f ? f : fmaf(kk, re[t][i], f);
+        }
+        dk[t][i] = be * re[t][i] - sv[t][i];
+        if (up == 0.0f) dk[t][i] = -sv[t][i];
+      }
+      c += __shfl_xor(c, 16, 64);
+      c += __shfl_xor(c, 32, 64);
+      d += __shfl_xor(d, 16, 64);
+      d += __shfl_xor(d, 32, 64);
+      f += __shfl_xor(f, 16, 64);
+      f += __shfl_xor(f, 32, 64);
+      if (g == 0) Dot[wave][0][tt] = c, Dot[wave][1][tt] = d, Dot[wave][2][tt] = f;
+    }
+  }
+  __syncthreads();  // E and dV have been read: their place is A's and B's
+  float *As = Big, *Bs = Big + TILE;
+  turn = 0;
+#pragma unroll
+  for (int ti = 0; ti < TT; ++ti)
+#pragma unroll
+    for (int si = 0; si <= ti; ++si, ++turn) {
+      if (turn % WAVES != wave) continue;
+      *reinterpret_cast<f32x4*>(&As[tile_of(ti, si) * 256 + n * 16 + 4 * g]) = At[turn / WAVES];
+      *reinterpret_cast<f32x4*>(&Bs[tile_of(ti, si) * 256 + n * 16 + 4 * g]) = Bt[turn / WAVES];
+    }
+  // one wave: what a token's sums come to, and the gradients of its decay and strength
+  if (wave == 0) {
+    const int t = lane < C ? lane : C - 1, own = t / 16;
+    float sum_p = 0.0f, sum_n = 0.0f, x = 0.0f, c = 0.0f, d = 0.0f, f = 0.0f, through = 0.0f;
+#pragma unroll
+    for (int i = 0; i < TT; ++i) {
+      if (i <= own) sum_p += Part[i][0][t], sum_n += Part[i][1][t];
+      if (i >= own) x += Part[i][2][t];
+    }
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) c += Dot[w][0][t], d += Dot[w][1][t], f += Dot[w][2][t], through += Through[w];
+    const float be = Row[BETA][t], whole = Row[IN][C - 1];
+    if (lane < C) {
+      Qd[t] = c + sum_p;
+      Kd[t] = be * (x + f) - sum_n - d;
+    }
+    // suffix sums within the texts that resets part, and of f those in front
+    const bool cut = lane < C && Row[DEC][t] < 0.0f;
+    const uint64_t cuts = __ballot(cut);
+    const uint64_t later = lane < 63 ? cuts & (~(uint64_t)0 << (lane + 1)) : 0, so_far = cuts & (((uint64_t)2 << lane) - 1);
+    const int end = later ? __builtin_ctzll(later) : C, start = so_far ? 63 - __builtin_clzll(so_far) : 0;
+    double suffix = lane < C ? (double)sum_p - sum_n + c - d - (double)be * x : 0.0, before = lane < C ? (double)be * f : 0.0;
+#pragma unroll
+    for (int m = 1; m < C; m <<= 1) {
+      const double up = __shfl_down(suffix, m, 64), low = __shfl_up(before, m, 64);
+      if (lane + m < end) suffix += up;
+      if (lane - m >= start) before += low;
+    }
+    before = __shfl_up(before, 1, 64);
+    if (lane == start) before = 0.0;
+    if (lane < left) {
+      const double dg = cut ? 0.0 : suffix + before + (cuts ? 0.0 : (double)kept(whole, through));
+      const int64_t at = (b * A.T + t0 + lane) * A.H + h;
+      if (A.dgamma) {
+        if (A.gamma_bf16) static_cast<__bf16*>(A.dgamma)[at] = from_f<__bf16>((float)dg);
+        else static_cast<float*>(A.dgamma)[at] = (float)dg;
+      }
+      if (A.dbeta) {
+        if (A.beta_bf16) static_cast<__bf16*>(A.dbeta)[at] = from_f<__bf16>(x + f);
+        else static_cast<float*>(A.dbeta)[at] = x + f;
+      }
+    }
+  }
+  __syncthreads();
+  if (!odd) {
+#pragma unroll
+    for (int s = 0; s < KB; ++s) {
+      const Frag kf = Op::column(&Ks[32 * s * KS], KS, r0, lane), qf = Op::column(&Qs[32 * s * KS], KS, r0, lane);
+      float rk[8], rq[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int t = 32 * s + (j < 4 ? 0 : 16) + 4 * g + j % 4;
+        rk[j] = Row[RK][t], rq[j] = Row[RQ][t] * A.scale;
+      }
+      auto times = [&](float(&x)[8], const float(&w)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] *= w[j];
+        return Op::pair(x);
+      };
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        float x[8];
+        if (s <= t / 2) {  // tokens s in front of t
+          triangle<true, TT>(As, t, s, lane, x);
+          dq[t] = Op::mma(kf, times(x, rk), dq[t]);
+          triangle<true, TT>(Bs, t, s, lane, x);
+          dk[t] = Op::mma(kf, times(x, rk), dk[t]);
+        }
+        if (s >= t / 2) {  // tokens behind t
+          triangle<false, TT>(As, t, s, lane, x);
+          dk[t] = Op::mma(qf, times(x, rq), dk[t]);
+          triangle<false, TT>(Bs, t, s, lane, x);
+          dk[t] = Op::mma(kf, times(x, rk), dk[t]);
+        }
+      }
+    }
+  } else {  // term by term, without those whose weight is 0
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      const int tt = 16 * t + n;
+      for (int s = 0; s < C; ++s) {
+        const int r = s > tt ? s : tt, c = s > tt ? tt : s;
+        const int at = tile_of(r / 16, c / 16) * 256 + r % 16 * 16 + c % 16;
+        const float a = As[at], bb = Bs[at], rk = Row[RK][s], rq = Row[RQ][s] * A.scale;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float kk = rk * to_f(Ks[s * KS + r0 + 4 * g + i]), qq = rq * to_f(Qs[s * KS + r0 + 4 * g + i]);
+          if (s <= tt && a != 0.0f) dq[t][i] = fmaf(a, kk, dq[t][i]);
+          if (s >= tt && a != 0.0f) dk[t][i] = fmaf(a, qq, dk[t][i]);
+          if (bb != 0.0f) dk[t][i] = fmaf(bb, kk, dk[t][i]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    const int tt = 16 * t + n;
+    const float rk = Row[RK][tt], rq = Row[RQ][tt];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = r0 + 4 * g + i;
+      const float qq = to_f(Qs[tt * KS + c]), kk = to_f(Ks[tt * KS + c]);
+      dq[t][i] *= rq * A.scale;
+      if (A.normalize) {  // the part along the vector itself is no change
+        dq[t][i] = fmaf(-qq * (rq * rq), Qd[tt], dq[t][i]);
+        dk[t][i] = rk * fmaf(-kk * rk, Kd[tt], dk[t][i]);
+      }
+    }
+    if (tt >= left) continue;
+    const int64_t at = ((b * A.T + t0 + tt) * A.H + h) * A.kd + r0 + 4 * g;
+    auto put = [&](auto* to, const f32x4& x) {
+      using Y = std::remove_pointer_t<decltype(to)>;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (r0 + 4 * g + i < A.kd) to[at + i] = from_f<Y>(x[i]);
+    };
+    if (A.dq) {
+      if (A.dq_f32) put(static_cast<float*>(A.dq), dq[t]);
+      else put(static_cast<T*>(A.dq), dq[t]);
+    }
+    if (A.dk) {
+      if (A.dk_f32) put(static_cast<float*>(A.dk), dk[t]);
+      else put(static_cast<T*>(A.dk), dk[t]);
+    }
+  }
+}
+
+// ---- launches --------------------------------------------------------------------------------------------------
+
+template <class T, int KD, int WAVES, int ET, bool BACK>
+int launch_delta_sweep(const Delta& A, hipStream_t s) {
+  Delta P = A;
+  P.colblocks = (int)ceil_div(A.vd, 16 * ET * WAVES);
+  return in_launches(A.B * A.H * P.colblocks, WAVES * 64, [&](int64_t first, dim3 grid) {
+    P.first = first / P.colblocks;
+    hipLaunchKernelGGL((delta_sweep_kernel<T, KD, WAVES, ET, BACK>), grid, dim3(WAVES * 64), 0, s, P);
+  }, P.colblocks);
+}
+
+template <class T, int KD, bool BACK>
+int launch_delta_sweeps(const Delta& A, hipStream_t s) {
+  if (A.vd <= 32) return launch_delta_sweep<T, KD, 2, 1, BACK>(A, s);
+  return launch_delta_sweep<T, KD, 4, 1, BACK>(A, s);
+}
+
+template <class T, int KD, int VD>
+int launch_delta_gradients(const Delta& A, hipStream_t s) {
+  return in_launches(A.B * A.H * A.chunks, KD / 16 * 64, [&](int64_t first, dim3 grid) {
+    Delta P = A;
+    P.first = first;
+    hipLaunchKernelGGL((delta_gradients_kernel<T, KD, VD>), grid, dim3(KD / 16 * 64), 0, s, P);
+  });
+}
+
+template <class T, int KD>
+int launch_delta(const Delta& A, int what, hipStream_t s) {
+  if (what == PREPARE)
+    return in_launches(A.B * A.H * A.chunks, 256, [&](int64_t first, dim3 grid) {
+      Delta P = A;
+      P.first = first;
+      hipLaunchKernelGGL((delta_prepare_kernel<T, KD>), grid, dim3(256), 0, s, P);
+    });
+  if (what == SWEEP) return launch_delta_sweeps<T, KD, false>(A, s);
+  if (what == SWEEP_BACK) return launch_delta_sweeps<T, KD, true>(A, s);
+  return A.vd <= 32   ? launch_delta_gradients<T, KD, 32>(A, s)
+         : A.vd <= 64 ? launch_delta_gradients<T, KD, 64>(A, s)
+                      : launch_delta_gradients<T, KD, 128>(A, s);
+}
+
+}  // namespace ttc
+
+#define TTC_DELTA_UNIT(T, KD)                                                                                        \
+  namespace ttc {                                                                                                    \
+  template <>                                                                                                        \
+  int launch_delta_kd##KD<T>(const Delta& A, int what, hipStream_t s) { return launch_delta<T, KD>(A, what, s); }   \
+  }

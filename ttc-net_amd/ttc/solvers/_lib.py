@@ -112,11 +112,11 @@ def _load():
     L.ttc_lqr_backward_host.argtypes = ([f32p] * 10 + [i64, i32, i32, i32, i32] + [f32p] * 9
                                         + [ctypes.c_float, f32p, i32])
     for name in ("ttc_rotary", "ttc_rotary_axes", "ttc_group_norm", "ttc_causal_conv", "ttc_causal_conv_step",
-                 "ttc_linear_attention", "ttc_linear_attention_step"):  # (block, stream)
+                 "ttc_linear_attention", "ttc_linear_attention_step", "ttc_delta_rule", "ttc_delta_rule_step"):  # (block, stream)
         getattr(L, name).restype = ctypes.c_int
         getattr(L, name).argtypes = [ctypes.c_char_p, ctypes.c_void_p]
     for name in ("ttc_group_norm_workspace_bytes", "ttc_causal_conv_workspace_bytes", "ttc_linear_attention_workspace_bytes",
-                 "ttc_linear_attention_saved_bytes"):
+                 "ttc_linear_attention_saved_bytes", "ttc_delta_rule_workspace_bytes", "ttc_delta_rule_saved_bytes"):
         getattr(L, name).restype = sz
         getattr(L, name).argtypes = [ctypes.c_char_p]
     for suffix in ("", "_bf16"):
