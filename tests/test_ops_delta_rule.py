@@ -465,13 +465,42 @@ def test_many_heads_and_far_rows():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("case", [(1, 5000, 2, 2, 2, 2, 128, 128), (2, 3333, 1, 1, 1, 1, 64, 32)])
-def test_long(case):
-    x = inputs(*case, torch.bfloat16, "cuda", True, normalize=True)
-    o, S = call(x, 0.1, True)
-    want = oracle(x, 0.1, normalize=True)
-    within(o, *want["o"])
-    within(S, *want["state"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["mixed", "reset"])
+@pytest.mark.parametrize("case", [(1, 1800, 2, 2, 2, 2, 128, 128), (2, 1111, 1, 1, 1, 1, 64, 32), (1, 900, 3, 1, 3, 1, 20, 70),
+                                  (1, 777, 2, 2, 2, 1, 128, 24), (1, 650, 1, 1, 1, 1, 30, 128)])
+def test_long(case, kind, dtype):
+    """Inputs whose chunks are split into segments."""
+    B, T, H, dk, dv = case[0], case[1], case[2], case[6], case[7]
+    x = inputs(*case, dtype, "cuda", True, kind, normalize=True)
+    d_o, d_state = make((B, T, H, dv), dtype, "cuda", 9), make((B, H, dk, dv), torch.float32, "cuda", 10)
+    got, want = grads(x, d_o, d_state, 0.1, True), oracle(x, 0.1, d_o, d_state, True)
+    check(got, want, ("o", "final") + NAMES, kind == "mixed")
+    with torch.no_grad():
+        o, S = call(x, 0.1, True)
+    assert torch.equal(o, got["o"]) and torch.equal(S, got["final"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("what", ["k", "v", "g", "beta", "q"])
+def test_not_finite_in_segments(dtype, what):
+    """A spoilt text among others, far apart: no effect in front of it, nor behind the reset after it, nor (its gradients) on the
+    text in front of it."""
+    B, T, H, dk, dv, first, second = 1, 1500, 1, 64, 48, 420, 1010
+    x = inputs(B, T, H, 1, 1, 1, dk, dv, dtype, "cuda", True)
+    x["g"][:, [first, second]] = -math.inf
+    d_o, d_state = make((B, T, H, dv), dtype, "cuda", 9), make((B, H, dk, dv), torch.float32, "cuda", 10)
+    clean = oracle(x, 0.4, d_o, d_state)
+    x[what][0, 700] = math.nan
+    got = grads(x, d_o, d_state, 0.4)
+    within(got["o"][:, :700], *(t[:, :700] for t in clean["o"]))
+    for n in ("o", "q", "k", "v", "beta", "g"):
+        within(got[n][:, :first], *(t[:, :first] for t in clean[n]))
+        within(got[n][:, second + 1:], *(t[:, second + 1:] for t in clean[n]))
+    within(got["final"], *clean["state"])
+    within(got["state"], *clean["d_state"])
+    assert not got["o"][:, 700:second].isfinite().all()
 
 
 def test_refusals():

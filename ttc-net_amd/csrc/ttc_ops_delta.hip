@@ -1,6 +1,7 @@
 // ttc_ops_delta.hip -- the gated delta rule: token by token (single tokens of a serving batch, short inputs), sums over shared
 // heads, and the C entries (formulas: ttc_ops_delta.hpp).
 #include "ttc_ops_delta.hpp"
+#include "ttc_ops_mfma.hpp"
 
 namespace ttc {
 
@@ -158,6 +159,76 @@ int launch_tokens(const Tokens& A, bool bf16, hipStream_t s) {
                                                                      : go(delta_tokens_kernel<float, 4>);
 }
 
+// The states in front of the segments: S_{j+1} = M_j S_j + own_j from state_in on, or (BACK) R_{j-1} = M_j' R_j + own_j from the
+// last one.  A workgroup has 16 columns, a wave 16 rows of them; what a segment's reset drops has no effect, whatever it holds.
+template <int KD, bool BACK>
+__global__ __launch_bounds__(KD / 16 * 64) void delta_join_kernel(Delta A) {
+  using Op = Operand<__bf16>;
+  constexpr int DB = KD / 32, RS = KD + 4;
+  __shared__ __attribute__((aligned(16))) float Now[2][16 * RS];  // the state's columns, by rows of them
+  const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int blocks = A.vdp / 16, c = (int)(blockIdx.x % blocks) * 16 + n, r0 = wave * 16;
+  const int64_t bh = A.first + blockIdx.x / blocks;
+  auto segment = [&](int i) { return bh * A.segs + (BACK ? A.segs - 1 - i : i); };
+  float m[DB][8], own[4];
+  int dead = 0;
+  f32x4 now;
+  auto fetch = [&](int i) {
+    const float* p = A.seg_matrix + segment(i) * KD * KD;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        m[d][j] = BACK ? p[(32 * d + 8 * g + j) * KD + r0 + n] : p[(r0 + n) * KD + 32 * d + 8 * g + j];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) own[j] = A.seg_state[(segment(i) * KD + r0 + 4 * g + j) * A.vdp + c];
+    dead = A.seg_dead[segment(i)];
+  };
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int r = r0 + 4 * g + j;
+    now[j] = A.state_in && r < A.kd && c < A.vd ? A.state_in[(bh * A.kd + r) * A.vd + c] : 0.0f;
+  }
+  fetch(0);
+  for (int i = 0;; ++i) {
+    f32x4 next;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) next[j] = own[j];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) A.seg_state[(segment(i) * KD + r0 + 4 * g + j) * A.vdp + c] = now[j];
+    if (i + 1 == A.segs) break;
+    float* to = Now[i & 1];
+    *reinterpret_cast<f32x4*>(&to[n * RS + r0 + 4 * g]) = now;
+    __syncthreads();  // the next round writes the other buffer, and meets this barrier before it comes back to this one
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = to[n * RS + 32 * d + 8 * g + j];
+      sum = Op::mma(Op::wide(m[d]), Op::wide(x), sum);
+    }
+    const bool drop = dead != 0;
+    fetch(i + 1);
+    now = drop ? next : next + sum;
+  }
+}
+
+int launch_delta_join(const Delta& A, bool back, hipStream_t s) {
+  const int blocks = A.vdp / 16;
+  auto go = [&](auto kernel, int threads) {
+    return in_launches(A.B * A.H * blocks, threads, [&](int64_t first, dim3 grid) {
+      Delta P = A;
+      P.first = first / blocks;
+      hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, P);
+    }, blocks);
+  };
+  if (A.kd <= 32) return back ? go(delta_join_kernel<32, true>, 128) : go(delta_join_kernel<32, false>, 128);
+  if (A.kd <= 64) return back ? go(delta_join_kernel<64, true>, 256) : go(delta_join_kernel<64, false>, 256);
+  return back ? go(delta_join_kernel<128, true>, 512) : go(delta_join_kernel<128, false>, 512);
+}
+
 // Gradients of shared heads: out [B, T, heads / share, d] = sums over `share` heads of `in`, element (b, t, h, i) at
 // b sb + t st + h sh + i
 template <class T>
@@ -199,11 +270,21 @@ inline int delta_check(const ttc_delta_rule_args& A) {  // a token's share of wh
 }
 
 struct DeltaLayout {  // bytes from the start of `saved` (inverse to E) and of the workspace; `saved` lies in it where none is given
-  int64_t inverse, scores, rows, odd, S, E, kept;
-  int64_t R, dV, dq, dk, total;
-  int64_t chunks;
-  int vdp;
+  int64_t inverse, scores, rows, odd, S, E, seg_matrix, seg_dead, kept;
+  int64_t R, dV, dq, dk, seg_state, total;
+  int64_t chunks, seg_chunks;
+  int vdp, segs;
 };
+
+// Segments: enough workgroups to fill the GPU's 256 CUs twice, of at least 4 chunks each
+inline void segments_of(const ttc_delta_rule_args& A, DeltaLayout& W) {
+  const int64_t sweeps = A.batch * A.heads * (A.dv > 64 ? 2 : 1);
+  int64_t count = sweeps > 0 ? 512 / sweeps : 1;
+  if (count > W.chunks / 4) count = W.chunks / 4;
+  if (count < 2) count = 1;
+  W.seg_chunks = ceil_div(W.chunks > 0 ? W.chunks : 1, count);
+  W.segs = (int)ceil_div(W.chunks > 0 ? W.chunks : 1, W.seg_chunks);
+}
 
 inline DeltaLayout delta_layout(const ttc_delta_rule_args& A) {
   DeltaLayout W{};
@@ -217,23 +298,29 @@ inline DeltaLayout delta_layout(const ttc_delta_rule_args& A) {
   const int64_t C = chunk_tokens(bf16), tiles = C / 16 * (C / 16 + 1) / 2;
   W.chunks = ceil_div(A.tokens, C);
   W.vdp = padded(A.dv);
+  segments_of(A, W);
   const int64_t units = A.batch * A.heads * W.chunks, state = (int64_t)padded(A.dk) * W.vdp * 4, values = C * W.vdp * 4;
-  W.inverse = take(units * tiles * 1024);
-  W.scores = take(units * tiles * 1024);
+  const int64_t tile = bf16 ? 3 * 512 : 1024;  // values in three parts of 16 bits
+  W.inverse = take(units * tiles * tile);
+  W.scores = take(units * tiles * tile);
   W.rows = take(units * ROWS * C * 4);
   W.odd = take(units * 4);
   W.S = take(keep ? units * state : 0);
   W.E = take(keep ? units * values : 0);
+  const int64_t parts = W.segs > 1 ? A.batch * A.heads * W.segs : 0;
+  W.seg_matrix = take(parts * padded(A.dk) * padded(A.dk) * 4);
+  W.seg_dead = take(parts * 4);
   W.kept = at;
+  if (A.backward || A.saved) at = 0;
+  W.seg_state = take(parts * state);
   if (A.backward) {
-    at = 0;
     W.R = take(units * state);
     W.dV = take(units * values);
     W.dq = take(A.heads != A.q_heads && A.dq ? A.batch * A.tokens * A.heads * A.dk * 4 : 0);
     W.dk = take(A.heads != A.k_heads && A.dk_out ? A.batch * A.tokens * A.heads * A.dk * 4 : 0);
     W.total = at;
   } else {
-    W.total = A.saved || A.tokens <= ONE_BY_ONE ? 0 : at;
+    W.total = !A.saved && A.tokens <= ONE_BY_ONE ? 0 : at;
   }
   return W;
 }
@@ -345,8 +432,11 @@ extern "C" int ttc_delta_rule(const ttc_delta_rule_args* args, void* stream) {
   P.scale = (float)A.scale, P.eps = (float)A.eps;
   char *ws = static_cast<char*>(A.workspace), *kept = A.saved ? static_cast<char*>(A.saved) : ws;
   auto floats = [](char* p, int64_t at) { return reinterpret_cast<float*>(p + at); };
-  P.inverse = floats(kept, W.inverse), P.scores = floats(kept, W.scores), P.rows = floats(kept, W.rows);
+  P.inverse = kept + W.inverse, P.scores = kept + W.scores, P.rows = floats(kept, W.rows);
   P.odd = reinterpret_cast<int*>(kept + W.odd);
+  P.segs = W.segs, P.seg_chunks = W.seg_chunks;
+  P.seg_matrix = floats(kept, W.seg_matrix), P.seg_state = floats(ws, W.seg_state);
+  P.seg_dead = reinterpret_cast<int*>(kept + W.seg_dead);
   if (A.saved) P.S = floats(kept, W.S), P.E = floats(kept, W.E);
   int rc = TTC_LQR_OK;
   if (!A.backward) {

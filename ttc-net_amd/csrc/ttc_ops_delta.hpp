@@ -15,10 +15,11 @@
 namespace ttc {
 
 // What prepare leaves for each chunk of each head
-enum { IN, UP, BETA, RK, RQ, DEC, HI, LO, PART, ROWS };  // C values each:
+enum { IN, UP, BETA, RK, RQ, DEC, HI, LO, PART, WK, WU, WQ, ROWS };  // C values each:
 // IN    e^{G_t}, 0 behind a reset                  UP    e^{G_C - G_t}, 0 in front of one
 // RK    1 / |k_t| (1 unless keys are normalised)   RQ    1 / |q_t|
 // DEC   e^{g_t}, -1 at a reset                     PART  resets so far
+// WK    IN RK      WU  UP RK b      WQ  IN RQ scale
 // HI, LO  the two parts of log2(e) G_t, whose sum starts anew at a reset; infinite where it is lost (a NaN, growth beyond e^128)
 
 struct Delta {
@@ -34,10 +35,16 @@ struct Delta {
   float* state_out;
   void* o;
   // [B, H, chunks, ...]
-  float *inverse, *scores;  // lower triangles of 16 x 16 tiles (the diagonal ones whole): (I + N b)^-1, P b
+  void *inverse, *scores;   // lower triangles of 16 x 16 tiles (the diagonal ones whole), each in its parts: (I + N b)^-1, P b
   float* rows;              // [ROWS, C]
   int* odd;                 // keys or inverse not finite
   float *S, *R;             // [KD, vdp]: states in front of the chunks, gradients behind them (NULL: not kept)
+  // Where heads are few their chunks are split into `segs` segments of seg_chunks (1: not split), [B, H, segs, ...]:
+  float* seg_state;         // [KD, vdp]: a segment's own part of the state behind it, then the state in front of it
+  float* seg_matrix;        // [KD, KD]: what becomes of the state in front of it (its transpose: of the gradient behind it)
+  int* seg_dead;            // nothing does, whatever it holds: a reset lies between
+  int segs;
+  int64_t seg_chunks;
   float *E, *dV;            // [C, vdp]
   // outputs of the gradients' kernel; fp32 for heads that share
   void *dq, *dk, *dv, *dgamma, *dbeta;
@@ -51,5 +58,7 @@ int launch_delta_kd64(const Delta& A, int what, hipStream_t s);
 template <class T>
 int launch_delta_kd128(const Delta& A, int what, hipStream_t s);
 enum { PREPARE, SWEEP, SWEEP_BACK, GRADIENTS };
+
+int launch_delta_join(const Delta& A, bool back, hipStream_t s);
 
 }  // namespace ttc

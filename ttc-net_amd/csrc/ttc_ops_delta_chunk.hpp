@@ -160,12 +160,18 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(Delta A) {
       qq = 1.0f / sqrtf(lane_sum(qq, SUB) + A.eps);
     }
     if (sub == 0) {
-      Row[RK][row] = row < left ? kk : 0.0f;
-      Row[RQ][row] = row < left ? qq : 0.0f;
+      const bool here = row < left;
+      const float in = Row[IN][row], up = Row[UP][row];
+      Row[RK][row] = here ? kk : 0.0f;
+      Row[RQ][row] = here ? qq : 0.0f;
+      Row[WK][row] = here ? kept(in, kk) : 0.0f;
+      Row[WU][row] = here ? kept(up, kk * Row[BETA][row]) : 0.0f;
+      Row[WQ][row] = here ? kept(in, qq * A.scale) : 0.0f;
     }
   }
   __syncthreads();
-  const int64_t tiles_at = unit * Z::TILES * 256;
+  constexpr int PLANE = Z::TILES * 256;
+  T *scores = static_cast<T*>(A.scores) + unit * Op::WIDE_PARTS * PLANE, *inverse = static_cast<T*>(A.inverse) + unit * Op::WIDE_PARTS * PLANE;
   for (int i = tid; i < ROWS * C / 4; i += 256)
     reinterpret_cast<f32x4*>(A.rows + unit * ROWS * C)[i] = reinterpret_cast<const f32x4*>(&Row[0][0])[i];
   int turn = 0;
@@ -191,7 +197,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(Delta A) {
         qk[i] = s + i <= t ? kept(w, qk[i] * rq * by) : 0.0f;
       }
       *reinterpret_cast<f32x4*>(&Lm[t * LS + s]) = kk;
-      *reinterpret_cast<f32x4*>(A.scores + tiles_at + tile_of(ti, si) * 256 + n * 16 + 4 * g) = qk;
+      Op::put_wide(scores + tile_of(ti, si) * 256 + n * 16 + 4 * g, PLANE, qk);
     }
   __syncthreads();
   // the diagonal blocks' inverses: a lane's column by forward substitution
@@ -242,7 +248,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(Delta A) {
       if (tile_of(ti, si) % 4 != wave) continue;
       const f32x4 x = *reinterpret_cast<const f32x4*>(&Tm[(16 * ti + n) * LS + 16 * si + 4 * g]);
       ok = ok && all_finite(x);
-      *reinterpret_cast<f32x4*>(A.inverse + tiles_at + tile_of(ti, si) * 256 + n * 16 + 4 * g) = x;
+      Op::put_wide(inverse + tile_of(ti, si) * 256 + n * 16 + 4 * g, PLANE, x);
     }
   const bool bad = __ballot(!ok) != 0;
   if (lane == 0) Odd[wave] |= bad;
@@ -252,7 +258,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(Delta A) {
 
 // ---- sweeps ----------------------------------------------------------------------------------------------------
 
-// Lower triangle of tiles in memory as operands.  ROW: row 16 t + n, columns 32 s + 4 g .. and 16 + 4 g ..; otherwise its
+// Lower triangle of tiles in shared memory as operands.  ROW: row 16 t + n, columns 32 s + 4 g .. and 16 + 4 g ..; otherwise its
 // transpose's: column 16 t + n, rows 32 s + ...
 template <bool ROW, int TT>
 __device__ __forceinline__ void triangle(const float* tiles, int t, int s, int lane, float (&x)[8]) {
@@ -280,7 +286,9 @@ __device__ __forceinline__ void eight(const f32x4& a, const f32x4& b, float (&x)
   for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
 }
 
-template <class T, int KD, int WAVES, int ET, bool BACK>
+// A segment's chunks.  STATE: nothing but the state behind them, of nothing in front; forwards also, by further workgroups, of the
+// unit matrix in front and no values.
+template <class T, int KD, int WAVES, int ET, bool BACK, bool STATE>
 __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
   using Z = DeltaShape<T, KD>;
   using Op = Operand<T>;
@@ -289,12 +297,18 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
   constexpr int C = Z::C, TT = Z::TT, KB = Z::KB, NT = WAVES * 64, COLS = 16 * ET * WAVES, QS = BACK ? Z::KS : Z::QS, KS = Z::KS,
                 VS = COLS + Op::COL_PAD;
   __shared__ __attribute__((aligned(16))) T Ks[C * KS], Qs[C * QS], Vs[C * VS];  // Vs: V, or dO
+  // the inverse's and the scores' tiles in parts; 16 digits of the scores are enough for outputs
+  constexpr int PLANE = Z::TILES * 256, PARTS = Op::WIDE_PARTS, USED = BACK || PARTS == 1 ? PARTS : 2;
+  __shared__ __attribute__((aligned(16))) T inverse[PARTS * PLANE], scores[USED * PLANE];
   __shared__ __attribute__((aligned(16))) float Row[ROWS][C];
   int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int lane = tid & 63, g = lane >> 4, n = lane & 15;
-  const int c0 = (int)(blockIdx.x % A.colblocks) * COLS, e0 = wave * 16 * ET;  // the workgroup's columns, the wave's of those
-  const int64_t bh = A.first + blockIdx.x / A.colblocks, b = bh / A.H;
+  const int blocks = STATE && !BACK ? A.colblocks + (KD + COLS - 1) / COLS : A.colblocks, block = (int)(blockIdx.x % blocks);
+  const bool matrix = STATE && !BACK && block >= A.colblocks;
+  const int c0 = (matrix ? block - A.colblocks : block) * COLS, e0 = wave * 16 * ET;  // the workgroup's columns, the wave's of those
+  const int64_t part = A.first + blockIdx.x / blocks, bh = part / A.segs, b = bh / A.H;
+  const int seg = (int)(part % A.segs);
   const int h = (int)(bh % A.H);
   const T *q = A.q.at<T>(b, h), *k = A.k.at<T>(b, h), *v = (BACK ? A.d_o : A.v).at<T>(b, h) + c0;
   const int64_t vst = BACK ? A.d_o.st : A.v.st;
@@ -311,42 +325,59 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) S[d][e][i] = f((float)S[d][e][i], 16 * d + r + i, c + 16 * e);
   };
-  {
-    const float* p = A.state_in ? A.state_in + bh * A.kd * A.vd : nullptr;
-    const auto from = bounded(p, p ? A.kd * A.vd * 4 : 0);
+  float* const seg_state = A.segs > 1 ? A.seg_state + part * KD * A.vdp : nullptr;
+  if constexpr (STATE) {
+    each([&](float, int r, int c) { return matrix && r == c ? 1.0f : 0.0f; });
+  } else {
+    const float* p = A.segs > 1 ? seg_state : A.state_in ? A.state_in + bh * A.kd * A.vd : nullptr;
+    const int rows = A.segs > 1 ? KD : A.kd, cols = A.segs > 1 ? A.vdp : A.vd;
+    const auto from = bounded(p, p ? rows * cols * 4 : 0);
     each([&](float, int r, int c) {
       return __builtin_bit_cast(
-          float, __builtin_amdgcn_raw_buffer_load_b32(from, r < A.kd && c < A.vd ? (r * A.vd + c) * 4 : BEYOND, 0, 0));
+          float, __builtin_amdgcn_raw_buffer_load_b32(from, r < rows && c < cols ? (r * cols + c) * 4 : BEYOND, 0, 0));
     });
   }
   Stage<T, KD, C, NT> kr, qr;
   Stage<T, COLS, C, NT> vr;
   Stage<float, C, ROWS, NT> rr;
-  auto chunk_of = [&](int64_t i) { return BACK ? A.chunks - 1 - i : i; };
+  Stage<T, 256, PARTS * Z::TILES, NT> ir;
+  Stage<T, 256, USED * Z::TILES, NT> sr;
+  int odd_next = 0;
+  const int64_t begin = seg * A.seg_chunks, end = begin + A.seg_chunks < A.chunks ? begin + A.seg_chunks : A.chunks;
+  auto chunk_of = [&](int64_t i) { return BACK ? end - 1 - i : begin + i; };
   auto fetch = [&](int64_t i) {
     const int64_t ch = chunk_of(i), t0 = ch * C;
     const int left = A.T - t0 < C ? (int)(A.T - t0) : C;
     kr.fetch(k + t0 * A.k.st, A.k.st, A.kd, left, A.wide_k, tid);
-    qr.fetch(q + t0 * A.q.st, A.q.st, A.kd, left, A.wide_q, tid);
-    vr.fetch(v + t0 * vst, vst, A.vd - c0, left, wide_v, tid);
-    rr.fetch(A.rows + (bh * A.chunks + ch) * ROWS * C, C, C, ROWS, true, tid);
+    if constexpr (BACK || !STATE) qr.fetch(q + t0 * A.q.st, A.q.st, A.kd, left, A.wide_q, tid);
+    if (matrix) vr.fetch(q, 1, 0, 0, true, tid);  // zeros
+    else vr.fetch(v + t0 * vst, vst, A.vd - c0, left, wide_v, tid);
+    const int64_t unit = bh * A.chunks + ch;
+    rr.fetch(A.rows + unit * ROWS * C, C, C, ROWS, true, tid);
+    ir.fetch(static_cast<const T*>(A.inverse) + unit * PARTS * PLANE, 256, 256, PARTS * Z::TILES, true, tid);
+    if constexpr (BACK || !STATE)
+      sr.fetch(static_cast<const T*>(A.scores) + unit * PARTS * PLANE, 256, 256, USED * Z::TILES, true, tid);
+    odd_next = A.odd[unit];
   };
   fetch(0);
-  for (int64_t i = 0; i < A.chunks; ++i) {
+  bool dead = false;
+  for (int64_t i = 0; i < end - begin; ++i) {
     asm volatile("" : "+v"(lane), "+v"(tid));
     g = lane >> 4, n = lane & 15;
     const int64_t ch = chunk_of(i), t0 = ch * C, unit = bh * A.chunks + ch;
     const int left = A.T - t0 < C ? (int)(A.T - t0) : C;
     kr.template put<KS>(Ks, tid);
-    qr.template put<QS>(Qs, tid);
+    if constexpr (BACK || !STATE) qr.template put<QS>(Qs, tid);
     vr.template put<VS>(Vs, tid);
     rr.template put<C>(&Row[0][0], tid);
+    ir.template put<256>(inverse, tid);
+    if constexpr (BACK || !STATE) sr.template put<256>(scores, tid);
+    bool odd = odd_next != 0;
     __syncthreads();
-    const float *inverse = A.inverse + unit * Z::TILES * 256, *scores = A.scores + unit * Z::TILES * 256;
-    bool odd = A.odd[unit] != 0;
-    if (i + 1 < A.chunks) fetch(i + 1);
+    if (i + 1 < end - begin) fetch(i + 1);
     const float whole = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(Row[IN][C - 1])));
-    float* kept_state = BACK ? A.R : A.S;
+    dead = dead || Row[PART][C - 1] > 0.0f;
+    float* kept_state = STATE ? nullptr : BACK ? A.R : A.S;
     if (kept_state) {
       float* p = kept_state + unit * KD * A.vdp;
       each([&](float s, int r, int c) {
@@ -357,13 +388,13 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
     auto row4 = [&](int which, int t) { return *reinterpret_cast<const f32x4*>(&Row[which][t]); };  // of 4 neighbouring tokens
 
     // X = K S: lane's tokens 16 t + 4 g + i, columns e0 + 16 e + n.  Forward's O' = S' Q': lane's token n, 4 columns
-    f32x4 X[TT][ET], O[BACK ? 1 : TT][ET];
+    f32x4 X[TT][ET], O[BACK || STATE ? 1 : TT][ET];
 #pragma unroll
     for (int t = 0; t < TT; ++t)
 #pragma unroll
       for (int e = 0; e < ET; ++e) {
         X[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if constexpr (!BACK) O[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (!BACK && !STATE) O[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
 #pragma unroll
     for (int d = 0; d < Z::DB; ++d) {
@@ -379,7 +410,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
         const Frag f = Op::row_split(&Ks[(16 * t + n) * KS + 32 * d + 4 * g]);
 #pragma unroll
         for (int e = 0; e < ET; ++e) X[t][e] = Op::mma(f, s[e], X[t][e]);
-        if constexpr (!BACK) {
+        if constexpr (!BACK && !STATE) {
           const Frag w = Op::row_split(&Qs[(16 * t + n) * QS + 32 * d + 4 * g]);
 #pragma unroll
           for (int e = 0; e < ET; ++e) O[t][e] = Op::mma(Op::first(s[e]), w, O[t][e]);
@@ -394,21 +425,21 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
       for (int e = 0; e < ET; ++e) vf[s][e] = Op::column(&Vs[32 * s * VS], VS, e0 + 16 * e, lane);
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
-      const f32x4 w = row4(BACK ? UP : IN, 16 * t + 4 * g), rk = row4(RK, 16 * t + 4 * g), be = row4(BETA, 16 * t + 4 * g);
+      // A weight of 0 does not select here: where the state is not finite, X is not, and the tokens go one by one below
+      const f32x4 w = row4(BACK ? WU : WK, 16 * t + 4 * g);
 #pragma unroll
       for (int e = 0; e < ET; ++e) {
         float y[8];
         if constexpr (!BACK) Op::values(vf[t / 2][e], y);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          X[t][e][j] = BACK ? kept(w[j], rk[j] * be[j] * X[t][e][j]) : y[t % 2 * 4 + j] - kept(w[j], rk[j] * X[t][e][j]);
+          X[t][e][j] = BACK ? w[j] * X[t][e][j] : fmaf(-w[j], X[t][e][j], y[t % 2 * 4 + j]);
       }
       if constexpr (BACK) {
 #pragma unroll
         for (int s = t / 2; s < KB; ++s) {
-          float y[8];
-          triangle<false, TT>(scores, t, s, lane, y);
-          const Wide f = Op::wide(y);
+          const Wide f = Op::template wide_tiles<false>(s * 2 >= t ? scores + tile_of(2 * s, t) * 256 : nullptr,
+                                                        scores + tile_of(2 * s + 1, t) * 256, PLANE, lane);
 #pragma unroll
           for (int e = 0; e < ET; ++e) X[t][e] = Op::mma(f, vf[s][e], X[t][e]);
         }
@@ -432,9 +463,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
         for (int e = 0; e < ET; ++e) E[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = BACK ? t / 2 : 0; s < (BACK ? KB : t / 2 + 1); ++s) {
-          float x[8];
-          triangle<!BACK, TT>(inverse, t, s, lane, x);
-          const Wide f = Op::wide(x);
+          // row tiles of the lower triangle, or (BACK) its columns'
+          const T *a = BACK ? 2 * s >= t ? inverse + tile_of(2 * s, t) * 256 : nullptr : inverse + tile_of(t, 2 * s) * 256,
+                  *c = BACK ? inverse + tile_of(2 * s + 1, t) * 256 : 2 * s < t ? inverse + tile_of(t, 2 * s + 1) * 256 : nullptr;
+          const Wide f = Op::template wide_tiles<!BACK>(a, c, PLANE, lane);
 #pragma unroll
           for (int e = 0; e < ET; ++e) E[t][e] = Op::mma(f, y[s][e], E[t][e]);
         }
@@ -446,7 +478,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
 #pragma unroll
       for (int e = 0; e < ET; ++e) fine = fine && all_finite(E[t][e]);
     odd = odd || __ballot(!fine) != 0;
-    float* kept_rows = (BACK ? A.dV : A.E) ? (BACK ? A.dV : A.E) + unit * C * A.vdp + c0 + e0 : nullptr;
+    float* const all_rows = STATE ? nullptr : BACK ? A.dV : A.E;
+    float* const kept_rows = all_rows ? all_rows + unit * C * A.vdp + c0 + e0 : nullptr;
     const int64_t first = ((b * A.T + t0) * A.H + h) * A.vd;  // of the output
     const int row = A.H * A.vd;
     if (!odd) {
@@ -458,7 +491,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) kept_rows[(16 * t + 4 * g + j) * A.vdp + 16 * e + n] = E[t][e][j];
       }
-      if constexpr (!BACK) {
+      if constexpr (!BACK && !STATE) {
         typename Op::Pair y[KB][ET];
 #pragma unroll
         for (int s = 0; s < KB; ++s)
@@ -470,16 +503,13 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
           }
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
-          const float w = Row[IN][16 * t + n], rq = Row[RQ][16 * t + n] * A.scale;
+          const float w = Row[WQ][16 * t + n];
 #pragma unroll
-          for (int e = 0; e < ET; ++e)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) O[t][e][j] = kept(w, rq * O[t][e][j]);
+          for (int e = 0; e < ET; ++e) O[t][e] *= w;
 #pragma unroll
           for (int s = 0; s <= t / 2; ++s) {
-            float x[8];
-            triangle<true, TT>(scores, t, s, lane, x);
-            const typename Op::Pair f = Op::pair(x);
+            const typename Op::Pair f = Op::template pair_tiles<true>(
+                scores + tile_of(t, 2 * s) * 256, 2 * s < t ? scores + tile_of(t, 2 * s + 1) * 256 : nullptr, PLANE, lane);
 #pragma unroll
             for (int e = 0; e < ET; ++e) O[t][e] = Op::mma(y[s][e], f, O[t][e]);
           }
@@ -509,30 +539,22 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
 #pragma unroll
       for (int d = 0; d < Z::DT; ++d)
 #pragma unroll
-        for (int e = 0; e < ET; ++e) S[d][e] = whole == 0.0f ? f32x4{0.f, 0.f, 0.f, 0.f} : S[d][e] * whole;
+        for (int e = 0; e < ET; ++e) S[d][e] *= whole;
 #pragma unroll
       for (int s = 0; s < KB; ++s) {
         Wide we[ET], wd[BACK ? ET : 1];
-        float w[8], wq[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int t = 32 * s + (j < 4 ? 0 : 16) + 4 * g + j % 4;
-          const float rk = Row[RK][t];
-          w[j] = BACK ? -rk : rk * Row[BETA][t];
-          wq[j] = Row[RQ][t] * A.scale;
-        }
-        const f32x4 ua = row4(BACK ? IN : UP, 32 * s + 4 * g), ub = row4(BACK ? IN : UP, 32 * s + 16 + 4 * g);
+        const f32x4 wa = row4(BACK ? WK : WU, 32 * s + 4 * g), wb = row4(BACK ? WK : WU, 32 * s + 16 + 4 * g);
+        const f32x4 qa = row4(WQ, 32 * s + 4 * g), qb = row4(WQ, 32 * s + 16 + 4 * g);
 #pragma unroll
         for (int e = 0; e < ET; ++e) {
           float x[8];
-          eight(E[2 * s][e], E[2 * s + 1][e], x);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = kept(j < 4 ? ua[j % 4] : ub[j % 4], w[j] * x[j]);
+          if constexpr (BACK) eight(E[2 * s][e] * -wa, E[2 * s + 1][e] * -wb, x);
+          else eight(E[2 * s][e] * wa, E[2 * s + 1][e] * wb, x);
           we[e] = Op::wide(x);
           if constexpr (BACK) {
             Op::values(vf[s][e], x);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = kept(j < 4 ? ua[j % 4] : ub[j % 4], wq[j] * x[j]);
+            for (int j = 0; j < 8; ++j) x[j] *= j < 4 ? qa[j % 4] : qb[j % 4];
             wd[e] = Op::wide(x);
           }
         }
@@ -561,7 +583,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int r = 16 * d + 4 * g + j;
-            const float kk = to_f(Ks[t * KS + r]), qq = to_f(Qs[t * QS + r]);
+            const float kk = to_f(Ks[t * KS + r]), qq = STATE && !BACK ? 0.0f : to_f(Qs[t * QS + r]);
 #pragma unroll
             for (int e = 0; e < ET; ++e) {
               S[d][e][j] = BACK ? fmaf(rq * qq, in[e], S[d][e][j]) : decay(S[d][e][j]);
@@ -580,7 +602,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int r = 16 * d + 4 * g + j;
-            const float kk = to_f(Ks[t * KS + r]), qq = to_f(Qs[t * QS + r]);
+            const float kk = to_f(Ks[t * KS + r]), qq = STATE && !BACK ? 0.0f : to_f(Qs[t * QS + r]);
 #pragma unroll
             for (int e = 0; e < ET; ++e) {
               if constexpr (BACK) {
@@ -591,7 +613,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
               }
             }
           }
-        if constexpr (!BACK) {
+        if constexpr (!BACK && !STATE) {
 #pragma unroll
           for (int e = 0; e < ET; ++e) {
             o[e] += __shfl_xor(o[e], 16, 64);
@@ -610,7 +632,15 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
     }
     __syncthreads();
   }
-  if (A.state_out) {
+  if constexpr (STATE) {
+    float* p = matrix ? A.seg_matrix + part * KD * KD : seg_state;
+    const int cols = matrix ? KD : A.vdp;
+    each([&](float s, int r, int c) {
+      if (c < cols) p[r * cols + c] = s;
+      return s;
+    });
+    if (matrix && c0 == 0 && tid == 0) A.seg_dead[part] = dead;
+  } else if (A.state_out && seg == (BACK ? 0 : A.segs - 1)) {
     float* p = A.state_out + bh * A.kd * A.vd;
     const auto to = bounded(p, A.kd * A.vd * 4);
     each([&](float s, int r, int c) {
@@ -943,14 +973,25 @@ __global__ __launch_bounds__((KD / 16 * 64), 2) void delta_gradients_kernel(Delt
 
 // ---- launches --------------------------------------------------------------------------------------------------
 
+template <class T, int KD, int WAVES, int ET, bool BACK, bool STATE>
+int launch_delta_part(const Delta& A, hipStream_t s) {
+  constexpr int COLS = 16 * ET * WAVES;
+  Delta P = A;
+  P.colblocks = (int)ceil_div(A.vd, COLS);
+  const int blocks = STATE && !BACK ? P.colblocks + (KD + COLS - 1) / COLS : P.colblocks;
+  return in_launches(A.B * A.H * A.segs * blocks, WAVES * 64, [&](int64_t first, dim3 grid) {
+    P.first = first / blocks;
+    hipLaunchKernelGGL((delta_sweep_kernel<T, KD, WAVES, ET, BACK, STATE>), grid, dim3(WAVES * 64), 0, s, P);
+  }, blocks);
+}
+
 template <class T, int KD, int WAVES, int ET, bool BACK>
 int launch_delta_sweep(const Delta& A, hipStream_t s) {
-  Delta P = A;
-  P.colblocks = (int)ceil_div(A.vd, 16 * ET * WAVES);
-  return in_launches(A.B * A.H * P.colblocks, WAVES * 64, [&](int64_t first, dim3 grid) {
-    P.first = first / P.colblocks;
-    hipLaunchKernelGGL((delta_sweep_kernel<T, KD, WAVES, ET, BACK>), grid, dim3(WAVES * 64), 0, s, P);
-  }, P.colblocks);
+  if (A.segs > 1) {
+    if (const int rc = launch_delta_part<T, KD, WAVES, ET, BACK, true>(A, s)) return rc;
+    if (const int rc = launch_delta_join(A, BACK, s)) return rc;
+  }
+  return launch_delta_part<T, KD, WAVES, ET, BACK, false>(A, s);
 }
 
 template <class T, int KD, bool BACK>

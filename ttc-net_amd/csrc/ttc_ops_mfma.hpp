@@ -101,6 +101,37 @@ struct Operand<__bf16> {
     return Pair{both(p), both(p + part)};
   }
   static __device__ __forceinline__ float score(const __bf16* p, int part) { return to_f(p[0]) + to_f(p[part]); }
+  // Values in memory as their three parts (WIDE_PARTS such arrays, `part` elements apart): 4 neighbours put at p, and two
+  // 16 x 16 tiles as an operand (NULL: zeros): rows n of both, or of their transposes, 24 or (first) 16 digits of them
+  static constexpr int WIDE_PARTS = 3;
+  static __device__ __forceinline__ void put_wide(__bf16* p, int part, f32x4 x) {
+    float d[4], e[4];
+    const u32x2 h = {cut(x[0], x[1], d[0], d[1]), cut(x[2], x[3], d[2], d[3])};
+    const u32x2 m = {cut(d[0], d[1], e[0], e[1]), cut(d[2], d[3], e[2], e[3])};
+    *reinterpret_cast<u32x2*>(p) = h;
+    *reinterpret_cast<u32x2*>(p + part) = m;
+    *reinterpret_cast<bf16x4*>(p + 2 * part) = bf16x4{(__bf16)e[0], (__bf16)e[1], (__bf16)e[2], (__bf16)e[3]};
+  }
+  template <bool ROW>
+  static __device__ __forceinline__ Frag tiles(const __bf16* a, const __bf16* b, int lane) {
+    const int g = lane >> 4, i = lane & 15;
+    typedef __attribute__((address_space(3))) i16x4 lds;
+    auto one = [&](const __bf16* p) {
+      if (ROW) return *reinterpret_cast<const i16x4*>(p + i * 16 + 4 * g);
+      return (i16x4)__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)(p + (4 * g + (i >> 2)) * 16 + (i & 3) * 4));
+    };
+    const i16x4 x = a ? one(a) : i16x4{0, 0, 0, 0}, y = b ? one(b) : i16x4{0, 0, 0, 0};
+    return __builtin_bit_cast(Frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  template <bool ROW>
+  static __device__ __forceinline__ Wide wide_tiles(const __bf16* a, const __bf16* b, int part, int lane) {
+    auto at = [&](const __bf16* p, int i) { return p ? p + i * part : nullptr; };
+    return Wide{tiles<ROW>(a, b, lane), tiles<ROW>(at(a, 1), at(b, 1), lane), tiles<ROW>(at(a, 2), at(b, 2), lane)};
+  }
+  template <bool ROW>
+  static __device__ __forceinline__ Pair pair_tiles(const __bf16* a, const __bf16* b, int part, int lane) {
+    return Pair{tiles<ROW>(a, b, lane), tiles<ROW>(a ? a + part : a, b ? b + part : b, lane)};
+  }
   static __device__ __forceinline__ Wide wide(const float (&x)[8]) {
     u32x4 h, m, l;
 #pragma unroll
@@ -175,6 +206,24 @@ struct Operand<float> {
     return Frag{{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
   }
   static __device__ __forceinline__ float score(const float* p, int) { return p[0]; }
+  static constexpr int WIDE_PARTS = 1;
+  static __device__ __forceinline__ void put_wide(float* p, int, f32x4 x) { *reinterpret_cast<f32x4*>(p) = x; }
+  template <bool ROW>
+  static __device__ __forceinline__ Frag wide_tiles(const float* a, const float* b, int, int lane) {
+    const int g = lane >> 4, n = lane & 15;
+    Frag r;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int at = ROW ? n * 16 + 4 * g + j : (4 * g + j) * 16 + n;
+      r.v[j] = a ? a[at] : 0.0f;
+      r.v[4 + j] = b ? b[at] : 0.0f;
+    }
+    return r;
+  }
+  template <bool ROW>
+  static __device__ __forceinline__ Frag pair_tiles(const float* a, const float* b, int part, int lane) {
+    return wide_tiles<ROW>(a, b, part, lane);
+  }
   static __device__ __forceinline__ Frag wide(const float (&x)[8]) {
     Frag r;
 #pragma unroll
