@@ -1,6 +1,6 @@
 // ttc_ops_delta_chunk.hpp -- the gated delta rule in chunks on the matrix cores (formulas: ttc_ops_delta.hpp).
 //
-// A sweep's wave holds 16 ET columns of the state in registers, all rows, and needs nothing of the other waves: the columns of
+// A sweep's wave holds 16 columns of the state in registers, all rows, and needs nothing of the other waves: the columns of
 // S, E, O, R and dV never meet.  Products are laid out so that no accumulator moves before it is an operand:
 //   K S         lane: column n, 4 neighbouring tokens       -> with V, rows of the next product's right side
 //   E = T Y     T's rows straight from memory as operands; E as it lies in the accumulators is the next right side
@@ -57,6 +57,14 @@ struct Stage {
       if (C * D / VEC % NT == 0 || row < C) *reinterpret_cast<u32x4*>(&to[row * STRIDE + c]) = r[j];
     }
   }
+  template <int STRIDE>
+  __device__ __forceinline__ void put_mixed(T* to, int tid) const {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int i = tid + j * NT, row = i / (D / VEC), c = i % (D / VEC) * VEC;
+      if (C * D / VEC % NT == 0 || row < C) Operand<T>::put_mixed(to, row, c, STRIDE, r[j]);
+    }
+  }
   __device__ __forceinline__ void largest(uint32_t& m) const {
 #pragma unroll
     for (int j = 0; j < N; ++j) Operand<T>::largest(r[j], m);
@@ -75,11 +83,36 @@ __device__ __forceinline__ float weight_of(const Place& t, const Place& s) {
   return t.part == s.part ? exp2_of((t.hi - s.hi) + (t.lo - s.lo)) : 0.0f;
 }
 
-__device__ __forceinline__ bool all_finite(const f32x4& x) {
-  bool ok = true;
+// m + 0 x: a sum that starts at 0 ends there only if all that it met is finite
+__device__ __forceinline__ float met(float m, const f32x4& x) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) ok = ok && (__float_as_uint(x[i]) & 0x7f800000u) != 0x7f800000u;
-  return ok;
+  for (int i = 0; i < 4; ++i) m = fmaf(x[i], 0.0f, m);
+  return m;
+}
+
+// c[i] += a[i] b, or b a[i], for i in [LO, HI): instructions of the different sums in turn
+template <class Op, int LO, int HI, int N, class A, class B, int M>
+__device__ __forceinline__ void mma_left(const A (&a)[N], const B& b, f32x4 (&c)[M]) {
+#pragma unroll
+  for (int p = 0; p < Op::steps((const A*)nullptr, (const B*)nullptr); ++p)
+#pragma unroll
+    for (int i = LO; i < HI; ++i) c[i] = Op::step(p, a[i], b, c[i]);
+}
+template <class Op, int LO, int HI, int N, class A, class B, int M>
+__device__ __forceinline__ void mma_right(const B& b, const A (&a)[N], f32x4 (&c)[M]) {
+#pragma unroll
+  for (int p = 0; p < Op::steps((const B*)nullptr, (const A*)nullptr); ++p)
+#pragma unroll
+    for (int i = LO; i < HI; ++i) c[i] = Op::step(p, b, a[i], c[i]);
+}
+
+// f(0), ..., f(N - 1) of constants
+template <int N, class F>
+__device__ __forceinline__ void unrolled(F f) {
+  if constexpr (N > 0) {
+    unrolled<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+  }
 }
 
 // ---- prepare: decays, lengths, scores and the triangle's inverse, one workgroup a chunk ----------------------------
@@ -197,7 +230,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(Delta A) {
         qk[i] = s + i <= t ? kept(w, qk[i] * rq * by) : 0.0f;
       }
       *reinterpret_cast<f32x4*>(&Lm[t * LS + s]) = kk;
-      Op::put_wide(scores + tile_of(ti, si) * 256 + n * 16 + 4 * g, PLANE, qk);
+      Op::put_wide(scores + tile_of(ti, si) * 256 + Op::tile_at(n, 4 * g), PLANE, qk);
     }
   __syncthreads();
   // the diagonal blocks' inverses: a lane's column by forward substitution
@@ -240,17 +273,17 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(Delta A) {
     put(2 + r, c, x, -1.0f);
   }
   __syncthreads();
-  bool ok = true;
+  float all = 0.0f;
 #pragma unroll
   for (int ti = 0; ti < TT; ++ti)
 #pragma unroll
     for (int si = 0; si <= ti; ++si) {
       if (tile_of(ti, si) % 4 != wave) continue;
       const f32x4 x = *reinterpret_cast<const f32x4*>(&Tm[(16 * ti + n) * LS + 16 * si + 4 * g]);
-      ok = ok && all_finite(x);
-      Op::put_wide(inverse + tile_of(ti, si) * 256 + n * 16 + 4 * g, PLANE, x);
+      all = met(all, x);
+      Op::put_wide(inverse + tile_of(ti, si) * 256 + Op::tile_at(n, 4 * g), PLANE, x);
     }
-  const bool bad = __ballot(!ok) != 0;
+  const bool bad = __ballot(all != 0.0f) != 0;
   if (lane == 0) Odd[wave] |= bad;
   __syncthreads();
   if (tid == 0) A.odd[unit] = Odd[0] | Odd[1] | Odd[2] | Odd[3];
@@ -288,15 +321,15 @@ __device__ __forceinline__ void eight(const f32x4& a, const f32x4& b, float (&x)
 
 // A segment's chunks.  STATE: nothing but the state behind them, of nothing in front; forwards also, by further workgroups, of the
 // unit matrix in front and no values.
-template <class T, int KD, int WAVES, int ET, bool BACK, bool STATE>
+template <class T, int KD, int WAVES, bool BACK, bool STATE>
 __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
   using Z = DeltaShape<T, KD>;
   using Op = Operand<T>;
   using Wide = typename Op::Wide;
   using Frag = typename Op::Frag;
-  constexpr int C = Z::C, TT = Z::TT, KB = Z::KB, NT = WAVES * 64, COLS = 16 * ET * WAVES, QS = BACK ? Z::KS : Z::QS, KS = Z::KS,
+  constexpr int C = Z::C, TT = Z::TT, KB = Z::KB, NT = WAVES * 64, COLS = 16 * WAVES, KS = Z::KS,
                 VS = COLS + Op::COL_PAD;
-  __shared__ __attribute__((aligned(16))) T Ks[C * KS], Qs[C * QS], Vs[C * VS];  // Vs: V, or dO
+  __shared__ __attribute__((aligned(16))) T Ks[C * KS], Qs[C * KS], Vs[C * VS];  // Vs: V, or dO
   // the inverse's and the scores' tiles in parts; 16 digits of the scores are enough for outputs
   constexpr int PLANE = Z::TILES * 256, PARTS = Op::WIDE_PARTS, USED = BACK || PARTS == 1 ? PARTS : 2;
   __shared__ __attribute__((aligned(16))) T inverse[PARTS * PLANE], scores[USED * PLANE];
@@ -304,26 +337,28 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
   int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int lane = tid & 63, g = lane >> 4, n = lane & 15;
-  const int blocks = STATE && !BACK ? A.colblocks + (KD + COLS - 1) / COLS : A.colblocks, block = (int)(blockIdx.x % blocks);
+  // Workgroup numbers go round the 8 XCDs: a segment's column blocks, which read the same keys, on one of them (its L2)
+  const int blocks = STATE && !BACK ? A.colblocks + (KD + COLS - 1) / COLS : A.colblocks;
+  const unsigned round = blockIdx.x / (8 * blocks), whole_rounds = gridDim.x / (8 * blocks), in_round = blockIdx.x % (8 * blocks);
+  const bool spread = round < whole_rounds;
+  const int block = (int)(spread ? in_round / 8 : in_round % blocks);
   const bool matrix = STATE && !BACK && block >= A.colblocks;
-  const int c0 = (matrix ? block - A.colblocks : block) * COLS, e0 = wave * 16 * ET;  // the workgroup's columns, the wave's of those
-  const int64_t part = A.first + blockIdx.x / blocks, bh = part / A.segs, b = bh / A.H;
+  const int c0 = (matrix ? block - A.colblocks : block) * COLS, e0 = wave * 16;  // the workgroup's columns, the wave's of those
+  const int64_t part = A.first + round * 8 + (spread ? in_round % 8 : in_round / blocks), bh = part / A.segs, b = bh / A.H;
   const int seg = (int)(part % A.segs);
   const int h = (int)(bh % A.H);
   const T *q = A.q.at<T>(b, h), *k = A.k.at<T>(b, h), *v = (BACK ? A.d_o : A.v).at<T>(b, h) + c0;
   const int64_t vst = BACK ? A.d_o.st : A.v.st;
   const bool wide_v = BACK ? A.wide_d : A.wide_v;
 
-  f32x4 S[Z::DT][ET];  // the state (BACK: its gradient): rows 16 d + 4 g + i, columns e0 + 16 e + n
+  f32x4 S[Z::DT];  // the state (BACK: its gradient): rows 16 d + 4 g + i, column e0 + n
   auto each = [&](auto f) {
     int r = 4 * g, c = c0 + e0 + n;
     asm volatile("" : "+v"(r), "+v"(c));  // otherwise the addresses stay in registers over the whole loop
 #pragma unroll
     for (int d = 0; d < Z::DT; ++d)
 #pragma unroll
-      for (int e = 0; e < ET; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) S[d][e][i] = f((float)S[d][e][i], 16 * d + r + i, c + 16 * e);
+      for (int i = 0; i < 4; ++i) S[d][i] = f((float)S[d][i], 16 * d + r + i, c);
   };
   float* const seg_state = A.segs > 1 ? A.seg_state + part * KD * A.vdp : nullptr;
   if constexpr (STATE) {
@@ -366,8 +401,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
     g = lane >> 4, n = lane & 15;
     const int64_t ch = chunk_of(i), t0 = ch * C, unit = bh * A.chunks + ch;
     const int left = A.T - t0 < C ? (int)(A.T - t0) : C;
-    kr.template put<KS>(Ks, tid);
-    if constexpr (BACK || !STATE) qr.template put<QS>(Qs, tid);
+    kr.template put_mixed<KS>(Ks, tid);
+    if constexpr (BACK || !STATE) qr.template put_mixed<KS>(Qs, tid);
     vr.template put<VS>(Vs, tid);
     rr.template put<C>(&Row[0][0], tid);
     ir.template put<256>(inverse, tid);
@@ -387,97 +422,79 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
     }
     auto row4 = [&](int which, int t) { return *reinterpret_cast<const f32x4*>(&Row[which][t]); };  // of 4 neighbouring tokens
 
-    // X = K S: lane's tokens 16 t + 4 g + i, columns e0 + 16 e + n.  Forward's O' = S' Q': lane's token n, 4 columns
-    f32x4 X[TT][ET], O[BACK || STATE ? 1 : TT][ET];
-#pragma unroll
-    for (int t = 0; t < TT; ++t)
-#pragma unroll
-      for (int e = 0; e < ET; ++e) {
-        X[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if constexpr (!BACK && !STATE) O[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
-      }
-#pragma unroll
-    for (int d = 0; d < Z::DB; ++d) {
-      Wide s[ET];
-#pragma unroll
-      for (int e = 0; e < ET; ++e) {
-        float y[8];
-        eight(S[2 * d][e], S[2 * d + 1][e], y);
-        s[e] = Op::wide(y);
-      }
-#pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        const Frag f = Op::row_split(&Ks[(16 * t + n) * KS + 32 * d + 4 * g]);
-#pragma unroll
-        for (int e = 0; e < ET; ++e) X[t][e] = Op::mma(f, s[e], X[t][e]);
-        if constexpr (!BACK && !STATE) {
-          const Frag w = Op::row_split(&Qs[(16 * t + n) * QS + 32 * d + 4 * g]);
-#pragma unroll
-          for (int e = 0; e < ET; ++e) O[t][e] = Op::mma(Op::first(s[e]), w, O[t][e]);
-        }
-      }
-    }
-    // what the triangle is solved for: V - e^G K S, or b (e^{G_C - G} K R + P' dO)
-    Frag vf[KB][ET];
-#pragma unroll
-    for (int s = 0; s < KB; ++s)
-#pragma unroll
-      for (int e = 0; e < ET; ++e) vf[s][e] = Op::column(&Vs[32 * s * VS], VS, e0 + 16 * e, lane);
+    const int rows_at = Op::row_place(KS, lane), columns_at = Op::column_place(KS, lane);
+    // X = K S: lane's tokens 16 t + 4 g + i, column e0 + n.  Forward's O' = S' Q': lane's token 16 t + n, 4 columns
+    f32x4 X[TT], O[BACK || STATE ? 1 : TT];
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
-      // A weight of 0 does not select here: where the state is not finite, X is not, and the tokens go one by one below
+      X[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (!BACK && !STATE) O[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int d = 0; d < Z::DB; ++d) {
+      Frag f[TT];
+#pragma unroll
+      for (int t = 0; t < TT; ++t) f[t] = Op::row_split(Ks + rows_at + 16 * t * KS + 32 * d);
+      float y[8];
+      eight(S[2 * d], S[2 * d + 1], y);
+      const Wide s = Op::wide(y);
+      mma_left<Op, 0, TT>(f, s, X);
+      if constexpr (!BACK && !STATE) {
+#pragma unroll
+        for (int t = 0; t < TT; ++t) f[t] = Op::row_split(Qs + rows_at + 16 * t * KS + 32 * d);
+        mma_right<Op, 0, TT>(Op::first(s), f, O);
+      }
+    }
+    // what the triangle is solved for: V - e^G K S, or b (e^{G_C - G} K R + P' dO).  A weight of 0 does not select here: where the
+    // state is not finite, X is not, and the tokens go one by one below
+    Frag vf[KB];
+#pragma unroll
+    for (int s = 0; s < KB; ++s) vf[s] = Op::column(&Vs[32 * s * VS], VS, e0, lane);
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
       const f32x4 w = row4(BACK ? WU : WK, 16 * t + 4 * g);
+      float y[8];
+      if constexpr (!BACK) Op::values(vf[t / 2], y);
 #pragma unroll
-      for (int e = 0; e < ET; ++e) {
-        float y[8];
-        if constexpr (!BACK) Op::values(vf[t / 2][e], y);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          X[t][e][j] = BACK ? w[j] * X[t][e][j] : fmaf(-w[j], X[t][e][j], y[t % 2 * 4 + j]);
-      }
-      if constexpr (BACK) {
-#pragma unroll
-        for (int s = t / 2; s < KB; ++s) {
-          const Wide f = Op::template wide_tiles<false>(s * 2 >= t ? scores + tile_of(2 * s, t) * 256 : nullptr,
-                                                        scores + tile_of(2 * s + 1, t) * 256, PLANE, lane);
-#pragma unroll
-          for (int e = 0; e < ET; ++e) X[t][e] = Op::mma(f, vf[s][e], X[t][e]);
-        }
-      }
+      for (int j = 0; j < 4; ++j) X[t][j] = BACK ? w[j] * X[t][j] : fmaf(-w[j], X[t][j], y[t % 2 * 4 + j]);
     }
-    // E (dV): the inverse's (its transpose's) rows times that
-    f32x4 E[TT][ET];
-    {
-      Wide y[KB][ET];
+    // E (dV): the inverse's (its transpose's) rows times that.  Row t of a lower triangle of tiles meets tiles up to t, of its
+    // transpose from t on
+    f32x4 E[TT];
 #pragma unroll
-      for (int s = 0; s < KB; ++s)
+    for (int t = 0; t < TT; ++t) E[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if constexpr (BACK)
+      unrolled<KB>([&](auto s_) {
+        constexpr int s = decltype(s_)::value;
+        Wide f[TT];
 #pragma unroll
-        for (int e = 0; e < ET; ++e) {
-          float x[8];
-          eight(X[2 * s][e], X[2 * s + 1][e], x);
-          y[s][e] = Op::wide(x);
-        }
+        for (int t = 0; t < 2 * s + 2; ++t)
+          f[t] = Op::template wide_tiles<false>(2 * s >= t, scores + tile_of(2 * s, t) * 256, true, scores + tile_of(2 * s + 1, t) * 256,
+                                                PLANE, lane);
+        mma_left<Op, 0, 2 * s + 2>(f, vf[s], X);
+      });
+    Wide y[KB];
 #pragma unroll
-      for (int t = 0; t < TT; ++t) {
-#pragma unroll
-        for (int e = 0; e < ET; ++e) E[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = BACK ? t / 2 : 0; s < (BACK ? KB : t / 2 + 1); ++s) {
-          // row tiles of the lower triangle, or (BACK) its columns'
-          const T *a = BACK ? 2 * s >= t ? inverse + tile_of(2 * s, t) * 256 : nullptr : inverse + tile_of(t, 2 * s) * 256,
-                  *c = BACK ? inverse + tile_of(2 * s + 1, t) * 256 : 2 * s < t ? inverse + tile_of(t, 2 * s + 1) * 256 : nullptr;
-          const Wide f = Op::template wide_tiles<!BACK>(a, c, PLANE, lane);
-#pragma unroll
-          for (int e = 0; e < ET; ++e) E[t][e] = Op::mma(f, y[s][e], E[t][e]);
-        }
-      }
+    for (int s = 0; s < KB; ++s) {
+      float x[8];
+      eight(X[2 * s], X[2 * s + 1], x);
+      y[s] = Op::wide(x);
     }
-    bool fine = true;
+    unrolled<KB>([&](auto s_) {
+      constexpr int s = decltype(s_)::value, LO = BACK ? 0 : 2 * s, HI = BACK ? 2 * s + 2 : TT;
+      Wide f[TT];
 #pragma unroll
-    for (int t = 0; t < TT; ++t)
+      for (int t = LO; t < HI; ++t)
+        f[t] = BACK ? Op::template wide_tiles<false>(2 * s >= t, inverse + tile_of(2 * s, t) * 256, true,
+                                                     inverse + tile_of(2 * s + 1, t) * 256, PLANE, lane)
+                    : Op::template wide_tiles<true>(true, inverse + tile_of(t, 2 * s) * 256, 2 * s < t,
+                                                    inverse + tile_of(t, 2 * s + 1) * 256, PLANE, lane);
+      mma_left<Op, LO, HI>(f, y[s], E);
+    });
+    float all = 0.0f;
 #pragma unroll
-      for (int e = 0; e < ET; ++e) fine = fine && all_finite(E[t][e]);
-    odd = odd || __ballot(!fine) != 0;
+    for (int t = 0; t < TT; ++t) all = met(all, E[t]);
+    odd = odd || __ballot(all != 0.0f) != 0;
     float* const all_rows = STATE ? nullptr : BACK ? A.dV : A.E;
     float* const kept_rows = all_rows ? all_rows + unit * C * A.vdp + c0 + e0 : nullptr;
     const int64_t first = ((b * A.T + t0) * A.H + h) * A.vd;  // of the output
@@ -487,147 +504,112 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
 #pragma unroll
         for (int t = 0; t < TT; ++t)
 #pragma unroll
-          for (int e = 0; e < ET; ++e)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) kept_rows[(16 * t + 4 * g + j) * A.vdp + 16 * e + n] = E[t][e][j];
+          for (int j = 0; j < 4; ++j) kept_rows[(16 * t + 4 * g + j) * A.vdp + n] = E[t][j];
       }
       if constexpr (!BACK && !STATE) {
-        typename Op::Pair y[KB][ET];
 #pragma unroll
-        for (int s = 0; s < KB; ++s)
+        for (int t = 0; t < TT; ++t) O[t] *= Row[WQ][16 * t + n];
+        unrolled<KB>([&](auto s_) {
+          constexpr int s = decltype(s_)::value;
+          float x[8];
+          eight(E[2 * s], E[2 * s + 1], x);
+          const typename Op::Pair e = Op::pair(x);
+          typename Op::Pair f[TT];
 #pragma unroll
-          for (int e = 0; e < ET; ++e) {
-            float x[8];
-            eight(E[2 * s][e], E[2 * s + 1][e], x);
-            y[s][e] = Op::pair(x);
-          }
+          for (int t = 2 * s; t < TT; ++t)
+            f[t] = Op::template pair_tiles<true>(true, scores + tile_of(t, 2 * s) * 256, 2 * s < t,
+                                                 scores + tile_of(t, 2 * s + 1) * 256, PLANE, lane);
+          mma_right<Op, 2 * s, TT>(e, f, O);
+        });
 #pragma unroll
-        for (int t = 0; t < TT; ++t) {
-          const float w = Row[WQ][16 * t + n];
+        for (int t = 0; t < TT; ++t) {  // a lane holds 4 neighbouring columns of one token
+          const int r = 16 * t + n, c = c0 + e0 + 4 * g;
+          T f[4];
 #pragma unroll
-          for (int e = 0; e < ET; ++e) O[t][e] *= w;
+          for (int j = 0; j < 4; ++j) f[j] = from_f<T>(O[t][j]);
+          T* to = static_cast<T*>(A.o) + first;
+          if (A.wide_o) {
+            const auto rows = bounded(to, ((left - 1) * row + A.vd) * (int)sizeof(T));
+            const int off = c < A.vd ? (r * row + c) * (int)sizeof(T) : BEYOND;
+            if constexpr (sizeof(T) == 4)
+              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f), rows, off, 0, 0);
+            else
+              __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f), rows, off, 0, 0);
+          } else if (r < left) {
 #pragma unroll
-          for (int s = 0; s <= t / 2; ++s) {
-            const typename Op::Pair f = Op::template pair_tiles<true>(
-                scores + tile_of(t, 2 * s) * 256, 2 * s < t ? scores + tile_of(t, 2 * s + 1) * 256 : nullptr, PLANE, lane);
-#pragma unroll
-            for (int e = 0; e < ET; ++e) O[t][e] = Op::mma(y[s][e], f, O[t][e]);
-          }
-#pragma unroll
-          for (int e = 0; e < ET; ++e) {  // a lane holds 4 neighbouring columns of one token
-            const int r = 16 * t + n, c = c0 + e0 + 16 * e + 4 * g;
-            T f[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) f[j] = from_f<T>(O[t][e][j]);
-            T* to = static_cast<T*>(A.o) + first;
-            if (A.wide_o) {
-              const auto rows = bounded(to, ((left - 1) * row + A.vd) * (int)sizeof(T));
-              const int off = c < A.vd ? (r * row + c) * (int)sizeof(T) : BEYOND;
-              if constexpr (sizeof(T) == 4)
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f), rows, off, 0, 0);
-              else
-                __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f), rows, off, 0, 0);
-            } else if (r < left) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (c + j < A.vd) to[(int64_t)r * row + c + j] = f[j];
-            }
+            for (int j = 0; j < 4; ++j)
+              if (c + j < A.vd) to[(int64_t)r * row + c + j] = f[j];
           }
         }
       }
       // the state behind the chunk, or its gradient in front of it
 #pragma unroll
-      for (int d = 0; d < Z::DT; ++d)
-#pragma unroll
-        for (int e = 0; e < ET; ++e) S[d][e] *= whole;
+      for (int d = 0; d < Z::DT; ++d) S[d] *= whole;
 #pragma unroll
       for (int s = 0; s < KB; ++s) {
-        Wide we[ET], wd[BACK ? ET : 1];
         const f32x4 wa = row4(BACK ? WK : WU, 32 * s + 4 * g), wb = row4(BACK ? WK : WU, 32 * s + 16 + 4 * g);
-        const f32x4 qa = row4(WQ, 32 * s + 4 * g), qb = row4(WQ, 32 * s + 16 + 4 * g);
+        float x[8];
+        if constexpr (BACK) eight(E[2 * s] * -wa, E[2 * s + 1] * -wb, x);
+        else eight(E[2 * s] * wa, E[2 * s + 1] * wb, x);
+        const Wide we = Op::wide(x);
+        Frag f[Z::DT];
 #pragma unroll
-        for (int e = 0; e < ET; ++e) {
-          float x[8];
-          if constexpr (BACK) eight(E[2 * s][e] * -wa, E[2 * s + 1][e] * -wb, x);
-          else eight(E[2 * s][e] * wa, E[2 * s + 1][e] * wb, x);
-          we[e] = Op::wide(x);
-          if constexpr (BACK) {
-            Op::values(vf[s][e], x);
+        for (int d = 0; d < Z::DT; ++d) f[d] = Op::column_mixed(Ks + columns_at + 32 * s * KS + 16 * d, KS);
+        mma_left<Op, 0, Z::DT>(f, we, S);
+        if constexpr (BACK) {
+          const f32x4 qa = row4(WQ, 32 * s + 4 * g), qb = row4(WQ, 32 * s + 16 + 4 * g);
+          Op::values(vf[s], x);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] *= j < 4 ? qa[j % 4] : qb[j % 4];
-            wd[e] = Op::wide(x);
-          }
-        }
+          for (int j = 0; j < 8; ++j) x[j] *= j < 4 ? qa[j % 4] : qb[j % 4];
+          const Wide wd = Op::wide(x);
 #pragma unroll
-        for (int d = 0; d < Z::DT; ++d) {
-          const Frag f = Op::column(&Ks[32 * s * KS], KS, 16 * d, lane);
-#pragma unroll
-          for (int e = 0; e < ET; ++e) S[d][e] = Op::mma(f, we[e], S[d][e]);
-          if constexpr (BACK) {
-            const Frag x = Op::column(&Qs[32 * s * QS], QS, 16 * d, lane);
-#pragma unroll
-            for (int e = 0; e < ET; ++e) S[d][e] = Op::mma(x, wd[e], S[d][e]);
-          }
+          for (int d = 0; d < Z::DT; ++d) f[d] = Op::column_mixed(Qs + columns_at + 32 * s * KS + 16 * d, KS);
+          mma_left<Op, 0, Z::DT>(f, wd, S);
         }
       }
     } else {  // token by token: a column needs nothing but its own entries
       for (int a = 0; a < left; ++a) {
         const int t = BACK ? left - 1 - a : a;
         const float rk = Row[RK][t], rq = Row[RQ][t] * A.scale, be = Row[BETA][t], dec = Row[DEC][t];
-        float in[ET], x[ET], o[ET];
-#pragma unroll
-        for (int e = 0; e < ET; ++e) in[e] = to_f(Vs[t * VS + e0 + 16 * e + n]), x[e] = o[e] = 0.0f;
+        const float in = to_f(Vs[t * VS + e0 + n]);
+        float x = 0.0f, o = 0.0f;
         auto decay = [&](float s) { return dec < 0.0f ? 0.0f : kept(dec, s); };
 #pragma unroll
         for (int d = 0; d < Z::DT; ++d)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int r = 16 * d + 4 * g + j;
-            const float kk = to_f(Ks[t * KS + r]), qq = STATE && !BACK ? 0.0f : to_f(Qs[t * QS + r]);
-#pragma unroll
-            for (int e = 0; e < ET; ++e) {
-              S[d][e][j] = BACK ? fmaf(rq * qq, in[e], S[d][e][j]) : decay(S[d][e][j]);
-              x[e] = r < A.kd ? fmaf(kk, S[d][e][j], x[e]) : x[e];
-            }
+            const float kk = to_f(Ks[Op::at(t, r, KS)]), qq = STATE && !BACK ? 0.0f : to_f(Qs[Op::at(t, r, KS)]);
+            S[d][j] = BACK ? fmaf(rq * qq, in, S[d][j]) : decay(S[d][j]);
+            x = r < A.kd ? fmaf(kk, S[d][j], x) : x;
           }
-#pragma unroll
-        for (int e = 0; e < ET; ++e) {
-          x[e] += __shfl_xor(x[e], 16, 64);
-          x[e] += __shfl_xor(x[e], 32, 64);
-          x[e] = BACK ? be * (rk * x[e]) : in[e] - rk * x[e];  // dV, or E
-          if (kept_rows && g == 0) kept_rows[t * A.vdp + 16 * e + n] = x[e];
-        }
+        x += __shfl_xor(x, 16, 64);
+        x += __shfl_xor(x, 32, 64);
+        x = BACK ? be * (rk * x) : in - rk * x;  // dV, or E
+        if (kept_rows && g == 0) kept_rows[t * A.vdp + n] = x;
 #pragma unroll
         for (int d = 0; d < Z::DT; ++d)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int r = 16 * d + 4 * g + j;
-            const float kk = to_f(Ks[t * KS + r]), qq = STATE && !BACK ? 0.0f : to_f(Qs[t * QS + r]);
-#pragma unroll
-            for (int e = 0; e < ET; ++e) {
-              if constexpr (BACK) {
-                S[d][e][j] = r < A.kd ? decay(fmaf(-rk * kk, x[e], S[d][e][j])) : 0.0f;
-              } else {
-                S[d][e][j] = r < A.kd ? fmaf(rk * kk, be * x[e], S[d][e][j]) : 0.0f;
-                o[e] = r < A.kd ? fmaf(qq, S[d][e][j], o[e]) : o[e];
-              }
+            const float kk = to_f(Ks[Op::at(t, r, KS)]), qq = STATE && !BACK ? 0.0f : to_f(Qs[Op::at(t, r, KS)]);
+            if constexpr (BACK) {
+              S[d][j] = r < A.kd ? decay(fmaf(-rk * kk, x, S[d][j])) : 0.0f;
+            } else {
+              S[d][j] = r < A.kd ? fmaf(rk * kk, be * x, S[d][j]) : 0.0f;
+              o = r < A.kd ? fmaf(qq, S[d][j], o) : o;
             }
           }
         if constexpr (!BACK && !STATE) {
-#pragma unroll
-          for (int e = 0; e < ET; ++e) {
-            o[e] += __shfl_xor(o[e], 16, 64);
-            o[e] += __shfl_xor(o[e], 32, 64);
-            const int c = c0 + e0 + 16 * e + n;
-            if (g == 0 && c < A.vd) static_cast<T*>(A.o)[first + (int64_t)t * row + c] = from_f<T>(rq * o[e]);
-          }
+          o += __shfl_xor(o, 16, 64);
+          o += __shfl_xor(o, 32, 64);
+          const int c = c0 + e0 + n;
+          if (g == 0 && c < A.vd) static_cast<T*>(A.o)[first + (int64_t)t * row + c] = from_f<T>(rq * o);
         }
       }
       if (kept_rows && left < C) {  // rows that do not exist
         for (int t = left; t < C; ++t)
-#pragma unroll
-          for (int e = 0; e < ET; ++e)
-            if (g == 0) kept_rows[t * A.vdp + 16 * e + n] = 0.0f;
+          if (g == 0) kept_rows[t * A.vdp + n] = 0.0f;
       }
     }
     __syncthreads();
@@ -973,31 +955,32 @@ __global__ __launch_bounds__((KD / 16 * 64), 2) void delta_gradients_kernel(Delt
 
 // ---- launches --------------------------------------------------------------------------------------------------
 
-template <class T, int KD, int WAVES, int ET, bool BACK, bool STATE>
+template <class T, int KD, int WAVES, bool BACK, bool STATE>
 int launch_delta_part(const Delta& A, hipStream_t s) {
-  constexpr int COLS = 16 * ET * WAVES;
+  constexpr int COLS = 16 * WAVES;
   Delta P = A;
   P.colblocks = (int)ceil_div(A.vd, COLS);
   const int blocks = STATE && !BACK ? P.colblocks + (KD + COLS - 1) / COLS : P.colblocks;
   return in_launches(A.B * A.H * A.segs * blocks, WAVES * 64, [&](int64_t first, dim3 grid) {
     P.first = first / blocks;
-    hipLaunchKernelGGL((delta_sweep_kernel<T, KD, WAVES, ET, BACK, STATE>), grid, dim3(WAVES * 64), 0, s, P);
+    hipLaunchKernelGGL((delta_sweep_kernel<T, KD, WAVES, BACK, STATE>), grid, dim3(WAVES * 64), 0, s, P);
   }, blocks);
 }
 
-template <class T, int KD, int WAVES, int ET, bool BACK>
+template <class T, int KD, int WAVES, bool BACK>
 int launch_delta_sweep(const Delta& A, hipStream_t s) {
   if (A.segs > 1) {
-    if (const int rc = launch_delta_part<T, KD, WAVES, ET, BACK, true>(A, s)) return rc;
+    if (const int rc = launch_delta_part<T, KD, WAVES, BACK, true>(A, s)) return rc;
     if (const int rc = launch_delta_join(A, BACK, s)) return rc;
   }
-  return launch_delta_part<T, KD, WAVES, ET, BACK, false>(A, s);
+  return launch_delta_part<T, KD, WAVES, BACK, false>(A, s);
 }
 
 template <class T, int KD, bool BACK>
 int launch_delta_sweeps(const Delta& A, hipStream_t s) {
-  if (A.vd <= 32) return launch_delta_sweep<T, KD, 2, 1, BACK>(A, s);
-  return launch_delta_sweep<T, KD, 4, 1, BACK>(A, s);
+  if (A.vd <= 32) return launch_delta_sweep<T, KD, 2, BACK>(A, s);
+  if (A.vd <= 64) return launch_delta_sweep<T, KD, 4, BACK>(A, s);
+  return launch_delta_sweep<T, KD, 8, BACK>(A, s);
 }
 
 template <class T, int KD, int VD>

@@ -46,6 +46,28 @@ struct Operand<__bf16> {
     return mma(a.h, b.h, mma(a.h, b.l, mma(a.l, b.h, c)));
   }
   static __device__ __forceinline__ Pair first(const Wide& a) { return Pair{a.h, a.m}; }  // 16 of its digits
+  // A product as single instructions, small terms first: those of several sums are issued in turn, so that none waits for the
+  // one before it
+  static constexpr int steps(const Frag*, const Wide*) { return 3; }
+  static constexpr int steps(const Wide*, const Frag*) { return 3; }
+  static constexpr int steps(const Wide*, const Wide*) { return 6; }
+  static constexpr int steps(const Pair*, const Frag*) { return 2; }
+  static constexpr int steps(const Frag*, const Pair*) { return 2; }
+  static constexpr int steps(const Pair*, const Pair*) { return 3; }
+  static __device__ __forceinline__ f32x4 step(int p, Frag a, const Wide& b, f32x4 c) {
+    return mma(a, p == 0 ? b.l : p == 1 ? b.m : b.h, c);
+  }
+  static __device__ __forceinline__ f32x4 step(int p, const Wide& a, Frag b, f32x4 c) {
+    return mma(p == 0 ? a.l : p == 1 ? a.m : a.h, b, c);
+  }
+  static __device__ __forceinline__ f32x4 step(int p, const Wide& a, const Wide& b, f32x4 c) {
+    return mma(p == 1 ? a.l : p == 2 || p == 3 ? a.m : a.h, p == 0 ? b.l : p == 2 || p == 4 ? b.m : b.h, c);
+  }
+  static __device__ __forceinline__ f32x4 step(int p, const Pair& a, Frag b, f32x4 c) { return mma(p == 0 ? a.l : a.h, b, c); }
+  static __device__ __forceinline__ f32x4 step(int p, Frag a, const Pair& b, f32x4 c) { return mma(a, p == 0 ? b.l : b.h, c); }
+  static __device__ __forceinline__ f32x4 step(int p, const Pair& a, const Pair& b, f32x4 c) {
+    return mma(p == 1 ? a.l : a.h, p == 0 ? b.l : b.h, c);
+  }
   static __device__ __forceinline__ f32x4 mma(const Pair& a, Frag b, f32x4 c) { return mma(a.h, b, mma(a.l, b, c)); }
   static __device__ __forceinline__ f32x4 mma(Frag a, const Pair& b, f32x4 c) { return mma(a, b.h, mma(a, b.l, c)); }
   static __device__ __forceinline__ Frag row(const __bf16* p) { return *reinterpret_cast<const Frag*>(p); }
@@ -101,8 +123,29 @@ struct Operand<__bf16> {
     return Pair{both(p), both(p + part)};
   }
   static __device__ __forceinline__ float score(const __bf16* p, int part) { return to_f(p[0]) + to_f(p[part]); }
+  // Rows of 8 banks' distance that are read along them and across them: 8 bytes of a row change places with its number / 4, so
+  // that both reads meet each bank once.  at: where an element of such an array (of tile_at: of a 16 x 16 tile) lies
+  static __device__ __forceinline__ int at(int row, int c, int stride) { return row * stride + (c ^ ((row >> 2 & 3) << 2)); }
+  static __device__ __forceinline__ int tile_at(int row, int c) { return row * 16 + (c ^ (row & 12)); }
+  static __device__ __forceinline__ void put_mixed(__bf16* p, int row, int c, int stride, u32x4 v) {
+    const bool swap = row & 4;
+    const u32x4 w = {swap ? v[2] : v[0], swap ? v[3] : v[1], swap ? v[0] : v[2], swap ? v[1] : v[3]};
+    *reinterpret_cast<u32x4*>(p + row * stride + (c ^ (row & 8))) = w;
+  }
+  // A lane's place for `row_split` (row n, elements 4 g on) and for `column_mixed` (as `column`); whole rows and multiples of 16
+  // elements are added to it
+  static __device__ __forceinline__ int row_place(int stride, int lane) { return at(lane & 15, lane >> 4 << 2, stride); }
+  static __device__ __forceinline__ int column_place(int stride, int lane) {
+    return at((lane >> 4 << 2) + (lane >> 2 & 3), (lane & 3) * 4, stride);
+  }
+  static __device__ __forceinline__ Frag column_mixed(const __bf16* a, int stride) {
+    typedef __attribute__((address_space(3))) i16x4 lds;
+    const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)(a));
+    const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)(a + 16 * stride));
+    return __builtin_bit_cast(Frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
   // Values in memory as their three parts (WIDE_PARTS such arrays, `part` elements apart): 4 neighbours put at p, and two
-  // 16 x 16 tiles as an operand (NULL: zeros): rows n of both, or of their transposes, 24 or (first) 16 digits of them
+  // 16 x 16 tiles as an operand (zeros for one that is not there): rows n of both, or of their transposes, 24 or (first) 16 digits of them
   static constexpr int WIDE_PARTS = 3;
   static __device__ __forceinline__ void put_wide(__bf16* p, int part, f32x4 x) {
     float d[4], e[4];
@@ -113,24 +156,24 @@ struct Operand<__bf16> {
     *reinterpret_cast<bf16x4*>(p + 2 * part) = bf16x4{(__bf16)e[0], (__bf16)e[1], (__bf16)e[2], (__bf16)e[3]};
   }
   template <bool ROW>
-  static __device__ __forceinline__ Frag tiles(const __bf16* a, const __bf16* b, int lane) {
+  static __device__ __forceinline__ Frag tiles(bool has_a, const __bf16* a, bool has_b, const __bf16* b, int lane) {
     const int g = lane >> 4, i = lane & 15;
     typedef __attribute__((address_space(3))) i16x4 lds;
     auto one = [&](const __bf16* p) {
-      if (ROW) return *reinterpret_cast<const i16x4*>(p + i * 16 + 4 * g);
-      return (i16x4)__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)(p + (4 * g + (i >> 2)) * 16 + (i & 3) * 4));
+      if (ROW) return *reinterpret_cast<const i16x4*>(p + tile_at(i, 4 * g));
+      return (i16x4)__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)(p + tile_at(4 * g + (i >> 2), (i & 3) * 4)));
     };
-    const i16x4 x = a ? one(a) : i16x4{0, 0, 0, 0}, y = b ? one(b) : i16x4{0, 0, 0, 0};
+    const i16x4 x = has_a ? one(a) : i16x4{0, 0, 0, 0}, y = has_b ? one(b) : i16x4{0, 0, 0, 0};
     return __builtin_bit_cast(Frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
   }
   template <bool ROW>
-  static __device__ __forceinline__ Wide wide_tiles(const __bf16* a, const __bf16* b, int part, int lane) {
-    auto at = [&](const __bf16* p, int i) { return p ? p + i * part : nullptr; };
-    return Wide{tiles<ROW>(a, b, lane), tiles<ROW>(at(a, 1), at(b, 1), lane), tiles<ROW>(at(a, 2), at(b, 2), lane)};
+  static __device__ __forceinline__ Wide wide_tiles(bool has_a, const __bf16* a, bool has_b, const __bf16* b, int part, int lane) {
+    return Wide{tiles<ROW>(has_a, a, has_b, b, lane), tiles<ROW>(has_a, a + part, has_b, b + part, lane),
+                tiles<ROW>(has_a, a + 2 * part, has_b, b + 2 * part, lane)};
   }
   template <bool ROW>
-  static __device__ __forceinline__ Pair pair_tiles(const __bf16* a, const __bf16* b, int part, int lane) {
-    return Pair{tiles<ROW>(a, b, lane), tiles<ROW>(a ? a + part : a, b ? b + part : b, lane)};
+  static __device__ __forceinline__ Pair pair_tiles(bool has_a, const __bf16* a, bool has_b, const __bf16* b, int part, int lane) {
+    return Pair{tiles<ROW>(has_a, a, has_b, b, lane), tiles<ROW>(has_a, a + part, has_b, b + part, lane)};
   }
   static __device__ __forceinline__ Wide wide(const float (&x)[8]) {
     u32x4 h, m, l;
@@ -184,6 +227,10 @@ struct Operand<float> {
     return c;
   }
   static __device__ __forceinline__ Frag first(const Frag& a) { return a; }
+  static constexpr int steps(const Frag*, const Frag*) { return 8; }
+  static __device__ __forceinline__ f32x4 step(int p, const Frag& a, const Frag& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[p], b.v[p], c, 0, 0, 0);
+  }
   static __device__ __forceinline__ Frag two(const float* p, const float* q) {
     const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(q);
     return Frag{{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
@@ -206,23 +253,36 @@ struct Operand<float> {
     return Frag{{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
   }
   static __device__ __forceinline__ float score(const float* p, int) { return p[0]; }
+  static __device__ __forceinline__ int at(int row, int c, int stride) { return row * stride + c; }
+  static __device__ __forceinline__ int tile_at(int row, int c) { return row * 16 + c; }
+  static __device__ __forceinline__ void put_mixed(float* p, int row, int c, int stride, u32x4 v) {
+    *reinterpret_cast<u32x4*>(p + row * stride + c) = v;
+  }
+  static __device__ __forceinline__ int row_place(int stride, int lane) { return (lane & 15) * stride + (lane >> 4 << 2); }
+  static __device__ __forceinline__ int column_place(int stride, int lane) { return (lane >> 4 << 2) * stride + (lane & 15); }
+  static __device__ __forceinline__ Frag column_mixed(const float* a, int stride) {
+    Frag r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r.v[j] = a[(j < 4 ? j : 12 + j) * stride];
+    return r;
+  }
   static constexpr int WIDE_PARTS = 1;
   static __device__ __forceinline__ void put_wide(float* p, int, f32x4 x) { *reinterpret_cast<f32x4*>(p) = x; }
   template <bool ROW>
-  static __device__ __forceinline__ Frag wide_tiles(const float* a, const float* b, int, int lane) {
+  static __device__ __forceinline__ Frag wide_tiles(bool has_a, const float* a, bool has_b, const float* b, int, int lane) {
     const int g = lane >> 4, n = lane & 15;
     Frag r;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int at = ROW ? n * 16 + 4 * g + j : (4 * g + j) * 16 + n;
-      r.v[j] = a ? a[at] : 0.0f;
-      r.v[4 + j] = b ? b[at] : 0.0f;
+      r.v[j] = has_a ? a[at] : 0.0f;
+      r.v[4 + j] = has_b ? b[at] : 0.0f;
     }
     return r;
   }
   template <bool ROW>
-  static __device__ __forceinline__ Frag pair_tiles(const float* a, const float* b, int part, int lane) {
-    return wide_tiles<ROW>(a, b, part, lane);
+  static __device__ __forceinline__ Frag pair_tiles(bool has_a, const float* a, bool has_b, const float* b, int part, int lane) {
+    return wide_tiles<ROW>(has_a, a, has_b, b, part, lane);
   }
   static __device__ __forceinline__ Frag wide(const float (&x)[8]) {
     Frag r;
