@@ -164,54 +164,58 @@ int launch_tokens(const Tokens& A, bool bf16, hipStream_t s) {
 template <int KD, bool BACK>
 __global__ __launch_bounds__(KD / 16 * 64) void delta_join_kernel(Delta A) {
   using Op = Operand<__bf16>;
-  constexpr int DB = KD / 32, RS = KD + 4;
-  __shared__ __attribute__((aligned(16))) float Now[2][16 * RS];  // the state's columns, by rows of them
+  constexpr int DB = KD / 32, RS = KD + 8, PLANE = 16 * RS;
+  __shared__ __attribute__((aligned(16))) __bf16 Now[2][3 * PLANE];  // the state's columns as rows, in their parts
   const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int blocks = A.vdp / 16, c = (int)(blockIdx.x % blocks) * 16 + n, r0 = wave * 16;
-  const int64_t bh = A.first + blockIdx.x / blocks;
+  const Spread W = spread(A.first, A.vdp / 16);
+  const int c = W.block * 16 + n, r0 = wave * 16;
+  const int64_t bh = W.group;
   auto segment = [&](int i) { return bh * A.segs + (BACK ? A.segs - 1 - i : i); };
-  float m[DB][8], own[4];
-  int dead = 0;
-  f32x4 now;
-  auto fetch = [&](int i) {
+  struct Part {
+    float m[DB][8], own[4];
+    int dead;
+  };
+  auto fetch = [&](int i, Part& P) {
     const float* p = A.seg_matrix + segment(i) * KD * KD;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        m[d][j] = BACK ? p[(32 * d + 8 * g + j) * KD + r0 + n] : p[(r0 + n) * KD + 32 * d + 8 * g + j];
+        P.m[d][j] = BACK ? p[(32 * d + 8 * g + j) * KD + r0 + n] : p[(r0 + n) * KD + 32 * d + 8 * g + j];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) own[j] = A.seg_state[(segment(i) * KD + r0 + 4 * g + j) * A.vdp + c];
-    dead = A.seg_dead[segment(i)];
+    for (int j = 0; j < 4; ++j) P.own[j] = A.seg_state[(segment(i) * KD + r0 + 4 * g + j) * A.vdp + c];
+    P.dead = A.seg_dead[segment(i)];
   };
+  f32x4 now;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int r = r0 + 4 * g + j;
     now[j] = A.state_in && r < A.kd && c < A.vd ? A.state_in[(bh * A.kd + r) * A.vd + c] : 0.0f;
   }
-  fetch(0);
-  for (int i = 0;; ++i) {
-    f32x4 next;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) next[j] = own[j];
+  // segment i, whose part is here, while that of the next one is on its way
+  auto pass = [&](int i, const Part& P, Part& ahead, __bf16* to) {
+    if (i + 1 < A.segs) fetch(i + 1, ahead);
 #pragma unroll
     for (int j = 0; j < 4; ++j) A.seg_state[(segment(i) * KD + r0 + 4 * g + j) * A.vdp + c] = now[j];
-    if (i + 1 == A.segs) break;
-    float* to = Now[i & 1];
-    *reinterpret_cast<f32x4*>(&to[n * RS + r0 + 4 * g]) = now;
-    __syncthreads();  // the next round writes the other buffer, and meets this barrier before it comes back to this one
-    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    if (i + 1 == A.segs) return;
+    Op::put_wide(&to[n * RS + r0 + 4 * g], PLANE, now);
+    __syncthreads();  // the next segment writes the other buffer, and meets this barrier before it comes back to this one
+    f32x4 sum[2] = {{P.own[0], P.own[1], P.own[2], P.own[3]}, {0.f, 0.f, 0.f, 0.f}};
+    if (!P.dead) {
 #pragma unroll
-    for (int d = 0; d < DB; ++d) {
-      float x[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = to[n * RS + 32 * d + 8 * g + j];
-      sum = Op::mma(Op::wide(m[d]), Op::wide(x), sum);
+      for (int d = 0; d < DB; ++d) {
+        const __bf16* x = &to[n * RS + 32 * d + 8 * g];
+        sum[d & 1] = Op::mma(Op::wide(P.m[d]), Op::Wide{Op::row(x), Op::row(x + PLANE), Op::row(x + 2 * PLANE)}, sum[d & 1]);
+      }
     }
-    const bool drop = dead != 0;
-    fetch(i + 1);
-    now = drop ? next : next + sum;
+    now = sum[0] + sum[1];
+  };
+  Part even, odd;
+  fetch(0, even);
+  for (int i = 0; i < A.segs; i += 2) {
+    pass(i, even, odd, Now[0]);
+    if (i + 1 < A.segs) pass(i + 1, odd, even, Now[1]);
   }
 }
 

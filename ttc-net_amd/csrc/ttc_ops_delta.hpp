@@ -59,6 +59,18 @@ template <class T>
 int launch_delta_kd128(const Delta& A, int what, hipStream_t s);
 enum { PREPARE, SWEEP, SWEEP_BACK, GRADIENTS };
 
+// Workgroup numbers go round the 8 XCDs.  Of `blocks` workgroups that read the same data (what they share: `group`), all go to
+// one XCD, whose L2 then reads it once.
+struct Spread {
+  int64_t group;
+  int block;
+};
+__device__ __forceinline__ Spread spread(int64_t first, int blocks) {
+  const unsigned round = blockIdx.x / (8 * blocks), at = blockIdx.x % (8 * blocks);
+  if (round < gridDim.x / (8 * blocks)) return {first + round * 8 + at % 8, (int)(at / 8)};
+  return {first + round * 8 + at / blocks, (int)(at % blocks)};  // fewer than 8 are left
+}
+
 int launch_delta_join(const Delta& A, bool back, hipStream_t s);
 
 }  // namespace ttc

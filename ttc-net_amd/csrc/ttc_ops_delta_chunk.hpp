@@ -26,43 +26,49 @@ struct DeltaShape {
 constexpr int tile_of(int t, int s) { return t * (t + 1) / 2 + s; }
 
 // A chunk's rows of D elements: 16-byte loads, all in flight at once, then to shared memory.  Rows that do not exist and
-// elements behind `dim` are 0.
+// elements behind `dim` are 0.  A thread's vectors lie in one column, STEP rows apart, so that its places follow from the first
+// one's.
 template <class T, int D, int C, int NT>
 struct Stage {
-  static constexpr int VEC = 16 / sizeof(T), N = (C * D / VEC + NT - 1) / NT;
+  static constexpr int VEC = 16 / sizeof(T), COLS = D / VEC, STEP = NT / COLS, N = (C + STEP - 1) / STEP;
+  static_assert(NT % COLS == 0, "whole rows of threads");
   u32x4 r[N];
   __device__ __forceinline__ void fetch(const T* p, int64_t st, int dim, int left, bool wide, int tid) {
+    const int row = tid / COLS, c = tid % COLS * VEC;
     if (wide) {
       const auto rows = bounded(p, left * (int)st * (int)sizeof(T));  // rows do not overlap: st >= dim
+      const unsigned at = c < dim ? (unsigned)(row * (int)st + c) * (unsigned)sizeof(T) : (unsigned)BEYOND;
+      const unsigned step = (unsigned)(STEP * (int)st) * (unsigned)sizeof(T);  // a chunk's rows lie within 2^30 bytes: no overflow
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const int i = tid + j * NT, row = i / (D / VEC), c = i % (D / VEC) * VEC;
-        r[j] = __builtin_amdgcn_raw_buffer_load_b128(
-            rows, row < C && c < dim ? (row * (int)st + c) * (int)sizeof(T) : BEYOND, 0, 0);
-      }
+      for (int j = 0; j < N; ++j) r[j] = __builtin_amdgcn_raw_buffer_load_b128(rows, (int)(at + j * step), 0, 0);
     } else {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const int i = tid + j * NT, row = i / (D / VEC), c = i % (D / VEC) * VEC;
         const u32x4 zero = {0, 0, 0, 0};
-        r[j] = row < C && row < left ? load_any(p + row * st, c, dim) : zero;
+        r[j] = row + j * STEP < left ? load_any(p + (int64_t)(row + j * STEP) * st, c, dim) : zero;
       }
     }
   }
   template <int STRIDE>
   __device__ __forceinline__ void put(T* to, int tid) const {
+    T* p = to + tid / COLS * STRIDE + tid % COLS * VEC;
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int i = tid + j * NT, row = i / (D / VEC), c = i % (D / VEC) * VEC;
-      if (C * D / VEC % NT == 0 || row < C) *reinterpret_cast<u32x4*>(&to[row * STRIDE + c]) = r[j];
-    }
+    for (int j = 0; j < N; ++j)
+      if (C % STEP == 0 || tid / COLS + j * STEP < C) *reinterpret_cast<u32x4*>(p + j * STEP * STRIDE) = r[j];
   }
   template <int STRIDE>
   __device__ __forceinline__ void put_mixed(T* to, int tid) const {
+    static_assert(C % STEP == 0, "whole rows");
+    if constexpr (STEP % 16 == 0) {  // rows that are mixed alike
+      T* p = to + Operand<T>::mixed_place(tid / COLS, tid % COLS * VEC, STRIDE);
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int i = tid + j * NT, row = i / (D / VEC), c = i % (D / VEC) * VEC;
-      if (C * D / VEC % NT == 0 || row < C) Operand<T>::put_mixed(to, row, c, STRIDE, r[j]);
+      for (int j = 0; j < N; ++j) *reinterpret_cast<u32x4*>(p + j * STEP * STRIDE) = Operand<T>::mixed(tid / COLS, r[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int row = tid / COLS + j * STEP;
+        *reinterpret_cast<u32x4*>(to + Operand<T>::mixed_place(row, tid % COLS * VEC, STRIDE)) = Operand<T>::mixed(row, r[j]);
+      }
     }
   }
   __device__ __forceinline__ void largest(uint32_t& m) const {
@@ -337,14 +343,12 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
   int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int lane = tid & 63, g = lane >> 4, n = lane & 15;
-  // Workgroup numbers go round the 8 XCDs: a segment's column blocks, which read the same keys, on one of them (its L2)
   const int blocks = STATE && !BACK ? A.colblocks + (KD + COLS - 1) / COLS : A.colblocks;
-  const unsigned round = blockIdx.x / (8 * blocks), whole_rounds = gridDim.x / (8 * blocks), in_round = blockIdx.x % (8 * blocks);
-  const bool spread = round < whole_rounds;
-  const int block = (int)(spread ? in_round / 8 : in_round % blocks);
+  const Spread W = spread(A.first, blocks);
+  const int block = W.block;
   const bool matrix = STATE && !BACK && block >= A.colblocks;
   const int c0 = (matrix ? block - A.colblocks : block) * COLS, e0 = wave * 16;  // the workgroup's columns, the wave's of those
-  const int64_t part = A.first + round * 8 + (spread ? in_round % 8 : in_round / blocks), bh = part / A.segs, b = bh / A.H;
+  const int64_t part = W.group, bh = part / A.segs, b = bh / A.H;
   const int seg = (int)(part % A.segs);
   const int h = (int)(bh % A.H);
   const T *q = A.q.at<T>(b, h), *k = A.k.at<T>(b, h), *v = (BACK ? A.d_o : A.v).at<T>(b, h) + c0;
@@ -979,8 +983,7 @@ int launch_delta_sweep(const Delta& A, hipStream_t s) {
 template <class T, int KD, bool BACK>
 int launch_delta_sweeps(const Delta& A, hipStream_t s) {
   if (A.vd <= 32) return launch_delta_sweep<T, KD, 2, BACK>(A, s);
-  if (A.vd <= 64) return launch_delta_sweep<T, KD, 4, BACK>(A, s);
-  return launch_delta_sweep<T, KD, 8, BACK>(A, s);
+  return launch_delta_sweep<T, KD, 4, BACK>(A, s);
 }
 
 template <class T, int KD, int VD>

@@ -127,10 +127,10 @@ struct Operand<__bf16> {
   // that both reads meet each bank once.  at: where an element of such an array (of tile_at: of a 16 x 16 tile) lies
   static __device__ __forceinline__ int at(int row, int c, int stride) { return row * stride + (c ^ ((row >> 2 & 3) << 2)); }
   static __device__ __forceinline__ int tile_at(int row, int c) { return row * 16 + (c ^ (row & 12)); }
-  static __device__ __forceinline__ void put_mixed(__bf16* p, int row, int c, int stride, u32x4 v) {
+  static __device__ __forceinline__ int mixed_place(int row, int c, int stride) { return row * stride + (c ^ (row & 8)); }
+  static __device__ __forceinline__ u32x4 mixed(int row, u32x4 v) {  // 8 elements as they lie there
     const bool swap = row & 4;
-    const u32x4 w = {swap ? v[2] : v[0], swap ? v[3] : v[1], swap ? v[0] : v[2], swap ? v[1] : v[3]};
-    *reinterpret_cast<u32x4*>(p + row * stride + (c ^ (row & 8))) = w;
+    return u32x4{swap ? v[2] : v[0], swap ? v[3] : v[1], swap ? v[0] : v[2], swap ? v[1] : v[3]};
   }
   // A lane's place for `row_split` (row n, elements 4 g on) and for `column_mixed` (as `column`); whole rows and multiples of 16
   // elements are added to it
@@ -255,9 +255,8 @@ struct Operand<float> {
   static __device__ __forceinline__ float score(const float* p, int) { return p[0]; }
   static __device__ __forceinline__ int at(int row, int c, int stride) { return row * stride + c; }
   static __device__ __forceinline__ int tile_at(int row, int c) { return row * 16 + c; }
-  static __device__ __forceinline__ void put_mixed(float* p, int row, int c, int stride, u32x4 v) {
-    *reinterpret_cast<u32x4*>(p + row * stride + c) = v;
-  }
+  static __device__ __forceinline__ int mixed_place(int row, int c, int stride) { return row * stride + c; }
+  static __device__ __forceinline__ u32x4 mixed(int, u32x4 v) { return v; }
   static __device__ __forceinline__ int row_place(int stride, int lane) { return (lane & 15) * stride + (lane >> 4 << 2); }
   static __device__ __forceinline__ int column_place(int stride, int lane) { return (lane >> 4 << 2) * stride + (lane & 15); }
   static __device__ __forceinline__ Frag column_mixed(const float* a, int stride) {
