@@ -459,6 +459,7 @@ extern "C" int ttc_delta_rule(const ttc_delta_rule_args* args, void* stream) {
   P.dk = !A.dk_out ? nullptr : dk_shared ? floats(ws, W.dk) : A.dk_out;
   P.dv = dv_shared ? nullptr : A.dv_out;
   P.dq_f32 = dq_shared || !bf16, P.dk_f32 = dk_shared || !bf16;
+  P.wide_dqk = A.dk % 4 == 0 && aligned16(P.dq) && aligned16(P.dk), P.wide_dv = A.dv % 8 == 0 && aligned16(P.dv);
   P.dgamma = A.d_log_gamma, P.dbeta = A.d_beta;
   if ((P.dq || P.dk || P.dv || P.dgamma || P.dbeta) && (rc = launch_delta_any(P, bf16, GRADIENTS, s))) return rc;
   const int64_t all = A.heads * A.dk, C = chunk_tokens(bf16), rows = W.chunks * C;

@@ -48,7 +48,7 @@ struct Delta {
   float *E, *dV;            // [C, vdp]
   // outputs of the gradients' kernel; fp32 for heads that share
   void *dq, *dk, *dv, *dgamma, *dbeta;
-  bool dq_f32, dk_f32;
+  bool dq_f32, dk_f32, wide_dqk, wide_dv;  // stores of 4 elements, of 8
 };
 
 template <class T>

@@ -644,192 +644,243 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
 // and with x_ts = P_ts L_ts - N_ts M_ts, f_s = e^{G_C - G_s} k_s . R E_s,
 //   db_s = sum_t x_ts + f_s,   dg_t = the sum over all terms of the loss's gradient that decay across token t: pairs s < t <= t',
 //   the state in front (into tokens from t on), the state behind (from tokens before t), and the state through the chunk.
-// Waves share the score tiles, then each takes 16 columns of the keys.  Lanes hold one token and 4 neighbouring columns.
-template <class T, int KD, int VD>
+// Values come 32 columns at a time, split into their parts once.  Waves share the score tiles, and each takes 16 columns of the
+// keys; its lanes hold one token and 4 neighbouring columns.
+template <class T, int KD>
 __global__ __launch_bounds__((KD / 16 * 64), 2) void delta_gradients_kernel(Delta A) {
   using Z = DeltaShape<T, KD>;
   using Op = Operand<T>;
   using Wide = typename Op::Wide;
+  using Pair = typename Op::Pair;
   using Frag = typename Op::Frag;
-  constexpr int C = Z::C, TT = Z::TT, KB = Z::KB, WAVES = KD / 16, NT = WAVES * 64, KS = Z::KS, VB = VD / 32;
-  constexpr int DS = VD + Op::ROW_PAD, ES = VD + 4, TILE = Z::TILES * 256;
-  __shared__ __attribute__((aligned(16))) T Ks[C * KS], Qs[C * KS], Ds[C * DS];
-  __shared__ __attribute__((aligned(16))) float Big[2 * C * ES > 2 * TILE ? 2 * C * ES : 2 * TILE];  // E and dV, then A and B
+  constexpr int C = Z::C, TT = Z::TT, KB = Z::KB, WAVES = KD / 16, NT = WAVES * 64, KS = Z::KS, MINE = (Z::TILES + WAVES - 1) / WAVES;
+  constexpr int W = 32, DS = W + Op::ROW_PAD, BLOCK = C * DS, PARTS = Op::WIDE_PARTS;  // columns of values, and their rows
+  constexpr int PLANE = Z::TILES * 256, SET = Op::SCORE_PARTS * PLANE, ROOM = (2 * PARTS + 1) * BLOCK;
+  __shared__ __attribute__((aligned(16))) T Ks[C * KS], Qs[C * KS];
+  __shared__ __attribute__((aligned(16))) T Big[ROOM > 4 * SET ? ROOM : 4 * SET];  // E, dV and dO, then A and B as they are used
   __shared__ __attribute__((aligned(16))) float Row[ROWS][C];
-  __shared__ float Part[TT][3][C];      // by tile: sums over s of b P L and of b N M (by si), over t of x (by ti)
-  __shared__ float Dot[WAVES][3][C];    // by wave: q . S dO, k . S dV, k . R E
+  __shared__ float Part[TT][3][C];    // by tile: sums over s of b P L and of b N M (by si), over t of x (by ti)
+  __shared__ float Dot[WAVES][3][C];  // by wave: q . S dO, k . S dV, k . R E
   __shared__ float Through[WAVES], Qd[C], Kd[C];
   __shared__ int Odd[WAVES];
-  float *Es = Big, *Vs = Big + C * ES;
+  T *Es = Big, *Vs = Big + PARTS * BLOCK, *Ds = Big + 2 * PARTS * BLOCK;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, n = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t unit = A.first + blockIdx.x, bh = unit / A.chunks, t0 = unit % A.chunks * C, b = bh / A.H;
-  const int h = (int)(bh % A.H), left = A.T - t0 < C ? (int)(A.T - t0) : C;
+  const int h = (int)(bh % A.H), left = A.T - t0 < C ? (int)(A.T - t0) : C, blocks = A.vdp / W;
+  uint32_t most = 0, most_f = 0;
   {
     Stage<T, KD, C, NT> k, q;
-    Stage<T, VD, C, NT> d;
     Stage<float, C, ROWS, NT> r;
-    Stage<float, VD, C, NT> e;
     k.fetch(A.k.at<T>(b, h) + t0 * A.k.st, A.k.st, A.kd, left, A.wide_k, tid);
     q.fetch(A.q.at<T>(b, h) + t0 * A.q.st, A.q.st, A.kd, left, A.wide_q, tid);
-    d.fetch(A.d_o.at<T>(b, h) + t0 * A.d_o.st, A.d_o.st, A.vd, left, A.wide_d, tid);
     r.fetch(A.rows + unit * ROWS * C, C, C, ROWS, true, tid);
-    uint32_t most = 0, mf = 0;
-    k.template put<KS>(Ks, tid);
-    q.template put<KS>(Qs, tid);
-    d.template put<DS>(Ds, tid);
+    k.template put_mixed<KS>(Ks, tid);
+    q.template put_mixed<KS>(Qs, tid);
     r.template put<C>(&Row[0][0], tid);
     k.largest(most);
     q.largest(most);
-    d.largest(most);
-    e.fetch(A.E + unit * C * A.vdp, A.vdp, A.vdp, C, true, tid);
-    e.template put<ES>(Es, tid);
-    e.largest(mf);
-    e.fetch(A.dV + unit * C * A.vdp, A.vdp, A.vdp, C, true, tid);
-    e.template put<ES>(Vs, tid);
-    e.largest(mf);
-    const bool odd = __ballot(!Op::finite(most) || !Operand<float>::finite(mf)) != 0;
-    if (lane == 0) Odd[wave] = odd;
+  }
+  // 8 neighbouring values of E and of dV a thread (UNITS of them)
+  constexpr int UNITS = (C * W / 8 + NT - 1) / NT;
+  u32x4 er[UNITS][2], vr[UNITS][2];
+  Stage<T, W, C, NT> dr;
+  auto fetch = [&](int d) {
+#pragma unroll
+    for (int j = 0; j < UNITS; ++j) {
+      const int u = tid + j * NT, row = u / 4 < C ? u / 4 : 0, c = d * W + u % 4 * 8;
+      const float *e = A.E + (unit * C + row) * A.vdp + c, *v = A.dV + (unit * C + row) * A.vdp + c;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) er[j][i] = reinterpret_cast<const u32x4*>(e)[i], vr[j][i] = reinterpret_cast<const u32x4*>(v)[i];
+    }
+    const int c0 = d * W;
+    dr.fetch(A.d_o.at<T>(b, h) + t0 * A.d_o.st + c0, A.d_o.st, A.vd - c0, left, A.wide_d, tid);
+  };
+  auto put = [&](int d) {
+#pragma unroll
+    for (int j = 0; j < UNITS; ++j) {
+      const int u = tid + j * NT, row = u / 4, c = u % 4 * 8;
+      if (row >= C) continue;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        Operand<float>::largest(er[j][i], most_f);
+        Operand<float>::largest(vr[j][i], most_f);
+        Op::put_wide(Es + row * DS + c + 4 * i, BLOCK, __builtin_bit_cast(f32x4, er[j][i]));
+        Op::put_wide(Vs + row * DS + c + 4 * i, BLOCK, __builtin_bit_cast(f32x4, vr[j][i]));
+      }
+      if (A.dv && row < left) {  // values' gradients, where each head has its own
+        T* to = static_cast<T*>(A.dv) + ((b * A.T + t0 + row) * A.H + h) * A.vd + d * W + c;
+        T f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = from_f<T>(__uint_as_float(vr[j][i / 4][i % 4]));
+        if (A.wide_dv && d * W + c < A.vd) {
+          __builtin_memcpy(__builtin_assume_aligned(to, 16), f, sizeof(f));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (d * W + c + i < A.vd) to[i] = f[i];
+        }
+      }
+    }
+    dr.template put<DS>(Ds, tid);
+    dr.largest(most);
+  };
+  auto wide_row = [&](const T* p, int row) {  // 8 neighbours
+    const T* at = p + row * DS + 8 * g;
+    if constexpr (PARTS == 3) return Wide{Op::row(at), Op::row(at + BLOCK), Op::row(at + 2 * BLOCK)};
+    else return Op::row(at);
+  };
+
+  // Over the columns of the values: L and M of the wave's tiles (lane: token t = n, 4 neighbouring s), and the state's parts S dO,
+  // S dV and R E (rows r0 + n of S and R; lane's token n, columns r0 + 4 g + i)
+  const int r0 = wave * 16;
+  f32x4 lt[MINE], mt[MINE], dq[TT], sv[TT], re[TT], dk[TT];
+#pragma unroll
+  for (int i = 0; i < MINE; ++i) lt[i] = mt[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int t = 0; t < TT; ++t) dq[t] = sv[t] = re[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const float *Sp = A.S + (unit * KD + r0 + n) * A.vdp + 8 * g, *Rp = A.R + (unit * KD + r0 + n) * A.vdp + 8 * g;
+  float through = 0.0f;
+  fetch(0);
+  for (int d = 0; d < blocks; ++d) {
+    f32x4 sr[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      sr[i] = reinterpret_cast<const f32x4*>(Sp + d * W)[i];
+      sr[2 + i] = reinterpret_cast<const f32x4*>(Rp + d * W)[i];
+    }
+    put(d);
+    __syncthreads();
+    if (d + 1 < blocks) fetch(d + 1);
+    int turn = 0;
+#pragma unroll
+    for (int ti = 0; ti < TT; ++ti)
+#pragma unroll
+      for (int si = 0; si <= ti; ++si, ++turn) {
+        if (turn % WAVES != wave) continue;
+        const Wide f = wide_row(Es, 16 * si + n);
+        lt[turn / WAVES] = Op::mma(f, Op::row(&Ds[(16 * ti + n) * DS + 8 * g]), lt[turn / WAVES]);
+        mt[turn / WAVES] = Op::mma(f, wide_row(Vs, 16 * ti + n), mt[turn / WAVES]);
+      }
+    float s8[8], r8[8];
+    eight(sr[0], sr[1], s8);
+    eight(sr[2], sr[3], r8);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) through = fmaf(s8[i], r8[i], through);
+    const Wide s = Op::wide(s8);
+    Wide f[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) f[t] = wide_row(Vs, 16 * t + n);
+    mma_right<Op, 0, TT>(s, f, sv);
+    Frag x[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) x[t] = Op::row(&Ds[(16 * t + n) * DS + 8 * g]);
+    mma_right<Op, 0, TT>(s, x, dq);
+    const Wide r = Op::wide(r8);
+#pragma unroll
+    for (int t = 0; t < TT; ++t) f[t] = wide_row(Es, 16 * t + n);
+    mma_right<Op, 0, TT>(r, f, re);
+    __syncthreads();
+  }
+  {
+    const bool odd_here = __ballot(!Op::finite(most) || !Operand<float>::finite(most_f)) != 0;
+    if (lane == 0) Odd[wave] = odd_here;
+  }
+
+  // the tiles: their sums, and A and B in the place of E, dV and dO, with the weights of what each is multiplied with
+  T *Ak = Big, *Aq = Big + SET, *Bs = Big + 2 * SET, *Bt = Big + 3 * SET;
+  const int rows_at = Op::row_place(KS, lane), columns_at = Op::column_place(KS, lane);
+  {
+    int turn = 0;
+#pragma unroll
+    for (int ti = 0; ti < TT; ++ti)
+#pragma unroll
+      for (int si = 0; si <= ti; ++si, ++turn) {
+        if (turn % WAVES != wave) continue;
+        f32x4 kk = {0.f, 0.f, 0.f, 0.f}, qk = kk;
+#pragma unroll
+        for (int d = 0; d < Z::DB; ++d) {
+          const Frag f = Op::row_split(Ks + rows_at + 16 * si * KS + 32 * d);
+          kk = Op::mma(f, Op::row_split(Ks + rows_at + 16 * ti * KS + 32 * d), kk);
+          qk = Op::mma(f, Op::row_split(Qs + rows_at + 16 * ti * KS + 32 * d), qk);
+        }
+        const int t = 16 * ti + n, s = 16 * si + 4 * g;
+        const Place at_t = {Row[HI][t], Row[LO][t], Row[PART][t]};
+        const float rk = Row[RK][t], rq = Row[RQ][t] * A.scale;
+        const f32x4 l = lt[turn / WAVES], m = mt[turn / WAVES];
+        float sum_p = 0.0f, sum_n = 0.0f, by_s[4];
+        f32x4 at, bt, as, bs;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float w = weight_of(at_t, Place{Row[HI][s + i], Row[LO][s + i], Row[PART][s + i]}), be = Row[BETA][s + i],
+                      rs = Row[RK][s + i];
+          const float pl = s + i <= t ? kept(w, rq * rs * qk[i] * l[i]) : 0.0f;
+          const float nm = s + i < t ? kept(w, rk * rs * kk[i] * m[i]) : 0.0f;
+          sum_p = s + i <= t && w != 0.0f ? fmaf(be, pl, sum_p) : sum_p;
+          sum_n = s + i < t && w != 0.0f ? fmaf(be, nm, sum_n) : sum_n;
+          by_s[i] = pl - nm;
+          at[i] = s + i <= t ? kept(w, be * l[i]) : 0.0f;
+          bt[i] = s + i < t ? kept(w, -be * m[i]) : 0.0f;
+          as[i] = at[i] * rs, bs[i] = bt[i] * rs;
+        }
+        const int tile = tile_of(ti, si) * 256 + Op::tile_at(n, 4 * g);
+        Op::put_scores(Ak + tile, PLANE, as);
+        Op::put_scores(Aq + tile, PLANE, at * rq);
+        Op::put_scores(Bs + tile, PLANE, bs);
+        Op::put_scores(Bt + tile, PLANE, bt * rk);
+        sum_p += __shfl_xor(sum_p, 16, 64);
+        sum_p += __shfl_xor(sum_p, 32, 64);
+        sum_n += __shfl_xor(sum_n, 16, 64);
+        sum_n += __shfl_xor(sum_n, 32, 64);
+        if (g == 0) Part[si][0][t] = sum_p, Part[si][1][t] = sum_n;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int x = 1; x <= 8; x <<= 1) by_s[i] += __shfl_xor(by_s[i], x, 64);
+          if (n == 0) Part[ti][2][s + i] = by_s[i];
+        }
+      }
+  }
+  // the state's parts with their weights, and their dots with q and k
+  auto four = [&](const T* p, int t) {  // the lane's columns of token t
+    struct alignas(4 * sizeof(T)) Four {
+      T v[4];
+    };
+    return *reinterpret_cast<const Four*>(p + Op::at(t, r0 + 4 * g, KS));
+  };
+  through = lane_sum(through, 64);
+  if (lane == 0) Through[wave] = through;
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    const int tt = 16 * t + n;
+    const float in = Row[IN][tt], up = Row[UP][tt], be = Row[BETA][tt], rq = Row[RQ][tt] * A.scale, rk = Row[RK][tt];
+    const auto q4 = four(Qs, tt), k4 = four(Ks, tt);
+    float c = 0.0f, d = 0.0f, f = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float qq = rq * to_f(q4.v[i]), kk = rk * to_f(k4.v[i]);
+      dq[t][i] = kept(in, dq[t][i]);
+      sv[t][i] = kept(in, sv[t][i]);
+      re[t][i] = kept(up, re[t][i]);
+      if (r0 + 4 * g + i < A.kd) {
+        c = in == 0.0f ? c : fmaf(qq, dq[t][i], c);
+        d = in == 0.0f ? d : fmaf(kk, sv[t][i], d);
+        f = up == 0.0f ? f : fmaf(kk, re[t][i], f);
+      }
+      dk[t][i] = up == 0.0f ? -sv[t][i] : be * re[t][i] - sv[t][i];
+    }
+    c += __shfl_xor(c, 16, 64);
+    c += __shfl_xor(c, 32, 64);
+    d += __shfl_xor(d, 16, 64);
+    d += __shfl_xor(d, 32, 64);
+    f += __shfl_xor(f, 16, 64);
+    f += __shfl_xor(f, 32, 64);
+    if (g == 0) Dot[wave][0][tt] = c, Dot[wave][1][tt] = d, Dot[wave][2][tt] = f;
   }
   __syncthreads();
   bool odd = A.odd[unit] != 0;
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) odd = odd || Odd[w];
-  auto wide_row = [&](const float* p) {  // 8 neighbours
-    const f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + 4);
-    float f[8];
-    eight(x, y, f);
-    return Op::wide(f);
-  };
-
-  // values' gradients, where each head has its own
-  if (A.dv) {
-    T* to = static_cast<T*>(A.dv) + ((b * A.T + t0) * A.H + h) * A.vd;
-    for (int i = tid; i < left * A.vd; i += NT) {
-      const int t = i / A.vd, c = i % A.vd;
-      to[(int64_t)t * A.H * A.vd + c] = from_f<T>(Vs[t * ES + c]);
-    }
-  }
-
-  // score tiles (lane: token t = n, 4 neighbouring s)
-  constexpr int MINE = (Z::TILES + WAVES - 1) / WAVES;
-  f32x4 At[MINE], Bt[MINE];
-  int turn = 0;
-#pragma unroll
-  for (int ti = 0; ti < TT; ++ti)
-#pragma unroll
-    for (int si = 0; si <= ti; ++si, ++turn) {
-      if (turn % WAVES != wave) continue;
-      f32x4 kk = {0.f, 0.f, 0.f, 0.f}, qk = kk, lt = kk, mt = kk;
-#pragma unroll
-      for (int d = 0; d < Z::DB; ++d) {
-        const Frag f = Op::row(&Ks[(16 * si + n) * KS + 32 * d + 8 * g]);
-        kk = Op::mma(f, Op::row(&Ks[(16 * ti + n) * KS + 32 * d + 8 * g]), kk);
-        qk = Op::mma(f, Op::row(&Qs[(16 * ti + n) * KS + 32 * d + 8 * g]), qk);
-      }
-#pragma unroll
-      for (int d = 0; d < VB; ++d) {
-        const Wide f = wide_row(&Es[(16 * si + n) * ES + 32 * d + 8 * g]);
-        lt = Op::mma(f, Op::row(&Ds[(16 * ti + n) * DS + 32 * d + 8 * g]), lt);
-        mt = Op::mma(f, wide_row(&Vs[(16 * ti + n) * ES + 32 * d + 8 * g]), mt);
-      }
-      const int t = 16 * ti + n, s = 16 * si + 4 * g;
-      const Place at_t = {Row[HI][t], Row[LO][t], Row[PART][t]};
-      const float rk = Row[RK][t], rq = Row[RQ][t] * A.scale;
-      float sum_p = 0.0f, sum_n = 0.0f, by_s[4];
-      f32x4 at, bt;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float w = weight_of(at_t, Place{Row[HI][s + i], Row[LO][s + i], Row[PART][s + i]}), be = Row[BETA][s + i], rs = Row[RK][s + i];
-        const float pl = s + i <= t ? kept(w, rq * rs * qk[i] * lt[i]) : 0.0f;
-        const float nm = s + i < t ? kept(w, rk * rs * kk[i] * mt[i]) : 0.0f;
-        sum_p = s + i <= t && w != 0.0f ? fmaf(be, pl, sum_p) : sum_p;
-        sum_n = s + i < t && w != 0.0f ? fmaf(be, nm, sum_n) : sum_n;
-        by_s[i] = pl - nm;
-        at[i] = s + i <= t ? kept(w, be * lt[i]) : 0.0f;
-        bt[i] = s + i < t ? kept(w, -be * mt[i]) : 0.0f;
-      }
-      At[turn / WAVES] = at, Bt[turn / WAVES] = bt;
-      sum_p += __shfl_xor(sum_p, 16, 64);
-      sum_p += __shfl_xor(sum_p, 32, 64);
-      sum_n += __shfl_xor(sum_n, 16, 64);
-      sum_n += __shfl_xor(sum_n, 32, 64);
-      if (g == 0) Part[si][0][t] = sum_p, Part[si][1][t] = sum_n;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int m = 1; m <= 8; m <<= 1) by_s[i] += __shfl_xor(by_s[i], m, 64);
-        if (n == 0) Part[ti][2][s + i] = by_s[i];
-      }
-    }
-
-  // the state's parts: S dO, S dV and R E (rows r0 + n of S and R, lane's token n, columns r0 + 4 g + i)
-  const int r0 = wave * 16;
-  f32x4 dq[TT], dk[TT];
-  {
-    f32x4 sv[TT], re[TT];
-#pragma unroll
-    for (int t = 0; t < TT; ++t) dq[t] = sv[t] = re[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const float *Sp = A.S + (unit * KD + r0 + n) * A.vdp + 8 * g, *Rp = A.R + (unit * KD + r0 + n) * A.vdp + 8 * g;
-    float through = 0.0f;
-#pragma unroll
-    for (int d = 0; d < VB; ++d) {
-      const f32x4 sa = *reinterpret_cast<const f32x4*>(Sp + 32 * d), sb = *reinterpret_cast<const f32x4*>(Sp + 32 * d + 4);
-      const f32x4 ra = *reinterpret_cast<const f32x4*>(Rp + 32 * d), rb = *reinterpret_cast<const f32x4*>(Rp + 32 * d + 4);
-      float s8[8], r8[8];
-      eight(sa, sb, s8);
-      eight(ra, rb, r8);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) through = fmaf(s8[i], r8[i], through);
-      const Wide s = Op::wide(s8), r = Op::wide(r8);
-#pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        dq[t] = Op::mma(s, Op::row(&Ds[(16 * t + n) * DS + 32 * d + 8 * g]), dq[t]);
-        sv[t] = Op::mma(s, wide_row(&Vs[(16 * t + n) * ES + 32 * d + 8 * g]), sv[t]);
-        re[t] = Op::mma(r, wide_row(&Es[(16 * t + n) * ES + 32 * d + 8 * g]), re[t]);
-      }
-    }
-    through = lane_sum(through, 64);
-    if (lane == 0) Through[wave] = through;
-#pragma unroll
-    for (int t = 0; t < TT; ++t) {
-      const int tt = 16 * t + n;
-      const float in = Row[IN][tt], up = Row[UP][tt], be = Row[BETA][tt], rq = Row[RQ][tt] * A.scale, rk = Row[RK][tt];
-      float c = 0.0f, d = 0.0f, f = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float qq = rq * to_f(Qs[tt * KS + r0 + 4 * g + i]), kk = rk * to_f(Ks[tt * KS + r0 + 4 * g + i]);
-        dq[t][i] = kept(in, dq[t][i]);
-        sv[t][i] = kept(in, sv[t][i]);
-        re[t][i] = kept(up, re[t][i]);
-        if (r0 + 4 * g + i < A.kd) {
-          c = in == 0.0f ? c : fmaf(qq, dq[t][i], c);
-          d = in == 0.0f ? d : fmaf(kk, sv[t][i], d);
-          f = up == 0.0f ? f : fmaf(kk, re[t][i], f);
-        }
-        dk[t][i] = be * re[t][i] - sv[t][i];
-        if (up == 0.0f) dk[t][i] = -sv[t][i];
-      }
-      c += __shfl_xor(c, 16, 64);
-      c += __shfl_xor(c, 32, 64);
-      d += __shfl_xor(d, 16, 64);
-      d += __shfl_xor(d, 32, 64);
-      f += __shfl_xor(f, 16, 64);
-      f += __shfl_xor(f, 32, 64);
-      if (g == 0) Dot[wave][0][tt] = c, Dot[wave][1][tt] = d, Dot[wave][2][tt] = f;
-    }
-  }
-  __syncthreads();  // E and dV have been read: their place is A's and B's
-  float *As = Big, *Bs = Big + TILE;
-  turn = 0;
-#pragma unroll
-  for (int ti = 0; ti < TT; ++ti)
-#pragma unroll
-    for (int si = 0; si <= ti; ++si, ++turn) {
-      if (turn % WAVES != wave) continue;
-      *reinterpret_cast<f32x4*>(&As[tile_of(ti, si) * 256 + n * 16 + 4 * g]) = At[turn / WAVES];
-      *reinterpret_cast<f32x4*>(&Bs[tile_of(ti, si) * 256 + n * 16 + 4 * g]) = Bt[turn / WAVES];
-    }
   // one wave: what a token's sums come to, and the gradients of its decay and strength
   if (wave == 0) {
     const int t = lane < C ? lane : C - 1, own = t / 16;
@@ -873,86 +924,88 @@ __global__ __launch_bounds__((KD / 16 * 64), 2) void delta_gradients_kernel(Delt
       }
     }
   }
-  __syncthreads();
   if (!odd) {
-#pragma unroll
-    for (int s = 0; s < KB; ++s) {
-      const Frag kf = Op::column(&Ks[32 * s * KS], KS, r0, lane), qf = Op::column(&Qs[32 * s * KS], KS, r0, lane);
-      float rk[8], rq[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int t = 32 * s + (j < 4 ? 0 : 16) + 4 * g + j % 4;
-        rk[j] = Row[RK][t], rq[j] = Row[RQ][t] * A.scale;
-      }
-      auto times = [&](float(&x)[8], const float(&w)[8]) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] *= w[j];
-        return Op::pair(x);
+    unrolled<KB>([&](auto s_) {
+      constexpr int s = decltype(s_)::value;
+      const Frag kf = Op::column_mixed(Ks + columns_at + 32 * s * KS + r0, KS);
+      const Frag qf = Op::column_mixed(Qs + columns_at + 32 * s * KS + r0, KS);
+      auto behind = [&](const T* p, int t) {  // the tokens of block s in front of token tile t
+        return Op::template pair_tiles<true>(true, p + tile_of(t, 2 * s) * 256, 2 * s < t, p + tile_of(t, 2 * s + 1) * 256, PLANE, lane);
       };
+      auto ahead = [&](const T* p, int t) {  // those behind it
+        return Op::template pair_tiles<false>(2 * s >= t, p + tile_of(2 * s, t) * 256, true, p + tile_of(2 * s + 1, t) * 256, PLANE, lane);
+      };
+      Pair f[TT];
 #pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        float x[8];
-        if (s <= t / 2) {  // tokens s in front of t
-          triangle<true, TT>(As, t, s, lane, x);
-          dq[t] = Op::mma(kf, times(x, rk), dq[t]);
-          triangle<true, TT>(Bs, t, s, lane, x);
-          dk[t] = Op::mma(kf, times(x, rk), dk[t]);
-        }
-        if (s >= t / 2) {  // tokens behind t
-          triangle<false, TT>(As, t, s, lane, x);
-          dk[t] = Op::mma(qf, times(x, rq), dk[t]);
-          triangle<false, TT>(Bs, t, s, lane, x);
-          dk[t] = Op::mma(kf, times(x, rk), dk[t]);
-        }
-      }
-    }
+      for (int t = 2 * s; t < TT; ++t) f[t] = behind(Ak, t);
+      mma_right<Op, 2 * s, TT>(kf, f, dq);
+#pragma unroll
+      for (int t = 2 * s; t < TT; ++t) f[t] = behind(Bs, t);
+      mma_right<Op, 2 * s, TT>(kf, f, dk);
+#pragma unroll
+      for (int t = 0; t < 2 * s + 2; ++t) f[t] = ahead(Aq, t);
+      mma_right<Op, 0, 2 * s + 2>(qf, f, dk);
+#pragma unroll
+      for (int t = 0; t < 2 * s + 2; ++t) f[t] = ahead(Bt, t);
+      mma_right<Op, 0, 2 * s + 2>(kf, f, dk);
+    });
   } else {  // term by term, without those whose weight is 0
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
       const int tt = 16 * t + n;
       for (int s = 0; s < C; ++s) {
-        const int r = s > tt ? s : tt, c = s > tt ? tt : s;
-        const int at = tile_of(r / 16, c / 16) * 256 + r % 16 * 16 + c % 16;
-        const float a = As[at], bb = Bs[at], rk = Row[RK][s], rq = Row[RQ][s] * A.scale;
+        const int r = s > tt ? s : tt, c = s > tt ? tt : s, at = tile_of(r / 16, c / 16) * 256 + Op::tile_at(r % 16, c % 16);
+        const float ak = Op::score(Ak + at, PLANE), aq = Op::score(Aq + at, PLANE), bs = Op::score(Bs + at, PLANE),
+                    bt = Op::score(Bt + at, PLANE);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float kk = rk * to_f(Ks[s * KS + r0 + 4 * g + i]), qq = rq * to_f(Qs[s * KS + r0 + 4 * g + i]);
-          if (s <= tt && a != 0.0f) dq[t][i] = fmaf(a, kk, dq[t][i]);
-          if (s >= tt && a != 0.0f) dk[t][i] = fmaf(a, qq, dk[t][i]);
-          if (bb != 0.0f) dk[t][i] = fmaf(bb, kk, dk[t][i]);
+          const float kk = to_f(Ks[Op::at(s, r0 + 4 * g + i, KS)]), qq = to_f(Qs[Op::at(s, r0 + 4 * g + i, KS)]);
+          if (s <= tt && ak != 0.0f) dq[t][i] = fmaf(ak, kk, dq[t][i]);
+          if (s >= tt && aq != 0.0f) dk[t][i] = fmaf(aq, qq, dk[t][i]);
+          if (s < tt && bs != 0.0f) dk[t][i] = fmaf(bs, kk, dk[t][i]);
+          if (s > tt && bt != 0.0f) dk[t][i] = fmaf(bt, kk, dk[t][i]);
         }
       }
     }
   }
+  __syncthreads();  // Qd and Kd
 #pragma unroll
   for (int t = 0; t < TT; ++t) {
     const int tt = 16 * t + n;
     const float rk = Row[RK][tt], rq = Row[RQ][tt];
+    if (A.normalize) {  // the part along the vector itself is no change
+      const auto q4 = four(Qs, tt), k4 = four(Ks, tt);
+      const float along_q = -Qd[tt] * (rq * rq), along_k = -Kd[tt] * rk;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = r0 + 4 * g + i;
-      const float qq = to_f(Qs[tt * KS + c]), kk = to_f(Ks[tt * KS + c]);
-      dq[t][i] *= rq * A.scale;
-      if (A.normalize) {  // the part along the vector itself is no change
-        dq[t][i] = fmaf(-qq * (rq * rq), Qd[tt], dq[t][i]);
-        dk[t][i] = rk * fmaf(-kk * rk, Kd[tt], dk[t][i]);
+      for (int i = 0; i < 4; ++i) {
+        dq[t][i] = fmaf(to_f(q4.v[i]), along_q, dq[t][i] * (rq * A.scale));
+        dk[t][i] = rk * fmaf(to_f(k4.v[i]), along_k, dk[t][i]);
       }
+    } else {
+      dq[t] *= A.scale;
     }
     if (tt >= left) continue;
     const int64_t at = ((b * A.T + t0 + tt) * A.H + h) * A.kd + r0 + 4 * g;
-    auto put = [&](auto* to, const f32x4& x) {
+    auto store = [&](auto* to, const f32x4& x) {
       using Y = std::remove_pointer_t<decltype(to)>;
+      Y f[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (r0 + 4 * g + i < A.kd) to[at + i] = from_f<Y>(x[i]);
+      for (int i = 0; i < 4; ++i) f[i] = from_f<Y>(x[i]);
+      if (A.wide_dqk && r0 + 4 * g < A.kd) {
+        __builtin_memcpy(__builtin_assume_aligned(to + at, 4 * sizeof(Y)), f, sizeof(f));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (r0 + 4 * g + i < A.kd) to[at + i] = f[i];
+      }
     };
     if (A.dq) {
-      if (A.dq_f32) put(static_cast<float*>(A.dq), dq[t]);
-      else put(static_cast<T*>(A.dq), dq[t]);
+      if (A.dq_f32) store(static_cast<float*>(A.dq), dq[t]);
+      else store(static_cast<T*>(A.dq), dq[t]);
     }
     if (A.dk) {
-      if (A.dk_f32) put(static_cast<float*>(A.dk), dk[t]);
-      else put(static_cast<T*>(A.dk), dk[t]);
+      if (A.dk_f32) store(static_cast<float*>(A.dk), dk[t]);
+      else store(static_cast<T*>(A.dk), dk[t]);
     }
   }
 }
@@ -986,12 +1039,12 @@ int launch_delta_sweeps(const Delta& A, hipStream_t s) {
   return launch_delta_sweep<T, KD, 4, BACK>(A, s);
 }
 
-template <class T, int KD, int VD>
+template <class T, int KD>
 int launch_delta_gradients(const Delta& A, hipStream_t s) {
   return in_launches(A.B * A.H * A.chunks, KD / 16 * 64, [&](int64_t first, dim3 grid) {
     Delta P = A;
     P.first = first;
-    hipLaunchKernelGGL((delta_gradients_kernel<T, KD, VD>), grid, dim3(KD / 16 * 64), 0, s, P);
+    hipLaunchKernelGGL((delta_gradients_kernel<T, KD>), grid, dim3(KD / 16 * 64), 0, s, P);
   });
 }
 
@@ -1005,9 +1058,7 @@ int launch_delta(const Delta& A, int what, hipStream_t s) {
     });
   if (what == SWEEP) return launch_delta_sweeps<T, KD, false>(A, s);
   if (what == SWEEP_BACK) return launch_delta_sweeps<T, KD, true>(A, s);
-  return A.vd <= 32   ? launch_delta_gradients<T, KD, 32>(A, s)
-         : A.vd <= 64 ? launch_delta_gradients<T, KD, 64>(A, s)
-                      : launch_delta_gradients<T, KD, 128>(A, s);
+  return launch_delta_gradients<T, KD>(A, s);
 }
 
 }  // namespace ttc
