@@ -124,11 +124,11 @@ __device__ __forceinline__ void unrolled(F f) {
 // ---- prepare: decays, lengths, scores and the triangle's inverse, one workgroup a chunk ----------------------------
 
 // acc + a b of 16 x 16 blocks in fp32
-__device__ __forceinline__ f32x4 block_mma(const float* a, const float* b, int stride, f32x4 acc, int lane) {
+__device__ __forceinline__ f32x4 block_mma(const float* a, int stride_a, const float* b, int stride_b, f32x4 acc, int lane) {
   const int g = lane >> 4, n = lane & 15;
 #pragma unroll
   for (int s = 0; s < 4; ++s)
-    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[n * stride + 4 * s + g], b[(4 * s + g) * stride + n], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[n * stride_a + 4 * s + g], b[(4 * s + g) * stride_b + n], acc, 0, 0, 0);
   return acc;
 }
 
@@ -136,9 +136,14 @@ template <class T, int KD>
 __global__ __launch_bounds__(256) void delta_prepare_kernel(Delta A) {
   using Z = DeltaShape<T, KD>;
   using Op = Operand<T>;
-  constexpr int C = Z::C, TT = Z::TT, QS = Z::QS, LS = C + 4, SUB = 256 / C;
-  __shared__ __attribute__((aligned(16))) T Ks[C * QS], Qs[C * QS];
-  __shared__ __attribute__((aligned(16))) float Lm[C * LS], Tm[C * LS];
+  constexpr int C = Z::C, TT = Z::TT, QS = Z::QS, LS = C + 4, SUB = 256 / C, BS = 20;
+  // Tiles of N b (rows of BS), and the inverse in the place of keys and queries, which are not needed any more: four workgroups a
+  // CU for keys of up to 64 (4,096 chunks: 52 us, with a place of its own, two workgroups: 77), three for 128
+  constexpr int ROOM = 2 * C * QS * (int)sizeof(T) > C * LS * 4 ? 2 * C * QS * (int)sizeof(T) : C * LS * 4;
+  __shared__ __attribute__((aligned(16))) char Room[ROOM];
+  __shared__ __attribute__((aligned(16))) float Lm[Z::TILES * 16 * BS];
+  T *Ks = reinterpret_cast<T*>(Room), *Qs = Ks + C * QS;
+  float* Tm = reinterpret_cast<float*>(Room);
   __shared__ __attribute__((aligned(16))) float Row[ROWS][C];
   __shared__ int Odd[4];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, n = lane & 15;
@@ -235,19 +240,19 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(Delta A) {
         kk[i] = s + i < t ? kept(w, kk[i] * rk * by) : 0.0f;
         qk[i] = s + i <= t ? kept(w, qk[i] * rq * by) : 0.0f;
       }
-      *reinterpret_cast<f32x4*>(&Lm[t * LS + s]) = kk;
+      *reinterpret_cast<f32x4*>(&Lm[(tile_of(ti, si) * 16 + n) * BS + 4 * g]) = kk;
       Op::put_wide(scores + tile_of(ti, si) * 256 + Op::tile_at(n, 4 * g), PLANE, qk);
     }
   __syncthreads();
   // the diagonal blocks' inverses: a lane's column by forward substitution
   if (wave == 0 && lane < C) {
-    const float* L = Lm + (lane & ~15) * (LS + 1);
+    const float* L = Lm + tile_of(lane >> 4, lane >> 4) * 16 * BS;
     float x[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float a = i == n ? 1.0f : 0.0f;
 #pragma unroll
-      for (int j = 0; j < i; ++j) a = fmaf(-L[i * LS + j], x[j], a);
+      for (int j = 0; j < i; ++j) a = fmaf(-L[i * BS + j], x[j], a);
       x[i] = a;
       Tm[((lane & ~15) + i) * LS + lane] = a;
     }
@@ -260,22 +265,23 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(Delta A) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) Tm[(16 * r + 4 * g + i) * LS + 16 * c + n] = sign * x[i];
   };
-  auto block = [&](const float* m, int r, int c) { return m + 16 * r * LS + 16 * c; };
+  auto inv = [&](int r, int c) { return Tm + 16 * r * LS + 16 * c; };
+  auto low = [&](int r, int c) { return Lm + tile_of(r, c) * 16 * BS; };
   if (wave < TT / 2)
-    put(2 * wave, 2 * wave + 1, block_mma(block(Lm, 2 * wave + 1, 2 * wave), block(Tm, 2 * wave, 2 * wave), LS, none, lane), 1.0f);
+    put(2 * wave, 2 * wave + 1, block_mma(low(2 * wave + 1, 2 * wave), BS, inv(2 * wave, 2 * wave), LS, none, lane), 1.0f);
   __syncthreads();
   if (wave < TT / 2)
-    put(2 * wave + 1, 2 * wave, block_mma(block(Tm, 2 * wave + 1, 2 * wave + 1), block(Tm, 2 * wave, 2 * wave + 1), LS, none, lane),
+    put(2 * wave + 1, 2 * wave, block_mma(inv(2 * wave + 1, 2 * wave + 1), LS, inv(2 * wave, 2 * wave + 1), LS, none, lane),
         -1.0f);
   if constexpr (TT == 4) {
     const int r = wave >> 1, c = wave & 1;
     __syncthreads();
     f32x4 x = none;
-    for (int k = c; k < 2; ++k) x = block_mma(block(Lm, 2 + r, k), block(Tm, k, c), LS, x, lane);
+    for (int k = c; k < 2; ++k) x = block_mma(low(2 + r, k), BS, inv(k, c), LS, x, lane);
     put(r, 2 + c, x, 1.0f);
     __syncthreads();
     x = none;
-    for (int k = 0; k <= r; ++k) x = block_mma(block(Tm, 2 + r, 2 + k), block(Tm, k, 2 + c), LS, x, lane);
+    for (int k = 0; k <= r; ++k) x = block_mma(inv(2 + r, 2 + k), LS, inv(k, 2 + c), LS, x, lane);
     put(2 + r, c, x, -1.0f);
   }
   __syncthreads();
