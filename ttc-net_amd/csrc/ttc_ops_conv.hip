@@ -3,7 +3,7 @@
 //   w = [state; x] (taps - 1 rows more than x),  p_t = bias + sum_j c_j w_{t + j},  y_t = act(p_t)
 // and with e_t = dy_t act'(p_t), zero outside [0, T),
 //   dw_i = sum_j c_j e_{i - j} (+ the final state's gradient),  dc_j = sum_t e_t w_{t + j},  dbias = sum_t e_t.
-// A thread holds 16 bytes of neighbouring channels and walks along a run of tokens with the last `taps` rows in registers,
+// A thread holds 4 neighbouring channels and walks along a run of tokens with the last `taps` rows in registers,
 // so that a row is read from memory once (and once more from the caches at the start of each run).
 #include "ttc_ops_common.hpp"
 
@@ -14,7 +14,7 @@ constexpr int MAX_TAPS = TTC_CAUSAL_CONV_MAX_TAPS;
 struct Conv {
   const void *x, *weight, *bias, *state;
   int64_t xb, xt, B, T, C;
-  bool weight_bf16;
+  bool weight_bf16, wide_weight;
   void *y, *final_state;
   const void *dy, *dfinal;
   int64_t yb, yt;
@@ -28,6 +28,16 @@ template <class T, int V>
 struct alignas(V * sizeof(T)) Vec {
   T v[V];
 };
+
+// 1 / (1 + e^-z): the reciprocal as one instruction, off by one unit in the last place, as an exact division costs as much as all
+// taps (16,381 tokens x 6,144 channels: 151 us, so 96)
+__device__ __forceinline__ float gate(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
+
+template <class T, int V>
+__device__ __forceinline__ void floats(const Vec<T, V>& a, float (&f)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) f[i] = to_f(a.v[i]);
+}
 
 template <class T, int V>
 __device__ __forceinline__ void get(const T* p, float (&f)[V]) {
@@ -44,32 +54,49 @@ __device__ __forceinline__ void put(T* p, const float (&f)[V]) {
   *reinterpret_cast<Vec<T, V>*>(p) = a;
 }
 
-__device__ __forceinline__ float param(const void* p, bool bf16, int64_t i) {
-  return bf16 ? to_f(static_cast<const __bf16*>(p)[i]) : static_cast<const float*>(p)[i];
+// A thread's V K taps lie one after the other: 16 bytes at a time where they can be (`wide`; the 32 of 8 channels in bf16 one by
+// one: prompt of 16,381 tokens x 6,144 channels 204 us, so 84)
+template <class W, int K, int V>
+__device__ __forceinline__ void taps_from(const W* p, bool wide, float (&w)[K][V]) {
+  constexpr int E = 16 / sizeof(W);
+  if constexpr (V > 1 && K * V % E == 0) {
+    if (wide) {
+#pragma unroll
+      for (int k = 0; k < K * V / E; ++k) {
+        const Vec<W, E> a = reinterpret_cast<const Vec<W, E>*>(p)[k];
+#pragma unroll
+        for (int i = 0; i < E; ++i) w[(k * E + i) % K][(k * E + i) / K] = to_f(a.v[i]);
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int j = 0; j < K; ++j) w[j][i] = to_f(p[i * K + j]);
 }
 
 template <int K, int V>
-__device__ __forceinline__ void weights(const void* weight, const void* bias, bool bf16, int64_t c, float (&w)[K][V],
-                                        float (&b)[V]) {
+__device__ __forceinline__ void weights(const Conv& A, int64_t c, float (&w)[K][V], float (&b)[V]) {
+  if (A.weight_bf16) taps_from<__bf16, K, V>(static_cast<const __bf16*>(A.weight) + c * K, A.wide_weight, w);
+  else taps_from<float, K, V>(static_cast<const float*>(A.weight) + c * K, A.wide_weight, w);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
+  for (int i = 0; i < V; ++i) b[i] = 0.0f;
+  if (A.bias == nullptr) return;
 #pragma unroll
-    for (int j = 0; j < K; ++j) w[j][i] = param(weight, bf16, (c + i) * K + j);
-    b[i] = bias ? param(bias, bf16, c + i) : 0.0f;
-  }
+  for (int i = 0; i < V; ++i)
+    b[i] = A.weight_bf16 ? to_f(static_cast<const __bf16*>(A.bias)[c + i]) : static_cast<const float*>(A.bias)[c + i];
 }
 
 // row i of w = [state; x], for 0 <= i < T + K - 1
 template <class T, int K, int V>
-__device__ __forceinline__ void wide_row(const Conv& A, int64_t b, int64_t i, int64_t c, float (&f)[V]) {
-  if (i >= K - 1) {
-    get<T, V>(static_cast<const T*>(A.x) + b * A.xb + (i - (K - 1)) * A.xt + c, f);
-  } else if (A.state) {
-    get<T, V>(static_cast<const T*>(A.state) + (b * (K - 1) + i) * A.C + c, f);
-  } else {
+__device__ __forceinline__ Vec<T, V> wide_row(const Conv& A, int64_t b, int64_t i, int64_t c) {
+  if (i >= K - 1) return *reinterpret_cast<const Vec<T, V>*>(static_cast<const T*>(A.x) + b * A.xb + (i - (K - 1)) * A.xt + c);
+  if (A.state) return *reinterpret_cast<const Vec<T, V>*>(static_cast<const T*>(A.state) + (b * (K - 1) + i) * A.C + c);
+  Vec<T, V> none;
 #pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = 0.0f;
-  }
+  for (int j = 0; j < V; ++j) none.v[j] = from_f<T>(0.0f);
+  return none;
 }
 
 template <int K, int V>
@@ -82,41 +109,50 @@ __device__ __forceinline__ void taps_of(const float (&w)[K][V], const float (&b)
   }
 }
 
-constexpr int FORWARD_RUN = 8;  // tokens a thread
+constexpr int FORWARD_RUN = 16;  // tokens a thread
 
-// All rows of a run are asked for at once.
+// All rows of a run are asked for at once, and taken from 16 bits when their turn comes.
 template <class T, int K, int V, bool SILU>
 __global__ __launch_bounds__(256) void conv_kernel(Conv A, int64_t first, int64_t items) {
   const int64_t item = (first + blockIdx.x) * 256 + threadIdx.x;
   if (item >= items) return;
   const int64_t c = item % A.cols * V, rest = item / A.cols, run = rest % A.runs, b = rest / A.runs;
   const int64_t t0 = run * FORWARD_RUN, last = A.T + K - 2;  // of w's rows
-  float w[K][V], bias[V], rows[FORWARD_RUN + K - 1][V];
+  Vec<T, V> rows[FORWARD_RUN + K - 1];
+  float w[K][V], bias[V], now[K][V];
+  if (t0 >= K - 1) {
+    const T* x = static_cast<const T*>(A.x) + b * A.xb + (t0 - (K - 1)) * A.xt + c;
+    const int left = last - t0 < FORWARD_RUN + K - 2 ? (int)(last - t0) : FORWARD_RUN + K - 2;
 #pragma unroll
-  for (int i = 0; i < FORWARD_RUN + K - 1; ++i) wide_row<T, K, V>(A, b, t0 + i < last ? t0 + i : last, c, rows[i]);
-  weights<K, V>(A.weight, A.bias, A.weight_bf16, c, w, bias);
+    for (int i = 0; i < FORWARD_RUN + K - 1; ++i) rows[i] = *reinterpret_cast<const Vec<T, V>*>(x + (i < left ? i : left) * A.xt);
+  } else {
+#pragma unroll
+    for (int i = 0; i < FORWARD_RUN + K - 1; ++i) rows[i] = wide_row<T, K, V>(A, b, t0 + i < last ? t0 + i : last, c);
+  }
+  weights<K, V>(A, c, w, bias);
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j) floats(rows[j], now[j + 1]);
 #pragma unroll
   for (int i = 0; i < FORWARD_RUN; ++i) {
     if (t0 + i >= A.T) break;
-    float now[K][V], p[V];
+    float p[V];
 #pragma unroll
-    for (int j = 0; j < K; ++j)
+    for (int j = 0; j + 1 < K; ++j)
 #pragma unroll
-      for (int k = 0; k < V; ++k) now[j][k] = rows[i + j][k];
+      for (int k = 0; k < V; ++k) now[j][k] = now[j + 1][k];
+    floats(rows[i + K - 1], now[K - 1]);
     taps_of<K, V>(w, bias, now, p);
     if (SILU) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) p[k] *= sigmoid(p[k]);
+      for (int k = 0; k < V; ++k) p[k] *= gate(p[k]);
     }
     put<T, V>(static_cast<T*>(A.y) + (b * A.T + t0 + i) * A.C + c, p);
   }
   if (K > 1 && A.final_state && run == A.runs - 1) {
 #pragma unroll
-    for (int i = 0; i < K - 1; ++i) {
-      float f[V];
-      wide_row<T, K, V>(A, b, A.T + i, c, f);
-      put<T, V>(static_cast<T*>(A.final_state) + (b * (K - 1) + i) * A.C + c, f);
-    }
+    for (int i = 0; i < K - 1; ++i)
+      *reinterpret_cast<Vec<T, V>*>(static_cast<T*>(A.final_state) + (b * (K - 1) + i) * A.C + c) =
+          wide_row<T, K, V>(A, b, A.T + i, c);
   }
 }
 
@@ -138,64 +174,86 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(Conv A, int64_t firs
     for (int i = 0; i < V; ++i) dw[j][i] = 0.0f;
   if (here) {
     float w[K][V], bias[V], rows[K][V], e[K][V];  // rows t .. t + K - 1 of w; e of tokens t - K + 1 .. t
-    weights<K, V>(A.weight, A.bias, A.weight_bf16, c, w, bias);
     const int64_t t0 = run * A.run, t1 = t0 + A.run < N ? t0 + A.run : N, lead = t0 - (K - 1) > 0 ? t0 - (K - 1) : 0;
+    const T *x = static_cast<const T*>(A.x) + b * A.xb + c, *dy = static_cast<const T*>(A.dy) + b * A.yb + c;
+    constexpr int AHEAD = 4;  // tokens that are on their way while as many are worked on
+    Vec<T, V> xs[AHEAD], ds[AHEAD];
+    auto fetch = [&](int64_t t) {
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        if (A.T == 0) break;
+        const int64_t at = t + u < A.T ? t + u : A.T - 1;
+        xs[u] = *reinterpret_cast<const Vec<T, V>*>(x + at * A.xt);
+        ds[u] = *reinterpret_cast<const Vec<T, V>*>(dy + at * A.yt);
+      }
+    };
+    fetch(lead);
+    weights<K, V>(A, c, w, bias);
 #pragma unroll
     for (int j = 0; j < K; ++j)
 #pragma unroll
       for (int i = 0; i < V; ++i) e[j][i] = rows[j][i] = 0.0f;
 #pragma unroll
     for (int j = 1; j < K; ++j)
-      if (lead + j - 1 < N) wide_row<T, K, V>(A, b, lead + j - 1, c, rows[j]);
-    const T* dy = static_cast<const T*>(A.dy) + b * A.yb + c;
-    for (int64_t t = lead; t < t1; ++t) {
+      if (lead + j - 1 < N) floats(wide_row<T, K, V>(A, b, lead + j - 1, c), rows[j]);
+    for (int64_t first_t = lead; first_t < t1; first_t += AHEAD) {
+      Vec<T, V> x_now[AHEAD], d_now[AHEAD];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
+      for (int u = 0; u < AHEAD; ++u) x_now[u] = xs[u], d_now[u] = ds[u];
+      if (first_t + AHEAD < t1) fetch(first_t + AHEAD);
 #pragma unroll
-        for (int j = 0; j + 1 < K; ++j) rows[j][i] = rows[j + 1][i], e[j][i] = e[j + 1][i];
-        e[K - 1][i] = 0.0f;
-      }
-      if (t < A.T) {
-        float p[V], d[V];
-        wide_row<T, K, V>(A, b, t + K - 1, c, rows[K - 1]);
-        get<T, V>(dy + t * A.yt, d);
-        if (SILU) {
-          taps_of<K, V>(w, bias, rows, p);
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float s = sigmoid(p[i]);
-            d[i] *= s * fmaf(p[i], 1.0f - s, 1.0f);
-          }
-        }
+      for (int u = 0; u < AHEAD; ++u) {
+        const int64_t t = first_t + u;
+        if (t >= t1) break;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          e[K - 1][i] = d[i];
-          if (t >= t0) {
 #pragma unroll
-            for (int j = 0; j < K; ++j) dw[j][i] = fmaf(d[i], rows[j][i], dw[j][i]);
-            dw[K][i] += d[i];
+          for (int j = 0; j + 1 < K; ++j) rows[j][i] = rows[j + 1][i], e[j][i] = e[j + 1][i];
+          e[K - 1][i] = 0.0f;
+        }
+        if (t < A.T) {
+          float p[V], d[V];
+          floats(x_now[u], rows[K - 1]);
+          floats(d_now[u], d);
+          if (SILU) {
+            taps_of<K, V>(w, bias, rows, p);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              const float s = gate(p[i]);
+              d[i] *= s * fmaf(p[i], 1.0f - s, 1.0f);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            e[K - 1][i] = d[i];
+            if (t >= t0) {
+#pragma unroll
+              for (int j = 0; j < K; ++j) dw[j][i] = fmaf(d[i], rows[j][i], dw[j][i]);
+              dw[K][i] += d[i];
+            }
           }
         }
-      }
-      if (t < t0) continue;
-      float g[V];
+        if (t < t0) continue;
+        float g[V];
+        const bool inner = t >= K - 1 && t < A.T;  // all taps meet tokens
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        g[i] = 0.0f;
+        for (int i = 0; i < V; ++i) {
+          g[i] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < K; ++j)  // of tokens that exist: a tap may be infinite
-          g[i] = t - j >= 0 && t - j < A.T ? fmaf(w[j][i], e[K - 1 - j][i], g[i]) : g[i];
-      }
-      if (t >= A.T && A.dfinal) {
-        float f[V];
-        get<T, V>(static_cast<const T*>(A.dfinal) + (b * (K - 1) + t - A.T) * A.C + c, f);
+          for (int j = 0; j < K; ++j)  // of tokens that exist: a tap may be infinite
+            g[i] = inner || (t - j >= 0 && t - j < A.T) ? fmaf(w[j][i], e[K - 1 - j][i], g[i]) : g[i];
+        }
+        if (t >= A.T && A.dfinal) {
+          float f[V];
+          get<T, V>(static_cast<const T*>(A.dfinal) + (b * (K - 1) + t - A.T) * A.C + c, f);
 #pragma unroll
-        for (int i = 0; i < V; ++i) g[i] += f[i];
-      }
-      if (t >= K - 1) {
-        if (A.dx) put<T, V>(static_cast<T*>(A.dx) + (b * A.T + t - (K - 1)) * A.C + c, g);
-      } else if (A.dstate) {
-        put<T, V>(static_cast<T*>(A.dstate) + (b * (K - 1) + t) * A.C + c, g);
+          for (int i = 0; i < V; ++i) g[i] += f[i];
+        }
+        if (t >= K - 1) {
+          if (A.dx) put<T, V>(static_cast<T*>(A.dx) + (b * A.T + t - (K - 1)) * A.C + c, g);
+        } else if (A.dstate) {
+          put<T, V>(static_cast<T*>(A.dstate) + (b * (K - 1) + t) * A.C + c, g);
+        }
       }
     }
   }
@@ -260,11 +318,11 @@ __global__ __launch_bounds__(256) void conv_step_kernel(Conv A, const int32_t* _
 #pragma unroll
   for (int j = 0; j < K - 1; ++j) get<T, V>(state + j * A.C, rows[j]);
   get<T, V>(static_cast<const T*>(A.x) + b * A.xb + c, rows[K - 1]);
-  weights<K, V>(A.weight, A.bias, A.weight_bf16, c, w, bias);
+  weights<K, V>(A, c, w, bias);
   taps_of<K, V>(w, bias, rows, p);
   if (SILU) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) p[i] *= sigmoid(p[i]);
+    for (int i = 0; i < V; ++i) p[i] *= gate(p[i]);
   }
   put<T, V>(y, p);
 #pragma unroll
@@ -313,15 +371,19 @@ inline int64_t backward_run(const ttc_causal_conv_args& A, int64_t cols) {
   return run < 8 ? 8 : run > 64 ? 64 : run;
 }
 
+// Channels a thread, where sizes, strides and addresses allow: 8 bytes in 16 bits, 16 in 32.  With 8 channels taps, rows and
+// sums leave two waves a SIMD (prompt of 16,381 tokens x 6,144 channels in bf16: 136 us, with four 100)
+constexpr int VECTOR = 4;
+
 template <class T>
-int64_t conv_vector(const ttc_causal_conv_args& A) {
-  constexpr int V = 16 / sizeof(T);
-  bool wide = A.channels % V == 0 && A.x_stride[0] % V == 0 && A.x_stride[1] % V == 0 && aligned16(A.x) && aligned16(A.y) &&
-              aligned16(A.initial_state) && aligned16(A.final_state);
+bool conv_wide(const ttc_causal_conv_args& A) {
+  auto ok = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % (VECTOR * sizeof(T)) == 0; };
+  bool wide = A.channels % VECTOR == 0 && A.x_stride[0] % VECTOR == 0 && A.x_stride[1] % VECTOR == 0 && ok(A.x) && ok(A.y) &&
+              ok(A.initial_state) && ok(A.final_state);
   if (A.backward)
-    wide = wide && A.d_y_stride[0] % V == 0 && A.d_y_stride[1] % V == 0 && aligned16(A.d_y) && aligned16(A.dx) &&
-           aligned16(A.d_final_state) && aligned16(A.d_initial_state);
-  return wide ? V : 1;
+    wide = wide && A.d_y_stride[0] % VECTOR == 0 && A.d_y_stride[1] % VECTOR == 0 && ok(A.d_y) && ok(A.dx) &&
+           ok(A.d_final_state) && ok(A.d_initial_state);
+  return wide;
 }
 
 // Sums of the weights' gradients: one row of them for each four runs of a sequence.  Of the block alone, whatever its
@@ -332,8 +394,7 @@ inline int64_t conv_parts(const ttc_causal_conv_args& A, int64_t cols) {
 
 inline int64_t conv_bytes(const ttc_causal_conv_args& A) {
   if (!A.backward || (!A.dweight && !A.dbias)) return 0;
-  const int64_t V = A.dtype == TTC_DTYPE_BF16 ? 8 : 4;
-  const int64_t a = conv_parts(A, ceil_div(A.channels, V)), b = conv_parts(A, A.channels);
+  const int64_t a = conv_parts(A, ceil_div(A.channels, VECTOR)), b = conv_parts(A, A.channels);
   return (a > b ? a : b) * (A.taps + 1) * A.channels * 4;
 }
 
@@ -343,7 +404,7 @@ int conv_run(const ttc_causal_conv_args& A, hipStream_t s) {
   P.x = A.x, P.weight = A.weight, P.bias = A.bias, P.state = A.initial_state;
   P.xb = A.x_stride[0], P.xt = A.x_stride[1];
   P.B = A.batch, P.T = A.tokens, P.C = A.channels;
-  P.weight_bf16 = A.weight_dtype == TTC_DTYPE_BF16;
+  P.weight_bf16 = A.weight_dtype == TTC_DTYPE_BF16, P.wide_weight = aligned16(A.weight);
   P.cols = A.channels / V;
   if (!A.backward) {
     P.y = A.y, P.final_state = A.final_state;
@@ -379,8 +440,7 @@ int conv_run(const ttc_causal_conv_args& A, hipStream_t s) {
 
 template <class T>
 int conv_typed(const ttc_causal_conv_args& A, hipStream_t s) {
-  constexpr int V = 16 / sizeof(T);
-  return conv_vector<T>(A) == V ? conv_run<T, V>(A, s) : conv_run<T, 1>(A, s);
+  return conv_wide<T>(A) ? conv_run<T, VECTOR>(A, s) : conv_run<T, 1>(A, s);
 }
 
 template <class T, int V>
@@ -389,7 +449,7 @@ int conv_step_run(const ttc_causal_conv_step_args& A, hipStream_t s) {
   P.x = A.x, P.weight = A.weight, P.bias = A.bias;
   P.xb = A.x_stride;
   P.C = A.channels;
-  P.weight_bf16 = A.weight_dtype == TTC_DTYPE_BF16;
+  P.weight_bf16 = A.weight_dtype == TTC_DTYPE_BF16, P.wide_weight = aligned16(A.weight);
   P.y = A.y, P.final_state = A.state;
   P.cols = A.channels / V;
   const int64_t items = A.batch * P.cols;
@@ -406,9 +466,9 @@ int conv_step_run(const ttc_causal_conv_step_args& A, hipStream_t s) {
 
 template <class T>
 int conv_step_typed(const ttc_causal_conv_step_args& A, hipStream_t s) {
-  constexpr int V = 16 / sizeof(T);
-  const bool wide = A.channels % V == 0 && A.x_stride % V == 0 && aligned16(A.x) && aligned16(A.y) && aligned16(A.state);
-  return wide ? conv_step_run<T, V>(A, s) : conv_step_run<T, 1>(A, s);
+  auto ok = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % (VECTOR * sizeof(T)) == 0; };
+  const bool wide = A.channels % VECTOR == 0 && A.x_stride % VECTOR == 0 && ok(A.x) && ok(A.y) && ok(A.state);
+  return wide ? conv_step_run<T, VECTOR>(A, s) : conv_step_run<T, 1>(A, s);
 }
 
 }  // namespace ttc
