@@ -18,7 +18,7 @@ CHUNK = 64
 
 def delta64(q, k, v, g, beta, scale, state=None, d_o=None, d_state=None, normalize=False, eps=1e-6):
     """{name: (value, bound)}: o, state, and for gradients d_o (and d_state) those of q, k, v, g, beta, d_state."""
-    dt, H = q.dtype, g.shape[-1]
+    dt, H = q.dtype if q.dtype in HALF else torch.float32, g.shape[-1]  # 64 bits: of a larger computation, whose bound counts
     d = lambda x: x.detach().double().cpu()  # noqa: E731
     wide = lambda x: x.repeat_interleave(H // x.shape[2], dim=2)  # noqa: E731
     length = lambda x: (d(x).square().sum(-1, keepdim=True) + (eps if normalize else 0)).sqrt()  # noqa: E731

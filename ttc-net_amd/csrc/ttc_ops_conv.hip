@@ -363,12 +363,17 @@ inline int conv_check(const ttc_causal_conv_args& A) {
   return conv_check(A.dtype, A.weight_dtype, {A.batch, A.tokens + MAX_TAPS, A.channels, MAX_TAPS + 1}, A.taps, A.activation);
 }
 
-// Rows of w a thread walks along backwards: the K - 1 tokens in front of a run are computed again, so runs of up to 64; as
-// many runs as give each of 256 CUs four workgroups where there are fewer tokens
+// Rows of w a thread walks along backwards: as many as let all workgroups run at once (three a CU, of four runs each), since the
+// K - 1 tokens in front of a run are computed again; 8 at least, 128 at most.  us by run:
+//                                               8     12     16     24     32     48     64     96    128
+//   4 x 2,048 tokens x 4,096 channels, bf16    84     74     70     68     73     63     78     91    115
+//   16,384 x 2,048                             82     74     69     68     69     63     68     91    103
+//   2,048 x 1,024                              14     16     19     24     29     40     51     73     95
+//   8 x 4,096 x 4,096, fp32                   495    457    430    399    393    386    360    372    354
 inline int64_t backward_run(const ttc_causal_conv_args& A, int64_t cols) {
   const int64_t tiles = ceil_div(cols, 64) * (A.batch > 0 ? A.batch : 1), N = A.tokens + A.taps - 1;
-  const int64_t run = N * tiles / (4 * 1024);
-  return run < 8 ? 8 : run > 64 ? 64 : run;
+  const int64_t run = ceil_div(N * tiles, 3072);
+  return run < 8 ? 8 : run > 128 ? 128 : run;
 }
 
 // Channels a thread, where sizes, strides and addresses allow: 8 bytes in 16 bits, 16 in 32.  With 8 channels taps, rows and

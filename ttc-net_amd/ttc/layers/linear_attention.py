@@ -17,12 +17,13 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ._angles import Angles
 from ..ops import group_norm, linear_attention, linear_attention_step, rotary, rotary_table
 
 __all__ = ["LinearAttentionLayer"]
 
 
-class LinearAttentionLayer(nn.Module):
+class LinearAttentionLayer(Angles, nn.Module):
     """``dim``: width of the model; ``key_dim``, ``value_dim``: a head's sizes (up to 128); ``kv_heads`` divides
     ``num_heads`` (shared keys and values); ``rotary_dim``: how much of a key is turned (``key_dim`` by default, 0: none, so that positions have no limit);
     ``max_positions``: of the table of angles; ``memory``: the heads' decays start, spread evenly over their logarithm, at
@@ -48,17 +49,6 @@ class LinearAttentionLayer(nn.Module):
         self.bias_gamma = nn.Parameter(torch.log(torch.expm1(rate)))
         self._table = dict(rotary or {}, length=max_positions, dim=key_dim if rotary_dim is None else rotary_dim)
         self.register_buffer("angles", rotary_table(**self._table), persistent=False)
-
-    def _apply(self, fn, recurse=True):
-        angles = self.angles
-        super()._apply(fn, recurse)
-        # No checkpoint holds the angles: whatever is done to the parameters (another type, to_empty), they keep their values
-        # in 32 bits, or get them where the layer was made without any
-        if angles.is_meta and not self.angles.is_meta:
-            self.angles = rotary_table(**dict(self._table, device=self.angles.device))
-        elif self.angles is not angles:
-            self.angles = angles.to(self.angles.device)
-        return self
 
     def _project(self, x):
         q, k, v, z, g = torch.split(self.in_proj(x), self._split, dim=-1)
