@@ -508,7 +508,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
     float* const all_rows = STATE ? nullptr : BACK ? A.dV : A.E;
     float* const kept_rows = all_rows ? all_rows + unit * C * A.vdp + c0 + e0 : nullptr;
     const int64_t first = ((b * A.T + t0) * A.H + h) * A.vd;  // of the output
-    const int row = A.H * A.vd;
+    const int64_t row = (int64_t)A.H * A.vd;
     if (!odd) {
       if (kept_rows) {
 #pragma unroll
@@ -539,8 +539,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
           for (int j = 0; j < 4; ++j) f[j] = from_f<T>(O[t][j]);
           T* to = static_cast<T*>(A.o) + first;
           if (A.wide_o) {
-            const auto rows = bounded(to, ((left - 1) * row + A.vd) * (int)sizeof(T));
-            const int off = c < A.vd ? (r * row + c) * (int)sizeof(T) : BEYOND;
+            const auto rows = bounded(to, ((left - 1) * (int)row + A.vd) * (int)sizeof(T));
+            const int off = c < A.vd ? (r * (int)row + c) * (int)sizeof(T) : BEYOND;
             if constexpr (sizeof(T) == 4)
               __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f), rows, off, 0, 0);
             else
@@ -548,7 +548,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
           } else if (r < left) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              if (c + j < A.vd) to[(int64_t)r * row + c + j] = f[j];
+              if (c + j < A.vd) to[r * row + c + j] = f[j];
           }
         }
       }
@@ -614,7 +614,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
           o += __shfl_xor(o, 16, 64);
           o += __shfl_xor(o, 32, 64);
           const int c = c0 + e0 + n;
-          if (g == 0 && c < A.vd) static_cast<T*>(A.o)[first + (int64_t)t * row + c] = from_f<T>(rq * o);
+          if (g == 0 && c < A.vd) static_cast<T*>(A.o)[first + t * row + c] = from_f<T>(rq * o);
         }
       }
       if (kept_rows && left < C) {  // rows that do not exist
@@ -675,23 +675,19 @@ __global__ __launch_bounds__((KD / 16 * 64), 2) void delta_gradients_kernel(Delt
   const int64_t unit = A.first + blockIdx.x, bh = unit / A.chunks, t0 = unit % A.chunks * C, b = bh / A.H;
   const int h = (int)(bh % A.H), left = A.T - t0 < C ? (int)(A.T - t0) : C, blocks = A.vdp / W;
   uint32_t most = 0, most_f = 0;
-  {
-    Stage<T, KD, C, NT> k, q;
-    Stage<float, C, ROWS, NT> r;
-    k.fetch(A.k.at<T>(b, h) + t0 * A.k.st, A.k.st, A.kd, left, A.wide_k, tid);
-    q.fetch(A.q.at<T>(b, h) + t0 * A.q.st, A.q.st, A.kd, left, A.wide_q, tid);
-    r.fetch(A.rows + unit * ROWS * C, C, C, ROWS, true, tid);
-    k.template put_mixed<KS>(Ks, tid);
-    q.template put_mixed<KS>(Qs, tid);
-    r.template put<C>(&Row[0][0], tid);
-    k.largest(most);
-    q.largest(most);
-  }
+  const int r0 = wave * 16;
   // 8 neighbouring values of E and of dV a thread (UNITS of them)
   constexpr int UNITS = (C * W / 8 + NT - 1) / NT;
   u32x4 er[UNITS][2], vr[UNITS][2];
   Stage<T, W, C, NT> dr;
+  f32x4 sr[4];  // 8 neighbours of a row of S and of R
+  const float *Sp = A.S + (unit * KD + r0 + n) * A.vdp + 8 * g, *Rp = A.R + (unit * KD + r0 + n) * A.vdp + 8 * g;
   auto fetch = [&](int d) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      sr[i] = reinterpret_cast<const f32x4*>(Sp + d * W)[i];
+      sr[2 + i] = reinterpret_cast<const f32x4*>(Rp + d * W)[i];
+    }
 #pragma unroll
     for (int j = 0; j < UNITS; ++j) {
       const int u = tid + j * NT, row = u / 4 < C ? u / 4 : 0, c = d * W + u % 4 * 8;
@@ -739,23 +735,30 @@ __global__ __launch_bounds__((KD / 16 * 64), 2) void delta_gradients_kernel(Delt
 
   // Over the columns of the values: L and M of the wave's tiles (lane: token t = n, 4 neighbouring s), and the state's parts S dO,
   // S dV and R E (rows r0 + n of S and R; lane's token n, columns r0 + 4 g + i)
-  const int r0 = wave * 16;
   f32x4 lt[MINE], mt[MINE], dq[TT], sv[TT], re[TT], dk[TT];
 #pragma unroll
   for (int i = 0; i < MINE; ++i) lt[i] = mt[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int t = 0; t < TT; ++t) dq[t] = sv[t] = re[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const float *Sp = A.S + (unit * KD + r0 + n) * A.vdp + 8 * g, *Rp = A.R + (unit * KD + r0 + n) * A.vdp + 8 * g;
   float through = 0.0f;
-  fetch(0);
+  {  // all loads of the first columns on their way together
+    Stage<T, KD, C, NT> k, q;
+    Stage<float, C, ROWS, NT> r;
+    k.fetch(A.k.at<T>(b, h) + t0 * A.k.st, A.k.st, A.kd, left, A.wide_k, tid);
+    q.fetch(A.q.at<T>(b, h) + t0 * A.q.st, A.q.st, A.kd, left, A.wide_q, tid);
+    r.fetch(A.rows + unit * ROWS * C, C, C, ROWS, true, tid);
+    fetch(0);
+    k.template put_mixed<KS>(Ks, tid);
+    q.template put_mixed<KS>(Qs, tid);
+    r.template put<C>(&Row[0][0], tid);
+    k.largest(most);
+    q.largest(most);
+  }
   for (int d = 0; d < blocks; ++d) {
-    f32x4 sr[4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      sr[i] = reinterpret_cast<const f32x4*>(Sp + d * W)[i];
-      sr[2 + i] = reinterpret_cast<const f32x4*>(Rp + d * W)[i];
-    }
     put(d);
+    float s8[8], r8[8];
+    eight(sr[0], sr[1], s8);
+    eight(sr[2], sr[3], r8);
     __syncthreads();
     if (d + 1 < blocks) fetch(d + 1);
     int turn = 0;
@@ -768,9 +771,6 @@ __global__ __launch_bounds__((KD / 16 * 64), 2) void delta_gradients_kernel(Delt
         lt[turn / WAVES] = Op::mma(f, Op::row(&Ds[(16 * ti + n) * DS + 8 * g]), lt[turn / WAVES]);
         mt[turn / WAVES] = Op::mma(f, wide_row(Vs, 16 * ti + n), mt[turn / WAVES]);
       }
-    float s8[8], r8[8];
-    eight(sr[0], sr[1], s8);
-    eight(sr[2], sr[3], r8);
 #pragma unroll
     for (int i = 0; i < 8; ++i) through = fmaf(s8[i], r8[i], through);
     const Wide s = Op::wide(s8);
