@@ -189,7 +189,8 @@ int ttc_linear_attention_step(const ttc_linear_attention_step_args* args, void* 
  * grow.  beta [batch, tokens, heads]: any strides, of type beta_dtype (fp32, or dtype), like log_gamma (which has all three
  * dimensions here).  Everything else as in ttc_linear_attention; resets (TTC_RESET_LOG_GAMMA) too.
  * saved: NULL, or ttc_delta_rule_saved_bytes() that the forward fills and the backward of the same inputs needs.
- * workspace: ttc_delta_rule_workspace_bytes() of the same block (whether `saved` is there counts). */
+ * workspace: ttc_delta_rule_workspace_bytes() of the same block (whether `saved` is there counts).  Both at addresses of 16
+ * bytes. */
 typedef struct {
   int64_t dtype, gamma_dtype, beta_dtype, normalize, backward;
   int64_t batch, tokens, heads, q_heads, k_heads, v_heads, dk, dv;

@@ -550,7 +550,8 @@ def test_c_entries_refuse():
                      (dict(Hk=3), 1), (dict(Hq=0), 1), (dict(dk=0), 1), (dict(dk=129), 1), (dict(dv=129), 1), (dict(eps=-1.0), 1),
                      (dict(eps=math.nan), 1), (dict(q=0), 1), (dict(k=0), 1), (dict(v=0), 1), (dict(g=0), 1), (dict(beta=0), 1),
                      (dict(o=0), 1), (dict(B=1 << 40, T=1 << 40), 1), (back | dict(saved=0), 1), (back | dict(saved_size=kept - 1), 1),
-                     (back | dict(d_o=0), 1), (dict(saved=64, saved_size=kept - 1), 1)]:
+                     (back | dict(d_o=0), 1), (dict(saved=64, saved_size=kept - 1), 1), (dict(ws=72), 1),
+                     (dict(saved=72, saved_size=kept), 1)]:
         assert lib.ttc_delta_rule(pack(**(room | kw)), None) == code, kw
     assert lib.ttc_delta_rule(pack(ws=64, size=need - 1), None) == 1 and lib.ttc_delta_rule(pack(), None) == 1
     assert lib.ttc_delta_rule(pack(**back, ws=64, size=wants - 1), None) == 1

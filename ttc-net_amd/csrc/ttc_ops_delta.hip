@@ -24,7 +24,8 @@ __device__ __forceinline__ float gate_of(const void* p, bool bf16, int64_t i) {
 
 // A workgroup holds 32 columns of one head's state in registers, a thread 4 of them for RPT rows.  Both reads of the state meet
 // in one sum over the rows, since S_t' q = e^g S' q + (k . q) b e: one exchange a token, and for one token the state is read and
-// written once (8 bytes an element against 9 flops): bound by memory.
+// written once (8 bytes an element against 9 flops): bound by memory.  192 sequences x 16 states of 128 x 128 in a pool: 95 us a
+// call for 406 MB, 4.3 TB/s where a copy of 1 GiB reaches 5.1; one sequence of 8 states of 64 x 64: 5.3 us, most of it latency.
 template <class T, int RPT>
 __global__ __launch_bounds__(256) void delta_tokens_kernel(Tokens A, int tiles, bool wide, int64_t first) {
   constexpr int COLS = 32, STEP = 32;  // columns of a workgroup, rows between a thread's
@@ -161,6 +162,7 @@ int launch_tokens(const Tokens& A, bool bf16, hipStream_t s) {
 
 // The states in front of the segments: S_{j+1} = M_j S_j + own_j from state_in on, or (BACK) R_{j-1} = M_j' R_j + own_j from the
 // last one.  A workgroup has 16 columns, a wave 16 rows of them; what a segment's reset drops has no effect, whatever it holds.
+// Bound by the chain: 16 segments x 16 heads of 128 x 128 53 us, 3 us a segment, for 17 MB of matrices that each XCD reads once.
 template <int KD, bool BACK>
 __global__ __launch_bounds__(KD / 16 * 64) void delta_join_kernel(Delta A) {
   using Op = Operand<__bf16>;
@@ -280,7 +282,16 @@ struct DeltaLayout {  // bytes from the start of `saved` (inverse to E) and of t
   int vdp, segs;
 };
 
-// Segments: enough workgroups to fill the GPU's 256 CUs twice, of at least 4 chunks each
+// Segments: enough workgroups to fill the GPU's 256 CUs twice, of at least 4 chunks each.  A split sweep does some three times
+// the work (own states, and what becomes of the one in front), so heads that fill the GPU by themselves are not split.  us a
+// call by the workgroups aimed at:                          1     128    256    384    512    768  1,024  1,536
+//   16,381 tokens x 16 heads of 128 x 128, bf16         1,403    629    447    468    426    468    484    532
+//   4 x 2,048 x 32 of 64 x 64, bf16, training             570    567    575    572    547    589    571    594
+//   2 x 2,048 x 32 of 128 x 128, bf16, training           708    707    711    713    691    759    745    791
+//   3 x 509 x 12 of 48 x 80, fp32, training               187    186    176    173    166    169    169    172
+//   4,096 x 16 of 128 x 128, fp32                         731    339    239    256    248    275    288    330
+//   4 x 4,096 x 8 of 32 x 32, bf16                        227    120     88     87     79     89     94     95
+//   8 x 2,048 x 32 of 128 x 128, bf16                     415    415    412    413    407    409    759    785
 inline void segments_of(const ttc_delta_rule_args& A, DeltaLayout& W) {
   const int64_t sweeps = A.batch * A.heads * (A.dv > 64 ? 2 : 1);
   int64_t count = sweeps > 0 ? 512 / sweeps : 1;
@@ -388,8 +399,8 @@ extern "C" int ttc_delta_rule(const ttc_delta_rule_args* args, void* stream) {
   if (some && (!A.q || !A.k || !A.v || !A.log_gamma || !A.beta)) return TTC_LQR_EINVAL;
   if (some && (A.backward ? !A.d_o || !A.saved : !A.o)) return TTC_LQR_EINVAL;
   const DeltaLayout W = delta_layout(A);
-  if (W.total > 0 && (!A.workspace || A.workspace_bytes < W.total)) return TTC_LQR_EINVAL;
-  if (A.saved && A.saved_bytes < W.kept) return TTC_LQR_EINVAL;
+  if (W.total > 0 && (!A.workspace || !aligned16(A.workspace) || A.workspace_bytes < W.total)) return TTC_LQR_EINVAL;
+  if (A.saved && (!aligned16(A.saved) || A.saved_bytes < W.kept)) return TTC_LQR_EINVAL;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (!some) {  // no tokens: the state passes
     const float* from = A.backward ? A.d_final_state : A.initial_state;

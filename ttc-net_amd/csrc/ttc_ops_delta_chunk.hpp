@@ -3,7 +3,7 @@
 // A sweep's wave holds 16 columns of the state in registers, all rows, and needs nothing of the other waves: the columns of
 // S, E, O, R and dV never meet.  Products are laid out so that no accumulator moves before it is an operand:
 //   K S         lane: column n, 4 neighbouring tokens       -> with V, rows of the next product's right side
-//   E = T Y     T's rows straight from memory as operands; E as it lies in the accumulators is the next right side
+//   E = T Y     T in tiles as operands; E as it lies in the accumulators is the next right side
 //   O' = S' Q' + E' (P b)'   lane: token n, 4 neighbouring columns -> stored 4 at once
 //   S += K' (w E)            K' by transposing reads of shared memory (bf16) or element by element (fp32)
 // Tokens that are not finite: where E (dV) of a wave's columns is not, the wave goes through that chunk token by token, so that
@@ -11,6 +11,27 @@
 //
 // Numerics.  In bf16 every operand that is not an input is split into bf16 parts: three (24 digits) on the way of the states,
 // E, dV and the dots that the decays' and strengths' gradients are made of, two (16 digits) where the result is a bf16 output.
+// Against 64 bits: bf16 outputs 1.7e-3 of their norm (one rounding), states and the decays' gradient 2e-7 to 4e-7.
+//
+// Bound.  Of a kernel's cycles (one MI355X)             vector ALU  matrix cores  waits  read, written (MB)    us
+//   16,381 tokens x 16 heads of 128 x 128, 16 segments
+//     prepare                                             40 %          9 %        57 %     70, 139            76
+//     sweep, STATE (values and matrix)                    59           40          24      105,  34           176
+//     join                                                14            5          46       17,  17            53
+//     sweep                                               49           32          36      168,  68           150
+//   training on 4 x 2,048 tokens x 32 heads of 64 x 64, 4 segments
+//     prepare                                             49           10          59       35, 139            56
+//     sweep, STATE (values and matrix)                    61           35          27       71,  17            66
+//     sweep, with what the backward needs                 36           17          27      114, 168            88
+//     sweep back, STATE                                   36           25          28      120,   8            69
+//     sweep back                                          34           20          22      124, 135            84
+//     gradients                                           38           14          54      193, 113           193
+// (read and written behind the XCDs' caches).  The sweeps wait for their own chain, one chunk after the other, and split three
+// ways what the state is multiplied with (176 of some 650 vector instructions a chunk at 128 rows); more waves a SIMD would
+// cover it, but a wave needs 150 to 250 registers.  Operands of different sums are read first and their instructions issued
+// in turn; arrays in shared memory are mixed so that reads along and across rows meet each bank once (with 4 reads of 5 in
+// conflict: STATE at 128 x 128 218 us, so 176).  8 waves of 16 columns a workgroup instead of two workgroups of 4: the same at
+// 128 x 128, fp32 of 48 x 80 slower (27 us against 19).
 #pragma once
 #include "ttc_ops_delta.hpp"
 #include "ttc_ops_mfma.hpp"
@@ -138,7 +159,8 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(Delta A) {
   using Op = Operand<T>;
   constexpr int C = Z::C, TT = Z::TT, QS = Z::QS, LS = C + 4, SUB = 256 / C, BS = 20;
   // Tiles of N b (rows of BS), and the inverse in the place of keys and queries, which are not needed any more: four workgroups a
-  // CU for keys of up to 64 (4,096 chunks: 52 us, with a place of its own, two workgroups: 77), three for 128
+  // CU for keys of up to 64 (4,096 chunks: 56 us, with a place of its own, two
+  // workgroups: 77), three for 128
   constexpr int ROOM = 2 * C * QS * (int)sizeof(T) > C * LS * 4 ? 2 * C * QS * (int)sizeof(T) : C * LS * 4;
   __shared__ __attribute__((aligned(16))) char Room[ROOM];
   __shared__ __attribute__((aligned(16))) float Lm[Z::TILES * 16 * BS];
@@ -241,7 +263,8 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(Delta A) {
         qk[i] = s + i <= t ? kept(w, qk[i] * rq * by) : 0.0f;
       }
       *reinterpret_cast<f32x4*>(&Lm[(tile_of(ti, si) * 16 + n) * BS + 4 * g]) = kk;
-      Op::put_wide(scores + tile_of(ti, si) * 256 + Op::tile_at(n, 4 * g), PLANE, qk);
+      // the third part is the backward's: 16 digits are enough for outputs
+      Op::put_wide(scores + tile_of(ti, si) * 256 + Op::tile_at(n, 4 * g), PLANE, qk, A.S != nullptr);
     }
   __syncthreads();
   // the diagonal blocks' inverses: a lane's column by forward substitution
@@ -303,28 +326,6 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(Delta A) {
 
 // ---- sweeps ----------------------------------------------------------------------------------------------------
 
-// Lower triangle of tiles in shared memory as operands.  ROW: row 16 t + n, columns 32 s + 4 g .. and 16 + 4 g ..; otherwise its
-// transpose's: column 16 t + n, rows 32 s + ...
-template <bool ROW, int TT>
-__device__ __forceinline__ void triangle(const float* tiles, int t, int s, int lane, float (&x)[8]) {
-  const int g = lane >> 4, n = lane & 15;
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int other = 2 * s + half, r = ROW ? t : other, c = ROW ? other : t;
-    if (c > r || r >= TT) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[4 * half + i] = 0.0f;
-    } else if (ROW) {
-      const f32x4 f = *reinterpret_cast<const f32x4*>(tiles + tile_of(r, c) * 256 + n * 16 + 4 * g);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[4 * half + i] = f[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[4 * half + i] = tiles[tile_of(r, c) * 256 + (4 * g + i) * 16 + n];
-    }
-  }
-}
-
 // 8 values of two accumulators: rows 4 g + i of both
 __device__ __forceinline__ void eight(const f32x4& a, const f32x4& b, float (&x)[8]) {
 #pragma unroll
@@ -372,6 +373,13 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
   };
   float* const seg_state = A.segs > 1 ? A.seg_state + part * KD * A.vdp : nullptr;
   if constexpr (STATE) {
+    // Nothing follows the last segment, and its matrix is the backward's alone; nothing is in front of the first one where no
+    // state comes in (training on 4 x 2,048 tokens x 32 heads of 64: 66 us forward and 68 back, so 64 and 58)
+    const bool last = seg == A.segs - 1, first = seg == 0;
+    if (BACK ? first : matrix ? (last && !A.S) || (first && !A.state_in) : last) {
+      if (matrix && c0 == 0 && tid == 0) A.seg_dead[part] = 1;
+      return;
+    }
     each([&](float, int r, int c) { return matrix && r == c ? 1.0f : 0.0f; });
   } else {
     const float* p = A.segs > 1 ? seg_state : A.state_in ? A.state_in + bh * A.kd * A.vd : nullptr;
@@ -650,8 +658,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
 // and with x_ts = P_ts L_ts - N_ts M_ts, f_s = e^{G_C - G_s} k_s . R E_s,
 //   db_s = sum_t x_ts + f_s,   dg_t = the sum over all terms of the loss's gradient that decay across token t: pairs s < t <= t',
 //   the state in front (into tokens from t on), the state behind (from tokens before t), and the state through the chunk.
-// Values come 32 columns at a time, split into their parts once.  Waves share the score tiles, and each takes 16 columns of the
-// keys; its lanes hold one token and 4 neighbouring columns.
+// Values come 32 columns at a time, split into their parts once (all at once, split by each wave that reads them: 4,096 chunks of
+// 64 x 64 265 us, so 193).  Waves share the score tiles, and each takes 16 columns of the keys; its lanes hold one token and 4
+// neighbouring columns.  Bound by latency: two workgroups a CU (71 KB at 64), each of which loads, meets, multiplies and stores;
+// without the second 32 columns 160 us, without the tiles' sums 175, without the products with keys and queries 182.
 template <class T, int KD>
 __global__ __launch_bounds__((KD / 16 * 64), 2) void delta_gradients_kernel(Delta A) {
   using Z = DeltaShape<T, KD>;

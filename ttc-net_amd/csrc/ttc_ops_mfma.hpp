@@ -147,13 +147,13 @@ struct Operand<__bf16> {
   // Values in memory as their three parts (WIDE_PARTS such arrays, `part` elements apart): 4 neighbours put at p, and two
   // 16 x 16 tiles as an operand (zeros for one that is not there): rows n of both, or of their transposes, 24 or (first) 16 digits of them
   static constexpr int WIDE_PARTS = 3;
-  static __device__ __forceinline__ void put_wide(__bf16* p, int part, f32x4 x) {
+  static __device__ __forceinline__ void put_wide(__bf16* p, int part, f32x4 x, bool all = true) {  // or its first two parts
     float d[4], e[4];
     const u32x2 h = {cut(x[0], x[1], d[0], d[1]), cut(x[2], x[3], d[2], d[3])};
     const u32x2 m = {cut(d[0], d[1], e[0], e[1]), cut(d[2], d[3], e[2], e[3])};
     *reinterpret_cast<u32x2*>(p) = h;
     *reinterpret_cast<u32x2*>(p + part) = m;
-    *reinterpret_cast<bf16x4*>(p + 2 * part) = bf16x4{(__bf16)e[0], (__bf16)e[1], (__bf16)e[2], (__bf16)e[3]};
+    if (all) *reinterpret_cast<bf16x4*>(p + 2 * part) = bf16x4{(__bf16)e[0], (__bf16)e[1], (__bf16)e[2], (__bf16)e[3]};
   }
   template <bool ROW>
   static __device__ __forceinline__ Frag tiles(bool has_a, const __bf16* a, bool has_b, const __bf16* b, int lane) {
@@ -266,7 +266,7 @@ struct Operand<float> {
     return r;
   }
   static constexpr int WIDE_PARTS = 1;
-  static __device__ __forceinline__ void put_wide(float* p, int, f32x4 x) { *reinterpret_cast<f32x4*>(p) = x; }
+  static __device__ __forceinline__ void put_wide(float* p, int, f32x4 x, bool = true) { *reinterpret_cast<f32x4*>(p) = x; }
   template <bool ROW>
   static __device__ __forceinline__ Frag wide_tiles(bool has_a, const float* a, bool has_b, const float* b, int, int lane) {
     const int g = lane >> 4, n = lane & 15;
