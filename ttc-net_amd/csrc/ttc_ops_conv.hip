@@ -375,7 +375,7 @@ inline int conv_check(const ttc_causal_conv_args& A) {
 //   8 x 4,096 x 4,096, fp32                   495    457    430    399    393    386    360    372    354
 inline int64_t backward_run(const ttc_causal_conv_args& A, int64_t cols) {
   const int64_t tiles = ceil_div(cols, 64) * (A.batch > 0 ? A.batch : 1), N = A.tokens + A.taps - 1;
-  const int64_t run = ceil_div(N * tiles, 3072);
+  const int64_t run = ceil_div(N * tiles, 3 * 256 * 4);
   return run < 8 ? 8 : run > 128 ? 128 : run;
 }
 

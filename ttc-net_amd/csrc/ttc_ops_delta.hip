@@ -18,10 +18,6 @@ struct Tokens {
   void* o;
 };
 
-__device__ __forceinline__ float gate_of(const void* p, bool bf16, int64_t i) {
-  return bf16 ? to_f(static_cast<const __bf16*>(p)[i]) : static_cast<const float*>(p)[i];
-}
-
 // A workgroup holds 32 columns of one head's state in registers, a thread 4 of them for RPT rows.  Both reads of the state meet
 // in one sum over the rows, since S_t' q = e^g S' q + (k . q) b e: one exchange a token, and for one token the state is read and
 // written once (8 bytes an element against 9 flops): bound by memory.  192 sequences x 16 states of 128 x 128 in a pool: 95 us a
@@ -70,8 +66,8 @@ __global__ __launch_bounds__(256) void delta_tokens_kernel(Tokens A, int tiles, 
   const T *q = A.q.at<T>(b, h), *k = A.k.at<T>(b, h), *v = A.v.at<T>(b, h);
   for (int64_t t = 0; t < A.T; ++t) {
     const int buf = t & 1;
-    const float lg = gate_of(A.gamma, A.gamma_bf16, b * A.gb + h * A.gh + t * A.gt);
-    const float be = gate_of(A.beta, A.beta_bf16, b * A.bb + h * A.bh + t * A.bt);
+    const float lg = gate_value(A.gamma, A.gamma_bf16, b * A.gb + h * A.gh + t * A.gt);
+    const float be = gate_value(A.beta, A.beta_bf16, b * A.bb + h * A.bh + t * A.bt);
     float vv[4], kk[RPT], qq[RPT], sk[4] = {0.f, 0.f, 0.f, 0.f}, sq[4] = {0.f, 0.f, 0.f, 0.f}, d[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < 4; ++j) vv[j] = to_f(v[t * A.v.st + col_at(j)]);

@@ -51,6 +51,11 @@ struct Delta {
   bool dq_f32, dk_f32, wide_dqk, wide_dv;  // stores of 4 elements, of 8
 };
 
+// a decay or a strength
+__device__ __forceinline__ float gate_value(const void* p, bool bf16, int64_t i) {
+  return bf16 ? to_f(static_cast<const __bf16*>(p)[i]) : static_cast<const float*>(p)[i];
+}
+
 template <class T>
 int launch_delta_kd32(const Delta& A, int what, hipStream_t s);
 template <class T>

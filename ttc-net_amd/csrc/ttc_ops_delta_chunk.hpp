@@ -21,9 +21,9 @@
 //     sweep                                               49           32          36      168,  68           150
 //   training on 4 x 2,048 tokens x 32 heads of 64 x 64, 4 segments
 //     prepare                                             49           10          59       35, 139            56
-//     sweep, STATE (values and matrix)                    61           35          27       71,  17            66
+//     sweep, STATE (values and matrix)                    61           35          27       71,  17            64
 //     sweep, with what the backward needs                 36           17          27      114, 168            88
-//     sweep back, STATE                                   36           25          28      120,   8            69
+//     sweep back, STATE                                   36           25          28      120,   8            58
 //     sweep back                                          34           20          22      124, 135            84
 //     gradients                                           38           14          54      193, 113           193
 // (read and written behind the XCDs' caches).  The sweeps wait for their own chain, one chunk after the other, and split three
@@ -41,8 +41,7 @@ namespace ttc {
 template <class T, int KD>
 struct DeltaShape {
   static constexpr int C = chunk_tokens(sizeof(T) == 2), TT = C / 16, KB = C / 32, DB = KD / 32, DT = KD / 16;
-  static constexpr int VEC = 16 / sizeof(T), TILES = TT * (TT + 1) / 2;
-  static constexpr int QS = KD + Operand<T>::ROW_PAD, KS = KD + Operand<T>::COL_PAD;
+  static constexpr int TILES = TT * (TT + 1) / 2, QS = KD + Operand<T>::ROW_PAD, KS = KD + Operand<T>::COL_PAD;
 };
 constexpr int tile_of(int t, int s) { return t * (t + 1) / 2 + s; }
 
@@ -97,10 +96,6 @@ struct Stage {
     for (int j = 0; j < N; ++j) Operand<T>::largest(r[j], m);
   }
 };
-
-__device__ __forceinline__ float gate_value(const void* p, bool bf16, int64_t i) {
-  return bf16 ? to_f(static_cast<const __bf16*>(p)[i]) : static_cast<const float*>(p)[i];
-}
 
 // A token's place among the decays, and e^{G_t - G_s}: 0 across a reset, whatever the sums hold
 struct Place {
@@ -159,8 +154,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(Delta A) {
   using Op = Operand<T>;
   constexpr int C = Z::C, TT = Z::TT, QS = Z::QS, LS = C + 4, SUB = 256 / C, BS = 20;
   // Tiles of N b (rows of BS), and the inverse in the place of keys and queries, which are not needed any more: four workgroups a
-  // CU for keys of up to 64 (4,096 chunks: 56 us, with a place of its own, two
-  // workgroups: 77), three for 128
+  // CU for keys of up to 64 (4,096 chunks: 56 us; with a place of its own, two workgroups: 77), three for 128
   constexpr int ROOM = 2 * C * QS * (int)sizeof(T) > C * LS * 4 ? 2 * C * QS * (int)sizeof(T) : C * LS * 4;
   __shared__ __attribute__((aligned(16))) char Room[ROOM];
   __shared__ __attribute__((aligned(16))) float Lm[Z::TILES * 16 * BS];
@@ -237,7 +231,8 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(Delta A) {
   }
   __syncthreads();
   constexpr int PLANE = Z::TILES * 256;
-  T *scores = static_cast<T*>(A.scores) + unit * Op::WIDE_PARTS * PLANE, *inverse = static_cast<T*>(A.inverse) + unit * Op::WIDE_PARTS * PLANE;
+  T* scores = static_cast<T*>(A.scores) + unit * Op::WIDE_PARTS * PLANE;
+  T* inverse = static_cast<T*>(A.inverse) + unit * Op::WIDE_PARTS * PLANE;
   for (int i = tid; i < ROWS * C / 4; i += 256)
     reinterpret_cast<f32x4*>(A.rows + unit * ROWS * C)[i] = reinterpret_cast<const f32x4*>(&Row[0][0])[i];
   int turn = 0;
@@ -258,7 +253,8 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(Delta A) {
       const float rk = Row[RK][t], rq = Row[RQ][t] * A.scale;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float w = weight_of(at_t, Place{Row[HI][s + i], Row[LO][s + i], Row[PART][s + i]}), by = Row[RK][s + i] * Row[BETA][s + i];
+        const float w = weight_of(at_t, Place{Row[HI][s + i], Row[LO][s + i], Row[PART][s + i]});
+        const float by = Row[RK][s + i] * Row[BETA][s + i];
         kk[i] = s + i < t ? kept(w, kk[i] * rk * by) : 0.0f;
         qk[i] = s + i <= t ? kept(w, qk[i] * rq * by) : 0.0f;
       }
