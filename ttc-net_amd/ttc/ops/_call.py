@@ -2,6 +2,8 @@
 that is itself recorded."""
 from __future__ import annotations
 
+import struct
+
 import torch
 
 from ..solvers._lib import check
@@ -34,6 +36,12 @@ def check_device(name: str, first, *xs) -> None:
 def unit_rows(x: torch.Tensor) -> torch.Tensor:
     """``x``, or a copy of it where its last dimension does not have stride 1."""
     return x if x.stride(-1) == 1 or x.shape[-1] <= 1 else x.contiguous()
+
+
+def with_spaces(block: bytes, *spaces) -> bytes:
+    """``block`` with these as its last fields: an address and a number of bytes each."""
+    tail = [n for x in spaces for n in ((0, 0) if x is None else (x.data_ptr(), x.numel()))]
+    return block[:-8 * len(tail)] + struct.pack(f"{len(tail)}q", *tail)
 
 
 def launch(fn, name: str, block: bytes, device: torch.device) -> None:

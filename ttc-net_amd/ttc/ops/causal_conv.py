@@ -16,7 +16,7 @@ import torch
 
 from .._dispatch import traced
 from ..solvers._lib import lib
-from ._call import DTYPES, check_device, check_types, launch, ptr, recorded_backward, unit_rows
+from ._call import DTYPES, check_device, check_types, launch, ptr, recorded_backward, unit_rows, with_spaces
 
 __all__ = ["causal_conv", "causal_conv_step", "causal_conv_torch", "MAX_TAPS"]
 
@@ -43,12 +43,12 @@ def causal_conv_torch(x, weight, bias=None, *, activation: str = "none", initial
 
 
 def _block(x, weight, bias, activation, initial, y, final, backward=0, d_y=None, d_final=None, dx=None, dweight=None,
-           dbias=None, d_initial=None, space=None):
+           dbias=None, d_initial=None):
     B, T, C = x.shape
     return _BLOCK.pack(DTYPES[x.dtype], DTYPES[weight.dtype], B, T, C, weight.shape[1], _ACTIVATIONS[activation], backward,
                        ptr(x), *x.stride()[:2], ptr(weight), ptr(bias), ptr(initial), ptr(y), ptr(final), ptr(d_y),
                        *((0, 0) if d_y is None else d_y.stride()[:2]), ptr(d_final), ptr(dx), ptr(dweight), ptr(dbias),
-                       ptr(d_initial), ptr(space), 0 if space is None else space.numel())
+                       ptr(d_initial), 0, 0)
 
 
 def _forward(x, weight, bias, activation, initial, want_state):
@@ -88,7 +88,7 @@ class _CausalConvFunc(torch.autograd.Function):
         size = lib.ttc_causal_conv_workspace_bytes(block)
         if size:
             space = torch.empty(size, dtype=torch.uint8, device=x.device)
-            block = _block(*args, space)
+            block = with_spaces(block, space)
         launch(lib.ttc_causal_conv, "ttc_causal_conv", block, x.device)
         return dx, dweight, dbias, d_initial, None, None
 

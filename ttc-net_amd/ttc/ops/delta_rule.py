@@ -17,7 +17,7 @@ import torch
 
 from .._dispatch import traced
 from ..solvers._lib import lib
-from ._call import DTYPES, check_device, check_types, launch, ptr, recorded_backward, unit_rows
+from ._call import DTYPES, check_device, check_types, launch, ptr, recorded_backward, unit_rows, with_spaces
 from .linear_attention import MAX_DIM, RESET
 
 __all__ = ["delta_rule", "delta_rule_step", "delta_rule_torch"]
@@ -91,24 +91,23 @@ def _in_chunks(q, k, v, log_gamma, beta, scale, initial_state, normalize, eps):
 
 
 def _block(q, k, v, log_gamma, beta, scale, normalize, eps, initial, o, final, backward=0, d_o=None, d_final=None, dq=None,
-           dk=None, dv=None, d_gamma=None, d_beta=None, d_initial=None, saved=None, space=None):
+           dk=None, dv=None, d_gamma=None, d_beta=None, d_initial=None):
     B, T = q.shape[:2]
-    size = lambda x: 0 if x is None else x.numel()  # noqa: E731
     return _BLOCK.pack(DTYPES[q.dtype], DTYPES[log_gamma.dtype], DTYPES[beta.dtype], normalize, backward, B, T,
                        log_gamma.shape[-1], q.shape[2], k.shape[2], v.shape[2], q.shape[3], v.shape[3], scale, eps, ptr(q),
                        ptr(k), ptr(v), ptr(log_gamma), ptr(beta), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
                        *log_gamma.stride(), *beta.stride(), ptr(initial), ptr(o), ptr(final), ptr(d_o),
                        *((0, 0, 0) if d_o is None else d_o.stride()[:3]), ptr(d_final), ptr(dq), ptr(dk), ptr(dv), ptr(d_gamma),
-                       ptr(d_beta), ptr(d_initial), ptr(saved), size(saved), ptr(space), size(space))
+                       ptr(d_beta), ptr(d_initial), 0, 0, 0, 0)  # what is kept for the backward, the workspace
 
 
-def _run(*args, **kw):
-    device = args[0].device
-    block = _block(*args, **kw)
+def _run(block, saved, device):
+    if saved is not None:
+        block = with_spaces(block, saved, None)  # the workspace holds what is not kept
     size = lib.ttc_delta_rule_workspace_bytes(block)
     if size:
         space = torch.empty(size, dtype=torch.uint8, device=device)
-        block = _block(*args, **kw, space=space)
+        block = with_spaces(block, space)
     launch(lib.ttc_delta_rule, "ttc_delta_rule", block, device)
 
 
@@ -119,11 +118,10 @@ def _forward(q, k, v, log_gamma, beta, scale, normalize, eps, initial, want_stat
     o = torch.empty(B, T, H, v.shape[-1], dtype=q.dtype, device=q.device)
     final = torch.empty(B, H, q.shape[-1], v.shape[-1], dtype=torch.float32, device=q.device) if want_state else None
     args = (unit_rows(q), unit_rows(k), unit_rows(v), log_gamma, beta, scale, normalize, eps, initial, o, final)
-    saved = None
+    block, saved = _block(*args), None  # args: what was copied for the block lives until the launch
     if train:
-        size = lib.ttc_delta_rule_saved_bytes(_block(*args))
-        saved = torch.empty(max(size, 1), dtype=torch.uint8, device=q.device)
-    _run(*args, saved=saved)
+        saved = torch.empty(max(lib.ttc_delta_rule_saved_bytes(block), 1), dtype=torch.uint8, device=q.device)
+    _run(block, saved, q.device)
     return o, final, saved
 
 
@@ -154,8 +152,9 @@ class _DeltaRuleFunc(torch.autograd.Function):
             d_o = torch.zeros(q.shape[0], q.shape[1], log_gamma.shape[-1], v.shape[-1], dtype=q.dtype, device=q.device)
         new = lambda x, wanted: torch.empty(x.shape, dtype=x.dtype, device=x.device) if wanted else None  # noqa: E731
         grads = tuple(new(x, n) for x, n in zip((q, k, v, log_gamma, beta, initial), needs))
-        _run(unit_rows(q), unit_rows(k), unit_rows(v), log_gamma, beta, *ctx.args, None, None, None, 1, unit_rows(d_o),
-             None if d_final is None else d_final.contiguous(), *grads, saved=saved)
+        args = (unit_rows(q), unit_rows(k), unit_rows(v), log_gamma, beta, *ctx.args, None, None, None, 1, unit_rows(d_o),
+                None if d_final is None else d_final.contiguous(), *grads)
+        _run(_block(*args), saved, q.device)
         return (*grads, None, None, None, None)
 
 
