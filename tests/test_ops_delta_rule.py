@@ -566,3 +566,23 @@ def test_c_entries_refuse():
                      (dict(g=0), 1), (dict(beta=0), 1), (dict(eps=-1.0), 1)]:
         assert lib.ttc_delta_rule_step(pack(**kw), None) == code, kw
     assert lib.ttc_delta_rule_step(None, None) == 1 and lib.ttc_delta_rule_step(pack(B=0, slots=0), None) == 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("train", [False, True])
+@pytest.mark.parametrize("case", [(5, 25, 8, 8, 8, 8, 128, 32), (2, 256, 4, 4, 4, 4, 41, 128), (3, 130, 4, 1, 2, 4, 64, 64),
+                                  (2, 90, 6, 6, 6, 6, 30, 20), (2, 70, 5, 5, 5, 5, 128, 128)])
+def test_sums_of_16_bit_outputs(device, train, case):
+    """Outputs in 16 bits are sums in 32, rounded once.  Some 400 roundings on a term's way, each of at most EPS and independent of
+    each other, leave a sum off by e = 20 EPS of the outputs' size.  One of z times that size, whose neighbours are at least 2^-8 z
+    of it apart, then rounds to the other one as often as e 2^8 / z, at most always: with z as normal values are, 0.8 dz near 0,
+    the mean of 1 / z from e 2^8 = 3e-4 on is 0.8 ln(1 / 3e-4) = 6.5, and 6.5 e 2^8 = 0.2 % of all differ from the rounded 64-bit
+    values; a count of n scatters by sqrt(n), four of which are added.  Their number and not their size is bounded: in the first
+    case one output of the largest, off by a step, is 2^-7 of 38 in the norm, more than all others together.  (Operands cut to 16
+    digits, the state and the scores, made 0.7 to 1.1 % differ.)"""
+    x = inputs(*case, torch.bfloat16, device, True, normalize=True)
+    leaves = {n: x[n].clone().requires_grad_(train) for n in NAMES}
+    o = call(leaves, 0.3, True)[0].detach().cpu()
+    want = oracle(x, 0.3, normalize=True)["o"][0].to(torch.bfloat16)
+    most = 6.5 * 20 * EPS * 2 ** 8 * o.numel()
+    assert int((o != want).sum()) <= most + 4 * math.sqrt(most), float((o != want).double().mean())

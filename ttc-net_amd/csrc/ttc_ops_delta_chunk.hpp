@@ -9,9 +9,11 @@
 // Tokens that are not finite: where E (dV) of a wave's columns is not, the wave goes through that chunk token by token, so that
 // no token has an effect on earlier ones and none passes a reset.
 //
-// Numerics.  In bf16 every operand that is not an input is split into bf16 parts: three (24 digits) on the way of the states,
-// E, dV and the dots that the decays' and strengths' gradients are made of, two (16 digits) where the result is a bf16 output.
-// Against 64 bits: bf16 outputs 1.7e-3 of their norm (one rounding), states and the decays' gradient 2e-7 to 4e-7.
+// Numerics.  In bf16 every operand that is not an input is split into three bf16 parts (24 digits), so that sums are those of 32
+// bits; but for the score tiles of the queries' and keys' gradients, in two (16 digits): a third part would take a workgroup's
+// shared memory beyond half a CU's.  Against 64 bits: bf16 outputs and gradients 1.7e-3 of their norm (one rounding), states and the
+// decays' gradient 2e-7 to 4e-7.  Of outputs 0.03 %, of those two gradients 0.4 %, round to the other neighbour of the exact value
+// (outputs from two parts: 1 %, and 1.5 % of a long prompt's time less; 6 % where heads fill the GPU by themselves).
 //
 // Bound.  Of a kernel's cycles (one MI355X)             vector ALU  matrix cores  waits  read, written (MB)    us
 //   16,381 tokens x 16 heads of 128 x 128, 16 segments
@@ -259,8 +261,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(Delta A) {
         qk[i] = s + i <= t ? kept(w, qk[i] * rq * by) : 0.0f;
       }
       *reinterpret_cast<f32x4*>(&Lm[(tile_of(ti, si) * 16 + n) * BS + 4 * g]) = kk;
-      // the third part is the backward's: 16 digits are enough for outputs
-      Op::put_wide(scores + tile_of(ti, si) * 256 + Op::tile_at(n, 4 * g), PLANE, qk, A.S != nullptr);
+      Op::put_wide(scores + tile_of(ti, si) * 256 + Op::tile_at(n, 4 * g), PLANE, qk);
     }
   __syncthreads();
   // the diagonal blocks' inverses: a lane's column by forward substitution
@@ -339,9 +340,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
   constexpr int C = Z::C, TT = Z::TT, KB = Z::KB, NT = WAVES * 64, COLS = 16 * WAVES, KS = Z::KS,
                 VS = COLS + Op::COL_PAD;
   __shared__ __attribute__((aligned(16))) T Ks[C * KS], Qs[C * KS], Vs[C * VS];  // Vs: V, or dO
-  // the inverse's and the scores' tiles in parts; 16 digits of the scores are enough for outputs
-  constexpr int PLANE = Z::TILES * 256, PARTS = Op::WIDE_PARTS, USED = BACK || PARTS == 1 ? PARTS : 2;
-  __shared__ __attribute__((aligned(16))) T inverse[PARTS * PLANE], scores[USED * PLANE];
+  constexpr int PLANE = Z::TILES * 256, PARTS = Op::WIDE_PARTS;
+  __shared__ __attribute__((aligned(16))) T inverse[PARTS * PLANE], scores[PARTS * PLANE];  // their tiles in parts
   __shared__ __attribute__((aligned(16))) float Row[ROWS][C];
   int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -389,8 +389,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
   Stage<T, KD, C, NT> kr, qr;
   Stage<T, COLS, C, NT> vr;
   Stage<float, C, ROWS, NT> rr;
-  Stage<T, 256, PARTS * Z::TILES, NT> ir;
-  Stage<T, 256, USED * Z::TILES, NT> sr;
+  Stage<T, 256, PARTS * Z::TILES, NT> ir, sr;
   int odd_next = 0;
   const int64_t begin = seg * A.seg_chunks, end = begin + A.seg_chunks < A.chunks ? begin + A.seg_chunks : A.chunks;
   auto chunk_of = [&](int64_t i) { return BACK ? end - 1 - i : begin + i; };
@@ -405,7 +404,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
     rr.fetch(A.rows + unit * ROWS * C, C, C, ROWS, true, tid);
     ir.fetch(static_cast<const T*>(A.inverse) + unit * PARTS * PLANE, 256, 256, PARTS * Z::TILES, true, tid);
     if constexpr (BACK || !STATE)
-      sr.fetch(static_cast<const T*>(A.scores) + unit * PARTS * PLANE, 256, 256, USED * Z::TILES, true, tid);
+      sr.fetch(static_cast<const T*>(A.scores) + unit * PARTS * PLANE, 256, 256, PARTS * Z::TILES, true, tid);
     odd_next = A.odd[unit];
   };
   fetch(0);
@@ -456,7 +455,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
       if constexpr (!BACK && !STATE) {
 #pragma unroll
         for (int t = 0; t < TT; ++t) f[t] = Op::row_split(Qs + rows_at + 16 * t * KS + 32 * d);
-        mma_right<Op, 0, TT>(Op::first(s), f, O);
+        mma_right<Op, 0, TT>(s, f, O);
       }
     }
     // what the triangle is solved for: V - e^G K S, or b (e^{G_C - G} K R + P' dO).  A weight of 0 does not select here: where the
@@ -527,11 +526,11 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
           constexpr int s = decltype(s_)::value;
           float x[8];
           eight(E[2 * s], E[2 * s + 1], x);
-          const typename Op::Pair e = Op::pair(x);
-          typename Op::Pair f[TT];
+          const Wide e = Op::wide(x);
+          Wide f[TT];
 #pragma unroll
           for (int t = 2 * s; t < TT; ++t)
-            f[t] = Op::template pair_tiles<true>(true, scores + tile_of(t, 2 * s) * 256, 2 * s < t,
+            f[t] = Op::template wide_tiles<true>(true, scores + tile_of(t, 2 * s) * 256, 2 * s < t,
                                                  scores + tile_of(t, 2 * s + 1) * 256, PLANE, lane);
           mma_right<Op, 2 * s, TT>(e, f, O);
         });

@@ -42,18 +42,12 @@ struct Operand<__bf16> {
     c = mma(a.m, b.m, mma(a.l, b.h, mma(a.h, b.l, c)));
     return mma(a.h, b.h, mma(a.h, b.m, mma(a.m, b.h, c)));
   }
-  static __device__ __forceinline__ f32x4 mma(const Pair& a, const Pair& b, f32x4 c) {  // 16 digits
-    return mma(a.h, b.h, mma(a.h, b.l, mma(a.l, b.h, c)));
-  }
-  static __device__ __forceinline__ Pair first(const Wide& a) { return Pair{a.h, a.m}; }  // 16 of its digits
   // A product as single instructions, small terms first: those of several sums are issued in turn, so that none waits for the
   // one before it
   static constexpr int steps(const Frag*, const Wide*) { return 3; }
   static constexpr int steps(const Wide*, const Frag*) { return 3; }
   static constexpr int steps(const Wide*, const Wide*) { return 6; }
-  static constexpr int steps(const Pair*, const Frag*) { return 2; }
   static constexpr int steps(const Frag*, const Pair*) { return 2; }
-  static constexpr int steps(const Pair*, const Pair*) { return 3; }
   static __device__ __forceinline__ f32x4 step(int p, Frag a, const Wide& b, f32x4 c) {
     return mma(a, p == 0 ? b.l : p == 1 ? b.m : b.h, c);
   }
@@ -63,11 +57,7 @@ struct Operand<__bf16> {
   static __device__ __forceinline__ f32x4 step(int p, const Wide& a, const Wide& b, f32x4 c) {
     return mma(p == 1 ? a.l : p == 2 || p == 3 ? a.m : a.h, p == 0 ? b.l : p == 2 || p == 4 ? b.m : b.h, c);
   }
-  static __device__ __forceinline__ f32x4 step(int p, const Pair& a, Frag b, f32x4 c) { return mma(p == 0 ? a.l : a.h, b, c); }
   static __device__ __forceinline__ f32x4 step(int p, Frag a, const Pair& b, f32x4 c) { return mma(a, p == 0 ? b.l : b.h, c); }
-  static __device__ __forceinline__ f32x4 step(int p, const Pair& a, const Pair& b, f32x4 c) {
-    return mma(p == 1 ? a.l : a.h, p == 0 ? b.l : b.h, c);
-  }
   static __device__ __forceinline__ f32x4 mma(const Pair& a, Frag b, f32x4 c) { return mma(a.h, b, mma(a.l, b, c)); }
   static __device__ __forceinline__ f32x4 mma(Frag a, const Pair& b, f32x4 c) { return mma(a, b.h, mma(a, b.l, c)); }
   static __device__ __forceinline__ Frag row(const __bf16* p) { return *reinterpret_cast<const Frag*>(p); }
@@ -145,15 +135,15 @@ struct Operand<__bf16> {
     return __builtin_bit_cast(Frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
   }
   // Values in memory as their three parts (WIDE_PARTS such arrays, `part` elements apart): 4 neighbours put at p, and two
-  // 16 x 16 tiles as an operand (zeros for one that is not there): rows n of both, or of their transposes, 24 or (first) 16 digits of them
+  // 16 x 16 tiles as an operand (zeros for one that is not there): rows n of both, or of their transposes
   static constexpr int WIDE_PARTS = 3;
-  static __device__ __forceinline__ void put_wide(__bf16* p, int part, f32x4 x, bool all = true) {  // or its first two parts
+  static __device__ __forceinline__ void put_wide(__bf16* p, int part, f32x4 x) {
     float d[4], e[4];
     const u32x2 h = {cut(x[0], x[1], d[0], d[1]), cut(x[2], x[3], d[2], d[3])};
     const u32x2 m = {cut(d[0], d[1], e[0], e[1]), cut(d[2], d[3], e[2], e[3])};
     *reinterpret_cast<u32x2*>(p) = h;
     *reinterpret_cast<u32x2*>(p + part) = m;
-    if (all) *reinterpret_cast<bf16x4*>(p + 2 * part) = bf16x4{(__bf16)e[0], (__bf16)e[1], (__bf16)e[2], (__bf16)e[3]};
+    *reinterpret_cast<bf16x4*>(p + 2 * part) = bf16x4{(__bf16)e[0], (__bf16)e[1], (__bf16)e[2], (__bf16)e[3]};
   }
   template <bool ROW>
   static __device__ __forceinline__ Frag tiles(bool has_a, const __bf16* a, bool has_b, const __bf16* b, int lane) {
@@ -226,7 +216,6 @@ struct Operand<float> {
     for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j], b.v[j], c, 0, 0, 0);
     return c;
   }
-  static __device__ __forceinline__ Frag first(const Frag& a) { return a; }
   static constexpr int steps(const Frag*, const Frag*) { return 8; }
   static __device__ __forceinline__ f32x4 step(int p, const Frag& a, const Frag& b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[p], b.v[p], c, 0, 0, 0);
@@ -266,7 +255,7 @@ struct Operand<float> {
     return r;
   }
   static constexpr int WIDE_PARTS = 1;
-  static __device__ __forceinline__ void put_wide(float* p, int, f32x4 x, bool = true) { *reinterpret_cast<f32x4*>(p) = x; }
+  static __device__ __forceinline__ void put_wide(float* p, int, f32x4 x) { *reinterpret_cast<f32x4*>(p) = x; }
   template <bool ROW>
   static __device__ __forceinline__ Frag wide_tiles(bool has_a, const float* a, bool has_b, const float* b, int, int lane) {
     const int g = lane >> 4, n = lane & 15;
