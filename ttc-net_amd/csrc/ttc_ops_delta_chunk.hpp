@@ -10,10 +10,9 @@
 // no token has an effect on earlier ones and none passes a reset.
 //
 // Numerics.  In bf16 every operand that is not an input is split into three bf16 parts (24 digits), so that sums are those of 32
-// bits; but for the score tiles of the queries' and keys' gradients, in two (16 digits): a third part would take a workgroup's
-// shared memory beyond half a CU's.  Against 64 bits: bf16 outputs and gradients 1.7e-3 of their norm (one rounding), states and the
-// decays' gradient 2e-7 to 4e-7.  Of outputs 0.03 %, of those two gradients 0.4 %, round to the other neighbour of the exact value
-// (outputs from two parts: 1 %, and 1.5 % of a long prompt's time less; 6 % where heads fill the GPU by themselves).
+// bits.  Against 64 bits: bf16 outputs and gradients 1.7e-3 of their norm (one rounding), states and the decays' gradient 2e-7 to
+// 4e-7; 0.03 % of the outputs round to the other neighbour of the exact value.  From two parts 1 % did (of queries' and keys'
+// gradients 0.4 %), for 1.5 % less time in a long prompt and in training, 6 % where heads fill the GPU by themselves.
 //
 // Bound.  Of a kernel's cycles (one MI355X)             vector ALU  matrix cores  waits  read, written (MB)    us
 //   16,381 tokens x 16 heads of 128 x 128, 16 segments
@@ -655,20 +654,19 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
 //   the state in front (into tokens from t on), the state behind (from tokens before t), and the state through the chunk.
 // Values come 32 columns at a time, split into their parts once (all at once, split by each wave that reads them: 4,096 chunks of
 // 64 x 64 265 us, so 193).  Waves share the score tiles, and each takes 16 columns of the keys; its lanes hold one token and 4
-// neighbouring columns.  Bound by latency: two workgroups a CU (71 KB at 64), each of which loads, meets, multiplies and stores;
+// neighbouring columns.  Bound by latency: two workgroups a CU (66 KB at 64), each of which loads, meets, multiplies and stores;
 // without the second 32 columns 160 us, without the tiles' sums 175, without the products with keys and queries 182.
 template <class T, int KD>
 __global__ __launch_bounds__((KD / 16 * 64), 2) void delta_gradients_kernel(Delta A) {
   using Z = DeltaShape<T, KD>;
   using Op = Operand<T>;
   using Wide = typename Op::Wide;
-  using Pair = typename Op::Pair;
   using Frag = typename Op::Frag;
   constexpr int C = Z::C, TT = Z::TT, KB = Z::KB, WAVES = KD / 16, NT = WAVES * 64, KS = Z::KS, MINE = (Z::TILES + WAVES - 1) / WAVES;
   constexpr int W = 32, DS = W + Op::ROW_PAD, BLOCK = C * DS, PARTS = Op::WIDE_PARTS;  // columns of values, and their rows
-  constexpr int PLANE = Z::TILES * 256, SET = Op::SCORE_PARTS * PLANE, ROOM = (2 * PARTS + 1) * BLOCK;
+  constexpr int PLANE = Z::TILES * 256, SET = PARTS * PLANE, ROOM = (2 * PARTS + 1) * BLOCK;
   __shared__ __attribute__((aligned(16))) T Ks[C * KS], Qs[C * KS];
-  __shared__ __attribute__((aligned(16))) T Big[ROOM > 4 * SET ? ROOM : 4 * SET];  // E, dV and dO, then A and B as they are used
+  __shared__ __attribute__((aligned(16))) T Big[ROOM > 2 * SET ? ROOM : 2 * SET];  // E, dV and dO, then A and B as they are used
   __shared__ __attribute__((aligned(16))) float Row[ROWS][C];
   __shared__ float Part[TT][3][C];    // by tile: sums over s of b P L and of b N M (by si), over t of x (by ti)
   __shared__ float Dot[WAVES][3][C];  // by wave: q . S dO, k . S dV, k . R E
@@ -798,8 +796,9 @@ __global__ __launch_bounds__((KD / 16 * 64), 2) void delta_gradients_kernel(Delt
     if (lane == 0) Odd[wave] = odd_here;
   }
 
-  // the tiles: their sums, and A and B in the place of E, dV and dO, with the weights of what each is multiplied with
-  T *Ak = Big, *Aq = Big + SET, *Bs = Big + 2 * SET, *Bt = Big + 3 * SET;
+  // the tiles: their sums, and A and B in the place of E, dV and dO, with the weights of what each is multiplied with: first that
+  // of the tokens in front, then, in the same place, of those behind (in lt and mt until then)
+  T *As = Big, *Bs = Big + SET;
   const int rows_at = Op::row_place(KS, lane), columns_at = Op::column_place(KS, lane);
   {
     int turn = 0;
@@ -835,10 +834,9 @@ __global__ __launch_bounds__((KD / 16 * 64), 2) void delta_gradients_kernel(Delt
           as[i] = at[i] * rs, bs[i] = bt[i] * rs;
         }
         const int tile = tile_of(ti, si) * 256 + Op::tile_at(n, 4 * g);
-        Op::put_scores(Ak + tile, PLANE, as);
-        Op::put_scores(Aq + tile, PLANE, at * rq);
-        Op::put_scores(Bs + tile, PLANE, bs);
-        Op::put_scores(Bt + tile, PLANE, bt * rk);
+        Op::put_wide(As + tile, PLANE, as);
+        Op::put_wide(Bs + tile, PLANE, bs);
+        lt[turn / WAVES] = at * rq, mt[turn / WAVES] = bt * rk;
         sum_p += __shfl_xor(sum_p, 16, 64);
         sum_p += __shfl_xor(sum_p, 32, 64);
         sum_n += __shfl_xor(sum_n, 16, 64);
@@ -935,51 +933,64 @@ __global__ __launch_bounds__((KD / 16 * 64), 2) void delta_gradients_kernel(Delt
       }
     }
   }
-  if (!odd) {
-    unrolled<KB>([&](auto s_) {
-      constexpr int s = decltype(s_)::value;
-      const Frag kf = Op::column_mixed(Ks + columns_at + 32 * s * KS + r0, KS);
-      const Frag qf = Op::column_mixed(Qs + columns_at + 32 * s * KS + r0, KS);
-      auto behind = [&](const T* p, int t) {  // the tokens of block s in front of token tile t
-        return Op::template pair_tiles<true>(true, p + tile_of(t, 2 * s) * 256, 2 * s < t, p + tile_of(t, 2 * s + 1) * 256, PLANE, lane);
-      };
-      auto ahead = [&](const T* p, int t) {  // those behind it
-        return Op::template pair_tiles<false>(2 * s >= t, p + tile_of(2 * s, t) * 256, true, p + tile_of(2 * s + 1, t) * 256, PLANE, lane);
-      };
-      Pair f[TT];
+  // products with the tokens in front (A K to dq, B K to dk), or with those behind (A' Q and B' K to dk); what is not finite: term
+  // by term, without those whose weight is 0
+  auto products = [&](auto front_) {
+    constexpr bool FRONT = decltype(front_)::value;
+    if (!odd) {
+      unrolled<KB>([&](auto s_) {
+        constexpr int s = decltype(s_)::value, LO = FRONT ? 2 * s : 0, HI = FRONT ? TT : 2 * s + 2;
+        const Frag kf = Op::column_mixed(Ks + columns_at + 32 * s * KS + r0, KS);
+        const Frag xf = FRONT ? kf : Op::column_mixed(Qs + columns_at + 32 * s * KS + r0, KS);
+        auto tiles = [&](const T* p, int t) {
+          if constexpr (FRONT)
+            return Op::template wide_tiles<true>(true, p + tile_of(t, 2 * s) * 256, 2 * s < t, p + tile_of(t, 2 * s + 1) * 256, PLANE, lane);
+          else
+            return Op::template wide_tiles<false>(2 * s >= t, p + tile_of(2 * s, t) * 256, true, p + tile_of(2 * s + 1, t) * 256, PLANE, lane);
+        };
+        Wide f[TT];
 #pragma unroll
-      for (int t = 2 * s; t < TT; ++t) f[t] = behind(Ak, t);
-      mma_right<Op, 2 * s, TT>(kf, f, dq);
+        for (int t = LO; t < HI; ++t) f[t] = tiles(As, t);
+        mma_right<Op, LO, HI>(xf, f, FRONT ? dq : dk);
 #pragma unroll
-      for (int t = 2 * s; t < TT; ++t) f[t] = behind(Bs, t);
-      mma_right<Op, 2 * s, TT>(kf, f, dk);
-#pragma unroll
-      for (int t = 0; t < 2 * s + 2; ++t) f[t] = ahead(Aq, t);
-      mma_right<Op, 0, 2 * s + 2>(qf, f, dk);
-#pragma unroll
-      for (int t = 0; t < 2 * s + 2; ++t) f[t] = ahead(Bt, t);
-      mma_right<Op, 0, 2 * s + 2>(kf, f, dk);
-    });
-  } else {  // term by term, without those whose weight is 0
+        for (int t = LO; t < HI; ++t) f[t] = tiles(Bs, t);
+        mma_right<Op, LO, HI>(kf, f, dk);
+      });
+      return;
+    }
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
       const int tt = 16 * t + n;
       for (int s = 0; s < C; ++s) {
-        const int r = s > tt ? s : tt, c = s > tt ? tt : s, at = tile_of(r / 16, c / 16) * 256 + Op::tile_at(r % 16, c % 16);
-        const float ak = Op::score(Ak + at, PLANE), aq = Op::score(Aq + at, PLANE), bs = Op::score(Bs + at, PLANE),
-                    bt = Op::score(Bt + at, PLANE);
+        if (FRONT ? s > tt : s < tt) continue;
+        const int r = FRONT ? tt : s, c = FRONT ? s : tt, at = tile_of(r / 16, c / 16) * 256 + Op::tile_at(r % 16, c % 16);
+        const float wa = Op::whole(As + at, PLANE), wb = Op::whole(Bs + at, PLANE);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float kk = to_f(Ks[Op::at(s, r0 + 4 * g + i, KS)]), qq = to_f(Qs[Op::at(s, r0 + 4 * g + i, KS)]);
-          if (s <= tt && ak != 0.0f) dq[t][i] = fmaf(ak, kk, dq[t][i]);
-          if (s >= tt && aq != 0.0f) dk[t][i] = fmaf(aq, qq, dk[t][i]);
-          if (s < tt && bs != 0.0f) dk[t][i] = fmaf(bs, kk, dk[t][i]);
-          if (s > tt && bt != 0.0f) dk[t][i] = fmaf(bt, kk, dk[t][i]);
+          if (FRONT && wa != 0.0f) dq[t][i] = fmaf(wa, kk, dq[t][i]);
+          if (!FRONT && wa != 0.0f) dk[t][i] = fmaf(wa, qq, dk[t][i]);
+          if (s != tt && wb != 0.0f) dk[t][i] = fmaf(wb, kk, dk[t][i]);
         }
       }
     }
+  };
+  products(std::true_type{});
+  __syncthreads();  // Qd and Kd; the tiles have been read
+  {
+    int turn = 0;
+#pragma unroll
+    for (int ti = 0; ti < TT; ++ti)
+#pragma unroll
+      for (int si = 0; si <= ti; ++si, ++turn) {
+        if (turn % WAVES != wave) continue;
+        const int tile = tile_of(ti, si) * 256 + Op::tile_at(n, 4 * g);
+        Op::put_wide(As + tile, PLANE, lt[turn / WAVES]);
+        Op::put_wide(Bs + tile, PLANE, mt[turn / WAVES]);
+      }
   }
-  __syncthreads();  // Qd and Kd
+  __syncthreads();
+  products(std::false_type{});
 #pragma unroll
   for (int t = 0; t < TT; ++t) {
     const int tt = 16 * t + n;

@@ -47,7 +47,6 @@ struct Operand<__bf16> {
   static constexpr int steps(const Frag*, const Wide*) { return 3; }
   static constexpr int steps(const Wide*, const Frag*) { return 3; }
   static constexpr int steps(const Wide*, const Wide*) { return 6; }
-  static constexpr int steps(const Frag*, const Pair*) { return 2; }
   static __device__ __forceinline__ f32x4 step(int p, Frag a, const Wide& b, f32x4 c) {
     return mma(a, p == 0 ? b.l : p == 1 ? b.m : b.h, c);
   }
@@ -57,7 +56,6 @@ struct Operand<__bf16> {
   static __device__ __forceinline__ f32x4 step(int p, const Wide& a, const Wide& b, f32x4 c) {
     return mma(p == 1 ? a.l : p == 2 || p == 3 ? a.m : a.h, p == 0 ? b.l : p == 2 || p == 4 ? b.m : b.h, c);
   }
-  static __device__ __forceinline__ f32x4 step(int p, Frag a, const Pair& b, f32x4 c) { return mma(a, p == 0 ? b.l : b.h, c); }
   static __device__ __forceinline__ f32x4 mma(const Pair& a, Frag b, f32x4 c) { return mma(a.h, b, mma(a.l, b, c)); }
   static __device__ __forceinline__ f32x4 mma(Frag a, const Pair& b, f32x4 c) { return mma(a, b.h, mma(a, b.l, c)); }
   static __device__ __forceinline__ Frag row(const __bf16* p) { return *reinterpret_cast<const Frag*>(p); }
@@ -161,10 +159,7 @@ struct Operand<__bf16> {
     return Wide{tiles<ROW>(has_a, a, has_b, b, lane), tiles<ROW>(has_a, a + part, has_b, b + part, lane),
                 tiles<ROW>(has_a, a + 2 * part, has_b, b + 2 * part, lane)};
   }
-  template <bool ROW>
-  static __device__ __forceinline__ Pair pair_tiles(bool has_a, const __bf16* a, bool has_b, const __bf16* b, int part, int lane) {
-    return Pair{tiles<ROW>(has_a, a, has_b, b, lane), tiles<ROW>(has_a, a + part, has_b, b + part, lane)};
-  }
+  static __device__ __forceinline__ float whole(const __bf16* p, int part) { return to_f(p[0]) + (to_f(p[part]) + to_f(p[2 * part])); }
   static __device__ __forceinline__ Wide wide(const float (&x)[8]) {
     u32x4 h, m, l;
 #pragma unroll
@@ -268,10 +263,7 @@ struct Operand<float> {
     }
     return r;
   }
-  template <bool ROW>
-  static __device__ __forceinline__ Frag pair_tiles(bool has_a, const float* a, bool has_b, const float* b, int part, int lane) {
-    return wide_tiles<ROW>(has_a, a, has_b, b, part, lane);
-  }
+  static __device__ __forceinline__ float whole(const float* p, int) { return p[0]; }
   static __device__ __forceinline__ Frag wide(const float (&x)[8]) {
     Frag r;
 #pragma unroll
