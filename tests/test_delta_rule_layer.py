@@ -171,3 +171,63 @@ def test_angles_and_refusals():
         layer(torch.zeros(1, 5, 48).bfloat16())
     with pytest.raises(ValueError):
         DeltaRuleLayer(16, 2, 8, 8, taps=9)(torch.zeros(1, 5, 16))
+
+
+def apart(got, want):
+    """The distance's part of the norm."""
+    return float((got.detach().double().cpu() - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_autocast(device):
+    """32-bit weights under autocast: prompts in pieces behind a new state and tokens one by one, the states in the weights' type,
+    as without autocast but for the projections' rounding; a state from either side goes on at the other.
+
+    Bound: as for a layer in 16 bits, eight roundings of 2^-8 (six stages, a key's roundings meet the state twice) of the norm."""
+    layer = make(device, torch.float32)
+    x, positions = tokens(2, 30, 2, device, torch.float32), grid_positions(2, 3, 5, device=device)
+    cast = lambda: torch.autocast(device, dtype=torch.bfloat16)  # noqa: E731
+    want, (want_before, want_S) = oracle(layer, x, positions)
+    with torch.no_grad():
+        state = layer.new_state(2)
+        assert state[0].dtype == torch.float32
+        with cast():
+            whole = layer(x, positions=positions)
+            y, state = layer(x[:, :20], state, positions[:20], output_state=True)
+            assert whole.dtype == y.dtype == torch.bfloat16 and state[0].dtype == torch.float32
+            got = [y]
+            for t in range(20, 30):
+                got.append(layer.step(x[:, t], state, positions[t].expand(2, 3))[:, None])
+        got = torch.cat(got, 1)
+        assert got.dtype == torch.bfloat16
+        for mine, ref in ((whole, want), (got, want), (state[0], want_before), (state[1], want_S)):
+            assert apart(mine, ref) <= 8 * 2.0 ** -8
+        with cast():  # a state of a prompt without one has the projection's type
+            _, state = layer(x[:, :20], positions=positions[:20], output_state=True)
+            assert state[0].dtype == torch.bfloat16
+            y, _ = layer(x[:, 20:], state, positions[20:], output_state=True)
+        assert apart(y, want[:, 20:]) <= 8 * 2.0 ** -8
+        y, after = layer(x[:, 20:], state, positions[20:], output_state=True)  # goes on in 32 bits
+        assert y.dtype == after[0].dtype == torch.float32 and apart(y, want[:, 20:]) <= 8 * 2.0 ** -8
+        with pytest.raises(ValueError):  # in place it cannot hold what comes
+            layer.step(x[:, 20], state, positions[20].expand(2, 3))
+    with cast():
+        loss = layer(x, layer.new_state(2), positions).float().square().sum()
+    for p, g in zip(layer.parameters(), torch.autograd.grad(loss, list(layer.parameters()))):
+        assert g.dtype == p.dtype and g.isfinite().all() and g.any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_wider_state(device):
+    """A layer in 16 bits with its convolution's state in 32: the same bits as with a state in 16, which hold its inputs exactly."""
+    layer = make(device, torch.bfloat16)
+    x, positions = tokens(2, 12, 2, device, torch.bfloat16), grid_positions(2, 2, 3, device=device)
+    with torch.no_grad():
+        narrow, wide = layer.new_state(2), tuple(s.float() for s in layer.new_state(2))
+        a, narrow = layer(x[:, :9], narrow, positions[:9], output_state=True)
+        b, wide = layer(x[:, :9], wide, positions[:9], output_state=True)
+        assert narrow[0].dtype == torch.bfloat16 and wide[0].dtype == torch.float32
+        for t in range(9, 12):
+            at = positions[t].expand(2, 3)
+            a, b = (torch.cat([y, layer.step(x[:, t], s, at)[:, None]], 1) for y, s in ((a, narrow), (b, wide)))
+        assert torch.equal(a, b) and torch.equal(narrow[0].float(), wide[0]) and torch.equal(narrow[1], wide[1])

@@ -60,6 +60,11 @@ class DeltaRuleLayer(Angles, nn.Module):
         mixed, z, b, g = torch.split(self.in_proj(x), [sum(self._mixed), H * self.value_dim, H, H], dim=-1)
         return mixed, z, torch.sigmoid(b.float()), -F.softplus(g.float() + self.bias_gamma.float())
 
+    def _beside(self, mixed, before):
+        """The convolution's inputs and taps in a type that holds a state of another one too."""
+        wide = mixed.dtype if before is None else torch.promote_types(mixed.dtype, before.dtype)
+        return mixed.to(wide), self.conv_weight.to(torch.promote_types(self.conv_weight.dtype, wide))
+
     def _heads(self, mixed, positions):
         q, k, v = torch.split(mixed, self._mixed, dim=-1)
         q, k, v = (t.unflatten(-1, (t.shape[-1] // d, d)) for t, d in ((q, self.key_dim), (k, self.key_dim), (v, self.value_dim)))
@@ -75,7 +80,8 @@ class DeltaRuleLayer(Angles, nn.Module):
         return self.out_proj(rows.view(*z.shape))
 
     def new_state(self, slots: int) -> tuple[torch.Tensor, torch.Tensor]:
-        """States of ``slots`` sequences that have not begun: the convolution's and the mixer's."""
+        """States of ``slots`` sequences that have not begun: the convolution's, of the weights' type (which holds exactly what a
+        projection in fewer bits gives under autocast), and the mixer's."""
         w = self.in_proj.weight
         return (torch.zeros(slots, self.taps - 1, sum(self._mixed), dtype=w.dtype, device=w.device),
                 torch.zeros(slots, self.num_heads, self.key_dim, self.value_dim, dtype=torch.float32, device=w.device))
@@ -83,11 +89,14 @@ class DeltaRuleLayer(Angles, nn.Module):
     def forward(self, x: torch.Tensor, state: tuple[torch.Tensor, torch.Tensor] | None = None,
                 positions: torch.Tensor | None = None, output_state: bool = False):
         """``x [batch, tokens, dim]`` behind ``state``, with ``rotary_sections`` at ``positions [tokens, axes]`` or ``[batch,
-        tokens, axes]``; with ``output_state`` also the state behind the last token."""
+        tokens, axes]``; with ``output_state`` also the state behind the last token, the convolution's of the projection's type or
+        that of ``state``, whichever is wider."""
         mixed, z, beta, log_gamma = self._project(x)
         before, S = (None, None) if state is None else state
-        mixed, before = causal_conv(mixed, self.conv_weight, activation="silu", initial_state=before, output_state=True)
-        q, k, v = self._heads(mixed, positions)
+        rows, weight = self._beside(mixed, before)
+        rows, before = causal_conv(rows, weight, activation="silu", output_state=True,
+                                   initial_state=None if before is None else before.to(rows.dtype))
+        q, k, v = self._heads(rows.to(mixed.dtype), positions)
         out = delta_rule(q, k, v, log_gamma, beta, initial_state=S, output_state=output_state, normalize=True)
         o, S = out if output_state else (out, None)
         y = self._finish(o, z)
@@ -97,9 +106,11 @@ class DeltaRuleLayer(Angles, nn.Module):
     def step(self, x: torch.Tensor, state: tuple[torch.Tensor, torch.Tensor], positions: torch.Tensor | None = None,
              slots: torch.Tensor | None = None) -> torch.Tensor:
         """``x [batch, dim]``, one token of each sequence, with ``rotary_sections`` at ``positions [batch, axes]``; ``state``
-        (:meth:`new_state`) is updated in place, row ``b``'s at ``slots[b]`` (int32; outside: the row is skipped) or ``b``."""
+        (:meth:`new_state`, or of a type no narrower than the projection's) is updated in place, row ``b``'s at ``slots[b]`` (int32;
+        outside: the row is skipped) or ``b``."""
         mixed, z, beta, log_gamma = self._project(x)
-        mixed = causal_conv_step(mixed, state[0], self.conv_weight, activation="silu", slots=slots)
-        q, k, v = self._heads(mixed.unsqueeze(1), None if positions is None else positions.unsqueeze(1))
+        rows, weight = self._beside(mixed, state[0])
+        rows = causal_conv_step(rows, state[0], weight, activation="silu", slots=slots)
+        q, k, v = self._heads(rows.to(mixed.dtype).unsqueeze(1), None if positions is None else positions.unsqueeze(1))
         o = delta_rule_step(q.squeeze(1), k.squeeze(1), v.squeeze(1), log_gamma, beta, state[1], slots=slots, normalize=True)
         return self._finish(o, z)
