@@ -55,7 +55,8 @@ def _forward(x, weight, bias, activation, initial, want_state):
     B, T, C = x.shape
     y = x.new_empty((B, T, C))
     final = x.new_empty((B, weight.shape[1] - 1, C)) if want_state else None
-    launch(lib.ttc_causal_conv, "ttc_causal_conv", _block(unit_rows(x), weight, bias, activation, initial, y, final), x.device)
+    x = unit_rows(x)  # a copy lives until the launch
+    launch(lib.ttc_causal_conv, "ttc_causal_conv", _block(x, weight, bias, activation, initial, y, final), x.device)
     return y, final
 
 
