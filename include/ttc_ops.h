@@ -68,7 +68,7 @@ int ttc_rotary_axes(const ttc_rotary_axes_args* args, void* stream);
  * TTC_CAUSAL_CONV_MAX_TAPS.  y contiguous; final_state (NULL: not wanted): the last taps - 1 rows of w, contiguous
  * [batch, taps - 1, channels] as initial_state, both of x's type.
  * The backward takes d_y (unit stride along the channels) and d_final_state (NULL: zero) and writes dx, d_initial_state
- * (contiguous, x's type), dweight and dbias (weight_dtype); NULL: not wanted.
+ * (contiguous, x's type), dweight and dbias (weight_dtype; zero where there are no sequences or no tokens); NULL: not wanted.
  * workspace: ttc_causal_conv_workspace_bytes() of the same block (0: none needed). */
 #define TTC_CAUSAL_CONV_MAX_TAPS 8
 typedef struct {

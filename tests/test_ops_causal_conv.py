@@ -12,6 +12,7 @@ import torch
 
 from _ops_oracle import EPS, HALF, quotient, within
 from ttc.ops import causal_conv, causal_conv_step
+from ttc.ops._call import with_spaces
 from ttc.ops.causal_conv import causal_conv_torch
 from ttc.solvers._lib import lib
 
@@ -325,3 +326,23 @@ def test_c_entries_refuse():
                      (dict(act=3), 1)]:
         assert lib.ttc_causal_conv_step(pack(**kw), None) == code, kw
     assert lib.ttc_causal_conv_step(None, None) == 1 and lib.ttc_causal_conv_step(pack(B=0, slots=0), None) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,K", [(0, 5, 4), (0, 0, 1), (2, 0, 1), (2, 0, 3)])
+def test_c_backward_of_nothing(dtype, B, T, K):
+    """No sequences or no tokens: the weights' gradients are written, as zeros, and the state's is the final state's."""
+    from ttc.ops.causal_conv import _block
+    x = torch.empty(B, T, 24, dtype=dtype, device="cuda")
+    w, bias = torch.ones(24, K, dtype=dtype, device="cuda"), torch.ones(24, dtype=dtype, device="cuda")
+    dw, db, d_final = torch.full_like(w, 7), torch.full_like(bias, 7), make((B, K - 1, 24), dtype, "cuda", 1)
+    d_state, space = torch.full_like(d_final, 7), torch.empty(1 << 16, dtype=torch.uint8, device="cuda")
+    block = _block(x, w, bias, "silu", None, None, None, 1, x, d_final, x, dw, db, d_state)
+    need = lib.ttc_causal_conv_workspace_bytes(block)
+    assert need <= space.numel() and (B > 0 or need == 0)
+    if need:
+        block = with_spaces(block, space)
+    assert lib.ttc_causal_conv(block, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert not dw.any() and not db.any() and torch.equal(d_state, d_final)

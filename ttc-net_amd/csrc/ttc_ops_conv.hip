@@ -440,7 +440,8 @@ int conv_run(const ttc_causal_conv_args& A, hipStream_t s) {
       else hipLaunchKernelGGL((conv_backward_kernel<T, K, V, false>), grid, dim3(256), 0, s, P, first);
     });
   });
-  if (rc || !P.part) return rc;
+  if (rc || (!A.dweight && !A.dbias)) return rc;
+  // of no parts, where there are no sequences or no rows: sums of nothing
   hipLaunchKernelGGL(conv_join_kernel, dim3((unsigned)ceil_div(A.channels * (A.taps + 1), 64)), dim3(256), 0, s, P.part, parts,
                      A.channels, (int)A.taps, P.weight_bf16, A.dweight, A.dbias);
   return launched();
@@ -493,9 +494,8 @@ extern "C" int ttc_causal_conv(const ttc_causal_conv_args* args, void* stream) {
   const ttc_causal_conv_args& A = *args;
   if (const int rc = conv_check(A)) return rc;
   if (A.channels == 0 || (!A.backward && (A.batch == 0 || A.tokens + A.taps == 1))) return TTC_LQR_OK;
-  if (!A.weight || (A.tokens > 0 && !A.x)) return TTC_LQR_EINVAL;
-  if (!A.backward && A.tokens > 0 && !A.y) return TTC_LQR_EINVAL;
-  if (A.backward && A.tokens > 0 && !A.d_y) return TTC_LQR_EINVAL;
+  const bool some = A.batch > 0 && A.tokens > 0;
+  if (!A.weight || (some && (!A.x || (A.backward ? !A.d_y : !A.y)))) return TTC_LQR_EINVAL;
   const int64_t bytes = conv_bytes(A);
   if (bytes > 0 && (!A.workspace || A.workspace_bytes < bytes)) return TTC_LQR_EINVAL;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
