@@ -107,7 +107,7 @@ int ttc_causal_conv_step(const ttc_causal_conv_step_args* args, void* stream);
  * variance.  y0 = (x - mean) rstd weight + bias; y = act(y0), or y0 act(gate) where gate is not NULL.
  * activation 0: none, 1: silu (z sigmoid(z)).  weight and bias (both or neither, type weight_dtype): [c].
  * mean, rstd [n, groups] fp32: written by the forward (NULL: not kept), read by the backward.  The backward
- * writes dx, dgate (with a gate), dweight and dbias (NULL: not wanted).
+ * writes dx, dgate (with a gate), dweight and dbias (zero where n or l is 0); NULL: not wanted.
  * workspace: ttc_group_norm_workspace_bytes() of the same block (0: none needed). */
 typedef struct {
   int64_t dtype, weight_dtype, n, l, c, groups, activation, backward;

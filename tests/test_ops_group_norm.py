@@ -264,3 +264,20 @@ def test_gradients_term_by_term(device, dtype, act, gate, shape, groups):
     for name in xs:
         assert float(bound[name].max()) < 0.05 * float(want[name].abs().max()), name
         within(got[name], want[name], bound[name] + HALF[dtype] * 1.01 * want[name].abs())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,l", [(0, 1), (0, 9), (3, 0)])
+def test_c_backward_of_nothing(dtype, n, l):
+    """No rows or no positions: the weights' gradients are written, as zeros."""
+    from ttc.ops._call import DTYPES
+    from ttc.ops.group_norm import _BLOCK
+    w = torch.ones(24, dtype=dtype, device="cuda")
+    dw, db = torch.full_like(w, 7), torch.full_like(w, 7)
+    block = _BLOCK.pack(DTYPES[dtype], DTYPES[dtype], n, l, 24, 4, 0, 1, 1e-5, 0, 0, w.data_ptr(), w.data_ptr(), 0, 0, 0, 0, 0, 0,
+                        dw.data_ptr(), db.data_ptr(), 0, 0)
+    assert lib.ttc_group_norm_workspace_bytes(block) == 0
+    assert lib.ttc_group_norm(block, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert not dw.any() and not db.any()

@@ -773,6 +773,20 @@ inline NormPlan norm_plan(const ttc_group_norm_args& A, bool wide) {
   return P;
 }
 
+// the weights' gradients from their parts: zeros where there are none
+inline int affine_sums(const ttc_group_norm_args& A, const float* ws, int64_t parts, hipStream_t s) {
+  if (A.dweight || A.dbias) {
+    const dim3 grid((unsigned)ceil_div(A.c, 16));
+    if (A.weight_dtype == TTC_DTYPE_BF16)
+      hipLaunchKernelGGL(norm_affine_sum_kernel<__bf16>, grid, dim3(1024), 0, s, ws, parts, A.c,
+                         static_cast<__bf16*>(A.dweight), static_cast<__bf16*>(A.dbias));
+    else
+      hipLaunchKernelGGL(norm_affine_sum_kernel<float>, grid, dim3(1024), 0, s, ws, parts, A.c,
+                         static_cast<float*>(A.dweight), static_cast<float*>(A.dbias));
+  }
+  return launched();
+}
+
 template <class T, int V, bool SILU, bool GATE>
 int norm_run(const ttc_group_norm_args& A, const NormPlan& P, hipStream_t s) {
   const T *x = static_cast<const T*>(A.x), *gate = static_cast<const T*>(A.gate), *dy = static_cast<const T*>(A.dy);
@@ -855,16 +869,7 @@ int norm_run(const ttc_group_norm_args& A, const NormPlan& P, hipStream_t s) {
     if (rc != TTC_LQR_OK) return rc;
     parts = A.n * S.slabs;
   }
-  if (A.dweight || A.dbias) {
-    const dim3 grid((unsigned)ceil_div(A.c, 16));
-    if (A.weight_dtype == TTC_DTYPE_BF16)
-      hipLaunchKernelGGL(norm_affine_sum_kernel<__bf16>, grid, dim3(1024), 0, s, ws, parts, A.c,
-                         static_cast<__bf16*>(A.dweight), static_cast<__bf16*>(A.dbias));
-    else
-      hipLaunchKernelGGL(norm_affine_sum_kernel<float>, grid, dim3(1024), 0, s, ws, parts, A.c,
-                         static_cast<float*>(A.dweight), static_cast<float*>(A.dbias));
-  }
-  return launched();
+  return affine_sums(A, ws, parts, s);
 }
 
 template <class T, int V>
@@ -902,7 +907,8 @@ extern "C" int ttc_group_norm(const ttc_group_norm_args* args, void* stream) {
   if (!args) return TTC_LQR_EINVAL;
   const ttc_group_norm_args& A = *args;
   if (const int rc = norm_check(A)) return rc;
-  if (A.n == 0 || A.l == 0 || A.c == 0) return TTC_LQR_OK;
+  if (A.n == 0 || A.l == 0 || A.c == 0)
+    return A.backward && A.c > 0 ? affine_sums(A, nullptr, 0, reinterpret_cast<hipStream_t>(stream)) : TTC_LQR_OK;
   if (!A.x || !A.weight != !A.bias || !A.mean != !A.rstd) return TTC_LQR_EINVAL;
   if (A.backward ? !A.dy || !A.mean || (A.dgate && !A.gate) : !A.y) return TTC_LQR_EINVAL;
   const size_t need = norm_floats(A) * sizeof(float);
