@@ -5,6 +5,8 @@ initialisation, so of about 1; 32-bit rounding of some hundred products and sums
 each of the six stages (projection, convolution, turn, mixing, norm, projection) rounds once to 2^-8 a value, and a key's
 rounding meets the state twice (what is read at it, what is written): about 3 % of a value of 1 at the output, 0.1 absolute at
 its largest."""
+import sys
+
 import pytest
 import torch
 import torch.nn.functional as F
@@ -231,3 +233,55 @@ def test_wider_state(device):
             at = positions[t].expand(2, 3)
             a, b = (torch.cat([y, layer.step(x[:, t], s, at)[:, None]], 1) for y, s in ((a, narrow), (b, wide)))
         assert torch.equal(a, b) and torch.equal(narrow[0].float(), wide[0]) and torch.equal(narrow[1], wide[1])
+
+
+# Parts of the norm: in 16 bits eight roundings of 2^-8 (six stages; a key's meets the state twice), in 32 bits eight stages of
+# some 160 EPS, as for the mixer alone
+PART = {torch.float32: 8 * 160 * 2.0 ** -24, torch.bfloat16: 8 * 2.0 ** -8}
+KINDS = [{}, dict(rotary_sections=(), key_heads=4, taps=1), dict(layout="interleaved", key_heads=1, taps=3)]
+
+
+def places(T, device):
+    """Far from each other on every axis, so that turns matter between any two tokens."""
+    return torch.randint(0, 64, (T, 3), generator=torch.Generator().manual_seed(8)).to(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T", [1, 7, 60])
+@pytest.mark.parametrize("kw", KINDS)
+def test_by_the_norm(device, dtype, T, kw):
+    """Outputs and states by the size that they have: whole sequences, and the last five tokens one by one behind a prompt."""
+    layer = make(device, dtype, **kw)
+    x, positions, first = tokens(2, T, 1, device, dtype), places(T, device), max(T - 5, 0)
+    want, (want_before, want_S) = oracle(layer, x, positions)
+    with torch.no_grad():
+        y, state = layer(x, positions=positions, output_state=True)
+        part, pool = layer(x[:, :first], layer.new_state(2), positions[:first], output_state=True)
+        rows = [part, *(layer.step(x[:, t], pool, positions[t].expand(2, 3))[:, None] for t in range(first, T))]
+    for got, (before, S) in ((y, state), (torch.cat(rows, 1), pool)):
+        assert apart(got, want) <= PART[dtype] and apart(S, want_S) <= PART[dtype]
+        assert layer.taps == 1 or apart(before, want_before) <= PART[dtype]
+
+
+@pytest.mark.parametrize("T", [7, 60])
+@pytest.mark.parametrize("kw", KINDS)
+def test_mistakes_are_seen(monkeypatch, T, kw):
+    """Formulas without the turns, the decays, the strengths or the keys' lengths are further off than the bounds in 16 bits."""
+    layer, positions = make("cpu", torch.bfloat16, **kw), places(T, "cpu")
+    x = tokens(2, T, 1, "cpu", torch.bfloat16)
+    want, (_, want_S) = oracle(layer, x, positions)
+    plain = delta64
+    mistakes = {"decays": lambda q, k, v, g, b, *a, **kw: plain(q, k, v, 0 * g, b, *a, **kw),
+                "strengths": lambda q, k, v, g, b, *a, **kw: plain(q, k, v, g, 0 * b + 1, *a, **kw),
+                "lengths": lambda *a, normalize: plain(*a)}
+    for form in mistakes.values():
+        with monkeypatch.context() as m:
+            m.setattr(sys.modules[__name__], "delta64", form)
+            got, (_, S) = oracle(layer, x, positions)
+        assert apart(got, want) > 2 * PART[torch.bfloat16] and apart(S, want_S) > 2 * PART[torch.bfloat16]
+    if layer.rotary_sections:
+        with monkeypatch.context() as m:
+            m.setattr(sys.modules[__name__], "axes64", lambda t, *a: t.double())
+            got, (_, S) = oracle(layer, x, positions)
+        assert apart(got, want) > 2 * PART[torch.bfloat16] and apart(S, want_S) > 2 * PART[torch.bfloat16]
