@@ -5,8 +5,8 @@
 //   dw_i = sum_j c_j e_{i - j} (+ the final state's gradient),  dc_j = sum_t e_t w_{t + j},  dbias = sum_t e_t.
 // A thread holds 4 neighbouring channels and walks along a run of tokens with the last `taps` rows in registers,
 // so that a row is read from memory once (and once more from the caches at the start of each run).
-// Bound: memory.  16,381 tokens x 6,144 channels of 4 taps in bf16: 75 us for 403 MB, 5.4 TB/s; training on 4 x 2,048 x 4,096: 28
-// us forward, 60 us backward for 201 MB (3.4 TB/s: the K - 1 tokens in front of each run, and three waves a SIMD); one token of
+// Bound: memory.  16,381 tokens x 6,144 channels of 4 taps in bf16: 76 us for 403 MB, 5.4 TB/s; training on 4 x 2,048 x 4,096: 28
+// us forward, 58 to 61 us backward for 201 MB (3.4 TB/s: the K - 1 tokens in front of each run, and three waves a SIMD); one token of
 // 16 sequences: 3.7 us.
 #include "ttc_ops_common.hpp"
 
@@ -395,7 +395,7 @@ bool conv_wide(const ttc_causal_conv_args& A) {
 }
 
 // Sums of the weights' gradients: one row of them for each four runs of a sequence.  Of the block alone, whatever its
-// pointers: those of 16-byte vectors are fewer.
+// pointers: with vectors of channels they are fewer.
 inline int64_t conv_parts(const ttc_causal_conv_args& A, int64_t cols) {
   return A.batch * ceil_div(ceil_div(A.tokens + A.taps - 1, backward_run(A, cols)), 4);
 }

@@ -248,7 +248,15 @@ __global__ __launch_bounds__(256) void head_sum_kernel(const float* __restrict__
 
 // ---- host ----------------------------------------------------------------------------------------------------
 
-// Up to this many tokens are taken one by one where nothing is kept for a backward
+// Up to this many tokens are taken one by one where nothing is kept for a backward.  The chunk kernels' time (12.8 to 72 us) hardly
+// depends on the number of tokens below a chunk's, and meets the other's between 5 and 8.  us on the GPU, states in and out, one by
+// one by tokens, and in a chunk:                                     1     2     3     4     5     6     8    chunk
+//   1 sequence x 8 heads of 64 x 64, fp32                          4.5   5.9   7.2   8.6   9.9  11.3  14.1     12.8
+//   1 x 16 of 128 x 128, bf16                                      5.1   6.5   8.0   9.5  11.0  12.5  15.6     19.2
+//   16 x 16 of 128 x 128, bf16                                    11.0  13.1  15.8  18.4  20.9  23.3  28.7     25.5
+//   64 x 16 of 128 x 128, bf16                                    29.9  36.2  43.5  51.4  60.1  68.2  84.5     71.6
+//   64 x 32 of 64 x 64, bf16                                      17.9  24.0  31.6  39.3  47.5  55.7  70.5     58.2
+//   32 x 16 of 64 x 64, fp32                                       7.7  10.6  12.9  15.6  17.9  20.4  25.3     19.1
 constexpr int64_t ONE_BY_ONE = 4;
 
 inline int padded(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
@@ -281,13 +289,13 @@ struct DeltaLayout {  // bytes from the start of `saved` (inverse to E) and of t
 // Segments: enough workgroups to fill the GPU's 256 CUs twice, of at least 4 chunks each.  A split sweep does some three times
 // the work (own states, and what becomes of the one in front), so heads that fill the GPU by themselves are not split.  us a
 // call by the workgroups aimed at:                          1     128    256    384    512    768  1,024  1,536
-//   16,381 tokens x 16 heads of 128 x 128, bf16         1,403    629    447    468    426    468    484    532
-//   4 x 2,048 x 32 of 64 x 64, bf16, training             570    567    575    572    547    589    571    594
-//   2 x 2,048 x 32 of 128 x 128, bf16, training           708    707    711    713    691    759    745    791
-//   3 x 509 x 12 of 48 x 80, fp32, training               187    186    176    173    166    169    169    172
-//   4,096 x 16 of 128 x 128, fp32                         731    339    239    256    248    275    288    330
-//   4 x 4,096 x 8 of 32 x 32, bf16                        227    120     88     87     79     89     94     95
-//   8 x 2,048 x 32 of 128 x 128, bf16                     415    415    412    413    407    409    759    785
+//   16,381 tokens x 16 heads of 128 x 128, bf16         1,463    669    433    448    412    449    464    520
+//   4 x 2,048 x 32 of 64 x 64, bf16, training             581    581    576    551    536    578    557    558
+//   2 x 2,048 x 32 of 128 x 128, bf16, training           714    714    720    710    675    753    735    737
+//   3 x 509 x 12 of 48 x 80, fp32, training               174    174    160    157    157    157    157    157
+//   4,096 x 16 of 128 x 128, fp32                         735    344    242    256    250    276    296    295
+//   4 x 4,096 x 8 of 32 x 32, bf16                        248    124     88     90     80     80     80     80
+//   8 x 2,048 x 32 of 128 x 128, bf16                     414    413    414    414    411    405    721    675
 inline void segments_of(const ttc_delta_rule_args& A, DeltaLayout& W) {
   const int64_t sweeps = A.batch * A.heads * (A.dv > 64 ? 2 : 1);
   int64_t count = sweeps > 0 ? 512 / sweeps : 1;

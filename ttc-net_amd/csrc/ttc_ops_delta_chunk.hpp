@@ -16,17 +16,17 @@
 //
 // Bound.  Of a kernel's cycles (one MI355X)             vector ALU  matrix cores  waits  read, written (MB)    us
 //   16,381 tokens x 16 heads of 128 x 128, 16 segments
-//     prepare                                             40 %          9 %        57 %     70, 139            76
-//     sweep, STATE (values and matrix)                    59           40          24      105,  34           176
-//     join                                                14            5          46       17,  17            53
-//     sweep                                               49           32          36      168,  68           150
+//     prepare                                             41 %          9 %        57 %     70, 139            74
+//     sweep, STATE (values and matrix)                    59           40          24       99,  32           173
+//     join                                                14            5          46       17,  17            52
+//     sweep                                               50           36          26      179,  68           163
 //   training on 4 x 2,048 tokens x 32 heads of 64 x 64, 4 segments
-//     prepare                                             49           10          59       35, 139            56
-//     sweep, STATE (values and matrix)                    61           35          27       71,  17            64
-//     sweep, with what the backward needs                 36           17          27      114, 168            88
-//     sweep back, STATE                                   36           25          28      120,   8            58
-//     sweep back                                          34           20          22      124, 135            84
-//     gradients                                           38           14          54      193, 113           193
+//     prepare                                             48           10          59       35, 139            56
+//     sweep, STATE (values and matrix)                    61           35          27       67,  13            62
+//     sweep, with what the backward needs                 35           20          24      124, 168            93
+//     sweep back, STATE                                   41           29          30       90,   6            58
+//     sweep back                                          33           20          22      124, 135            83
+//     gradients                                           39           15          48      195, 112           205
 // (read and written behind the XCDs' caches).  The sweeps wait for their own chain, one chunk after the other, and split three
 // ways what the state is multiplied with (176 of some 650 vector instructions a chunk at 128 rows); more waves a SIMD would
 // cover it, but a wave needs 150 to 250 registers.  Operands of different sums are read first and their instructions issued
@@ -653,9 +653,11 @@ __global__ __launch_bounds__(WAVES * 64, 2) void delta_sweep_kernel(Delta A) {
 //   db_s = sum_t x_ts + f_s,   dg_t = the sum over all terms of the loss's gradient that decay across token t: pairs s < t <= t',
 //   the state in front (into tokens from t on), the state behind (from tokens before t), and the state through the chunk.
 // Values come 32 columns at a time, split into their parts once (all at once, split by each wave that reads them: 4,096 chunks of
-// 64 x 64 265 us, so 193).  Waves share the score tiles, and each takes 16 columns of the keys; its lanes hold one token and 4
-// neighbouring columns.  Bound by latency: two workgroups a CU (66 KB at 64), each of which loads, meets, multiplies and stores;
-// without the second 32 columns 160 us, without the tiles' sums 175, without the products with keys and queries 182.
+// 64 x 64 265 us, so 193 with score tiles in two parts).  Waves share the score tiles, in three parts of which those that meet the
+// tokens in front of each take turns with those that meet the tokens behind (205 us; all four sets in two parts 193), and each wave
+// takes 16 columns of the keys; its lanes hold one token and 4 neighbouring columns.  Bound by latency: two workgroups a CU (66 KB at
+// 64), each of which loads, meets, multiplies and stores; of the 193, without the second 32 columns 160 us, without the tiles' sums
+// 175, without the products with keys and queries 182.
 template <class T, int KD>
 __global__ __launch_bounds__((KD / 16 * 64), 2) void delta_gradients_kernel(Delta A) {
   using Z = DeltaShape<T, KD>;

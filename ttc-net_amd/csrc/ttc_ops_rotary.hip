@@ -52,7 +52,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const T* __restrict__ q, co
   float c[PAIRS], s[PAIRS];
   if (turn && AXES) {
     // Every axis's position at once, then each pair's entry, 8 bytes from the cache: a vector's pairs lie in one section or in
-    // several.  HEADS heads share them: 16,381 tokens x (16 + 16) heads of 128 on three axes 52 us, on one 48
+    // several.  HEADS heads share them: 16,381 tokens x (16 + 16) heads of 128 on three axes 53 us, on one 48
     const int pair = INTER ? at / 2 : at;
     int64_t p[TTC_ROTARY_MAX_AXES];
 #pragma unroll

@@ -7,8 +7,8 @@ several axes (:func:`ttc.ops.rotary_axes`), the gated delta rule mixes them (:fu
     q, k, v, z, b, g = in_proj(x);   q, k, v = silu(conv(q, k, v))
     o = delta_rule(q, k, v, log_gamma = -softplus(g + bias_gamma), beta = sigmoid(b));   y = out_proj(group_norm(o) * silu(z))
 
-:meth:`forward` takes whole sequences (training, prompts), :meth:`step` one token of each sequence of a batch, whose states it
-updates in place.  A sequence's state, whatever its length, is the last ``taps - 1`` inputs of the convolution and
+:meth:`forward` takes whole sequences (training, prompts) of one text each, :meth:`step` one token of each sequence of a batch, whose
+states it updates in place.  A sequence's state, whatever its length, is the last ``taps - 1`` inputs of the convolution and
 ``[heads, key_dim, value_dim]`` float32.
 """
 from __future__ import annotations
