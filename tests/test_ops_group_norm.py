@@ -281,3 +281,9 @@ def test_c_backward_of_nothing(dtype, n, l):
     assert lib.ttc_group_norm(block, torch.cuda.current_stream().cuda_stream) == 0
     torch.cuda.synchronize()
     assert not dw.any() and not db.any()
+
+
+def test_c_backward_of_nothing_that_is_wanted():
+    """No gradients asked for: nothing is launched (no GPU is touched)."""
+    from ttc.ops.group_norm import _BLOCK
+    assert lib.ttc_group_norm(_BLOCK.pack(0, 0, 0, 1, 24, 4, 0, 1, 1e-5, *(0,) * 14), None) == 0

@@ -908,7 +908,8 @@ extern "C" int ttc_group_norm(const ttc_group_norm_args* args, void* stream) {
   const ttc_group_norm_args& A = *args;
   if (const int rc = norm_check(A)) return rc;
   if (A.n == 0 || A.l == 0 || A.c == 0)
-    return A.backward && A.c > 0 ? affine_sums(A, nullptr, 0, reinterpret_cast<hipStream_t>(stream)) : TTC_LQR_OK;
+    return A.backward && A.c > 0 && (A.dweight || A.dbias) ? affine_sums(A, nullptr, 0, reinterpret_cast<hipStream_t>(stream))
+                                                           : TTC_LQR_OK;
   if (!A.x || !A.weight != !A.bias || !A.mean != !A.rstd) return TTC_LQR_EINVAL;
   if (A.backward ? !A.dy || !A.mean || (A.dgate && !A.gate) : !A.y) return TTC_LQR_EINVAL;
   const size_t need = norm_floats(A) * sizeof(float);
